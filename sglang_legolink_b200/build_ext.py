@@ -25,6 +25,8 @@ CUDA_SOURCES = [
     "bindings.cpp",
     "gemm_tcgen05.cu",
     "elementwise.cu",
+    "lora.cu",
+    "sampling.cu",
     "attention.cu",
     "attention_tc.cu",
     "gemm_small_m_noalloc.cu",

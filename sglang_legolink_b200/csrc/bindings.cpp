@@ -9,6 +9,8 @@
 using bf16 = __nv_bfloat16;
 
 #include "gemm_epi.h"
+#include "lora.h"
+#include "sampling.h"
 #include "tp_fused.h"
 
 extern "C" {
@@ -21,6 +23,13 @@ int ll_gemm_small_m_splits(int N, int K);
 int ll_gemm_bf16_small_m_ex(const bf16* A, int lda, const bf16* W, int ldw, bf16* C, int ldc, const bf16* bias,
                             int M, int N, int K, int splits, float* ws, size_t ws_floats, int* tickets, int* err,
                             int flags, cudaStream_t stream);
+int ll_lora_low(const bf16* x, int64_t ldx, int M, int K, const LLLora* lo, int* err, cudaStream_t stream);
+int ll_gemm_bf16_small_m_lora(const void* A, int lda, const void* W, int ldw, void* C, int ldc, const void* bias,
+                              int M, int N, int K, int splits, float* ws, size_t ws_floats, int* tickets, int* err,
+                              int w_tiled, const LLSmallMEpi* epi, const LLLora* lo, void* stream);
+int ll_gemm_bf16_lora(const void* A, int lda, const void* W, int ldw, void* C, int ldc, const void* bias, int M,
+                      int N, int K, int epilogue, const LLLora* lo, int* err, void* stream);
+int ll_sample(const LLSample* p, cudaStream_t stream);
 int ll_rmsnorm(bf16* out, const bf16* x, bf16* residual, const bf16* w, int rows, int hidden, float eps,
                cudaStream_t stream);
 int ll_rope_qkv_write(const bf16* qkv, const int* positions, const int64_t* slots, const float* cos_sin, bf16* q_out,
@@ -65,7 +74,12 @@ inline bf16* bp(const at::Tensor& t) { return reinterpret_cast<bf16*>(t.data_ptr
 inline bf16* bp_opt(const c10::optional<at::Tensor>& t) { return t.has_value() ? bp(*t) : nullptr; }
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
-void check_rc(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
+// Numbers go into error messages as strings: the toolchain may link its C++
+// library into this extension statically, and a stream that formats a number
+// with the facets of two copies of it crashes.
+inline std::string num(int64_t v) { return std::to_string(v); }
+
+void check_rc(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", num(rc)); }
 
 // out[M, N] = a[M, K] @ w[N, K]^T (+ bias).  a/out may be row-strided views.
 void gemm(const at::Tensor& a, const at::Tensor& w, const c10::optional<at::Tensor>& bias, at::Tensor& out,
@@ -341,6 +355,119 @@ void gemm_small_m_epi(const at::Tensor& a, const at::Tensor& w, const c10::optio
            "ll_gemm_bf16_small_m_epi");
 }
 
+// A projection with per-row low-rank adapters (lora.h): the low-rank rows,
+// then the shared product with the adapters' B as further k-blocks.  The
+// scratch is this call's own, so calls on different streams share nothing.
+// plan: int32 [row_slot M | tile_ptr tiles + 1 | plane_adapter max_planes].
+void lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, at::Tensor& out,
+                 const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale, const at::Tensor& plan,
+                 int64_t tile_rows, int64_t max_planes, bool small_m, int64_t splits, bool swiglu,
+                 const at::Tensor& err) {
+  CHECK_CUDA(x); CHECK_BF16(x); CHECK_BF16(w); CHECK_BF16(out); CHECK_BF16(a); CHECK_BF16(b); CHECK_F32(scale);
+  CHECK_I32(plan); CHECK_I32(err); CHECK_CONTIG(w); CHECK_CONTIG(a); CHECK_CONTIG(b); CHECK_CONTIG(scale);
+  CHECK_CONTIG(plan); CHECK_ALIGN16(x); CHECK_ALIGN16(w); CHECK_ALIGN16(a); CHECK_ALIGN16(b); CHECK_ALIGN16(out);
+  for (const at::Tensor* t : {&w, static_cast<const at::Tensor*>(&out), &a, &b, &scale, &plan, &err})
+    TORCH_CHECK(t->device() == x.device(), "all tensors must be on ", x.device().str());
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && out.dim() == 2 && a.dim() == 3 && b.dim() == 3);
+  TORCH_CHECK(x.stride(1) == 1 && out.stride(1) == 1, "inner dim must be contiguous");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0), n = a.size(0), R = a.size(1);
+  TORCH_CHECK(M > 0 && M < (1 << 28) && K > 0 && N > 0 && n > 0, "empty projection");
+  TORCH_CHECK(w.size(1) == K && a.size(2) == K, "K of x, w and the adapters differ");
+  TORCH_CHECK(b.size(0) == n && b.size(1) == N && b.size(2) == R && scale.numel() == n, "adapter shapes differ");
+  TORCH_CHECK(R % 8 == 0 && R <= LL_LORA_MAX_RANK, "adapter rank must be a multiple of 8, at most ", num(LL_LORA_MAX_RANK));
+  TORCH_CHECK(K % 8 == 0 && N % 8 == 0 && (!swiglu || N % 32 == 0), "K and N must be multiples of 8 (N of 32: SwiGLU)");
+  TORCH_CHECK(x.stride(0) % 8 == 0 && out.stride(0) % 8 == 0, "row strides must be multiples of 8");
+  TORCH_CHECK(x.stride(0) < (1ll << 31) && out.stride(0) < (1ll << 31), "row strides must be below 2^31");
+  TORCH_CHECK(out.size(0) == M && out.size(1) == (swiglu ? N / 2 : N), "bad output shape");
+  if (bias.has_value()) {
+    CHECK_BF16(*bias); CHECK_CONTIG(*bias);
+    TORCH_CHECK(bias->numel() == N && bias->device() == x.device(), "bad bias");
+  }
+  const int64_t tiles = (M + tile_rows - 1) / tile_rows;
+  TORCH_CHECK(tile_rows == (M <= 128 ? 128 : 256) && max_planes >= 1, "bad plan");
+  TORCH_CHECK(plan.numel() == M + tiles + 1 + max_planes, "the plan is for another batch");
+  TORCH_CHECK(max_planes * tile_rows < (1ll << 31), "too many adapters per tile of rows");
+  TORCH_CHECK(!small_m || (M <= 128 && splits >= 1), "bad split count");
+  c10::cuda::CUDAGuard g(x.device());
+  const int nt = small_m ? (int)((N + 127) / 128) : 0;
+  auto low = at::empty({max_planes * tile_rows, R}, x.options());
+  at::Tensor ws, tickets;
+  if (small_m && splits > 1) {
+    ws = at::empty({splits * M * N}, scale.options());
+    tickets = at::empty({nt}, plan.options());
+  }
+  LLLora lo{};
+  lo.a = bp(a);
+  lo.b = bp(b);
+  lo.scale = scale.data_ptr<float>();
+  lo.row_slot = plan.data_ptr<int>();
+  lo.tile_ptr = lo.row_slot + M;
+  lo.plane_adapter = lo.tile_ptr + tiles + 1;
+  lo.low = bp(low);
+  lo.tickets = tickets.defined() ? tickets.data_ptr<int>() : nullptr;
+  lo.num_tickets = tickets.defined() ? nt : 0;
+  lo.adapters = (int)n;
+  lo.rank = (int)R;
+  lo.tiles = (int)tiles;
+  lo.tile_rows = (int)tile_rows;
+  lo.max_planes = (int)max_planes;
+  check_rc(ll_lora_low(bp(x), x.stride(0), (int)M, (int)K, &lo, err.data_ptr<int>(), cur_stream()), "ll_lora_low");
+  void* bias_p = bias.has_value() ? bias->data_ptr() : nullptr;
+  if (small_m) {
+    LLSmallMEpi epi{};
+    epi.mode = swiglu ? LL_EPI_SWIGLU : LL_EPI_STORE;
+    check_rc(ll_gemm_bf16_small_m_lora(x.data_ptr(), (int)x.stride(0), w.data_ptr(), (int)K, out.data_ptr(),
+                                       (int)out.stride(0), bias_p, (int)M, (int)N, (int)K, (int)splits,
+                                       ws.defined() ? ws.data_ptr<float>() : nullptr,
+                                       ws.defined() ? (size_t)ws.numel() : 0, lo.tickets, err.data_ptr<int>(), 0, &epi,
+                                       &lo, cur_stream()),
+             "ll_gemm_bf16_small_m_lora");
+  } else {
+    check_rc(ll_gemm_bf16_lora(x.data_ptr(), (int)x.stride(0), w.data_ptr(), (int)K, out.data_ptr(),
+                               (int)out.stride(0), bias_p, (int)M, (int)N, (int)K, swiglu ? 1 : 0, &lo,
+                               err.data_ptr<int>(), cur_stream()),
+             "ll_gemm_bf16_lora");
+  }
+}
+
+// One token per row of logits (sampling.h).
+void sample(const at::Tensor& logits, const at::Tensor& u, const c10::optional<at::Tensor>& temperature,
+            const c10::optional<at::Tensor>& top_k, const c10::optional<at::Tensor>& top_p,
+            const c10::optional<at::Tensor>& min_p, at::Tensor& out, const c10::optional<at::Tensor>& logprob) {
+  CHECK_CUDA(logits); CHECK_I32(out);
+  TORCH_CHECK(logits.dim() == 2, "logits must be [rows, vocabulary]");
+  TORCH_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat,
+              "logits must be bfloat16 or float32");
+  const int64_t B = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V > 0 && V <= LL_SAMPLE_MAX_VOCAB, "the vocabulary must have 1 to ", num(LL_SAMPLE_MAX_VOCAB), " tokens");
+  TORCH_CHECK(B < (1 << 27), "too many rows");
+  TORCH_CHECK(V == 1 || logits.stride(1) == 1, "a row of logits must be contiguous");
+  LLSample p{};
+  auto arg = [&](const at::Tensor& t, at::ScalarType type, const char* name) -> void* {
+    TORCH_CHECK(t.device() == logits.device(), name, " must be on ", logits.device().str());
+    TORCH_CHECK(t.scalar_type() == type, name, " must be ", c10::toString(type));
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == B && t.is_contiguous(), name, " must be a contiguous [rows] tensor");
+    return t.data_ptr();
+  };
+  p.u = static_cast<const double*>(arg(u, at::kDouble, "uniforms"));
+  if (temperature.has_value()) p.temperature = static_cast<const float*>(arg(*temperature, at::kFloat, "temperature"));
+  if (top_k.has_value()) p.top_k = static_cast<const int*>(arg(*top_k, at::kInt, "top_k"));
+  if (top_p.has_value()) p.top_p = static_cast<const float*>(arg(*top_p, at::kFloat, "top_p"));
+  if (min_p.has_value()) p.min_p = static_cast<const float*>(arg(*min_p, at::kFloat, "min_p"));
+  p.out = static_cast<int*>(arg(out, at::kInt, "out"));
+  if (logprob.has_value()) p.logprob = static_cast<float*>(arg(*logprob, at::kFloat, "logprobs"));
+  if (B == 0) return;
+  p.logits = logits.data_ptr();
+  p.stride = logits.stride(0);
+  p.B = (int)B;
+  p.V = (int)V;
+  p.fp32 = logits.scalar_type() == at::kFloat;
+  c10::cuda::CUDAGuard g(logits.device());
+  const int rc = ll_sample(&p, cur_stream());
+  TORCH_CHECK(rc != -4, "a row of ", num(V), " fp32 logits does not fit a cluster's shared memory");
+  check_rc(rc, "ll_sample");
+}
+
 void rmsnorm(at::Tensor& out, const at::Tensor& x, const c10::optional<at::Tensor>& residual, const at::Tensor& w,
              double eps) {
   CHECK_CUDA(x); CHECK_BF16(x); CHECK_BF16(out); CHECK_BF16(w); CHECK_CONTIG(x); CHECK_CONTIG(out);
@@ -489,6 +616,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_small_m", &gemm_small_m);
   m.def("gemm_small_m_splits", &gemm_small_m_splits);
   m.def("gemm_small_m_epi", &gemm_small_m_epi);
+  m.def("lora_linear", &lora_linear);
+  m.def("sample", &sample);
   m.def("rmsnorm", &rmsnorm);
   m.def("rope_qkv_write", &rope_qkv_write);
   m.def("kv_link_rope", &kv_link_rope);

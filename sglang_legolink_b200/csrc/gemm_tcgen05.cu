@@ -32,6 +32,7 @@
 
 #include "common.cuh"
 #include "gemm_epi.h"
+#include "lora.h"
 #include "tp_fused.h"
 
 namespace ll {
@@ -46,6 +47,27 @@ enum Epilogue : int { kEpiPlain = 0, kEpiSwiGLU = 1, kEpiScatter = 2 };
 
 // Tensor-parallel hooks of the 2-SM kernel (tp_fused.h, tp_fused.cu).
 using TpArgs = LLTpArgs;
+
+// Low-rank adapters beside the shared product (lora.h): after the k-blocks of
+// K, an output tile runs more k-blocks, 64 ranks of one adapter each, over
+// the adapter's low-rank rows (`low`, the A side of the product) and its
+// B matrix.  They accumulate into the same TMEM accumulator, so the adapters'
+// term joins the product in fp32, before the epilogue, and costs no pass over
+// the output: at 5087 rows x 4608 outputs a separate pass would read and write
+// 94 MB (14 us at HBM rate), the extra k-block adds 1 to 56 (2 us of 118).
+// NoLora compiles the kernels without any of it.
+struct NoLora {
+  static constexpr bool on = false;
+};
+struct alignas(64) LoraBlocks {
+  static constexpr bool on = true;
+  CUtensorMap tm_low;        // [planes * tile_rows, rank]
+  CUtensorMap tm_b;          // [adapters, N, rank]
+  const int* tile_ptr;       // planes of row tile t: [tile_ptr[t], tile_ptr[t + 1])
+  const int* plane_adapter;  // adapter of each plane
+  int rank_blocks;           // 64-rank blocks of an adapter
+  int tile_rows;             // rows of a plane
+};
 
 template <int BN>
 struct GemmCfg {
@@ -489,12 +511,12 @@ struct SwapCfg {
 //
 // kTile (BNX == 16, 2 <= M <= 16, MODE >= 0): the tile epilogue (TileEpi)
 // instead of the one-row-at-a-time one.
-template <int BNX, int RING_KB, bool kRowPrefetch, int MODE = -1, bool kTile = false>
+template <int BNX, int RING_KB, bool kRowPrefetch, int MODE = -1, bool kTile = false, class Lora = NoLora>
 __global__ void __launch_bounds__(192, 2)
     gemm_swapab_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                        bf16* __restrict__ C, const bf16* __restrict__ bias, int M, int N, int K, int ldc,
                        int kb_per_split, float* __restrict__ ws, int* __restrict__ tickets, int* err,
-                       int w_tiled, const __grid_constant__ LLSmallMEpi epi) {
+                       int w_tiled, const __grid_constant__ LLSmallMEpi epi, const __grid_constant__ Lora lora) {
   const int mode = MODE >= 0 ? MODE : epi.mode;
   using Cfg = SwapCfg<BNX, RING_KB>;
   constexpr int STAGES = Cfg::STAGES;
@@ -514,8 +536,15 @@ __global__ void __launch_bounds__(192, 2)
   const int nb = blockIdx.x;  // feature tile
   const int split = blockIdx.y, nsplit = gridDim.y;
   const int num_kb = (K + GEMM_BK - 1) / GEMM_BK;
-  const int kb0 = split * kb_per_split;
-  const int kb1 = min(num_kb, kb0 + kb_per_split);
+  int kb_all = num_kb, kb_per = kb_per_split;
+  if constexpr (Lora::on) {
+    // the adapters' k-blocks follow those of K; how many there are is known
+    // on the device only (a captured graph replays with other adapters)
+    kb_all += lora.tile_ptr[1] * lora.rank_blocks;
+    kb_per = (kb_all + nsplit - 1) / nsplit;
+  }
+  const int kb0 = split * kb_per;
+  const int kb1 = min(kb_all, kb0 + kb_per);
   pdl_trigger();
 
   if (threadIdx.x == 0) {
@@ -542,7 +571,8 @@ __global__ void __launch_bounds__(192, 2)
       // The weights do not depend on the previous kernel: start streaming the
       // first ring's worth of them before waiting for it, then add the
       // activation tiles once its output is visible.
-      const int pre = (kb1 - kb0) < STAGES ? (kb1 - kb0) : STAGES;
+      const int base1 = min(kb1, num_kb);  // k-blocks of K in this split
+      const int pre = max(0, min(base1 - kb0, STAGES));
       for (int i = 0; i < pre; ++i) {
         mbar_arrive_expect_tx(&full[i], Cfg::W_BYTES + Cfg::X_BYTES);
         if (w_tiled)  // one contiguous 16 KB tile
@@ -554,12 +584,27 @@ __global__ void __launch_bounds__(192, 2)
       for (int i = 0; i < pre; ++i)
         tma_load_2d(sX + i * Cfg::X_BYTES, &tmX, &full[i], (kb0 + i) * GEMM_BK, 0);
       if (pre == STAGES) phase = 1;  // stage wrapped around exactly once
+      else stage = pre;
       for (int kb = kb0 + pre; kb < kb1; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
           ok = false;
           break;
         }
         mbar_arrive_expect_tx(&full[stage], Cfg::W_BYTES + Cfg::X_BYTES);
+        if constexpr (Lora::on) {
+          if (kb >= num_kb) {  // 64 ranks of one adapter
+            const int plane = (kb - num_kb) / lora.rank_blocks, rb = (kb - num_kb) % lora.rank_blocks;
+            tma_load_3d(sW + stage * Cfg::W_BYTES, &lora.tm_b, &full[stage], rb * GEMM_BK, nb * GEMM_BM,
+                        lora.plane_adapter[plane]);
+            tma_load_2d(sX + stage * Cfg::X_BYTES, &lora.tm_low, &full[stage], rb * GEMM_BK,
+                        plane * lora.tile_rows);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+            continue;
+          }
+        }
         if (w_tiled)
           tma_load_4d_(sW + stage * Cfg::W_BYTES, &tmW, &full[stage], 0, 0, kb, nb);
         else
@@ -956,6 +1001,15 @@ __device__ __forceinline__ void tma_load_2d_2sm(void* smem_dst, const void* tmap
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_3d_2sm(void* smem_dst, const void* tmap, uint32_t leader_bar, int x, int y,
+                                                int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(tmap), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 __device__ __forceinline__ void umma_bf16_2sm(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                               uint32_t accumulate) {
   asm volatile(
@@ -1068,12 +1122,12 @@ struct Gemm2Cfg {
   static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + EPI_BYTES + 1024 + 256;
 };
 
-template <int BN, int EPI>
+template <int BN, int EPI, class Lora = NoLora>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     gemm_tcgen05_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                             const __grid_constant__ CUtensorMap tmC, int c_bulk, bf16* __restrict__ C,
                             const bf16* __restrict__ bias, int M, int N, int K, int ldc, int* err,
-                            const __grid_constant__ TpArgs tp, int group_m) {
+                            const __grid_constant__ TpArgs tp, int group_m, const __grid_constant__ Lora lora) {
   using Cfg = Gemm2Cfg<BN>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -1149,6 +1203,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
             phase ^= 1;
           }
         }
+        if constexpr (Lora::on) {
+          const int p0 = lora.tile_ptr[mb], n_extra = (lora.tile_ptr[mb + 1] - p0) * lora.rank_blocks;
+          for (int e = 0; e < n_extra && ok; ++e) {
+            if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
+              ok = false;
+              break;
+            }
+            const int plane = p0 + e / lora.rank_blocks, rb = e % lora.rank_blocks;
+            const uint32_t leader_full = mapa_shared(smem_u32(&full[stage]), 0);
+            if (crank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
+            tma_load_2d_2sm(sA + stage * Cfg::A_BYTES, &lora.tm_low, leader_full, rb * GEMM_BK,
+                            plane * lora.tile_rows + (int)crank * GEMM_BM);
+            tma_load_3d_2sm(sB + stage * Cfg::B_BYTES, &lora.tm_b, leader_full, rb * GEMM_BK,
+                            nb * BN + (int)crank * (BN / 2), lora.plane_adapter[plane]);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
       }
       if (!ok) {
         unsigned long long t0 = globaltimer_ns();
@@ -1166,7 +1240,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         if (!mbar_wait(&tempty[acc], aphase ^ 1, err, kErrTmemEmptyTimeout)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        int num_kb_t = num_kb;
+        if constexpr (Lora::on) {
+          int mb, nb;
+          tile_coords(t, num_m, num_n, group_m, mb, nb);
+          num_kb_t += (lora.tile_ptr[mb + 1] - lora.tile_ptr[mb]) * lora.rank_blocks;
+        }
+        for (int kb = 0; kb < num_kb_t; ++kb) {
           if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) {
             ok = false;
             break;
@@ -1492,7 +1572,7 @@ extern "C" int ll_gemm_bf16(const bf16* A, int lda, const bf16* W, int ldw, bf16
       init = true;                                                                                    \
     }                                                                                                 \
     kern<<<2 * pairs, 192, Gemm2Cfg<256>::SMEM, stream>>>(tA, tB, tC, c_bulk, C, bias, M, N, K, ldc, err, \
-                                                           TpArgs{}, gemm_group_m(M, K, 2 * GEMM_BM)); \
+                                                           TpArgs{}, gemm_group_m(M, K, 2 * GEMM_BM), NoLora{}); \
   } while (0)
     if (epilogue == kEpiSwiGLU) LL_LAUNCH2(kEpiSwiGLU); else LL_LAUNCH2(kEpiPlain);
 #undef LL_LAUNCH2
@@ -1564,7 +1644,7 @@ extern "C" int ll_gemm_bf16_tp(const void* A_, int lda, const void* W_, int ldw,
       init = true;                                                                                    \
     }                                                                                                 \
     kern<<<2 * pairs, 192, Gemm2Cfg<256>::SMEM, stream>>>(tA, tB, tC, c_bulk, C, bias, M, N, K, ldc, err, \
-                                                           *tp, gemm_group_m(M, K, 2 * GEMM_BM));    \
+                                                           *tp, gemm_group_m(M, K, 2 * GEMM_BM), NoLora{}); \
   } while (0)
   if (epilogue == kEpiSwiGLU) LL_LAUNCH_TP(kEpiSwiGLU);
   else if (epilogue == kEpiScatter) LL_LAUNCH_TP(kEpiScatter);
@@ -1657,13 +1737,8 @@ static bool small_m_tile_ok(const bf16* C, int ldc, const bf16* bias, int M, int
   }
 }
 
-static int small_m_launch(const bf16* A, int lda, const bf16* W, int ldw, bf16* C, int ldc, const bf16* bias, int M,
-                          int N, int K, int splits, float* ws, size_t ws_floats, int* tickets, int* err, int w_tiled,
-                          const LLSmallMEpi& epi, cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (M > 128) return -3;
-  if ((K % 8) || (lda % 8) || (ldw % 8)) return -3;
-  if (w_tiled && ((N % 128) || (K % 64))) return -3;
+// Arguments that the epilogue of a small-M launch needs.
+static int small_m_check_epi(const bf16* C, int N, const LLSmallMEpi& epi) {
   switch (epi.mode) {
     case LL_EPI_STORE:
       if (C == nullptr) return -3;
@@ -1685,6 +1760,17 @@ static int small_m_launch(const bf16* A, int lda, const bf16* W, int ldw, bf16* 
     default:
       return -3;
   }
+  return 0;
+}
+
+static int small_m_launch(const bf16* A, int lda, const bf16* W, int ldw, bf16* C, int ldc, const bf16* bias, int M,
+                          int N, int K, int splits, float* ws, size_t ws_floats, int* tickets, int* err, int w_tiled,
+                          const LLSmallMEpi& epi, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M > 128) return -3;
+  if ((K % 8) || (lda % 8) || (ldw % 8)) return -3;
+  if (w_tiled && ((N % 128) || (K % 64))) return -3;
+  if (const int rc = small_m_check_epi(C, N, epi)) return rc;
   const int ntiles = (N + GEMM_BM - 1) / GEMM_BM;
   const int num_kb = (K + GEMM_BK - 1) / GEMM_BK;
   if (splits <= 0) {
@@ -1712,7 +1798,7 @@ static int small_m_launch(const bf16* A, int lda, const bf16* W, int ldw, bf16* 
       init = true;                                                                                       \
     }                                                                                                    \
     launch_pdl(kern, grid, dim3(192), C_::SMEM, stream, tW, tX, C, bias, M, N, K, ldc, kb_per, ws, tickets, \
-               err, w_tiled, epi);                                                                       \
+               err, w_tiled, epi, NoLora{});                                                             \
   } while (0)
 #define LL_LAUNCH_SM(BNX_, RING_, PF_, MODE_) LL_LAUNCH_SMT(BNX_, RING_, PF_, MODE_, false)
 #define LL_LAUNCH_S(BNX_, RING_, PF_) LL_LAUNCH_SM(BNX_, RING_, PF_, -1)
@@ -1808,4 +1894,146 @@ extern "C" int ll_gemm_small_m_splits(int N, int K) {
   if (splits < 1) splits = 1;
   int kb_per = (num_kb + splits - 1) / splits;
   return (num_kb + kb_per - 1) / kb_per;
+}
+
+// ---------------------------------------------------------------------------
+// Projections with low-rank adapters: the planes of `low` (written by
+// ll_lora_low on the same stream) as further k-blocks of the product.
+
+// 3-D map over B [adapters, N, rank]: box = [1, 128 outputs, 64 ranks].
+static int make_tmap_lora_b(CUtensorMap* tm, const LLLora& lo, int N) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return -1;
+  cuuint64_t dims[3] = {(cuuint64_t)lo.rank, (cuuint64_t)N, (cuuint64_t)lo.adapters};
+  cuuint64_t strides[2] = {(cuuint64_t)lo.rank * 2, (cuuint64_t)lo.rank * 2 * (cuuint64_t)N};
+  cuuint32_t box[3] = {64, 128, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(lo.b), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
+// Opt-in shared memory of a kernel, once on every device that launches it.
+template <class Kern>
+static bool smem_on_device(Kern kern, int bytes, unsigned long long& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done |= bit;
+  return true;
+}
+
+static int make_lora_blocks(LoraBlocks* lb, const LLLora& lo, int N, int low_box_rows) {
+  if (lo.rank <= 0 || (lo.rank % 8) || lo.rank > LL_LORA_MAX_RANK || lo.adapters <= 0 || lo.tile_rows <= 0) return -3;
+  if (make_tmap_2d(&lb->tm_low, lo.low, lo.max_planes * lo.tile_rows, lo.rank, lo.rank, low_box_rows)) return -2;
+  if (make_tmap_lora_b(&lb->tm_b, lo, N)) return -2;
+  lb->tile_ptr = lo.tile_ptr;
+  lb->plane_adapter = lo.plane_adapter;
+  lb->rank_blocks = (lo.rank + GEMM_BK - 1) / GEMM_BK;
+  lb->tile_rows = lo.tile_rows;
+  return 0;
+}
+
+// Small M (<= 128 rows, one row tile).  Same workspace rules as
+// ll_gemm_bf16_small_m_epi; W row-major or tile-major.
+extern "C" int ll_gemm_bf16_small_m_lora(const void* A_, int lda, const void* W_, int ldw, void* C_, int ldc,
+                                         const void* bias_, int M, int N, int K, int splits, float* ws,
+                                         size_t ws_floats, int* tickets, int* err, int w_tiled,
+                                         const LLSmallMEpi* epi_, const LLLora* lo, void* stream_) {
+  const bf16* A = static_cast<const bf16*>(A_);
+  const bf16* W = static_cast<const bf16*>(W_);
+  bf16* C = static_cast<bf16*>(C_);
+  const bf16* bias = static_cast<const bf16*>(bias_);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (epi_ == nullptr || lo == nullptr) return -3;
+  const LLSmallMEpi& epi = *epi_;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M > 128 || lo->tiles != 1 || lo->tile_rows < M) return -3;
+  if ((K % 8) || (lda % 8) || (ldw % 8)) return -3;
+  if (w_tiled && ((N % 128) || (K % 64))) return -3;
+  if (const int rc = small_m_check_epi(C, N, epi)) return rc;
+  if (splits < 1) return -3;
+  if (splits > 1 && (ws == nullptr || tickets == nullptr || ws_floats < (size_t)splits * M * N)) return -6;
+  const int BNX = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
+  CUtensorMap tW, tX;
+  LoraBlocks lb;
+  if (w_tiled ? make_tmap_w_tiled(&tW, W, N, K) : make_tmap_2d(&tW, W, N, K, ldw, GEMM_BM)) return -2;
+  if (make_tmap_2d(&tX, A, M, K, lda, BNX)) return -2;
+  if (const int rc = make_lora_blocks(&lb, *lo, N, BNX)) return rc;
+  const dim3 grid((N + GEMM_BM - 1) / GEMM_BM, splits);
+  cudaError_t e = cudaSuccess;
+#define LL_LAUNCH_LORA(BNX_, PF_, MODE_, TILE_)                                                          \
+  do {                                                                                                   \
+    auto kern = gemm_swapab_kernel<BNX_, 108, PF_, MODE_, TILE_, LoraBlocks>;                            \
+    using C_ = SwapCfg<BNX_, 108>;                                                                       \
+    static unsigned long long done = 0;                                                                  \
+    if (!smem_on_device(kern, C_::SMEM, done)) return -7;                                                \
+    e = launch_pdl(kern, grid, dim3(192), C_::SMEM, stream, tW, tX, C, bias, M, N, K, ldc, 0, ws, tickets, err, \
+                   w_tiled, epi, lb);                                                                    \
+  } while (0)
+#define LL_LAUNCH_LORA_MODE(PF_, TILE_)                                              \
+  do {                                                                               \
+    switch (epi.mode) {                                                              \
+      case LL_EPI_STORE: LL_LAUNCH_LORA(16, PF_, LL_EPI_STORE, TILE_); break;       \
+      case LL_EPI_SWIGLU: LL_LAUNCH_LORA(16, PF_, LL_EPI_SWIGLU, TILE_); break;     \
+      case LL_EPI_RESIDUAL: LL_LAUNCH_LORA(16, PF_, LL_EPI_RESIDUAL, TILE_); break; \
+      default: LL_LAUNCH_LORA(16, PF_, LL_EPI_QKV_ROPE, TILE_); break;              \
+    }                                                                                \
+  } while (0)
+  switch (BNX) {
+    case 16:
+      if (M == 1) LL_LAUNCH_LORA_MODE(false, false);
+      else if (small_m_tile_ok(C, ldc, bias, M, N, ws, epi)) LL_LAUNCH_LORA_MODE(true, true);
+      else LL_LAUNCH_LORA(16, true, -1, false);
+      break;
+    case 32: LL_LAUNCH_LORA(32, true, -1, false); break;
+    case 64: LL_LAUNCH_LORA(64, true, -1, false); break;
+    default: LL_LAUNCH_LORA(128, true, -1, false); break;
+  }
+#undef LL_LAUNCH_LORA_MODE
+#undef LL_LAUNCH_LORA
+  return e == cudaSuccess ? 0 : -5;
+}
+
+// Any M: 256 x 256 tiles on CTA pairs.  epilogue 0 plain, 1 SwiGLU.
+extern "C" int ll_gemm_bf16_lora(const void* A_, int lda, const void* W_, int ldw, void* C_, int ldc,
+                                 const void* bias_, int M, int N, int K, int epilogue, const LLLora* lo, int* err,
+                                 void* stream_) {
+  const bf16* A = static_cast<const bf16*>(A_);
+  const bf16* W = static_cast<const bf16*>(W_);
+  bf16* C = static_cast<bf16*>(C_);
+  const bf16* bias = static_cast<const bf16*>(bias_);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if ((K % 8) || (N % 8) || (lda % 8) || (ldw % 8) || (ldc % 8) || (reinterpret_cast<uintptr_t>(C) & 15)) return -3;
+  if (epilogue != kEpiPlain && epilogue != kEpiSwiGLU) return -4;
+  if (epilogue == kEpiSwiGLU && (N % 32)) return -4;
+  const int num_m = (M + 2 * GEMM_BM - 1) / (2 * GEMM_BM);
+  // one row tile per 256-row output tile, or all (<= 128) rows in one
+  if (lo->tiles != num_m || (num_m > 1 && lo->tile_rows != 2 * GEMM_BM)) return -3;
+  CUtensorMap tA, tB, tC;
+  LoraBlocks lb;
+  if (make_tmap_2d(&tA, A, M, K, lda, GEMM_BM)) return -2;
+  if (make_tmap_2d(&tB, W, N, K, ldw, 128)) return -2;
+  if (const int rc = make_lora_blocks(&lb, *lo, N, GEMM_BM)) return rc;
+  const int c_bulk =
+      gemm_bulk_store_enabled() && make_tmap_c(&tC, C, M, epilogue == kEpiSwiGLU ? N / 2 : N, ldc) == 0;
+  if (!c_bulk) tC = tA;  // not read
+  const int ntiles = num_m * ((N + 255) / 256);
+  const int pairs = ntiles < num_sms() / 2 ? ntiles : num_sms() / 2;
+#define LL_LAUNCH_LORA2(EPI_)                                                                          \
+  do {                                                                                                 \
+    auto kern = gemm_tcgen05_2sm_kernel<256, EPI_, LoraBlocks>;                                        \
+    static unsigned long long done = 0;                                                                \
+    if (!smem_on_device(kern, Gemm2Cfg<256>::SMEM, done)) return -7;                                   \
+    kern<<<2 * pairs, 192, Gemm2Cfg<256>::SMEM, stream>>>(tA, tB, tC, c_bulk, C, bias, M, N, K, ldc, err, \
+                                                           TpArgs{}, gemm_group_m(M, K, 2 * GEMM_BM), lb); \
+  } while (0)
+  if (epilogue == kEpiSwiGLU) LL_LAUNCH_LORA2(kEpiSwiGLU);
+  else LL_LAUNCH_LORA2(kEpiPlain);
+#undef LL_LAUNCH_LORA2
+  return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }

@@ -22,12 +22,13 @@ import torch
 
 from . import reference as ref
 from ._ext import ExtensionMissing, cuda as _cuda  # noqa: F401
+from .lora import LORA_MAX_RANK, LoraPlan, LoraStack, lora_plan  # noqa: F401
 
 __all__ = [
     "ExtensionMissing", "linear", "rmsnorm", "fused_add_rmsnorm", "rope_qkv_write", "attention_prefill",
     "attention_decode", "swiglu", "embedding", "argmax", "kv_link_rope", "interleave_gate_up",
     "deinterleave_gate_up", "prefill_tiles", "workspace", "check_errors", "gemv_rownorm", "gemv_residual",
-    "gemv_qkv_rope",
+    "gemv_qkv_rope", "LoraStack", "LoraPlan", "lora_plan", "linear_lora", "sample",
 ]
 
 SMALL_M_MAX = 128
@@ -291,6 +292,42 @@ def gemv_qkv_rope(x, w, bias, positions, slots, cos_sin, q_out, k_pool_l, v_pool
                              q_out, k_pool_l, v_pool_l, q_norm_w, k_norm_w, num_heads, num_kv_heads,
                              k_pool_l.shape[-2], eps)
     return q_out
+
+
+def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], lora: LoraStack, plan: LoraPlan,
+                out: Optional[torch.Tensor] = None, swiglu_epilogue: bool = False) -> torch.Tensor:
+    """:func:`linear` with each row's own low-rank adapter:
+
+    ``y[m] = x[m] @ w.T + bias + scale[j] * (x[m] @ a[j].T) @ b[j].T`` for the
+    adapter j that ``plan`` (:func:`lora_plan`) gives row m, if any; with
+    ``swiglu_epilogue`` the result is ``silu(gate) * up`` of the interleaved
+    gate/up product.  bf16, row strides and K multiples of 8, N of 8 (of 32
+    with SwiGLU); ``w`` row-major.  CUDA: two launches, the low-rank rows and
+    the product; their scratch belongs to the call, so calls on several
+    streams may share a stack and a plan."""
+    M, N = x.shape[0], w.shape[0]
+    if plan.rows != M:
+        raise ValueError(f"the plan is for {plan.rows} rows, x has {M}")
+    if plan.top_adapter >= lora.a.shape[0]:
+        raise ValueError(f"the plan names adapter {plan.top_adapter}, the stack has {lora.a.shape[0]}")
+    if out is None:
+        out = torch.empty(M, N // 2 if swiglu_epilogue else N, dtype=x.dtype, device=x.device)
+    if not x.is_cuda:
+        y = ref.linear_lora(x, w, bias, lora.a, lora.b, lora.scale, plan.row_adapters)
+        out.copy_(ref_swiglu_interleaved(y) if swiglu_epilogue else y)
+        return out
+    if M == 0:
+        return out
+    ext = _cuda()
+    small = M <= SMALL_M_MAX and not (M > 64 and N >= 148 * 256)  # as linear()
+    splits = 1
+    if small:
+        splits = ext.gemm_small_m_splits(N, x.shape[1])
+        if 1 < M <= 16:
+            splits = min(splits, _TILE_MAX_SPLITS)
+    ext.lora_linear(x, w, bias, out, lora.a, lora.b, lora.scale, plan.buf, plan.tile_rows, plan.max_planes, small,
+                    splits, swiglu_epilogue, workspace(x.device).err)
+    return out
 
 
 def ref_swiglu_interleaved(gu: torch.Tensor) -> torch.Tensor:
@@ -606,6 +643,36 @@ def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Te
         out = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
     _cuda().argmax(out, logits)
     return out
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+           min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, return_logprobs: bool = False):
+    """One token per row of ``logits`` [B, V] (bf16 or fp32, rows of any
+    stride, V <= 2^19), drawn with ``uniforms`` (float64 [B] in [0, 1)).
+
+    Per row, each a [B] tensor or None: ``temperature`` (fp32; <= 0: the
+    largest logit), ``top_k`` (int32; <= 0: off), ``top_p`` (fp32; >= 1: off)
+    and ``min_p`` (fp32, relative to the largest probability; <= 0: off),
+    applied in that order; equal logits rank by index.  Returns int32 [B], -1
+    where a row has no logit above -inf (NaN counts as -inf); with
+    ``return_logprobs`` also fp32 [B], the log of the token's share of what
+    the filters keep (0 for a greedy row).  The result for a row does not
+    depend on the rest of the batch.  :func:`.reference.sample` states it."""
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocabulary]")
+    if not logits.is_cuda:
+        ids, logp = ref.sample(logits, uniforms, temperature, top_k, top_p, min_p)
+        if out is not None:
+            out.copy_(ids)
+            ids = out
+        return (ids, logp) if return_logprobs else ids
+    B = logits.shape[0]
+    if out is None:
+        out = torch.empty(B, dtype=torch.int32, device=logits.device)
+    logp = torch.empty(B, dtype=torch.float32, device=logits.device) if return_logprobs else None
+    _cuda().sample(logits, uniforms, temperature, top_k, top_p, min_p, out, logp)
+    return (out, logp) if return_logprobs else out
 
 
 def kv_link_rope(k_pool, v_pool, src_slots, dst_slots, local_pos, global_pos, cos_sin,

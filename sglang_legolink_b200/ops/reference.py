@@ -158,6 +158,67 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     return y.to(x.dtype)
 
 
+def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor,
+                scale: torch.Tensor, row_adapters: torch.Tensor) -> torch.Tensor:
+    """``x @ w.T (+ bias)`` plus, for each row m with an adapter
+    ``j = row_adapters[m] >= 0``, ``scale[j] * (x[m] @ a[j].T) @ b[j].T``;
+    fp32 throughout, the result in fp32 (the caller rounds it)."""
+    y = x.float() @ w.float().t()
+    if bias is not None:
+        y = y + bias.float()
+    for j in torch.unique(row_adapters[row_adapters >= 0]).tolist():
+        rows = (row_adapters == j).nonzero()[:, 0]
+        y[rows] += float(scale[j]) * ((x[rows].float() @ a[j].float().t()) @ b[j].float().t())
+    return y
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+           min_p: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """One token per row (int32) and the log of its share of what the filters
+    keep (fp32), in float64.  With ``w = exp((x - max x) / temperature)`` and
+    the tokens in descending order of x (equal ones by index) a row keeps its
+    first ``top_k`` tokens; of those, the ones whose predecessors hold less
+    than ``top_p`` of their mass; of those, the ones with ``w >= min_p``.  The
+    token is the first kept one, in index order, whose running sum of w
+    exceeds ``u`` times the kept sum.  NaN counts as -inf; a row with nothing
+    above -inf gives token -1; +inf logits share all of the mass."""
+    B, V = logits.shape
+    x = logits.double()
+    x = torch.where(torch.isnan(x), torch.full_like(x, float("-inf")), x)
+    col = lambda t, v: (torch.full((B, 1), v, dtype=torch.float64, device=x.device) if t is None  # noqa: E731
+                        else t.double()[:, None])
+    t, p, m = col(temperature, 1.0), col(top_p, 1.0), col(min_p, 0.0)
+    k = col(top_k, 0).long()
+    top = x.max(dim=1, keepdim=True).values
+    none = top == float("-inf")
+    greedy = ~(t > 0)
+    w = torch.exp((x - top) / torch.where(greedy, torch.ones_like(t), t))
+    w = torch.where(x == top, torch.ones_like(w), w)
+    w = torch.where((x == float("-inf")) | torch.isnan(w), torch.zeros_like(w), w)
+    order = torch.sort(x, dim=1, descending=True, stable=True).indices
+    ws = w.gather(1, order)
+    ar = torch.arange(V, device=x.device)[None, :]
+    keep = ar < torch.where((k <= 0) | (k > V), torch.full_like(k, V), k)
+    ws = ws * keep
+    cum = torch.cumsum(ws, dim=1)
+    keep &= (ar == 0) | ~(p < 1) | (cum - ws < p * cum[:, -1:])
+    keep &= ~(m > 0) | (ws >= m.clamp(max=1.0))
+    wk = w * torch.zeros_like(keep).scatter_(1, order, keep)
+    cum = torch.cumsum(wk, dim=1)
+    total = cum[:, -1:]
+    uu = u.double()[:, None].clamp(0.0, 1.0)
+    ids = ((cum > uu * total) & (wk > 0)).to(torch.uint8).argmax(dim=1, keepdim=True)
+    last = torch.where(wk > 0, ar, torch.full_like(ar, -1)).max(dim=1, keepdim=True).values
+    ids = torch.where(uu * total >= total, last.clamp(min=0), ids)
+    ids = torch.where(greedy, order[:, :1], ids)
+    logp = torch.log(w.gather(1, ids) / total)
+    logp = torch.where(greedy, torch.zeros_like(logp), logp)
+    ids = torch.where(none, torch.full_like(ids, -1), ids)
+    logp = torch.where(none, torch.full_like(logp, float("-inf")), logp)
+    return ids[:, 0].to(torch.int32), logp[:, 0].float()
+
+
 def remap_delta(cos_sin: torch.Tensor, local_pos: torch.Tensor, global_pos: torch.Tensor):
     """Rotation that maps RoPE(local) to RoPE(global): R(global) R(local)^-1.
 
