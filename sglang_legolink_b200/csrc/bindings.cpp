@@ -358,7 +358,8 @@ void gemm_small_m_epi(const at::Tensor& a, const at::Tensor& w, const c10::optio
 // A projection with per-row low-rank adapters (lora.h): the low-rank rows,
 // then the shared product with the adapters' B as further k-blocks.  The
 // scratch is this call's own, so calls on different streams share nothing.
-// plan: int32 [row_slot M | tile_ptr tiles + 1 | plane_adapter max_planes].
+// plan: int32 [row_slot M | tile_ptr tiles + 1 | plane_adapter max_planes |
+// plane_tile max_planes].
 void lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, at::Tensor& out,
                  const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale, const at::Tensor& plan,
                  int64_t tile_rows, int64_t max_planes, bool small_m, int64_t splits, bool swiglu,
@@ -385,12 +386,12 @@ void lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<a
   }
   const int64_t tiles = (M + tile_rows - 1) / tile_rows;
   TORCH_CHECK(tile_rows == (M <= 128 ? 128 : 256) && max_planes >= 1, "bad plan");
-  TORCH_CHECK(plan.numel() == M + tiles + 1 + max_planes, "the plan is for another batch");
-  TORCH_CHECK(max_planes * tile_rows < (1ll << 31), "too many adapters per tile of rows");
+  TORCH_CHECK(plan.numel() == M + tiles + 1 + 2 * max_planes, "the plan is for another batch");
+  TORCH_CHECK(max_planes <= 65535, "too many adapters per tile of rows");
   TORCH_CHECK(!small_m || (M <= 128 && splits >= 1), "bad split count");
   c10::cuda::CUDAGuard g(x.device());
   const int nt = small_m ? (int)((N + 127) / 128) : 0;
-  auto low = at::empty({max_planes * tile_rows, R}, x.options());
+  auto low = at::empty({max_planes * 2 * tile_rows, R}, x.options());
   at::Tensor ws, tickets;
   if (small_m && splits > 1) {
     ws = at::empty({splits * M * N}, scale.options());
@@ -403,6 +404,7 @@ void lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<a
   lo.row_slot = plan.data_ptr<int>();
   lo.tile_ptr = lo.row_slot + M;
   lo.plane_adapter = lo.tile_ptr + tiles + 1;
+  lo.plane_tile = lo.plane_adapter + max_planes;
   lo.low = bp(low);
   lo.tickets = tickets.defined() ? tickets.data_ptr<int>() : nullptr;
   lo.num_tickets = tickets.defined() ? nt : 0;

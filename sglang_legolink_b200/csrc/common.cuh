@@ -289,6 +289,19 @@ inline bool pdl_enabled() {
   return v == 1;
 }
 
+// Opt-in shared memory of a kernel, set once on every device that launches
+// it; `done` is the caller's per-kernel record.
+template <class Kern>
+inline bool smem_on_device(Kern kern, int bytes, unsigned long long& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done |= bit;
+  return true;
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                               Args&&... args) {

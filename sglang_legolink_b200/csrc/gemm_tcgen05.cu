@@ -50,18 +50,18 @@ using TpArgs = LLTpArgs;
 
 // Low-rank adapters beside the shared product (lora.h): after the k-blocks of
 // K, an output tile runs more k-blocks, 64 ranks of one adapter each, over
-// the adapter's low-rank rows (`low`, the A side of the product) and its
-// B matrix.  They accumulate into the same TMEM accumulator, so the adapters'
+// the adapter's low-rank rows (`low`, the A side of the product; hi, then lo)
+// and its B matrix.  They accumulate into the same TMEM accumulator, so the adapters'
 // term joins the product in fp32, before the epilogue, and costs no pass over
 // the output: at 5087 rows x 4608 outputs a separate pass would read and write
-// 94 MB (14 us at HBM rate), the extra k-block adds 1 to 56 (2 us of 118).
+// 94 MB (14 us at HBM rate), the extra k-blocks add 2 to 56.
 // NoLora compiles the kernels without any of it.
 struct NoLora {
   static constexpr bool on = false;
 };
 struct alignas(64) LoraBlocks {
   static constexpr bool on = true;
-  CUtensorMap tm_low;        // [planes * tile_rows, rank]
+  CUtensorMap tm_low;        // [planes * 2 (hi, lo) * tile_rows, rank]
   CUtensorMap tm_b;          // [adapters, N, rank]
   const int* tile_ptr;       // planes of row tile t: [tile_ptr[t], tile_ptr[t + 1])
   const int* plane_adapter;  // adapter of each plane
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(192, 2)
   if constexpr (Lora::on) {
     // the adapters' k-blocks follow those of K; how many there are is known
     // on the device only (a captured graph replays with other adapters)
-    kb_all += lora.tile_ptr[1] * lora.rank_blocks;
+    kb_all += lora.tile_ptr[1] * 2 * lora.rank_blocks;
     kb_per = (kb_all + nsplit - 1) / nsplit;
   }
   const int kb0 = split * kb_per;
@@ -593,11 +593,12 @@ __global__ void __launch_bounds__(192, 2)
         mbar_arrive_expect_tx(&full[stage], Cfg::W_BYTES + Cfg::X_BYTES);
         if constexpr (Lora::on) {
           if (kb >= num_kb) {  // 64 ranks of one adapter
-            const int plane = (kb - num_kb) / lora.rank_blocks, rb = (kb - num_kb) % lora.rank_blocks;
+            const int e = (kb - num_kb) >> 1, half = (kb - num_kb) & 1;
+            const int plane = e / lora.rank_blocks, rb = e % lora.rank_blocks;
             tma_load_3d(sW + stage * Cfg::W_BYTES, &lora.tm_b, &full[stage], rb * GEMM_BK, nb * GEMM_BM,
                         lora.plane_adapter[plane]);
             tma_load_2d(sX + stage * Cfg::X_BYTES, &lora.tm_low, &full[stage], rb * GEMM_BK,
-                        plane * lora.tile_rows);
+                        (2 * plane + half) * lora.tile_rows);
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1;
@@ -1204,17 +1205,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           }
         }
         if constexpr (Lora::on) {
-          const int p0 = lora.tile_ptr[mb], n_extra = (lora.tile_ptr[mb + 1] - p0) * lora.rank_blocks;
+          const int p0 = lora.tile_ptr[mb], n_extra = (lora.tile_ptr[mb + 1] - p0) * 2 * lora.rank_blocks;
           for (int e = 0; e < n_extra && ok; ++e) {
             if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
               ok = false;
               break;
             }
-            const int plane = p0 + e / lora.rank_blocks, rb = e % lora.rank_blocks;
+            const int plane = p0 + (e >> 1) / lora.rank_blocks, rb = (e >> 1) % lora.rank_blocks;
             const uint32_t leader_full = mapa_shared(smem_u32(&full[stage]), 0);
             if (crank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
             tma_load_2d_2sm(sA + stage * Cfg::A_BYTES, &lora.tm_low, leader_full, rb * GEMM_BK,
-                            plane * lora.tile_rows + (int)crank * GEMM_BM);
+                            (2 * plane + (e & 1)) * lora.tile_rows + (int)crank * GEMM_BM);
             tma_load_3d_2sm(sB + stage * Cfg::B_BYTES, &lora.tm_b, leader_full, rb * GEMM_BK,
                             nb * BN + (int)crank * (BN / 2), lora.plane_adapter[plane]);
             if (++stage == STAGES) {
@@ -1244,7 +1245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         if constexpr (Lora::on) {
           int mb, nb;
           tile_coords(t, num_m, num_n, group_m, mb, nb);
-          num_kb_t += (lora.tile_ptr[mb + 1] - lora.tile_ptr[mb]) * lora.rank_blocks;
+          num_kb_t += (lora.tile_ptr[mb + 1] - lora.tile_ptr[mb]) * 2 * lora.rank_blocks;
         }
         for (int kb = 0; kb < num_kb_t; ++kb) {
           if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) {
@@ -1914,21 +1915,9 @@ static int make_tmap_lora_b(CUtensorMap* tm, const LLLora& lo, int N) {
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
-// Opt-in shared memory of a kernel, once on every device that launches it.
-template <class Kern>
-static bool smem_on_device(Kern kern, int bytes, unsigned long long& done) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (done & bit) return true;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-  done |= bit;
-  return true;
-}
-
 static int make_lora_blocks(LoraBlocks* lb, const LLLora& lo, int N, int low_box_rows) {
   if (lo.rank <= 0 || (lo.rank % 8) || lo.rank > LL_LORA_MAX_RANK || lo.adapters <= 0 || lo.tile_rows <= 0) return -3;
-  if (make_tmap_2d(&lb->tm_low, lo.low, lo.max_planes * lo.tile_rows, lo.rank, lo.rank, low_box_rows)) return -2;
+  if (make_tmap_2d(&lb->tm_low, lo.low, lo.max_planes * 2 * lo.tile_rows, lo.rank, lo.rank, low_box_rows)) return -2;
   if (make_tmap_lora_b(&lb->tm_b, lo, N)) return -2;
   lb->tile_ptr = lo.tile_ptr;
   lb->plane_adapter = lo.plane_adapter;

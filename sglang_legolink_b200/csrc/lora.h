@@ -4,10 +4,11 @@
 //
 // in two launches (lora.cu, gemm_tcgen05.cu):
 //
-//   1. low[plane][row] = bf16(scale[a] x[row] A[a]^T), one plane per adapter
-//      that a tile of rows uses, with zeros in the rows of other adapters;
+//   1. low[plane][row] = scale[a] x[row] A[a]^T, one plane per adapter that a
+//      tile of rows uses, with zeros in the rows of other adapters; each value
+//      as the sum of two bf16, hi and lo;
 //   2. the shared product, whose k-loop goes on over the planes:
-//      [x | low_0 | low_1 | ...] . [W | B[a_0] | B[a_1] | ...]^T.
+//      [x | hi_0 | lo_0 | hi_1 | ...] . [W | B[a_0] | B[a_0] | B[a_1] | ...]^T.
 //
 // Rows are cut into tiles of `tile_rows`; the planes of tile t are
 // [tile_ptr[t], tile_ptr[t + 1]) and plane_adapter names their adapters.
@@ -24,7 +25,8 @@ struct LLLora {
   const int* row_slot;      // [M] plane of the row within its tile, -1: no adapter
   const int* tile_ptr;      // [tiles + 1]
   const int* plane_adapter; // [max_planes]
-  __nv_bfloat16* low;       // [max_planes * tile_rows, rank]
+  const int* plane_tile;    // [max_planes]
+  __nv_bfloat16* low;       // [max_planes, 2 (hi, lo), tile_rows, rank]
   int* tickets;             // split-K tickets of the second launch, zeroed by the first
   int adapters, rank, tiles, tile_rows, max_planes, num_tickets;
 };

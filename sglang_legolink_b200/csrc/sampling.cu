@@ -497,13 +497,7 @@ static int sample_launch(const LLSample& p, cudaStream_t stream) {
   while (cs < SMP_MAX_CLUSTER && (int64_t)p.B * cs * 2 <= 148 && nvec / (2 * cs) >= SMP_THREADS) cs *= 2;
   auto kern = sample_kernel<Raw>;
   static unsigned long long done = 0;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return -5;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (!(done & bit)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)limit) != cudaSuccess) return -7;
-    done |= bit;
-  }
+  if (!smem_on_device(kern, (int)limit, done)) return -7;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.B * cs));
   cfg.blockDim = dim3(SMP_THREADS);

@@ -66,11 +66,11 @@ class LoraPlan:
         self.max_planes = max(1, planes if max_planes is None else int(max_planes))
         if planes > self.max_planes:
             raise ValueError(f"the rows need {planes} planes, max_planes is {self.max_planes}")
-        self.buf = torch.empty(self.rows + self.tiles + 1 + self.max_planes, dtype=torch.int32, device=self.device)
+        self.buf = torch.empty(self.rows + self.tiles + 1 + 2 * self.max_planes, dtype=torch.int32, device=self.device)
         self._store(ids, host)
 
     def _build(self, ids: np.ndarray):
-        """(row slots, tile offsets, plane adapters) and the plane count."""
+        """(row slots, tile offsets, plane keys) and the plane count."""
         tile = np.arange(self.rows, dtype=np.int64) // self.tile_rows
         live = ids >= 0
         # one key per (tile, adapter): planes in tile order, adapters ascending
@@ -78,14 +78,16 @@ class LoraPlan:
         ptr = np.searchsorted(keys, np.arange(self.tiles + 1, dtype=np.int64) << 32)
         slot = np.full(self.rows, -1, dtype=np.int64)
         slot[live] = inverse.reshape(-1) - ptr[tile[live]]
-        return (slot, ptr, keys & 0xFFFFFFFF), len(keys)
+        return (slot, ptr, keys), len(keys)
 
     def _store(self, ids: np.ndarray, host) -> None:
-        slot, ptr, adapters = host
+        slot, ptr, keys = host
         flat = np.zeros(self.buf.numel(), dtype=np.int32)
         flat[: self.rows] = slot
         flat[self.rows : self.rows + self.tiles + 1] = ptr
-        flat[self.rows + self.tiles + 1 :][: len(adapters)] = adapters
+        planes = flat[self.rows + self.tiles + 1 :].reshape(2, self.max_planes)
+        planes[0, : len(keys)] = keys & 0xFFFFFFFF
+        planes[1, : len(keys)] = keys >> 32
         self.buf.copy_(torch.from_numpy(flat))
         self.top_adapter = int(ids.max()) if self.rows else -1
         self.row_adapters = torch.from_numpy(ids)
