@@ -24,9 +24,8 @@ int ll_gemm_bf16_small_m_ex(const bf16* A, int lda, const bf16* W, int ldw, bf16
                             int M, int N, int K, int splits, float* ws, size_t ws_floats, int* tickets, int* err,
                             int flags, cudaStream_t stream);
 int ll_lora_low(const bf16* x, int64_t ldx, int M, int K, const LLLora* lo, int* err, cudaStream_t stream);
-int ll_gemm_bf16_small_m_lora(const void* A, int lda, const void* W, int ldw, void* C, int ldc, const void* bias,
-                              int M, int N, int K, int splits, float* ws, size_t ws_floats, int* tickets, int* err,
-                              int w_tiled, const LLSmallMEpi* epi, const LLLora* lo, void* stream);
+int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, int64_t ldc, const bf16* bias, int M, int N,
+                 int K, int swiglu, const LLLora* lo, int* err, cudaStream_t stream);
 int ll_gemm_bf16_lora(const void* A, int lda, const void* W, int ldw, void* C, int ldc, const void* bias, int M,
                       int N, int K, int epilogue, const LLLora* lo, int* err, void* stream);
 int ll_sample(const LLSample* p, cudaStream_t stream);
@@ -360,16 +359,20 @@ void gemm_small_m_epi(const at::Tensor& a, const at::Tensor& w, const c10::optio
 // scratch is this call's own, so calls on different streams share nothing.
 // plan: int32 [row_slot M | tile_ptr tiles + 1 | plane_adapter max_planes |
 // plane_tile max_planes].
-void lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, at::Tensor& out,
-                 const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale, const at::Tensor& plan,
-                 int64_t tile_rows, int64_t max_planes, bool small_m, int64_t splits, bool swiglu,
-                 const at::Tensor& err) {
-  CHECK_CUDA(x); CHECK_BF16(x); CHECK_BF16(w); CHECK_BF16(out); CHECK_BF16(a); CHECK_BF16(b); CHECK_F32(scale);
+at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
+                       const c10::optional<at::Tensor>& out_, const at::Tensor& a, const at::Tensor& b,
+                       const at::Tensor& scale, const at::Tensor& plan, int64_t tile_rows, int64_t max_planes,
+                       bool small_m, bool swiglu, const at::Tensor& err) {
+  CHECK_CUDA(x); CHECK_BF16(x); CHECK_BF16(w); CHECK_BF16(a); CHECK_BF16(b); CHECK_F32(scale);
   CHECK_I32(plan); CHECK_I32(err); CHECK_CONTIG(w); CHECK_CONTIG(a); CHECK_CONTIG(b); CHECK_CONTIG(scale);
-  CHECK_CONTIG(plan); CHECK_ALIGN16(x); CHECK_ALIGN16(w); CHECK_ALIGN16(a); CHECK_ALIGN16(b); CHECK_ALIGN16(out);
-  for (const at::Tensor* t : {&w, static_cast<const at::Tensor*>(&out), &a, &b, &scale, &plan, &err})
+  CHECK_CONTIG(plan); CHECK_ALIGN16(x); CHECK_ALIGN16(w); CHECK_ALIGN16(a); CHECK_ALIGN16(b);
+  for (const at::Tensor* t : {&w, &a, &b, &scale, &plan, &err})
     TORCH_CHECK(t->device() == x.device(), "all tensors must be on ", x.device().str());
-  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && out.dim() == 2 && a.dim() == 3 && b.dim() == 3);
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && a.dim() == 3 && b.dim() == 3);
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor out = out_.has_value() ? *out_ : at::empty({x.size(0), swiglu ? w.size(0) / 2 : w.size(0)}, x.options());
+  CHECK_BF16(out); CHECK_ALIGN16(out);
+  TORCH_CHECK(out.device() == x.device() && out.dim() == 2, "out must be a matrix on ", x.device().str());
   TORCH_CHECK(x.stride(1) == 1 && out.stride(1) == 1, "inner dim must be contiguous");
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0), n = a.size(0), R = a.size(1);
   TORCH_CHECK(M > 0 && M < (1 << 28) && K > 0 && N > 0 && n > 0, "empty projection");
@@ -382,21 +385,15 @@ void lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<a
   TORCH_CHECK(out.size(0) == M && out.size(1) == (swiglu ? N / 2 : N), "bad output shape");
   if (bias.has_value()) {
     CHECK_BF16(*bias); CHECK_CONTIG(*bias);
+    CHECK_ALIGN16(*bias);
     TORCH_CHECK(bias->numel() == N && bias->device() == x.device(), "bad bias");
   }
   const int64_t tiles = (M + tile_rows - 1) / tile_rows;
   TORCH_CHECK(tile_rows == (M <= 128 ? 128 : 256) && max_planes >= 1, "bad plan");
   TORCH_CHECK(plan.numel() == M + tiles + 1 + 2 * max_planes, "the plan is for another batch");
   TORCH_CHECK(max_planes <= 65535, "too many adapters per tile of rows");
-  TORCH_CHECK(!small_m || (M <= 128 && splits >= 1), "bad split count");
-  c10::cuda::CUDAGuard g(x.device());
-  const int nt = small_m ? (int)((N + 127) / 128) : 0;
+  TORCH_CHECK(!small_m || M <= 128, "the small-M kernel takes at most 128 rows");
   auto low = at::empty({max_planes * 2 * tile_rows, R}, x.options());
-  at::Tensor ws, tickets;
-  if (small_m && splits > 1) {
-    ws = at::empty({splits * M * N}, scale.options());
-    tickets = at::empty({nt}, plan.options());
-  }
   LLLora lo{};
   lo.a = bp(a);
   lo.b = bp(b);
@@ -406,30 +403,23 @@ void lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<a
   lo.plane_adapter = lo.tile_ptr + tiles + 1;
   lo.plane_tile = lo.plane_adapter + max_planes;
   lo.low = bp(low);
-  lo.tickets = tickets.defined() ? tickets.data_ptr<int>() : nullptr;
-  lo.num_tickets = tickets.defined() ? nt : 0;
   lo.adapters = (int)n;
   lo.rank = (int)R;
   lo.tiles = (int)tiles;
   lo.tile_rows = (int)tile_rows;
   lo.max_planes = (int)max_planes;
   check_rc(ll_lora_low(bp(x), x.stride(0), (int)M, (int)K, &lo, err.data_ptr<int>(), cur_stream()), "ll_lora_low");
-  void* bias_p = bias.has_value() ? bias->data_ptr() : nullptr;
   if (small_m) {
-    LLSmallMEpi epi{};
-    epi.mode = swiglu ? LL_EPI_SWIGLU : LL_EPI_STORE;
-    check_rc(ll_gemm_bf16_small_m_lora(x.data_ptr(), (int)x.stride(0), w.data_ptr(), (int)K, out.data_ptr(),
-                                       (int)out.stride(0), bias_p, (int)M, (int)N, (int)K, (int)splits,
-                                       ws.defined() ? ws.data_ptr<float>() : nullptr,
-                                       ws.defined() ? (size_t)ws.numel() : 0, lo.tickets, err.data_ptr<int>(), 0, &epi,
-                                       &lo, cur_stream()),
-             "ll_gemm_bf16_small_m_lora");
+    check_rc(ll_lora_gemv(bp(x), x.stride(0), bp(w), bp(out), out.stride(0), bp_opt(bias), (int)M, (int)N, (int)K,
+                          swiglu ? 1 : 0, &lo, err.data_ptr<int>(), cur_stream()),
+             "ll_lora_gemv");
   } else {
     check_rc(ll_gemm_bf16_lora(x.data_ptr(), (int)x.stride(0), w.data_ptr(), (int)K, out.data_ptr(),
-                               (int)out.stride(0), bias_p, (int)M, (int)N, (int)K, swiglu ? 1 : 0, &lo,
+                               (int)out.stride(0), bp_opt(bias), (int)M, (int)N, (int)K, swiglu ? 1 : 0, &lo,
                                err.data_ptr<int>(), cur_stream()),
              "ll_gemm_bf16_lora");
   }
+  return out;
 }
 
 // One token per row of logits (sampling.h).

@@ -110,11 +110,11 @@ __device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int gro
   nb = r / gm;
 }
 
-template <int BN, int EPI>
+template <int BN, int EPI, class Lora = NoLora>
 __global__ void __launch_bounds__(192, 1)
     gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         bf16* __restrict__ C, const bf16* __restrict__ bias, int M, int N, int K, int ldc,
-                        int* err, int group_m) {
+                        int* err, int group_m, const __grid_constant__ Lora lora) {
   using Cfg = GemmCfg<BN>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(192, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (Lora::on) pdl_wait();  // set up while the low-rank kernel ran
 
   if (warp == 0) {
     if (lane == 0) {
@@ -175,6 +176,26 @@ __global__ void __launch_bounds__(192, 1)
             phase ^= 1;
           }
         }
+        if constexpr (Lora::on) {
+          const int t0 = mb * GEMM_BM / lora.tile_rows, r0 = mb * GEMM_BM % lora.tile_rows;
+          const int p0 = lora.tile_ptr[t0], n_extra = (lora.tile_ptr[t0 + 1] - p0) * 2 * lora.rank_blocks;
+          for (int e = 0; e < n_extra && ok; ++e) {
+            if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
+              ok = false;
+              break;
+            }
+            const int plane = p0 + (e >> 1) / lora.rank_blocks, rb = (e >> 1) % lora.rank_blocks;
+            mbar_arrive_expect_tx(&full[stage], Cfg::A_BYTES + Cfg::B_BYTES);
+            tma_load_2d(sA + stage * Cfg::A_BYTES, &lora.tm_low, &full[stage], rb * GEMM_BK,
+                        (2 * plane + (e & 1)) * lora.tile_rows + r0);
+            tma_load_3d(sB + stage * Cfg::B_BYTES, &lora.tm_b, &full[stage], rb * GEMM_BK, nb * BN,
+                        lora.plane_adapter[plane]);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
       }
       if (!ok) {
         // Give in-flight bulk copies time to land before the CTA exits.
@@ -193,7 +214,14 @@ __global__ void __launch_bounds__(192, 1)
         if (!mbar_wait(&tempty[acc], aphase ^ 1, err, kErrTmemEmptyTimeout)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        int num_kb_t = num_kb;
+        if constexpr (Lora::on) {
+          int mb, nb;
+          tile_coords(t, num_m, num_n, group_m, mb, nb);
+          const int t0 = mb * GEMM_BM / lora.tile_rows;
+          num_kb_t += (lora.tile_ptr[t0 + 1] - lora.tile_ptr[t0]) * 2 * lora.rank_blocks;
+        }
+        for (int kb = 0; kb < num_kb_t; ++kb) {
           if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) {
             ok = false;
             break;
@@ -511,12 +539,12 @@ struct SwapCfg {
 //
 // kTile (BNX == 16, 2 <= M <= 16, MODE >= 0): the tile epilogue (TileEpi)
 // instead of the one-row-at-a-time one.
-template <int BNX, int RING_KB, bool kRowPrefetch, int MODE = -1, bool kTile = false, class Lora = NoLora>
+template <int BNX, int RING_KB, bool kRowPrefetch, int MODE = -1, bool kTile = false>
 __global__ void __launch_bounds__(192, 2)
     gemm_swapab_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                        bf16* __restrict__ C, const bf16* __restrict__ bias, int M, int N, int K, int ldc,
                        int kb_per_split, float* __restrict__ ws, int* __restrict__ tickets, int* err,
-                       int w_tiled, const __grid_constant__ LLSmallMEpi epi, const __grid_constant__ Lora lora) {
+                       int w_tiled, const __grid_constant__ LLSmallMEpi epi) {
   const int mode = MODE >= 0 ? MODE : epi.mode;
   using Cfg = SwapCfg<BNX, RING_KB>;
   constexpr int STAGES = Cfg::STAGES;
@@ -536,15 +564,8 @@ __global__ void __launch_bounds__(192, 2)
   const int nb = blockIdx.x;  // feature tile
   const int split = blockIdx.y, nsplit = gridDim.y;
   const int num_kb = (K + GEMM_BK - 1) / GEMM_BK;
-  int kb_all = num_kb, kb_per = kb_per_split;
-  if constexpr (Lora::on) {
-    // the adapters' k-blocks follow those of K; how many there are is known
-    // on the device only (a captured graph replays with other adapters)
-    kb_all += lora.tile_ptr[1] * 2 * lora.rank_blocks;
-    kb_per = (kb_all + nsplit - 1) / nsplit;
-  }
-  const int kb0 = split * kb_per;
-  const int kb1 = min(kb_all, kb0 + kb_per);
+  const int kb0 = split * kb_per_split;
+  const int kb1 = min(num_kb, kb0 + kb_per_split);
   pdl_trigger();
 
   if (threadIdx.x == 0) {
@@ -571,8 +592,7 @@ __global__ void __launch_bounds__(192, 2)
       // The weights do not depend on the previous kernel: start streaming the
       // first ring's worth of them before waiting for it, then add the
       // activation tiles once its output is visible.
-      const int base1 = min(kb1, num_kb);  // k-blocks of K in this split
-      const int pre = max(0, min(base1 - kb0, STAGES));
+      const int pre = (kb1 - kb0) < STAGES ? (kb1 - kb0) : STAGES;
       for (int i = 0; i < pre; ++i) {
         mbar_arrive_expect_tx(&full[i], Cfg::W_BYTES + Cfg::X_BYTES);
         if (w_tiled)  // one contiguous 16 KB tile
@@ -584,28 +604,12 @@ __global__ void __launch_bounds__(192, 2)
       for (int i = 0; i < pre; ++i)
         tma_load_2d(sX + i * Cfg::X_BYTES, &tmX, &full[i], (kb0 + i) * GEMM_BK, 0);
       if (pre == STAGES) phase = 1;  // stage wrapped around exactly once
-      else stage = pre;
       for (int kb = kb0 + pre; kb < kb1; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
           ok = false;
           break;
         }
         mbar_arrive_expect_tx(&full[stage], Cfg::W_BYTES + Cfg::X_BYTES);
-        if constexpr (Lora::on) {
-          if (kb >= num_kb) {  // 64 ranks of one adapter
-            const int e = (kb - num_kb) >> 1, half = (kb - num_kb) & 1;
-            const int plane = e / lora.rank_blocks, rb = e % lora.rank_blocks;
-            tma_load_3d(sW + stage * Cfg::W_BYTES, &lora.tm_b, &full[stage], rb * GEMM_BK, nb * GEMM_BM,
-                        lora.plane_adapter[plane]);
-            tma_load_2d(sX + stage * Cfg::X_BYTES, &lora.tm_low, &full[stage], rb * GEMM_BK,
-                        (2 * plane + half) * lora.tile_rows);
-            if (++stage == STAGES) {
-              stage = 0;
-              phase ^= 1;
-            }
-            continue;
-          }
-        }
         if (w_tiled)
           tma_load_4d_(sW + stage * Cfg::W_BYTES, &tmW, &full[stage], 0, 0, kb, nb);
         else
@@ -1173,6 +1177,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (Lora::on) pdl_wait();  // set up while the low-rank kernel ran
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1593,7 +1598,7 @@ extern "C" int ll_gemm_bf16(const bf16* A, int lda, const bf16* W, int ldw, bf16
       init = true;                                                                                    \
     }                                                                                                 \
     kern<<<grid, 192, GemmCfg<BN_>::SMEM, stream>>>(tA, tB, C, bias, M, N, K, ldc, err,               \
-                                                    gemm_group_m(M, K, GEMM_BM));                   \
+                                                    gemm_group_m(M, K, GEMM_BM), NoLora{});         \
   } while (0)
   if (BN == 256) {
     if (epilogue == kEpiSwiGLU) LL_LAUNCH(256, kEpiSwiGLU); else LL_LAUNCH(256, kEpiPlain);
@@ -1738,8 +1743,13 @@ static bool small_m_tile_ok(const bf16* C, int ldc, const bf16* bias, int M, int
   }
 }
 
-// Arguments that the epilogue of a small-M launch needs.
-static int small_m_check_epi(const bf16* C, int N, const LLSmallMEpi& epi) {
+static int small_m_launch(const bf16* A, int lda, const bf16* W, int ldw, bf16* C, int ldc, const bf16* bias, int M,
+                          int N, int K, int splits, float* ws, size_t ws_floats, int* tickets, int* err, int w_tiled,
+                          const LLSmallMEpi& epi, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M > 128) return -3;
+  if ((K % 8) || (lda % 8) || (ldw % 8)) return -3;
+  if (w_tiled && ((N % 128) || (K % 64))) return -3;
   switch (epi.mode) {
     case LL_EPI_STORE:
       if (C == nullptr) return -3;
@@ -1761,17 +1771,6 @@ static int small_m_check_epi(const bf16* C, int N, const LLSmallMEpi& epi) {
     default:
       return -3;
   }
-  return 0;
-}
-
-static int small_m_launch(const bf16* A, int lda, const bf16* W, int ldw, bf16* C, int ldc, const bf16* bias, int M,
-                          int N, int K, int splits, float* ws, size_t ws_floats, int* tickets, int* err, int w_tiled,
-                          const LLSmallMEpi& epi, cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (M > 128) return -3;
-  if ((K % 8) || (lda % 8) || (ldw % 8)) return -3;
-  if (w_tiled && ((N % 128) || (K % 64))) return -3;
-  if (const int rc = small_m_check_epi(C, N, epi)) return rc;
   const int ntiles = (N + GEMM_BM - 1) / GEMM_BM;
   const int num_kb = (K + GEMM_BK - 1) / GEMM_BK;
   if (splits <= 0) {
@@ -1799,7 +1798,7 @@ static int small_m_launch(const bf16* A, int lda, const bf16* W, int ldw, bf16* 
       init = true;                                                                                       \
     }                                                                                                    \
     launch_pdl(kern, grid, dim3(192), C_::SMEM, stream, tW, tX, C, bias, M, N, K, ldc, kb_per, ws, tickets, \
-               err, w_tiled, epi, NoLora{});                                                             \
+               err, w_tiled, epi);                                                                       \
   } while (0)
 #define LL_LAUNCH_SM(BNX_, RING_, PF_, MODE_) LL_LAUNCH_SMT(BNX_, RING_, PF_, MODE_, false)
 #define LL_LAUNCH_S(BNX_, RING_, PF_) LL_LAUNCH_SM(BNX_, RING_, PF_, -1)
@@ -1901,13 +1900,13 @@ extern "C" int ll_gemm_small_m_splits(int N, int K) {
 // Projections with low-rank adapters: the planes of `low` (written by
 // ll_lora_low on the same stream) as further k-blocks of the product.
 
-// 3-D map over B [adapters, N, rank]: box = [1, 128 outputs, 64 ranks].
-static int make_tmap_lora_b(CUtensorMap* tm, const LLLora& lo, int N) {
+// 3-D map over B [adapters, N, rank]: box = [1, box_rows outputs, 64 ranks].
+static int make_tmap_lora_b(CUtensorMap* tm, const LLLora& lo, int N, int box_rows) {
   EncodeTiledFn enc = get_encode_fn();
   if (enc == nullptr) return -1;
   cuuint64_t dims[3] = {(cuuint64_t)lo.rank, (cuuint64_t)N, (cuuint64_t)lo.adapters};
   cuuint64_t strides[2] = {(cuuint64_t)lo.rank * 2, (cuuint64_t)lo.rank * 2 * (cuuint64_t)N};
-  cuuint32_t box[3] = {64, 128, 1};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(lo.b), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1915,10 +1914,10 @@ static int make_tmap_lora_b(CUtensorMap* tm, const LLLora& lo, int N) {
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
-static int make_lora_blocks(LoraBlocks* lb, const LLLora& lo, int N, int low_box_rows) {
+static int make_lora_blocks(LoraBlocks* lb, const LLLora& lo, int N, int b_box_rows) {
   if (lo.rank <= 0 || (lo.rank % 8) || lo.rank > LL_LORA_MAX_RANK || lo.adapters <= 0 || lo.tile_rows <= 0) return -3;
-  if (make_tmap_2d(&lb->tm_low, lo.low, lo.max_planes * 2 * lo.tile_rows, lo.rank, lo.rank, low_box_rows)) return -2;
-  if (make_tmap_lora_b(&lb->tm_b, lo, N)) return -2;
+  if (make_tmap_2d(&lb->tm_low, lo.low, lo.max_planes * 2 * lo.tile_rows, lo.rank, lo.rank, GEMM_BM)) return -2;
+  if (make_tmap_lora_b(&lb->tm_b, lo, N, b_box_rows)) return -2;
   lb->tile_ptr = lo.tile_ptr;
   lb->plane_adapter = lo.plane_adapter;
   lb->rank_blocks = (lo.rank + GEMM_BK - 1) / GEMM_BK;
@@ -1926,68 +1925,12 @@ static int make_lora_blocks(LoraBlocks* lb, const LLLora& lo, int N, int low_box
   return 0;
 }
 
-// Small M (<= 128 rows, one row tile).  Same workspace rules as
-// ll_gemm_bf16_small_m_epi; W row-major or tile-major.
-extern "C" int ll_gemm_bf16_small_m_lora(const void* A_, int lda, const void* W_, int ldw, void* C_, int ldc,
-                                         const void* bias_, int M, int N, int K, int splits, float* ws,
-                                         size_t ws_floats, int* tickets, int* err, int w_tiled,
-                                         const LLSmallMEpi* epi_, const LLLora* lo, void* stream_) {
-  const bf16* A = static_cast<const bf16*>(A_);
-  const bf16* W = static_cast<const bf16*>(W_);
-  bf16* C = static_cast<bf16*>(C_);
-  const bf16* bias = static_cast<const bf16*>(bias_);
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (epi_ == nullptr || lo == nullptr) return -3;
-  const LLSmallMEpi& epi = *epi_;
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (M > 128 || lo->tiles != 1 || lo->tile_rows < M) return -3;
-  if ((K % 8) || (lda % 8) || (ldw % 8)) return -3;
-  if (w_tiled && ((N % 128) || (K % 64))) return -3;
-  if (const int rc = small_m_check_epi(C, N, epi)) return rc;
-  if (splits < 1) return -3;
-  if (splits > 1 && (ws == nullptr || tickets == nullptr || ws_floats < (size_t)splits * M * N)) return -6;
-  const int BNX = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
-  CUtensorMap tW, tX;
-  LoraBlocks lb;
-  if (w_tiled ? make_tmap_w_tiled(&tW, W, N, K) : make_tmap_2d(&tW, W, N, K, ldw, GEMM_BM)) return -2;
-  if (make_tmap_2d(&tX, A, M, K, lda, BNX)) return -2;
-  if (const int rc = make_lora_blocks(&lb, *lo, N, BNX)) return rc;
-  const dim3 grid((N + GEMM_BM - 1) / GEMM_BM, splits);
-  cudaError_t e = cudaSuccess;
-#define LL_LAUNCH_LORA(BNX_, PF_, MODE_, TILE_)                                                          \
-  do {                                                                                                   \
-    auto kern = gemm_swapab_kernel<BNX_, 108, PF_, MODE_, TILE_, LoraBlocks>;                            \
-    using C_ = SwapCfg<BNX_, 108>;                                                                       \
-    static unsigned long long done = 0;                                                                  \
-    if (!smem_on_device(kern, C_::SMEM, done)) return -7;                                                \
-    e = launch_pdl(kern, grid, dim3(192), C_::SMEM, stream, tW, tX, C, bias, M, N, K, ldc, 0, ws, tickets, err, \
-                   w_tiled, epi, lb);                                                                    \
-  } while (0)
-#define LL_LAUNCH_LORA_MODE(PF_, TILE_)                                              \
-  do {                                                                               \
-    switch (epi.mode) {                                                              \
-      case LL_EPI_STORE: LL_LAUNCH_LORA(16, PF_, LL_EPI_STORE, TILE_); break;       \
-      case LL_EPI_SWIGLU: LL_LAUNCH_LORA(16, PF_, LL_EPI_SWIGLU, TILE_); break;     \
-      case LL_EPI_RESIDUAL: LL_LAUNCH_LORA(16, PF_, LL_EPI_RESIDUAL, TILE_); break; \
-      default: LL_LAUNCH_LORA(16, PF_, LL_EPI_QKV_ROPE, TILE_); break;              \
-    }                                                                                \
-  } while (0)
-  switch (BNX) {
-    case 16:
-      if (M == 1) LL_LAUNCH_LORA_MODE(false, false);
-      else if (small_m_tile_ok(C, ldc, bias, M, N, ws, epi)) LL_LAUNCH_LORA_MODE(true, true);
-      else LL_LAUNCH_LORA(16, true, -1, false);
-      break;
-    case 32: LL_LAUNCH_LORA(32, true, -1, false); break;
-    case 64: LL_LAUNCH_LORA(64, true, -1, false); break;
-    default: LL_LAUNCH_LORA(128, true, -1, false); break;
-  }
-#undef LL_LAUNCH_LORA_MODE
-#undef LL_LAUNCH_LORA
-  return e == cudaSuccess ? 0 : -5;
-}
-
-// Any M: 256 x 256 tiles on CTA pairs.  epilogue 0 plain, 1 SwiGLU.
+// The tiles are those of ll_gemm_bf16 for the same sizes: CTA pairs with 256 x
+// 256 tiles past 256 rows and from N = 2048 on, else 128 x 256 or 128 x 128.
+// Launched as ll_lora_low's dependent, so that its set-up overlaps that kernel;
+// it waits for it before its first tile.  (Starting the k-blocks of K at once
+// was slower at 5087 rows, 163 us for 142: the pairs that got their SMs last
+// finished last.)
 extern "C" int ll_gemm_bf16_lora(const void* A_, int lda, const void* W_, int ldw, void* C_, int ldc,
                                  const void* bias_, int M, int N, int K, int epilogue, const LLLora* lo, int* err,
                                  void* stream_) {
@@ -2000,29 +1943,59 @@ extern "C" int ll_gemm_bf16_lora(const void* A_, int lda, const void* W_, int ld
   if ((K % 8) || (N % 8) || (lda % 8) || (ldw % 8) || (ldc % 8) || (reinterpret_cast<uintptr_t>(C) & 15)) return -3;
   if (epilogue != kEpiPlain && epilogue != kEpiSwiGLU) return -4;
   if (epilogue == kEpiSwiGLU && (N % 32)) return -4;
-  const int num_m = (M + 2 * GEMM_BM - 1) / (2 * GEMM_BM);
-  // one row tile per 256-row output tile, or all (<= 128) rows in one
-  if (lo->tiles != num_m || (num_m > 1 && lo->tile_rows != 2 * GEMM_BM)) return -3;
+  if (lo->tile_rows != (M <= GEMM_BM ? GEMM_BM : 2 * GEMM_BM) || lo->tiles != (M + lo->tile_rows - 1) / lo->tile_rows)
+    return -3;
+  const int BN = N >= 2048 ? 256 : 128;
+  const bool pair = BN == 256 && M > 2 * GEMM_BM;
   CUtensorMap tA, tB, tC;
   LoraBlocks lb;
   if (make_tmap_2d(&tA, A, M, K, lda, GEMM_BM)) return -2;
-  if (make_tmap_2d(&tB, W, N, K, ldw, 128)) return -2;
-  if (const int rc = make_lora_blocks(&lb, *lo, N, GEMM_BM)) return rc;
-  const int c_bulk =
-      gemm_bulk_store_enabled() && make_tmap_c(&tC, C, M, epilogue == kEpiSwiGLU ? N / 2 : N, ldc) == 0;
-  if (!c_bulk) tC = tA;  // not read
-  const int ntiles = num_m * ((N + 255) / 256);
-  const int pairs = ntiles < num_sms() / 2 ? ntiles : num_sms() / 2;
-#define LL_LAUNCH_LORA2(EPI_)                                                                          \
-  do {                                                                                                 \
-    auto kern = gemm_tcgen05_2sm_kernel<256, EPI_, LoraBlocks>;                                        \
-    static unsigned long long done = 0;                                                                \
-    if (!smem_on_device(kern, Gemm2Cfg<256>::SMEM, done)) return -7;                                   \
-    kern<<<2 * pairs, 192, Gemm2Cfg<256>::SMEM, stream>>>(tA, tB, tC, c_bulk, C, bias, M, N, K, ldc, err, \
-                                                           TpArgs{}, gemm_group_m(M, K, 2 * GEMM_BM), lb); \
+  if (make_tmap_2d(&tB, W, N, K, ldw, pair ? BN / 2 : BN)) return -2;
+  if (const int rc = make_lora_blocks(&lb, *lo, N, pair ? BN / 2 : BN)) return rc;
+  const int bm = pair ? 2 * GEMM_BM : GEMM_BM;
+  const int ntiles = ((M + bm - 1) / bm) * ((N + BN - 1) / BN);
+  const int slots = pair ? num_sms() / 2 : num_sms();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((ntiles < slots ? ntiles : slots) * (pair ? 2 : 1));
+  cfg.blockDim = dim3(192);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  const int group_m = gemm_group_m(M, K, bm);
+  cudaError_t e;
+#define LL_LAUNCH_LORA2(EPI_)                                                                            \
+  do {                                                                                                   \
+    auto kern = gemm_tcgen05_2sm_kernel<256, EPI_, LoraBlocks>;                                          \
+    static unsigned long long done = 0;                                                                  \
+    if (!smem_on_device(kern, Gemm2Cfg<256>::SMEM, done)) return -7;                                     \
+    cfg.dynamicSmemBytes = Gemm2Cfg<256>::SMEM;                                                          \
+    e = cudaLaunchKernelEx(&cfg, kern, tA, tB, tC, c_bulk, C, bias, M, N, K, ldc, err, TpArgs{}, group_m, lb); \
   } while (0)
-  if (epilogue == kEpiSwiGLU) LL_LAUNCH_LORA2(kEpiSwiGLU);
-  else LL_LAUNCH_LORA2(kEpiPlain);
+#define LL_LAUNCH_LORA1(BN_, EPI_)                                                                       \
+  do {                                                                                                   \
+    auto kern = gemm_tcgen05_kernel<BN_, EPI_, LoraBlocks>;                                              \
+    static unsigned long long done = 0;                                                                  \
+    if (!smem_on_device(kern, GemmCfg<BN_>::SMEM, done)) return -7;                                      \
+    cfg.dynamicSmemBytes = GemmCfg<BN_>::SMEM;                                                           \
+    e = cudaLaunchKernelEx(&cfg, kern, tA, tB, C, bias, M, N, K, ldc, err, group_m, lb);                 \
+  } while (0)
+  if (pair) {
+    const int c_bulk =
+        gemm_bulk_store_enabled() && make_tmap_c(&tC, C, M, epilogue == kEpiSwiGLU ? N / 2 : N, ldc) == 0;
+    if (!c_bulk) tC = tA;  // not read
+    if (epilogue == kEpiSwiGLU) LL_LAUNCH_LORA2(kEpiSwiGLU);
+    else LL_LAUNCH_LORA2(kEpiPlain);
+  } else if (BN == 256) {
+    if (epilogue == kEpiSwiGLU) LL_LAUNCH_LORA1(256, kEpiSwiGLU);
+    else LL_LAUNCH_LORA1(256, kEpiPlain);
+  } else {
+    if (epilogue == kEpiSwiGLU) LL_LAUNCH_LORA1(128, kEpiSwiGLU);
+    else LL_LAUNCH_LORA1(128, kEpiPlain);
+  }
+#undef LL_LAUNCH_LORA1
 #undef LL_LAUNCH_LORA2
-  return cudaGetLastError() == cudaSuccess ? 0 : -5;
+  return e == cudaSuccess ? 0 : -5;
 }

@@ -25,6 +25,7 @@ constexpr int LOW_BM = 128;
 constexpr int LOW_BK = 64;
 constexpr int LOW_MAX_CLUSTER = 8;
 constexpr int LOW_RING = 96 * 1024;
+constexpr int64_t LOW_ROWS_BYTES = 24 << 20;
 
 struct LowShape {
   int npad;      // ranks rounded up to the MMA's multiple of 16
@@ -67,12 +68,8 @@ __global__ void __launch_bounds__(128, 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cs = gridDim.x, crank = blockIdx.x;
   const int plane = blockIdx.z;
-  pdl_trigger();
 
-  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && lo.num_tickets > 0) {
-    pdl_wait();  // the previous kernel may be the product of an earlier call on this scratch
-    for (int i = tid; i < lo.num_tickets; i += blockDim.x) lo.tickets[i] = 0;
-  }
+  pdl_trigger();
 
   // which rows and which adapter: the same for every CTA of the cluster
   const int planes = lo.tile_ptr[lo.tiles];
@@ -227,6 +224,289 @@ __global__ void __launch_bounds__(128, 2)
   if (warp == 1) tmem_dealloc(tmem, shp.tmem_cols);
 }
 
+// ---------------------------------------------------------------------------
+// The product for up to 128 rows (decode): as the small-M GEMM, the weight
+// tile is the M = 128 side of the MMA and the rows are the N side, and K is
+// split so that every SM streams weights.  Here the splits of a feature tile
+// are a cluster: their fp32 partials stay in shared memory and each CTA sums,
+// in split order, and stores its share of the rows.  Nothing goes through
+// global memory and no CTA waits for a last one to add up 128 features x M
+// rows x all splits (at 61 rows x 5120 features, 7 splits, that fix-up alone
+// was 40 of 62 us).  Each split takes its share of the k-blocks of K, then its
+// share of the adapters'.  The first ring of weights is on its way before the
+// wait for the low-rank kernel.
+constexpr int GEMV_RING = 108 * 1024;
+// Clusters do not fill the SMs to the last place (two CTAs a SM, 296 places):
+// 36 clusters of 8 and 40 of 7 ran a second round.  us a call with 2 / 4 / 6 /
+// 8 (7) CTAs: 1 row x 4608 features 12.9 / 10.1 / 8.6 / 14.3, 61 rows x 5120
+// 43.2 / 31.1 / 27.9 / 38.7.
+constexpr int GEMV_MAX_CLUSTER = 6;
+constexpr int GEMV_PLACES = 248;
+template <int BNX>
+struct GemvCfg {
+  static constexpr int W_BYTES = 128 * LOW_BK * 2;
+  static constexpr int X_BYTES = BNX * LOW_BK * 2;
+  static constexpr int STAGES = GEMV_RING / (W_BYTES + X_BYTES);
+  static constexpr int TMEM_COLS = BNX < 32 ? 32 : BNX;
+  static constexpr int LD = 132;  // floats per row of the partials
+  static constexpr int SMEM = STAGES * (W_BYTES + X_BYTES) + 1024;
+  static_assert(BNX * LD * 4 <= STAGES * (W_BYTES + X_BYTES), "the partials overlay the ring");
+};
+
+struct alignas(64) GemvMaps {
+  CUtensorMap w, x, low, b;
+};
+
+__device__ __forceinline__ float gemv_silu(float x) { return x / (1.0f + __expf(-x)); }
+
+template <int BNX, bool SWIGLU>
+__global__ void __launch_bounds__(192, 2)
+    lora_gemv_kernel(const __grid_constant__ GemvMaps tm, bf16* __restrict__ C, int64_t ldc,
+                     const bf16* __restrict__ bias, int M, int N, int K, const __grid_constant__ LLLora lo,
+                     int* err) {
+  using Cfg = GemvCfg<BNX>;
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sW = smem;
+  uint8_t* sX = smem + STAGES * Cfg::W_BYTES;
+  float* part = reinterpret_cast<float*>(smem);  // [M][LD], over the ring, once the product is done
+  __shared__ uint64_t full[STAGES], empty[STAGES], tfull;
+  __shared__ uint32_t tmem_slot;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cs = gridDim.x, crank = blockIdx.x, nb = blockIdx.y;
+  const int num_kb = (K + LOW_BK - 1) / LOW_BK;
+  const int rank_blocks = (lo.rank + LOW_BK - 1) / LOW_BK;
+  const int num_extra = min(lo.tile_ptr[1], lo.max_planes) * 2 * rank_blocks;
+  const int per = (num_kb + cs - 1) / cs, eper = (num_extra + cs - 1) / cs;
+  const int kb0 = min(num_kb, crank * per), kb1 = min(num_kb, kb0 + per);
+  const int e0 = min(num_extra, crank * eper), e1 = min(num_extra, e0 + eper);
+  const int steps = kb1 - kb0 + e1 - e0;
+  pdl_trigger();
+
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&tfull, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&tmem_slot, Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const int pre = min(kb1 - kb0, STAGES);
+      for (int i = 0; i < pre; ++i) {
+        mbar_arrive_expect_tx(&full[i], Cfg::W_BYTES + Cfg::X_BYTES);
+        tma_load_2d(sW + i * Cfg::W_BYTES, &tm.w, &full[i], (kb0 + i) * LOW_BK, nb * 128);
+      }
+      pdl_wait();
+      for (int i = 0; i < steps; ++i) {
+        const int kb = kb0 + i;
+        if (i >= pre) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[stage], Cfg::W_BYTES + Cfg::X_BYTES);
+        }
+        if (kb < kb1) {
+          if (i >= pre) tma_load_2d(sW + stage * Cfg::W_BYTES, &tm.w, &full[stage], kb * LOW_BK, nb * 128);
+          tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.x, &full[stage], kb * LOW_BK, 0);
+        } else {
+          const int e = e0 + kb - kb1;
+          const int plane = (e >> 1) / rank_blocks, rb = (e >> 1) % rank_blocks;
+          tma_load_3d(sW + stage * Cfg::W_BYTES, &tm.b, &full[stage], rb * LOW_BK, nb * 128,
+                      lo.plane_adapter[plane]);
+          tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.low, &full[stage], rb * LOW_BK,
+                      (2 * plane + (e & 1)) * lo.tile_rows);
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) {  // let the copies in flight land before the CTA exits
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 2000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_bf16_f32(128, BNX);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < steps; ++i) {
+        if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) break;
+        tc_fence_after();
+        const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sW + stage * Cfg::W_BYTES));
+        const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sX + stage * Cfg::X_BYTES));
+#pragma unroll
+        for (int k = 0; k < LOW_BK / 16; ++k) umma_bf16(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0 ? 1u : 0u);
+        umma_commit(&empty[stage]);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      umma_commit(&tfull);
+    }
+  }
+  __syncwarp();
+  pdl_wait();  // the output may still be read by an earlier kernel's successor
+  const bool ok = __syncthreads_and(mbar_wait(&tfull, 0, err, kErrTmemFullTimeout));
+  tc_fence_after();
+  if (warp >= 2) {  // TMEM lane quarter of this warp: features; columns: rows
+    const int f = (warp & 3) * 32 + lane;
+#pragma unroll 1
+    for (int c = 0; c < BNX && c < M; c += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tmem + (uint32_t((warp & 3) * 32) << 16) + c, r);  // BNX 16: columns 16.. unused
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (c + i < M && c + i < BNX) part[(c + i) * Cfg::LD + f] = steps > 0 ? __uint_as_float(r[i]) : 0.f;
+    }
+  }
+  tc_fence_before();
+  low_cluster_sync();
+  tc_fence_after();
+  if (ok) {
+    const uint32_t base = smem_u32(part);
+    auto sum4 = [&](int row, int f) {
+      float4 p[GEMV_MAX_CLUSTER];
+      const uint32_t at = base + (uint32_t)(row * Cfg::LD + f) * 4;
+#pragma unroll
+      for (int r = 0; r < GEMV_MAX_CLUSTER; ++r) p[r] = r < cs ? ld_cluster_f32x4(low_mapa(at, r)) : make_float4(0, 0, 0, 0);
+      float4 v = p[0];
+#pragma unroll
+      for (int r = 1; r < GEMV_MAX_CLUSTER; ++r) {
+        v.x += p[r].x;
+        v.y += p[r].y;
+        v.z += p[r].z;
+        v.w += p[r].w;
+      }
+      if (bias != nullptr) {
+        const uint2 bv = *reinterpret_cast<const uint2*>(bias + nb * 128 + f);
+        const float2 b0 = unpack_bf16x2(bv.x), b1 = unpack_bf16x2(bv.y);
+        v.x += b0.x;
+        v.y += b0.y;
+        v.z += b1.x;
+        v.w += b1.y;
+      }
+      return v;
+    };
+    constexpr int GROUPS = SWIGLU ? 16 : 32;  // 4-feature groups a row
+    for (int i = crank * 192 + tid; i < M * GROUPS; i += cs * 192) {
+      const int row = i / GROUPS, g = i % GROUPS;
+      if constexpr (SWIGLU) {  // 16 gate features, then the matching 16 up features
+        const int f = (g >> 2) * 32 + (g & 3) * 4;
+        if (nb * 128 + f >= N) continue;
+        const float4 a = sum4(row, f), u = sum4(row, f + 16);
+        *reinterpret_cast<uint2*>(C + row * ldc + nb * 64 + 4 * g) =
+            make_uint2(pack_bf16x2(gemv_silu(a.x) * u.x, gemv_silu(a.y) * u.y),
+                       pack_bf16x2(gemv_silu(a.z) * u.z, gemv_silu(a.w) * u.w));
+      } else {
+        if (nb * 128 + 4 * g >= N) continue;
+        const float4 v = sum4(row, 4 * g);
+        *reinterpret_cast<uint2*>(C + row * ldc + nb * 128 + 4 * g) =
+            make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+      }
+    }
+  }
+  low_cluster_sync();  // the partials live until every CTA has read them
+  if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);
+}
+
+// Few rows (decode): dot products, `ks` warps of a CTA to each (row, rank),
+// every warp with its share of the adapter's row in registers before the wait
+// for x.  No shared tiles, so these CTAs fit beside the product's, which are
+// loading weights meanwhile; what counts is the time from x to the stored
+// value: 2-3 us, against 5-6 for the tensor-core kernel's chain (tiles, TMEM,
+// partials, cluster).  A is read once per row here, from L2 where rows share it.
+constexpr int ROWS_VEC = 8;  // 16-byte vectors a lane holds: 2048 elements of K a warp
+__global__ void __launch_bounds__(256, 2) lora_low_rows_kernel(const bf16* __restrict__ x, int64_t ldx, int M, int K,
+                                                               const __grid_constant__ LLLora lo, int ks, int* err) {
+  __shared__ float parts[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = 8 / ks, share = warp % ks;
+  const int m = blockIdx.x, r = blockIdx.y * per + warp / ks;
+  pdl_trigger();
+  const int t = m / lo.tile_rows;
+  const int p0 = lo.tile_ptr[t], np = lo.tile_ptr[t + 1] - p0, slot = lo.row_slot[m];
+  if (p0 < 0 || np < 0 || p0 + np > lo.max_planes || slot >= np) {
+    if (threadIdx.x == 0) record_error(err, kErrBadIndex);
+    return;
+  }
+  int a = slot >= 0 ? lo.plane_adapter[p0 + slot] : -1;
+  if (slot >= 0 && (a < 0 || a >= lo.adapters)) {
+    if (threadIdx.x == 0) record_error(err, kErrBadIndex);
+    a = -1;
+  }
+  float v = 0.f;
+  if (a >= 0 && r < lo.rank) {
+    const int nv = K / 8, chunk = (nv + ks - 1) / ks;
+    const int v0 = share * chunk, v1 = min(nv, v0 + chunk);
+    const uint4* xr = reinterpret_cast<const uint4*>(x + m * ldx);
+    const uint4* ar = reinterpret_cast<const uint4*>(lo.a + ((size_t)a * lo.rank + r) * K);
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    uint4 av[ROWS_VEC], xv[ROWS_VEC];
+    for (int b = v0; b < v1; b += 32 * ROWS_VEC) {
+#pragma unroll
+      for (int i = 0; i < ROWS_VEC; ++i) {
+        const int j = b + lane + 32 * i;
+        av[i] = j < v1 ? ar[j] : make_uint4(0, 0, 0, 0);
+      }
+      if (b == v0) pdl_wait();
+#pragma unroll
+      for (int i = 0; i < ROWS_VEC; ++i) {
+        const int j = b + lane + 32 * i;
+        xv[i] = j < v1 ? xr[j] : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < ROWS_VEC; ++i) {
+        const uint32_t xu[4] = {xv[i].x, xv[i].y, xv[i].z, xv[i].w}, au[4] = {av[i].x, av[i].y, av[i].z, av[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 p = unpack_bf16x2(xu[j]), q = unpack_bf16x2(au[j]);
+          s[j] = fmaf(p.x, q.x, s[j]);
+          s[j] = fmaf(p.y, q.y, s[j]);
+        }
+      }
+    }
+    v = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
+  }
+  pdl_wait();  // `low` may still be read by an earlier product
+  if (ks > 1) {
+    if (lane == 0) parts[warp] = v;
+    __syncthreads();
+    if (share != 0) return;
+    v = parts[warp];
+    for (int i = 1; i < ks; ++i) v += parts[warp + i];
+  }
+  if (r >= lo.rank) return;
+  if (a >= 0) v *= lo.scale[a];
+  const bf16 hi = __float2bfloat16(v);
+  const float rest = v - __bfloat162float(hi);
+  const bf16 rem = __float2bfloat16(rest == rest && fabsf(rest) < 3.0e38f ? rest : 0.f);  // none of an infinite value
+  const bf16 zero = __float2bfloat16(0.f);
+  for (int j = lane; j < np; j += 32) {
+    bf16* d = lo.low + ((size_t)(p0 + j) * 2 * lo.tile_rows + m % lo.tile_rows) * lo.rank + r;
+    d[0] = j == slot ? hi : zero;
+    d[(size_t)lo.tile_rows * lo.rank] = j == slot ? rem : zero;
+  }
+}
+
 typedef CUresult (*LowEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -262,6 +542,15 @@ extern "C" int ll_lora_low(const bf16* x, int64_t ldx, int M, int K, const LLLor
   if (M <= 0) return 0;
   if ((K % 8) || (ldx % 8) || lo->rank <= 0 || lo->rank > LL_LORA_MAX_RANK || (lo->rank % 8)) return -3;
   if (lo->max_planes < 1 || lo->max_planes > 65535) return -3;
+  // one A row per row and rank through L2, up to this many bytes
+  if ((int64_t)M * lo->rank * K * 2 <= LOW_ROWS_BYTES) {
+    int ks = 1;
+    while (ks < 8 && ks * ROWS_VEC * 256 < K) ks *= 2;
+    const dim3 grid(M, (lo->rank + 8 / ks - 1) / (8 / ks));
+    const cudaError_t e =
+        launch_pdl(lora_low_rows_kernel, grid, dim3(256), 0, stream, x, ldx, M, K, *lo, ks, err);
+    return e == cudaSuccess ? 0 : -5;
+  }
   LowShape shp;
   shp.npad = (lo->rank + 15) / 16 * 16;
   shp.x_rows = M < LOW_BM ? (M + 7) / 8 * 8 : LOW_BM;
@@ -306,4 +595,65 @@ extern "C" int ll_lora_low(const bf16* x, int64_t ldx, int M, int K, const LLLor
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, lora_low_kernel, tmX, tmA, M, K, *lo, shp, err) == cudaSuccess ? 0 : -5;
+}
+
+// One to 128 rows, one row tile.  N a multiple of 8 (32 with SwiGLU); out and
+// bias on 8-byte boundaries.  K splits: as many CTAs (two a SM) as the feature
+// tiles leave room for, up to a cluster of 6.
+extern "C" int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, int64_t ldc, const bf16* bias, int M,
+                            int N, int K, int swiglu, const LLLora* lo, int* err, cudaStream_t stream) {
+  if (M <= 0 || M > 128 || lo->tiles != 1 || lo->tile_rows != 128) return -3;
+  if ((K % 8) || (N % 8) || (swiglu && (N % 32)) || (ldx % 8) || (ldc % 4)) return -3;
+  const int bnx = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
+  GemvMaps tm;
+  const cuuint32_t box2w[2] = {64, 128}, box2x[2] = {64, (cuuint32_t)bnx}, box3[3] = {64, 128, 1};
+  const cuuint64_t dw[2] = {(cuuint64_t)K, (cuuint64_t)N}, sw[1] = {(cuuint64_t)K * 2};
+  const cuuint64_t dx[2] = {(cuuint64_t)K, (cuuint64_t)M}, sx[1] = {(cuuint64_t)ldx * 2};
+  const cuuint64_t dl[2] = {(cuuint64_t)lo->rank, (cuuint64_t)lo->max_planes * 2 * lo->tile_rows};
+  const cuuint64_t sl[1] = {(cuuint64_t)lo->rank * 2};
+  const cuuint64_t db[3] = {(cuuint64_t)lo->rank, (cuuint64_t)N, (cuuint64_t)lo->adapters};
+  const cuuint64_t sb[2] = {(cuuint64_t)lo->rank * 2, (cuuint64_t)lo->rank * 2 * N};
+  if (!low_tmap(&tm.w, w, 2, dw, sw, box2w) || !low_tmap(&tm.x, x, 2, dx, sx, box2x) ||
+      !low_tmap(&tm.low, lo->low, 2, dl, sl, box2x) || !low_tmap(&tm.b, lo->b, 3, db, sb, box3))
+    return -2;
+  const int ntiles = (N + 127) / 128, num_kb = (K + LOW_BK - 1) / LOW_BK;
+  if (ntiles > 65535) return -3;
+  int cs = GEMV_PLACES / ntiles;
+  if (cs > GEMV_MAX_CLUSTER) cs = GEMV_MAX_CLUSTER;
+  if (cs > (num_kb + 1) / 2) cs = (num_kb + 1) / 2;
+  if (cs < 1) cs = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cs, ntiles);
+  cfg.blockDim = dim3(192);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)cs, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cudaError_t e;
+#define LL_GEMV(BNX_, SW_)                                                                      \
+  do {                                                                                          \
+    auto kern = lora_gemv_kernel<BNX_, SW_>;                                                    \
+    static unsigned long long done = 0;                                                         \
+    if (!smem_on_device(kern, GemvCfg<BNX_>::SMEM, done)) return -7;                            \
+    cfg.dynamicSmemBytes = GemvCfg<BNX_>::SMEM;                                                 \
+    e = cudaLaunchKernelEx(&cfg, kern, tm, C, ldc, bias, M, N, K, *lo, err);                    \
+  } while (0)
+#define LL_GEMV_SW(BNX_)              \
+  do {                                \
+    if (swiglu) LL_GEMV(BNX_, true);  \
+    else LL_GEMV(BNX_, false);        \
+  } while (0)
+  switch (bnx) {
+    case 16: LL_GEMV_SW(16); break;
+    case 32: LL_GEMV_SW(32); break;
+    case 64: LL_GEMV_SW(64); break;
+    default: LL_GEMV_SW(128); break;
+  }
+#undef LL_GEMV_SW
+#undef LL_GEMV
+  return e == cudaSuccess ? 0 : -5;
 }

@@ -27,8 +27,7 @@ struct LLLora {
   const int* plane_adapter; // [max_planes]
   const int* plane_tile;    // [max_planes]
   __nv_bfloat16* low;       // [max_planes, 2 (hi, lo), tile_rows, rank]
-  int* tickets;             // split-K tickets of the second launch, zeroed by the first
-  int adapters, rank, tiles, tile_rows, max_planes, num_tickets;
+  int adapters, rank, tiles, tile_rows, max_planes;
 };
 
 constexpr int LL_LORA_MAX_RANK = 256;

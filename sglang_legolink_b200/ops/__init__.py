@@ -308,26 +308,15 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
     M, N = x.shape[0], w.shape[0]
     if plan.rows != M:
         raise ValueError(f"the plan is for {plan.rows} rows, x has {M}")
-    if plan.top_adapter >= lora.a.shape[0]:
-        raise ValueError(f"the plan names adapter {plan.top_adapter}, the stack has {lora.a.shape[0]}")
-    if out is None:
-        out = torch.empty(M, N // 2 if swiglu_epilogue else N, dtype=x.dtype, device=x.device)
-    if not x.is_cuda:
+    if plan.top_adapter >= lora.count:
+        raise ValueError(f"the plan names adapter {plan.top_adapter}, the stack has {lora.count}")
+    if M == 0 or not x.is_cuda:
         y = ref.linear_lora(x, w, bias, lora.a, lora.b, lora.scale, plan.row_adapters)
-        out.copy_(ref_swiglu_interleaved(y) if swiglu_epilogue else y)
-        return out
-    if M == 0:
-        return out
-    ext = _cuda()
+        y = (ref_swiglu_interleaved(y) if swiglu_epilogue else y).to(x.dtype)
+        return y if out is None else out.copy_(y)
     small = M <= SMALL_M_MAX and not (M > 64 and N >= 148 * 256)  # as linear()
-    splits = 1
-    if small:
-        splits = ext.gemm_small_m_splits(N, x.shape[1])
-        if 1 < M <= 16:
-            splits = min(splits, _TILE_MAX_SPLITS)
-    ext.lora_linear(x, w, bias, out, lora.a, lora.b, lora.scale, plan.buf, plan.tile_rows, plan.max_planes, small,
-                    splits, swiglu_epilogue, workspace(x.device).err)
-    return out
+    return _cuda().lora_linear(x, w, bias, out, lora.a, lora.b, lora.scale, plan.buf, plan.tile_rows, plan.max_planes,
+                               small, swiglu_epilogue, workspace(x.device).err)
 
 
 def ref_swiglu_interleaved(gu: torch.Tensor) -> torch.Tensor:

@@ -40,6 +40,7 @@ class LoraStack:
             raise ValueError("a, b and scale must share a device, a and b a dtype")
         self.a, self.b = a.contiguous(), b.contiguous()
         self.scale = scale.float().contiguous()
+        self.count, self.rank = n, rank
         if not bool(torch.isfinite(self.a).all() & torch.isfinite(self.b).all() & torch.isfinite(self.scale).all()):
             raise ValueError("adapter weights must be finite")
 
