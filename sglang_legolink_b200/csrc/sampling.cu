@@ -11,27 +11,18 @@
 // sorted.
 //
 // Few candidates (top-k to 1024, a nucleus or a min-p set of that size): a
-// lower bound on tau that one pass finds (the ranges' own maxima bound the
-// k-th largest; the mass per power of two of the weight bounds the nucleus;
-// min-p is a bound) picks them out of the row, and one CTA sorts them.  Else tau comes from radix selection on the values' order-preserving
-// integer keys, with token counts (top-k) or weights (top-p) summed per bin;
-// top-p selects within the power of two that its cut falls in.
+// lower bound on tau picks them out of the row (the ranges' own maxima bound
+// the k-th largest; the mass per power of two of the weight bounds the
+// nucleus; min-p is a bound), and one CTA sorts them.  Else tau comes from
+// radix selection on the values' order-preserving integer keys, with token
+// counts (top-k) or weights (top-p) summed per bin; top-p selects within the
+// power of two that its cut falls in.
 //
-// Exact weights are integers: w in units of 2^-44, computed in double.
-// Integer sums do not depend on their order, so a row gives the same token
-// whatever batch, cluster size or device it is drawn on, and the sums over a
-// whole vocabulary (2^19 tokens at most: 2^63) are exact to 2^-45 of the
-// largest weight per token.  A token below 2^-45 of it has weight 0 and is
-// never drawn.
-//
-// An exact weight takes some 25 instructions, and a row of 152064 tokens is
-// 150 a thread of a cluster.  Sums over many tokens are therefore first taken
-// with the hardware's 2^x (4 instructions a token) together with a bound on
-// their error, 2^-22 (1.75 + 0.35 |log2 w|) of each weight:
-//   ex2.approx 2^-22; its argument |log2 w| 2^-24 from the product's rounding
-//   and as much from the factor's, times ln 2; three rounded additions.
-// Where the bound leaves one answer possible, that is the exact one; else (a
-// border closer than about 1e-6 of the sum) the row is summed exactly.
+// Weights are integers: w in units of 2^-44, computed in double.  Integer sums
+// do not depend on their order, so a row gives the same token whatever batch,
+// cluster size or device it is drawn on, and the sums over a whole vocabulary
+// (2^19 tokens at most: 2^63) are exact to 2^-45 of the largest weight per
+// token.  A token below 2^-45 of it has weight 0 and is never drawn.
 //
 // A cluster of CTAs owns a row and holds it in shared memory, so the logits
 // are read from memory once; the passes over the row run on shared memory and
@@ -133,17 +124,16 @@ constexpr int SMP_RANGES = SMP_MAX_CLUSTER * SMP_WARPS;  // warp ranges of a row
 constexpr int SMP_OCTAVES = 16;            // powers of two of the weight, the last one open
 constexpr int SMP_LIST = 2048;             // candidates, in one segment per CTA
 constexpr int SMP_FEW = 2 * SMP_THREADS;   // of them that one CTA sorts
-constexpr double SMP_FAST_ONE = 1099511627776.0;  // 2^40: unit of the approximate sums
 constexpr float SMP_LOWEST = -3.4028234663852886e38f;
 
 // What a row's passes need to know of it.
 struct Row {
   double xmax, inv_t, k1;  // t = (x - xmax) k1 is 32 log2 w
-  double shift;            // approximate weights times it are true to their own error
   double u, top_p, min_w;
+  double shift;            // approximate weights times it are true to their own error
+  float fc, fm;            // approximately log2 w = x fc + fm, a little below 0 at the largest
   float top;               // xmax
   float zero;              // smaller logits weigh less than half a unit
-  float fc, fm;            // approximately log2 w = x fc + fm, a little below 0 at the largest
   uint32_t kmax;
 };
 
@@ -153,8 +143,8 @@ struct SampleShared {
   float wkth[SMP_RANGES];                // the r-th largest of its lanes' largest
   unsigned long long wsum[SMP_RANGES];   // kept weight of each range
   uint32_t wties[SMP_RANGES];            // its tokens equal to tau
-  float werr[SMP_RANGES];                // error bound of an approximate sum, in units of 2^-22
-  unsigned long long octave[2][SMP_MAX_CLUSTER][SMP_OCTAVES];  // each CTA's mass per bin; levels alternate
+  unsigned long long whigh[SMP_RANGES];  // weight of each range above the keys that top-p selects in
+  uint32_t octave[2][SMP_MAX_CLUSTER][SMP_OCTAVES];  // each CTA's mass per bin; levels alternate
   uint32_t listed[SMP_MAX_CLUSTER];      // candidates of each CTA
   unsigned long long scan[SMP_WARPS];
   unsigned long long found_above, total, at_target;
@@ -162,9 +152,9 @@ struct SampleShared {
   float bound;
   uint32_t minp_key;
   uint32_t edge[2];
+  int redo;
   int at_range;
   uint32_t at_ties;
-  int redo;
   uint32_t count_here;
   double exp2_table[32];
   union {
@@ -174,7 +164,7 @@ struct SampleShared {
     };
     struct {
       alignas(16) unsigned long long list[SMP_LIST];  // key << 32 | ~index
-      alignas(16) unsigned long long flat[SMP_FEW];   // the same without gaps
+      alignas(16) unsigned long long flat[SMP_FEW];   // of the sort
     };
     uint32_t mine[SMP_OCTAVES][SMP_THREADS];  // each thread's mass per bin
   };
@@ -186,24 +176,25 @@ static_assert(offsetof(SampleShared, count) % 16 == 0 && offsetof(SampleShared, 
 // degree 4 (within 1.2e-12), 2^(n / 32) from a table and the exponent.  Eleven
 // double operations; the library's exponential takes about three times that.
 // For zero <= x <= max.
-__device__ __forceinline__ unsigned long long exact_weight(float x, double xmax, double k1, const double* table) {
+__device__ __forceinline__ double real_weight(float x, double xmax, double k1, const double* table) {
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
   constexpr double c1 = 0.02166084939249829, c2 = 2.3459619820224677e-4, c3 = 1.6938509724371819e-6,
                    c4 = 9.172562701824643e-9;    // (ln 2 / 32)^i / i!
-  // float -> double by its bits (the conversion unit is slow); a subnormal
-  // becomes a number of about its size, infinity a finite number
-  const uint32_t b = __float_as_uint(x);
-  const double xd = __hiloint2double((int)(((b & 0x7FFFFFFFu) >> 3) + (896u << 20) + (b & 0x80000000u)), (int)(b << 29));
-  const double t = (xd - xmax) * k1;
+  const double t = ((double)x - xmax) * k1;
   const double m = t + kMagic;
   const int n = __double2loint(m);
   const double f = t - (m - kMagic);
   double p = fma(fma(fma(fma(c4, f, c3), f, c2), f, c1), f, 1.0);
   p *= table[n & 31];
-  // * 2^(n >> 5) * 2^44, then to a whole number
-  p = __hiloint2double(__double2hiint(p) + (((n >> 5) + 44) << 20), __double2loint(p));
-  p += kMagic;
-  return (((unsigned long long)(uint32_t)__double2hiint(p) << 32) | (uint32_t)__double2loint(p)) - 0x4338000000000000ull;
+  // * 2^(n >> 5) * 2^44
+  return __hiloint2double(__double2hiint(p) + (((n >> 5) + 44) << 20), __double2loint(p));
+}
+__device__ __forceinline__ unsigned long long to_whole(double w) {
+  w += 6755399441055744.0;
+  return (((unsigned long long)(uint32_t)__double2hiint(w) << 32) | (uint32_t)__double2loint(w)) - 0x4338000000000000ull;
+}
+__device__ __forceinline__ unsigned long long exact_weight(float x, double xmax, double k1, const double* table) {
+  return to_whole(real_weight(x, xmax, k1, table));
 }
 // any logit; without a branch, so that several run at once
 __device__ __forceinline__ unsigned long long weight_from(float x, float from, double xmax, double k1,
@@ -213,12 +204,6 @@ __device__ __forceinline__ unsigned long long weight_from(float x, float from, d
 }
 __device__ __noinline__ unsigned long long weight_of(const SampleShared& sh, float x) {
   return weight_from(x, sh.row.zero, sh.row.xmax, sh.row.k1, sh.exp2_table);
-}
-
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ unsigned long long warp_add(unsigned long long v) {
@@ -248,52 +233,71 @@ __device__ __noinline__ ulonglong2 block_exclusive(unsigned long long v, unsigne
   return make_ulonglong2((warp > 0 ? before : 0ull) + inc - v, __shfl_sync(0xffffffffu, w, 31));
 }
 
-// Bitonic sort of n (a power of two, at most 2 SMP_THREADS) values in shared
-// memory, largest first; a pair a thread and step.  Up to 64 values are one
-// warp's, which needs no barrier of the block.
-__device__ __noinline__ void sort_descending(unsigned long long* a, uint32_t n) {
-  __syncthreads();
-  const bool one_warp = n <= 64;
-  if (!one_warp || threadIdx.x < 32)
-    for (uint32_t k = 2; k <= n; k *= 2)
-      for (uint32_t j = k / 2; j > 0; j /= 2) {
-        const uint32_t i = 2 * threadIdx.x - (threadIdx.x & (j - 1));
-        if (i + j < n) {
-          const unsigned long long x = a[i], y = a[i + j];
-          if ((x < y) == ((i & k) == 0)) {
-            a[i] = y;
-            a[i + j] = x;
-          }
-        }
-        if (one_warp) __syncwarp();
-        else __syncthreads();
+// Bitonic sort of n (a power of two, at most 2 SMP_THREADS) values, largest
+// first: thread t holds values 2t and 2t + 1.  Steps within a warp's 64 values
+// are shuffles, wider ones go through `buf`.
+__device__ __noinline__ ulonglong2 sort_descending(ulonglong2 c, unsigned long long* buf, uint32_t n) {
+  const uint32_t i = 2 * threadIdx.x;
+  for (uint32_t k = 2; k <= n; k *= 2)
+    for (uint32_t j = k / 2; j > 0; j /= 2) {
+      ulonglong2 o;  // the partners i ^ j, (i + 1) ^ j
+      if (j >= 64) {
+        __syncthreads();
+        buf[i] = c.x;
+        buf[i + 1] = c.y;
+        __syncthreads();
+        o.x = buf[i ^ j];
+        o.y = buf[(i ^ j) + 1];
+      } else if (j >= 2) {
+        o.x = __shfl_xor_sync(0xffffffffu, c.x, j / 2);
+        o.y = __shfl_xor_sync(0xffffffffu, c.y, j / 2);
+      } else {
+        o.x = c.y;
+        o.y = c.x;
       }
-  __syncthreads();
-}
-
-template <int N>
-__device__ __forceinline__ float tree_sum(const float (&a)[N]) {
-  if constexpr (N == 8) return ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
-  else return (a[0] + a[1]) + (a[2] + a[3]);
+      // the lower index of a pair keeps the larger value where (i & k) == 0
+      const bool down = (i & k) == 0, low = (i & j) == 0;
+      const bool large = down == low, large1 = j == 1 ? !large : large;
+      c.x = large == (o.x > c.x) ? o.x : c.x;
+      c.y = large1 == (o.y > c.y) ? o.y : c.y;
+    }
+  return c;
 }
 
 // ---- passes over a warp's range [a, b) of vectors, results per lane
 
-// Exact weight of the logits >= from.
-template <typename Raw>
-__device__ __noinline__ unsigned long long exact_sum(const uint4* vals, int a, int b, float from, double xmax,
-                                                     double k1, const double* table) {
+// Weight of the logits within [from, upto], and (BOTH) of those above upto
+// too.  The weights are added up as the bits of 1.5 * 2^52 + w, a masked one
+// as those of w = 0.
+struct ExactSum {
+  unsigned long long s, high;
+};
+template <typename Raw, bool BOTH>
+__device__ __noinline__ ExactSum exact_sum(const uint4* vals, int a, int b, float from, float upto, double xmax,
+                                           double k1, const double* table) {
   using K = Key<Raw>;
-  unsigned long long s = 0;
+  unsigned long long s = 0, high = 0;
+  uint32_t vectors = 0;
   for (int v = a + (threadIdx.x & 31); v < b; v += 32) {
     const uint4 q = vals[v];
     if (K::largest(q) < from) continue;
+    ++vectors;
     float x[K::kPerVec];
     K::unpack(q, x);
 #pragma unroll
-    for (int i = 0; i < K::kPerVec; ++i) s += weight_from(x[i], from, xmax, k1, table);
+    for (int i = 0; i < K::kPerVec; ++i) {
+      const double w = real_weight(x[i], xmax, k1, table);  // anything below from
+      const bool in = x[i] >= from && x[i] <= upto;
+      const double r = __hiloint2double(in ? __double2hiint(w) : 0, __double2loint(w)) + 6755399441055744.0;
+      s += __double_as_longlong(r);
+      if (BOTH) {
+        const double h = __hiloint2double(x[i] > upto ? __double2hiint(w) : 0, __double2loint(w)) + 6755399441055744.0;
+        high += __double_as_longlong(h);
+      }
+    }
   }
-  return s;
+  const unsigned long long zero = (unsigned long long)(vectors * K::kPerVec) * 0x4338000000000000ull;
+  return ExactSum{s - zero, high - (BOTH ? zero : 0ull)};
 }
 
 template <typename Raw>
@@ -309,48 +313,12 @@ __device__ __noinline__ uint32_t count_equal(const uint4* vals, int a, int b, fl
   return n;
 }
 
-// Approximate weights of a vector's logits >= from; their sum, and the error
-// bound of it in units of 2^-22 added to `err`.
-template <typename Raw>
-__device__ __forceinline__ float fast_vector(const uint4& q, float fc, float fm, float from,
-                                             float (&w)[Key<Raw>::kPerVec], float& err) {
-  using K = Key<Raw>;
-  float x[K::kPerVec], e[K::kPerVec];
-  K::unpack(q, x);
-#pragma unroll
-  for (int i = 0; i < K::kPerVec; ++i) {
-    const float arg = fmaf(x[i], fc, fm);
-    w[i] = x[i] >= from ? ex2_approx(arg) : 0.f;
-    e[i] = w[i] * fmaxf(arg, -150.f);  // -inf: no weight
-  }
-  const float s = tree_sum(w);
-  err += 1.75f * s - 0.35f * tree_sum(e);
-  return s;
-}
-struct FastSum {
-  unsigned long long s;
-  float err;
-};
-template <typename Raw>
-__device__ __noinline__ FastSum fast_sum(const uint4* vals, int a, int b, float fc, float fm, float from) {
-  using K = Key<Raw>;
-  FastSum r{0, 0.f};
-  for (int v = a + (threadIdx.x & 31); v < b; v += 32) {
-    float w[K::kPerVec];
-    r.s += __float2ull_rn(fast_vector<Raw>(vals[v], fc, fm, from, w, r.err) * (float)SMP_FAST_ONE);
-  }
-  return r;
-}
-
-// Mass per bin of -log2 w, to the thread's own sums: w 2^(e + 23) <= 2^23,
-// rounded to a whole number.  All logits, bins floor(-log2 w); or those within
-// [flo, fhi], bins floor((-log2 w - a0) sc).
-__device__ __forceinline__ void put_mass(uint32_t* mine, uint32_t b, uint32_t e, float arg) {
-  const float m = fmaf(ex2_approx(arg), __uint_as_float((127u + 23u + e) << 23), 8388608.f);
-  mine[b * SMP_THREADS] += __float_as_uint(m) - 0x4B000000u;
-}
-__device__ __forceinline__ float bin_of(float x, float fc, float fm, float a0, float sc) {  // + 2^23
-  return __fadd_rd(fminf(fmaxf((-fmaf(x, fc, fm) - a0) * sc, 0.f), (float)(SMP_OCTAVES - 1)), 8388608.f);
+// Approximate mass per bin floor(-log2 w) of all logits, to the thread's own
+// sums: w 2^(bin + 23) <= 2^23, rounded to a whole number.
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 template <typename Raw>
 __device__ __noinline__ void octave_sums(const uint4* vals, int a, int b, float fc, float fm, uint32_t* mine) {
@@ -362,13 +330,20 @@ __device__ __noinline__ void octave_sums(const uint4* vals, int a, int b, float 
     for (int i = 0; i < K::kPerVec; ++i) {
       const float arg = fmaf(x[i], fc, fm);  // < 0
       const uint32_t bin = __float_as_uint(__fadd_rd(fminf(-arg, (float)(SMP_OCTAVES - 1)), 8388608.f)) - 0x4B000000u;
-      put_mass(mine, bin, bin, arg);
+      const float m = fmaf(ex2_approx(arg), __uint_as_float((127u + 23u + bin) << 23), 8388608.f);
+      mine[bin * SMP_THREADS] += __float_as_uint(m) - 0x4B000000u;
     }
   }
 }
+
+// Mass (approximate) of the logits within [flo, fhi] per sixteenth of their
+// range of arguments: bins floor((a1 - x) sc).
+__device__ __forceinline__ float bin_of(float x, float a1, float sc) {  // + 2^23
+  return __fadd_rd(fminf(fmaxf((a1 - x) * sc, 0.f), (float)(SMP_OCTAVES - 1)), 8388608.f);
+}
 template <typename Raw>
-__device__ __noinline__ void refine_sums(const uint4* vals, int a, int b, float fc, float fm, float a0, float sc,
-                                         uint32_t oct, float flo, float fhi, uint32_t* mine) {
+__device__ __noinline__ void refine_sums(const uint4* vals, int a, int b, float a1, float sc, float k, float flo,
+                                         float fhi, uint32_t* mine) {
   using K = Key<Raw>;
   for (int v = a + (threadIdx.x & 31); v < b; v += 32) {
     const uint4 q = vals[v];
@@ -378,8 +353,9 @@ __device__ __noinline__ void refine_sums(const uint4* vals, int a, int b, float 
 #pragma unroll
     for (int i = 0; i < K::kPerVec; ++i) {  // outside: no mass, without a branch
       const bool in = x[i] >= flo && x[i] <= fhi;
-      put_mass(mine, __float_as_uint(bin_of(x[i], fc, fm, a0, sc)) - 0x4B000000u, oct,
-               in ? fmaf(x[i], fc, fm) : -INFINITY);
+      const uint32_t bin = __float_as_uint(bin_of(x[i], a1, sc)) - 0x4B000000u;
+      // of the heaviest within the keys: at most 2^23
+      mine[bin * SMP_THREADS] += (uint32_t)ex2_approx(in ? fmaf(x[i] - fhi, k, 23.f) : -INFINITY);
     }
   }
 }
@@ -407,10 +383,10 @@ __device__ __noinline__ void histogram(const uint4* vals, int a, int b, float fl
   }
 }
 
-// Candidates >= xlo into this CTA's segment of the first CTA's list.
+// Candidates within [xlo, xhi] into this CTA's segment of the first CTA's list.
 template <typename Raw>
-__device__ __noinline__ void collect(const uint4* vals, int a, int b, int token0, float xlo, uint32_t* counter,
-                                     unsigned long long* to, uint32_t segment) {
+__device__ __noinline__ void collect(const uint4* vals, int a, int b, int token0, float xlo, float xhi,
+                                     uint32_t* counter, unsigned long long* to, uint32_t segment) {
   using K = Key<Raw>;
   for (int v = a + (threadIdx.x & 31); v < b; v += 32) {
     const uint4 q = vals[v];
@@ -419,7 +395,7 @@ __device__ __noinline__ void collect(const uint4* vals, int a, int b, int token0
     K::unpack(q, x);
 #pragma unroll
     for (int i = 0; i < K::kPerVec; ++i)
-      if (x[i] >= xlo) {
+      if (x[i] >= xlo && x[i] <= xhi) {
         const uint32_t at = atomicAdd(counter, 1u);
         if (at < segment)
           to[at] = (unsigned long long)K::of(x[i]) << 32 | (0xFFFFFFFFu - (uint32_t)(token0 + v * K::kPerVec + i));
@@ -428,8 +404,8 @@ __device__ __noinline__ void collect(const uint4* vals, int a, int b, int token0
 }
 
 // Running sums of kept weight over the n <= 128 ranges: weight above tau and
-// tokens at tau, of which the first `quota` count `wtau` each.  One warp; lane
-// l holds entries [l per, (l + 1) per).  The lane whose entry passes u times
+// tokens at tau, of which the first `quota` count `wtau` each.  One warp, four
+// entries a lane.  The lane whose entry passes u times
 // the total returns entry >= 0, what is left of that target before the entry,
 // and of the quota.
 struct Found {
@@ -437,48 +413,45 @@ struct Found {
   unsigned long long t, total;
   uint32_t quota;
 };
-__device__ __noinline__ Found find_entry(const unsigned long long* wsum, const uint32_t* wties, int n, uint32_t quota,
-                                         unsigned long long wtau, double u) {
-  constexpr int MOST = SMP_RANGES / 32;
+__device__ __forceinline__ Found find_entry(const unsigned long long* wsum, const uint32_t* wties, int n,
+                                            uint32_t quota, unsigned long long wtau, double u) {
+  constexpr int PER = SMP_RANGES / 32;
   const int lane = threadIdx.x & 31;
-  const int per = (n + 31) / 32;
-  unsigned long long s[MOST], mine = 0;
-  uint32_t k[MOST], ties = 0;
+  unsigned long long s[PER], mine = 0;
+  uint32_t left[PER] = {};
 #pragma unroll
-  for (int j = 0; j < MOST; ++j) {
-    const int i = lane * per + j;
-    const bool in = j < per && i < n;
-    s[j] = in ? wsum[i] : 0ull;
-    k[j] = in && quota > 0 ? wties[i] : 0u;
-    ties += k[j];
-  }
-  uint32_t before = quota > 0 ? warp_inclusive(ties, lane) - ties : 0u;
-  Found f{-1, 0, 0, 0};
+  for (int j = 0; j < PER; ++j) s[j] = lane * PER + j < n ? wsum[lane * PER + j] : 0ull;
+  if (quota > 0) {
+    uint32_t k[PER], ties = 0;
 #pragma unroll
-  for (int j = 0; j < MOST; ++j) {
-    const uint32_t left = quota > before ? quota - before : 0u;
-    before += k[j];
-    s[j] += (unsigned long long)min(left, k[j]) * wtau;
-    k[j] = left;
-    mine += s[j];
+    for (int j = 0; j < PER; ++j) {
+      k[j] = lane * PER + j < n ? wties[lane * PER + j] : 0u;
+      ties += k[j];
+    }
+    uint32_t before = warp_inclusive(ties, lane) - ties;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      left[j] = quota > before ? quota - before : 0u;
+      before += k[j];
+      s[j] += (unsigned long long)min(left[j], k[j]) * wtau;
+    }
   }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) mine += s[j];
   const unsigned long long inc = warp_inclusive(mine, lane);
-  f.total = __shfl_sync(0xffffffffu, inc, 31);
+  Found f{-1, 0, __shfl_sync(0xffffffffu, inc, 31), 0};
   unsigned long long t = u > 0.0 ? (u < 1.0 ? (unsigned long long)(u * (double)f.total) : f.total - 1) : 0ull;
   if (t >= f.total) t = f.total - 1;
   unsigned long long run = inc - mine;
   if (run <= t && t < inc) {
 #pragma unroll
-    for (int j = 0; j < MOST; ++j) {
-      if (f.entry < 0) {
-        if (t < run + s[j]) {
-          f.entry = lane * per + j;
-          f.t = t - run;
-          f.quota = k[j];
-        } else {
-          run += s[j];
-        }
+    for (int j = 0; j < PER; ++j) {
+      if (run <= t) {
+        f.entry = lane * PER + j;
+        f.t = t - run;
+        f.quota = left[j];
       }
+      run += s[j];
     }
   }
   return f;
@@ -491,27 +464,28 @@ __device__ __noinline__ float log_share(const Row& r, float x, double total) {
 
 // w >= min_p, in the definition's own terms
 __device__ __noinline__ bool heavy(const Row& r, float x) {
-  return x == r.top || (!isinf(r.top) && exp(((double)x - r.xmax) * r.inv_t) >= r.min_w);
+  return x == r.top || exp(((double)x - r.xmax) * r.inv_t) >= r.min_w;
 }
 
 // Largest key in [lo, hi] at which `above` (the sum over keys larger than hi)
 // plus the sum over keys from it to hi reaches a target: tokens, or their
-// weights (W).  The target is `target`, or with below >= 0
-// ceil(top_p (above + all of [lo, hi] + below)), at least 1.
+// weights (W).  Tokens: the search may end with the lower end of a bin of keys,
+// once no more than `enough` tokens are at or above it.
 struct Selected {
   bool ok;  // false: never reached
-  uint32_t key, count;             // the key, tokens equal to it
-  unsigned long long above, goal;  // sum over larger keys
+  uint32_t key, count;       // the key, tokens equal to it
+  unsigned long long above;  // sum over larger keys
 };
 template <typename Raw, bool W>
 __device__ __noinline__ Selected select(SampleShared& sh, const uint4* vals, int v0, int v1, uint32_t lo, uint32_t hi,
-                                        unsigned long long above, unsigned long long target, double below) {
+                                        unsigned long long above, unsigned long long target,
+                                        unsigned long long enough = 0) {
   using K = Key<Raw>;
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = (int)cluster.num_blocks(), tid = threadIdx.x;
-  Selected r{false, 0, 0, above, target};
+  Selected r{false, 0, 0, above};
   if (lo > hi) return r;
-  for (bool first = true;; first = false) {
+  while (true) {
     constexpr int PER = SMP_BINS / SMP_THREADS;
     static_assert(PER == 4, "a thread's bins are one 16-byte read");
     const uint32_t span = hi - lo;
@@ -561,16 +535,14 @@ __device__ __noinline__ Selected select(SampleShared& sh, const uint4* vals, int
       }
     }
     const ulonglong2 ex = block_exclusive(mine, sh.scan);
-    if (first && below >= 0.0)
-      r.goal = (unsigned long long)fmax(1.0, ceil(sh.row.top_p * ((double)r.above + (double)ex.y + below)));
-    if (r.above >= r.goal || r.above + ex.y < r.goal) {  // uniform over the cluster
+    if (r.above >= target || r.above + ex.y < target) {  // uniform over the cluster
       cluster.sync();
       return r;
     }
     unsigned long long before = r.above + ex.x;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      if (before < r.goal && before + val[j] >= r.goal) {
+      if (before < target && before + val[j] >= target) {
         sh.found_bin = b0 + PER - 1 - j;
         sh.found_above = before;
         sh.found_count = cnt[j];
@@ -580,9 +552,9 @@ __device__ __noinline__ Selected select(SampleShared& sh, const uint4* vals, int
     cluster.sync();  // the found bin, and every read of the bins
     const uint32_t b = sh.found_bin;
     r.above = sh.found_above;
-    if (shift == 0) {
+    if (shift == 0 || (!W && r.above + sh.found_count <= enough)) {
       r.ok = true;
-      r.key = lo + b;
+      r.key = lo + (b << shift);
       r.count = sh.found_count;
       return r;
     }
@@ -613,173 +585,213 @@ __device__ __forceinline__ uint32_t first_key(uint32_t lo, uint32_t hi, In in) {
   return lo;
 }
 
-// top-p over the whole row: where its cut falls.  The mass per power of two of
-// the weight (bins floor(-log2 w), the last one open), then, while the bin in
-// which the cut falls holds many tokens, the mass of its sixteenths.
+// top-p over the whole row: the keys within which its cut falls, from
+// approximate masses.  The mass per power of two of the weight (bins
+// floor(-log2 w), the last one open), then, while the bin of the cut holds
+// many tokens for one histogram, the mass of its sixteenths.  What is selected
+// within the keys is checked against exact sums; the few tokens of a small
+// nucleus are enough with the mass below them and its error.
 struct Nucleus {
-  double above, err_above;  // keys > hi: mass (units of 1), its error
-  double below, err_below;  // keys < lo
   uint32_t lo, hi;
-  double tokens;            // at most so many tokens >= lo
+  double tokens, inside;    // at most so many tokens >= lo of the first level; within [lo, hi]
+  double below, err_below;  // mass (units of 1) of the keys < lo of the first level, its error
 };
 template <typename Raw>
-__device__ __noinline__ Nucleus find_nucleus(SampleShared& sh, const uint4* vals, int v0, int v1, int V) {
+__device__ __noinline__ Nucleus find_nucleus(SampleShared& sh, const uint4* vals, int v0, int v1, int V, float T) {
   using K = Key<Raw>;
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float fc = sh.row.fc, fm = sh.row.fm;
-  const double pd = sh.row.top_p;
-  Nucleus r{0.0, 0.0, 0.0, 0.0, K::kNegInf + 1, sh.row.kmax, 1e30};
-  float a0 = 0.f, sc = 1.f;
-  int oct = 0;
+  Nucleus r{K::kNegInf + 1, sh.row.kmax, 1e30, 1e30, 0.0, 0.0};
+  double goal = 0.0;  // mass still to pass
   for (int level = 0;; ++level) {
 #pragma unroll
     for (int b = 0; b < SMP_OCTAVES; ++b) sh.mine[b][tid] = 0;
+    const float flo = K::value(r.lo), fhi = K::value(r.hi), sc = (float)SMP_OCTAVES / (fhi - flo);
     if (level == 0) octave_sums<Raw>(vals, v0, v1, fc, fm, &sh.mine[0][tid]);
-    else refine_sums<Raw>(vals, v0, v1, fc, fm, a0, sc, (uint32_t)oct, K::value(r.lo), K::value(r.hi), &sh.mine[0][tid]);
+    else refine_sums<Raw>(vals, v0, v1, fhi, sc, 1.442695f / T, flo, fhi, &sh.mine[0][tid]);
     __syncthreads();
-    {  // one warp a bin
-      static_assert(SMP_WARPS == SMP_OCTAVES, "a warp a bin");
+    {  // one warp a bin, in units 512 times coarser: a bin of a CTA fits 32 bits
+      static_assert(SMP_WARPS == SMP_OCTAVES && SMP_THREADS == 512, "a warp a bin");
       unsigned long long m = 0;
 #pragma unroll
       for (int i = 0; i < SMP_THREADS; i += 32) m += sh.mine[warp][i + lane];
       m = warp_add(m);
-      if (lane < cs) cluster.map_shared_rank(&sh.octave[level & 1][0][0], lane)[rank * SMP_OCTAVES + warp] = m;
+      if (lane < cs)
+        cluster.map_shared_rank(&sh.octave[level & 1][0][0], lane)[rank * SMP_OCTAVES + warp] = (uint32_t)(m >> 9);
     }
     cluster.sync();
-    // every warp, a lane a bin: mass, error, the bin in which the cut falls
-    double mass = 0.0, err = 0.0;
+    // every warp, a lane a bin: the bin in which the cut falls
+    double mass = 0.0;
     if (lane < SMP_OCTAVES) {
       unsigned long long m = 0;
       for (int c = 0; c < cs; ++c) m += sh.octave[level & 1][c][lane];
-      const int e = level == 0 ? lane : oct;
-      mass = (double)m * __hiloint2double((1023 - 23 - e) << 20, 0);
-      // 2^-22 (ex2) + 2^-23 (rounded to a whole) + 2 * 2^-24 |arg| ln 2
-      // (argument; the open bin: at most 46); its wholes are of its upper end
-      err = mass * ((1.5 + 0.35 * (e == SMP_OCTAVES - 1 ? 46.0 : e + 1.0)) * (1.01 / 4194304.0)) +
-            (e == SMP_OCTAVES - 1 ? (double)V * __hiloint2double((1023 - 24 - (SMP_OCTAVES - 1)) << 20, 0) : 0.0);
+      // units: of bin b 2^(9 - 23 - b); of a later level, the weight of hi 2^(9 - 23)
+      mass = (double)m * (level == 0 ? __hiloint2double((1023 - 14 - lane) << 20, 0)
+                                     : (double)ex2_approx(fmaf(fhi, fc, fm)) * (1.0 / 16384.0));
     }
-    const double upto = warp_inclusive(mass, lane), err_upto = warp_inclusive(err, lane);
-    const double all = __shfl_sync(0xffffffffu, upto, 31), err_all = __shfl_sync(0xffffffffu, err_upto, 31);
-    // top_p (above + all + below) - above, and how far it may be off
-    const double goal = pd * (r.above + all + r.below) - r.above;
-    const double e = (1.0 - pd) * r.err_above + pd * (err_all + r.err_below) + err_all;
+    const double upto = warp_inclusive(mass, lane), all = __shfl_sync(0xffffffffu, upto, 31);
+    if (level == 0) goal = sh.row.top_p * all;
     const uint32_t past = __ballot_sync(0xffffffffu, lane < SMP_OCTAVES - 1 && upto >= goal);
-    const uint32_t past0 = __ballot_sync(0xffffffffu, lane < SMP_OCTAVES - 1 && upto >= goal - e);
-    const uint32_t past1 = __ballot_sync(0xffffffffu, lane < SMP_OCTAVES - 1 && upto >= goal + e);
-    if (level > 0 && (past0 != past || past1 != past)) break;  // on a border: stay with the wider bin
     const int at = past ? __ffs(past) - 1 : SMP_OCTAVES - 1;
-    const double here = __shfl_sync(0xffffffffu, upto, at), err_here = __shfl_sync(0xffffffffu, err_upto, at);
-    const double in = __shfl_sync(0xffffffffu, mass, at), err_in = __shfl_sync(0xffffffffu, err, at);
-    r.above += here - in;
-    r.err_above += err_here - err_in;
-    r.below += all - here;
-    r.err_below += err_all - err_here;
+    const double in = __shfl_sync(0xffffffffu, mass, at), here = __shfl_sync(0xffffffffu, upto, at);
+    goal -= here - in;
     if (level == 0) {
-      oct = at;
-      const double n = warp_inclusive(lane < SMP_OCTAVES - 1 ? mass * (double)(2u << lane) * 1.001 : 1e30, lane);
-      r.tokens = __shfl_sync(0xffffffffu, n, at);
+      // tokens: by the bins' smallest weights, and what the coarser units dropped
+      const double n = lane < SMP_OCTAVES - 1 ? mass * (double)(2u << lane) * 1.001 + 1.0 : 1e30;
+      r.tokens = __shfl_sync(0xffffffffu, warp_inclusive(n, lane), at);
+      // error: 2^-22 (ex2) + 2^-23 (rounded to a whole) + 2 * 2^-24 |arg| ln 2
+      // (argument; the open bin: at most 46); its wholes, and the coarser units
+      double err = lane < SMP_OCTAVES
+                       ? mass * ((1.5 + 0.35 * (lane == SMP_OCTAVES - 1 ? 46.0 : lane + 1.0)) * (1.01 / 4194304.0)) +
+                             (lane == SMP_OCTAVES - 1 ? (double)V : 0.0) * __hiloint2double((1023 - 39) << 20, 0) +
+                             cs * __hiloint2double((1023 - 14 - lane) << 20, 0)
+                       : 0.0;
+      err = warp_inclusive(err, lane);
+      r.below = all - here;
+      r.err_below = __shfl_sync(0xffffffffu, err, 31) - __shfl_sync(0xffffffffu, err, at);
     }
-    // the bin's keys: bin_of does not rise with x
+    // the bin's keys
     if (warp < 2) {
-      const float border = 8388608.f + (float)(at + 1 - warp);  // bins < at + 1; < at
-      uint32_t k = warp == 0 ? r.lo : r.hi + 1;
+      const int b = at + 1 - warp;  // warp 0: first key of bins < at + 1; warp 1: of bins < at
+      uint32_t k = warp == 0 ? max(r.lo, K::of(sh.row.zero)) : r.hi + 1;
       if (warp == 0 ? at < SMP_OCTAVES - 1 : at > 0)
-        k = first_key(r.lo, r.hi, [&](uint32_t q) { return bin_of(K::value(q), fc, fm, a0, sc) < border; });
+        k = first_key(r.lo, r.hi, [&](uint32_t q) {
+          const float x = K::value(q);
+          return level == 0 ? fmaf(x, fc, fm) > -(float)b : bin_of(x, fhi, sc) < 8388608.f + (float)b;
+        });
       if (lane == 0) sh.edge[warp] = k;
     }
     __syncthreads();
     r.lo = sh.edge[0];
     r.hi = sh.edge[1] - 1;
-    const double tokens = oct == SMP_OCTAVES - 1 ? 1e30 : in * (double)(2u << oct);
     // (a bin per key takes 32-bit counts: cheaper than another level up to more tokens)
-    if (r.tokens <= SMP_FEW || tokens <= (r.hi - r.lo < SMP_BINS ? 8192.0 : 1024.0) || r.lo >= r.hi || level == 3) break;
-    a0 += (float)at / sc;
-    sc *= level == 0 && oct == SMP_OCTAVES - 1 ? 0.5f : 16.f;
+    r.inside = in / (double)ex2_approx(fmaf(K::value(r.lo), fc, fm)) * 1.001 + 1.0;
+    if (r.tokens <= SMP_FEW || r.inside <= (r.hi - r.lo < SMP_BINS ? 8192.0 : (double)SMP_FEW) || r.lo >= r.hi ||
+        level == 3)
+      break;
+    __syncthreads();  // the edges are read
   }
   return r;
 }
 
+// Every CTA's candidates within [xlo, xhi] to the first CTA's list; how many,
+// or more than SMP_FEW where they do not fit.  All threads of the cluster.
+template <typename Raw>
+__device__ __noinline__ uint32_t collect_all(SampleShared& sh, const uint4* vals, int a, int b, int token0, float xlo,
+                                             float xhi) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x;
+  const uint32_t segment = SMP_LIST / cs;
+  if (tid == 0) sh.count_here = 0;
+  __syncthreads();
+  collect<Raw>(vals, a, b, token0, xlo, xhi, &sh.count_here, cluster.map_shared_rank(sh.list, 0) + rank * segment,
+               segment);
+  __syncthreads();
+  if (tid < cs) cluster.map_shared_rank(sh.listed, tid)[rank] = sh.count_here;
+  cluster.sync();
+  uint32_t n = 0;
+  for (int c = 0; c < cs; ++c) {
+    const uint32_t m = sh.listed[c];
+    n = n > SMP_FEW || m > segment ? SMP_FEW + 1 : n + m;
+  }
+  return n;
+}
+
+// The n listed candidates in the order, two a thread, on the first CTA.
+__device__ __noinline__ ulonglong2 sorted_list(SampleShared& sh, int cs, uint32_t n) {
+  const int tid = threadIdx.x, segment = SMP_LIST / cs;
+  ulonglong2 c = make_ulonglong2(0, 0);
+  uint32_t base = 0, size = 2;
+  for (int r = 0; r < cs; ++r) {
+    const uint32_t m = sh.listed[r], i = 2 * tid - base;  // wraps where 2 tid < base
+    if (i < m) c.x = sh.list[r * segment + i];
+    if (i + 1 < m) c.y = sh.list[r * segment + i + 1];
+    base += m;
+  }
+  while (size < n) size *= 2;
+  return sort_descending(c, sh.flat, size);
+}
+
+// top-p's cut among the n listed candidates, `above` the weight of all larger
+// ones: its key and how many tokens equal to it are kept, to every CTA (0: the
+// cut is not among them).
+template <typename Raw>
+__device__ __noinline__ void cut_in_list(SampleShared& sh, int cs, uint32_t n, unsigned long long above,
+                                         unsigned long long goal) {
+  using K = Key<Raw>;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
+  const ulonglong2 c = sorted_list(sh, cs, n);
+  const uint32_t k0 = (uint32_t)(c.x >> 32), k1 = (uint32_t)(c.y >> 32);
+  const unsigned long long w0 = c.x != 0 ? weight_of(sh, K::value(k0)) : 0ull;
+  const unsigned long long w1 = c.y != 0 ? weight_of(sh, K::value(k1)) : 0ull;
+  if (tid == 0) sh.found_bin = 0;
+  const ulonglong2 ex = block_exclusive(w0 + w1, sh.scan);
+  const unsigned long long b0 = above + ex.x, b1 = b0 + w0;
+  // the last kept token: what is before it is below the goal, with it no more
+  if (b0 < goal && goal <= b0 + w0) sh.found_bin = k0;
+  if (b1 < goal && goal <= b1 + w1) sh.found_bin = k1;
+  __syncthreads();
+  const uint32_t key = sh.found_bin;
+  const uint32_t kept = __syncthreads_count(key != 0 && k0 == key && b0 < goal) +
+                        __syncthreads_count(key != 0 && k1 == key && b1 < goal);
+  if (tid < cs) {
+    *cluster.map_shared_rank(&sh.found_bin, tid) = key;
+    *cluster.map_shared_rank(&sh.found_count, tid) = kept;
+  }
+}
+
 // The few candidates in sh.list, in segments of one CTA each: filters, draw.
-// `below` and its error: mass (units of 1) of the lighter tokens, for a top-p
-// over the whole row (below >= 0).  False: too near a border.
+// `below`, `err`: mass (units of 1) of the row's other tokens and its error,
+// for a top-p over the whole row; else -1.  False: too near a border.
 template <typename Raw>
 __device__ __noinline__ bool finish_list(SampleShared& sh, const LLSample& p, int64_t row, int cs, uint32_t n,
                                          uint32_t limit, bool use_p, bool use_m, double below, double err) {
   using K = Key<Raw>;
-  const int tid = threadIdx.x, segment = SMP_LIST / cs;
-  uint32_t base = 0;
-  for (int c = 0; c < cs; ++c) {
-    const uint32_t m = sh.listed[c];
-    for (uint32_t i = tid; i < m; i += SMP_THREADS) sh.flat[base + i] = sh.list[c * segment + i];
-    base += m;
-  }
+  const int tid = threadIdx.x;
   // two tokens a thread, in the order: weights and what is before them
-  uint32_t size = 2;
-  while (size < n) size *= 2;
-  for (uint32_t i = n + tid; i < size; i += SMP_THREADS) sh.flat[i] = 0;
-  sort_descending(sh.flat, size);
+  ulonglong2 c = sorted_list(sh, cs, n);
   limit = min(limit, n);
-  unsigned long long c[2], w[2], before[2];
-#pragma unroll
-  for (int o = 0; o < 2; ++o) {
-    const uint32_t i = 2 * tid + o;
-    c[o] = i < n ? sh.flat[i] : 0ull;
-    w[o] = i < limit ? weight_of(sh, K::value((uint32_t)(c[o] >> 32))) : 0ull;
-  }
-  ulonglong2 ex = block_exclusive(w[0] + w[1], sh.scan);
-  before[0] = ex.x;
-  before[1] = ex.x + w[0];
-  double goal = 0.0, goal0 = 0.0, goal1 = 0.0;
+  if (2 * tid >= limit) c.x = 0;
+  if (2 * tid + 1 >= limit) c.y = 0;
+  unsigned long long w0 = c.x != 0 ? weight_of(sh, K::value((uint32_t)(c.x >> 32))) : 0ull;
+  unsigned long long w1 = c.y != 0 ? weight_of(sh, K::value((uint32_t)(c.y >> 32))) : 0ull;
   if (use_p) {
-    const double pd = sh.row.top_p, s = (double)ex.y + (below > 0.0 ? below * sh.row.shift * SMP_ONE : 0.0);
-    goal = goal0 = goal1 = fmax(1.0, ceil(pd * s));
+    const ulonglong2 ex = block_exclusive(w0 + w1, sh.scan);
+    // predecessors' mass below top_p of all; the first token is always kept
+    const double scale = below >= 0.0 ? sh.row.shift * SMP_ONE : 0.0;
+    const double goal = fmax(1.0, ceil(sh.row.top_p * ((double)ex.y + below * scale)));
     if (below >= 0.0) {
-      const double e = pd * err * sh.row.shift * SMP_ONE + 2.0;
-      goal0 = fmax(1.0, goal - e);
-      goal1 = goal + e;
+      // the cut for any mass within the error: before the same token, and within the list
+      const double e = sh.row.top_p * err * scale + 2.0, b0 = (double)ex.x, b1 = (double)(ex.x + w0);
+      const bool near = (c.x != 0 && tid > 0 && fabs(b0 - goal) <= e) || (c.y != 0 && fabs(b1 - goal) <= e) ||
+                        (double)ex.y < goal + e;
+      if (__syncthreads_or(near)) return false;
     }
+    if ((double)ex.x >= goal && tid > 0) c.x = 0;
+    if ((double)(ex.x + w0) >= goal) c.y = 0;
   }
-  bool near = false;
-#pragma unroll
-  for (int o = 0; o < 2; ++o) {
-    const uint32_t i = 2 * tid + o;
-    bool in = i < limit;
-    if (in && use_p && i > 0) {
-      near |= (double)before[o] >= goal0 && (double)before[o] < goal1;
-      in = (double)before[o] < goal;
-    }
-    // the list ends above the lighter tokens: the cut must lie inside it
-    if (below >= 0.0 && i == n - 1) near |= (double)(before[o] + w[o]) < goal1;
-    if (in && use_m) in = heavy(sh.row, K::value((uint32_t)(c[o] >> 32)));
-    if (!in) c[o] = 0;
+  if (use_m) {
+    if (c.x != 0 && !heavy(sh.row, K::value((uint32_t)(c.x >> 32)))) c.x = 0;
+    if (c.y != 0 && !heavy(sh.row, K::value((uint32_t)(c.y >> 32)))) c.y = 0;
   }
-  if (__syncthreads_or(near && below >= 0.0)) return false;
   // the kept ones, which are the first: by index (~index, key), and their running sum
-  const uint32_t kept = __syncthreads_count(c[0] != 0) + __syncthreads_count(c[1] != 0);
-  size = 2;
+  const uint32_t kept = __syncthreads_count(c.x != 0) + __syncthreads_count(c.y != 0);
+  uint32_t size = 2;
   while (size < kept) size *= 2;
-#pragma unroll
-  for (int o = 0; o < 2; ++o)
-    if (2 * tid + o < size) sh.flat[2 * tid + o] = c[o] << 32 | c[o] >> 32;
-  sort_descending(sh.flat, size);
-#pragma unroll
-  for (int o = 0; o < 2; ++o) {
-    c[o] = 2 * tid + o < kept ? sh.flat[2 * tid + o] : 0ull;
-    w[o] = c[o] != 0 ? weight_of(sh, K::value((uint32_t)c[o])) : 0ull;
-  }
-  ex = block_exclusive(w[0] + w[1], sh.scan);
+  c = sort_descending(make_ulonglong2(c.x << 32 | c.x >> 32, c.y << 32 | c.y >> 32), sh.flat, size);
+  w0 = 2 * tid < kept ? weight_of(sh, K::value((uint32_t)c.x)) : 0ull;
+  w1 = 2 * tid + 1 < kept ? weight_of(sh, K::value((uint32_t)c.y)) : 0ull;
+  const ulonglong2 ex = block_exclusive(w0 + w1, sh.scan);
   const double u = sh.row.u;
   unsigned long long t = u > 0.0 ? (u < 1.0 ? (unsigned long long)(u * (double)ex.y) : ex.y - 1) : 0ull;
   if (t >= ex.y) t = ex.y - 1;
-#pragma unroll
-  for (int o = 0; o < 2; ++o) {
-    if (ex.x <= t && t < ex.x + w[o]) {
-      p.out[row] = (int)(0xFFFFFFFFu - (uint32_t)(c[o] >> 32));
-      if (p.logprob) p.logprob[row] = log_share(sh.row, K::value((uint32_t)c[o]), (double)ex.y / SMP_ONE);
-    }
-    ex.x += w[o];
+  if (ex.x <= t && t < ex.x + w0 + w1) {
+    const unsigned long long d = t < ex.x + w0 ? c.x : c.y;
+    p.out[row] = (int)(0xFFFFFFFFu - (uint32_t)(d >> 32));
+    if (p.logprob) p.logprob[row] = log_share(sh.row, K::value((uint32_t)d), (double)ex.y / SMP_ONE);
   }
   return true;
 }
@@ -800,8 +812,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
   const int V = p.V, ranges = cs * SMP_WARPS;
 
   pdl_trigger();
-  if (tid < 32) sh.exp2_table[tid] = exp2((double)tid / 32.0);
   if (tid == 0) sh.redo = 0;
+  if (tid < 32) sh.exp2_table[tid] = exp2((double)tid / 32.0);
   pdl_wait();
   const float T = p.temperature ? p.temperature[row] : 1.f;
   const int top_k = p.top_k ? p.top_k[row] : 0;
@@ -811,7 +823,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
   // few candidates: at least k_of tokens lie at or above the k_of-th largest
   // of the ranges' maxima; with r_want of them wanted from every range, at or
   // above the smallest of the ranges' r_want-th largest lane maxima
-  const int r_want = k_of <= SMP_FEW ? (k_of + ranges - 1) / ranges : 0;
+  const int r_want = (k_of + ranges - 1) / ranges;
 
   // ---- load: the row to shared memory, and its largest logit.  Every CTA
   // has a run of 16-byte vectors, every warp of it a range [v0, v1) of them.
@@ -910,189 +922,183 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
     }
     return;
   }
+  if (xmax == INFINITY) {  // all mass is on the infinities, alike: they become 0, the others -inf
+    __syncthreads();       // the ranges' maxima are read
+    for (int v = v0 + lane; v < v1; v += 32) {
+      float x[PV];
+      K::unpack(vals[v], x);
+      uint32_t w[4] = {K::kFill, K::kFill, K::kFill, K::kFill};
+#pragma unroll
+      for (int i = 0; i < PV; ++i)
+        if (x[i] == INFINITY) {
+          if constexpr (PV == 8) w[i / 2] &= (i & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+          else w[i] = 0u;
+        }
+      vals[v] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (tid < ranges) {
+      sh.wmax[tid] = sh.wmax[tid] == INFINITY ? 0.f : kNone;
+      sh.wkth[tid] = sh.wkth[tid] == INFINITY ? 0.f : kNone;
+    }
+    xmax = 0.f;
+    __syncthreads();
+  }
   if (tid == 0) {
     Row& r = sh.row;
-    const bool inf = isinf(xmax);  // then all mass is on the infinities, alike
     r.top = xmax;
     r.kmax = K::of(xmax);
     r.xmax = (double)xmax;
     r.inv_t = 1.0 / (double)T;
-    r.k1 = inf ? 0.0 : 46.16624130844683 * r.inv_t;  // 32 / ln 2
+    r.k1 = 46.16624130844683 * r.inv_t;  // 32 / ln 2
     // rounded up: no logit from it on is outside the polynomial's range
-    float z = fminf(xmax, __double2float_ru(r.xmax - 31.2 * (double)T));
-    z = inf ? xmax : K::up(z == kNone ? SMP_LOWEST : z);
-    r.zero = z;
+    const float z = fminf(xmax, __double2float_ru(r.xmax - 31.2 * (double)T));
+    r.zero = K::up(fmaxf(z, SMP_LOWEST));
     r.fc = (float)(1.4426950408889634 * r.inv_t);
     r.fm = fmaf(-xmax, r.fc, -0.001953125f);  // every argument is below 0
     // 2^-(fm + xmax fc), the exponent within 2^-8: by its series
     const double d = -0.6931471805599453 * ((double)r.fm + r.xmax * (double)r.fc);
     r.shift = 1.0 + d * (1.0 + d * (0.5 + d * (1.0 / 6 + d * (1.0 / 24 + d * (1.0 / 120)))));
-    if (inf) r.xmax = 0.0;  // (x - xmax) k1 = 0
     r.u = p.u[row];
     r.top_p = fmax((double)top_p, 0.0);
     r.min_w = fmin((double)min_p, 1.0);
   }
-  // where the approximate sums' bound holds: no overflow or cancellation in
-  // the arguments, fm rounded to 2^-12 at most
-  const float fm_size = fabsf(xmax) / T * 1.4427f;
-  const bool fast_ok = T >= 1e-3f && T <= 1e4f && fm_size <= 4000.f && V >= 2048;
   __syncthreads();
 
   const bool use_p = top_p < 1.f, use_m = min_p > 0.f;
-  const bool nucleus = use_p && k_of == 0 && fast_ok;
-  Nucleus nu{0.0, 0.0, -1.0, 0.0, K::kNegInf + 1, 0u, 1e30};
-  if (nucleus) nu = find_nucleus<Raw>(sh, vals, v0, v1, V);
+  // approximate masses: where their arguments neither overflow nor cancel, fm
+  // rounded to 2^-12 at most
+  const bool nucleus = use_p && k_of == 0 && T >= 1e-3f && T <= 1e4f && fabsf(xmax) / T * 1.4427f <= 4000.f;
+  Nucleus nu{K::kNegInf + 1, sh.row.kmax, 1e30, 1e30, -1.0, 0.0};
+  if (nucleus) nu = find_nucleus<Raw>(sh, vals, v0, v1, V, T);
+
+  // What is kept, where it is not few: logits above tau, and the first `quota`
+  // equal to it.
+  float tau = kNone;
+  uint32_t quota = 0;
+
+  // ---- top-k: a lower bound on the k-th largest; with a larger k, itself
+  float xlo = INFINITY;
+  if (r_want == 1) {
+    if (tid < ranges) {
+      const float mine = sh.wmax[tid];
+      int larger = 0;
+#pragma unroll 8
+      for (int i = 0; i < ranges; ++i) {
+        const float o = sh.wmax[i];
+        larger += o > mine || (o == mine && i < tid);
+      }
+      if (larger == k_of - 1) sh.bound = mine;
+    }
+    __syncthreads();
+    xlo = fmaxf(sh.bound, SMP_LOWEST);
+  } else if (k_of > 0) {
+    float b = r_want <= 32 ? INFINITY : kNone;
+    for (int i = lane; i < ranges; i += 32) b = fminf(b, sh.wkth[i]);
+    xlo = fmaxf(-warp_max(-b), SMP_LOWEST);
+    const Selected r =
+        select<Raw, false>(sh, vals, v0, v1, K::of(xlo), sh.row.kmax, 0, (unsigned long long)k_of, SMP_FEW);
+    if (r.ok) {
+      xlo = K::value(r.key);
+      if (r.above + r.count > SMP_FEW) {
+        tau = xlo;
+        quota = (uint32_t)(k_of - r.above);
+      }
+    }
+  } else if (use_p) {
+    if (nu.tokens <= SMP_FEW) xlo = K::value(nu.lo);
+  } else if (min_p >= 1e-4f) {
+    // a little below max + T log(min_p)
+    xlo = __double2float_rd(sh.row.xmax + (double)T * (log(sh.row.min_w) - 1e-6) - 1e-6 * fabs(sh.row.xmax));
+    xlo = K::up(fmaxf(xlo, SMP_LOWEST));
+    if (!(xlo <= xmax)) xlo = xmax;
+  }
 
   // ---- few candidates: every token at or above `xlo`, finished by one CTA
-  {
-    float xlo = INFINITY;
-    if (r_want == 1) {
-      if (tid < ranges) {
-        const float mine = sh.wmax[tid];
-        int larger = 0;
-#pragma unroll 8
-        for (int i = 0; i < ranges; ++i) {
-          const float o = sh.wmax[i];
-          larger += o > mine || (o == mine && i < tid);
-        }
-        if (larger == k_of - 1) sh.bound = mine;
-      }
-      __syncthreads();
-      xlo = sh.bound;
-    } else if (r_want > 1) {
-      float b = r_want <= 32 ? INFINITY : kNone;
-      for (int i = lane; i < ranges; i += 32) b = fminf(b, sh.wkth[i]);
-      xlo = -warp_max(-b);
-    } else if (nucleus) {
-      if (nu.tokens <= SMP_FEW) xlo = K::value(nu.lo);
-    } else if (k_of == 0 && !use_p && min_p >= 1e-4f && !isinf(xmax)) {
-      // a little below max + T log(min_p)
-      xlo = __double2float_rd(sh.row.xmax + (double)T * (log(sh.row.min_w) - 1e-6) - 1e-6 * fabs(sh.row.xmax));
-      xlo = K::up(fmaxf(xlo, SMP_LOWEST));
-      if (!(xlo <= xmax)) xlo = xmax;
-    }
-    if (xlo != INFINITY || isinf(xmax)) {
-      xlo = fmaxf(fminf(xlo, xmax), SMP_LOWEST);
-      const uint32_t segment = SMP_LIST / cs;
-      if (tid == 0) sh.count_here = 0;
-      __syncthreads();
-      collect<Raw>(vals, v0, v1, token0, xlo, &sh.count_here, cluster.map_shared_rank(sh.list, 0) + rank * segment,
-                   segment);
-      __syncthreads();
-      if (tid < cs) cluster.map_shared_rank(sh.listed, tid)[rank] = sh.count_here;
+  if (xlo != INFINITY && tau == kNone) {
+    const uint32_t n = collect_all<Raw>(sh, vals, v0, v1, token0, xlo, INFINITY);
+    if (n <= SMP_FEW) {
+      if (rank == 0 &&
+          !finish_list<Raw>(sh, p, row, cs, n, k_of > 0 ? (uint32_t)k_of : n, use_p, use_m, nu.below, nu.err_below) &&
+          tid < cs)
+        *cluster.map_shared_rank(&sh.redo, tid) = 1;
+      if (!nucleus) return;
       cluster.sync();
-      uint32_t n = 0;
-      bool fits = true;
-      for (int c = 0; c < cs; ++c) {
-        fits = fits && sh.listed[c] <= segment;
-        n += sh.listed[c];
-      }
-      if (fits && n <= SMP_FEW) {
-        if (rank == 0 && !finish_list<Raw>(sh, p, row, cs, n, k_of > 0 ? (uint32_t)k_of : n, use_p, use_m, nu.below,
-                                           nu.err_below) &&
-            tid < cs)
-          *cluster.map_shared_rank(&sh.redo, tid) = 1;
-        if (!nucleus) return;
-        cluster.sync();
-        if (!sh.redo) return;
-      }
+      if (!sh.redo) return;
     }
   }
 
-  // ---- many: what is kept is logits above tau, and the first `quota` equal to it
-  float tau = kNone;
-  uint32_t quota = 0;
-  // The smallest logit above tau with weight; NaN where there is none.
-  auto above_tau = [&](bool fast) {
-    if (tau >= xmax) return __int_as_float(0x7FFFFFFF);
-    const float next = tau == kNone ? SMP_LOWEST : K::value(K::of(tau) + 1);
-    return fast ? next : fmaxf(next, sh.row.zero);
+  // ---- many: the threshold, selected in the row
+  // The smallest logit above x with weight; NaN where there is none.
+  auto above_of = [&](float x) {
+    if (x >= xmax) return __int_as_float(0x7FFFFFFF);
+    return fmaxf(x == kNone ? SMP_LOWEST : K::value(K::of(x) + 1), sh.row.zero);
   };
-  // Weight above tau and tokens at tau per warp range, to every CTA.
-  auto sum_pass = [&](bool fast) {
-    const float next = above_tau(fast);
-    unsigned long long s;
-    float err = 0.f;
-    if (fast) {
-      const FastSum f = fast_sum<Raw>(vals, v0, v1, sh.row.fc, sh.row.fm, next);
-      s = f.s;
-      err = warp_sum(f.err);
-    } else {
-      s = exact_sum<Raw>(vals, v0, v1, next, sh.row.xmax, sh.row.k1, sh.exp2_table);
-    }
-    s = warp_add(s);
+  // Weight within [from, upto] and tokens at tau per warp range, to every CTA;
+  // `both`: and the weight above upto.
+  auto sum_pass = [&](float from, float upto, bool both) {
+    const ExactSum e = both ? exact_sum<Raw, true>(vals, v0, v1, from, upto, sh.row.xmax, sh.row.k1, sh.exp2_table)
+                            : exact_sum<Raw, false>(vals, v0, v1, from, upto, sh.row.xmax, sh.row.k1, sh.exp2_table);
+    const unsigned long long s = warp_add(e.s), high = both ? warp_add(e.high) : 0ull;
     const uint32_t ties = quota > 0 ? __reduce_add_sync(0xffffffffu, count_equal<Raw>(vals, v0, v1, tau)) : 0u;
     if (lane < cs) {
       const int i = rank * SMP_WARPS + warp;
       cluster.map_shared_rank(sh.wsum, lane)[i] = s;
       cluster.map_shared_rank(sh.wties, lane)[i] = ties;
-      cluster.map_shared_rank(sh.werr, lane)[i] = err;
+      if (both) cluster.map_shared_rank(sh.whigh, lane)[i] = high;
     }
     cluster.sync();
   };
-  if (k_of > 0) {
-    const Selected r = select<Raw, false>(sh, vals, v0, v1, K::kNegInf + 1, sh.row.kmax, 0, (unsigned long long)k_of, -1.0);
+  float split = INFINITY;  // whigh holds the ranges' weight above it
+  if (k_of > 0 && tau == kNone) {  // too many at or above the bound, or fewer tokens than k
+    const Selected r =
+        select<Raw, false>(sh, vals, v0, v1, K::kNegInf + 1, sh.row.kmax, 0, (unsigned long long)k_of);
     if (r.ok) {
       tau = K::value(r.key);
       quota = (uint32_t)(k_of - r.above);
     }
   }
-  double kept_bound = k_of > 0 ? k_of : V;  // at most so many tokens are kept
   if (use_p) {
+    // all weights; of a row whose cut is known to lie within keys, apart from those above them
+    if (nucleus && nu.lo <= nu.hi) split = K::value(nu.hi);
+    sum_pass(above_of(tau), split, true);
+    unsigned long long s = 0, above = 0;
+    uint32_t ties = 0;
+    for (int i = lane; i < ranges; i += 32) {
+      s += sh.wsum[i];
+      above += sh.whigh[i];
+      ties += sh.wties[i];
+    }
+    above = warp_add(above);
+    const unsigned long long total =
+        warp_add(s) + above +
+        (quota > 0 ? (unsigned long long)min(__reduce_add_sync(0xffffffffu, ties), quota) * weight_of(sh, tau) : 0ull);
+    // predecessors' mass below top_p of all; the first token is always kept
+    const unsigned long long goal = (unsigned long long)fmax(1.0, ceil(sh.row.top_p * (double)total));
     const uint32_t floor_key = max(K::of(fmaxf(fmaxf(tau, SMP_LOWEST), sh.row.zero)), K::kNegInf + 1);
-    // pass 0: from the approximate masses, if they leave one answer; 1: from
-    // exact ones, within the same keys; 2: over all keys
-    for (int pass = !nucleus ? 2 : (sh.redo ? 1 : 0); pass < 3; ++pass) {
-      const float tau0 = tau;
-      const uint32_t quota0 = quota;
-      unsigned long long above = 0, goal = 0;
-      double below = -1.0, e = 0.0;
-      uint32_t lo = floor_key, hi = sh.row.kmax;
-      if (pass < 2) {
-        lo = max(lo, nu.lo);
-        hi = nu.hi;
-      }
-      if (pass == 0) {
-        above = (unsigned long long)(nu.above * sh.row.shift * SMP_ONE);
-        below = nu.below * sh.row.shift * SMP_ONE;
-        // of top_p (above + between + below) - above, and a unit's rounding
-        e = ((1.0 - sh.row.top_p) * nu.err_above + sh.row.top_p * nu.err_below) * sh.row.shift * SMP_ONE + 2.0;
-      } else {
-        for (int part = pass == 1 ? 0 : 1; part < 2; ++part) {  // above the keys; all
-          if (part == 0) {
-            tau = K::value(hi);
-            quota = 0;
-          }
-          sum_pass(false);
-          if (warp == 0) {
-            const Found f = find_entry(sh.wsum, sh.wties, ranges, quota, quota > 0 ? weight_of(sh, tau) : 0ull, 0.0);
-            if (lane == 0) sh.total = f.total;
-          }
-          __syncthreads();
-          if (part == 0) above = sh.total;
-          else goal = (unsigned long long)fmax(1.0, ceil(sh.row.top_p * (double)sh.total));
-          tau = tau0;
-          quota = quota0;
-          cluster.sync();  // every CTA has read its sums
+    Selected r{false, 0, 0, 0};
+    bool found = false;
+    if (split != INFINITY && nu.inside <= SMP_FEW) {
+      const uint32_t n = collect_all<Raw>(sh, vals, v0, v1, token0, K::value(max(floor_key, nu.lo)), split);
+      if (n <= SMP_FEW) {
+        if (rank == 0) cut_in_list<Raw>(sh, cs, n, above, goal);
+        cluster.sync();
+        if (sh.found_count > 0) {
+          found = true;
+          tau = K::value(sh.found_bin);
+          quota = sh.found_count;
         }
       }
-      // predecessors' mass below top_p of all; the first token is always kept
-      const Selected r = select<Raw, true>(sh, vals, v0, v1, lo, hi, above, goal, below);
-      if (!r.ok) {
-        if (pass < 2) continue;
-        break;  // everything with weight is kept
-      }
+    } else if (split != INFINITY) {
+      r = select<Raw, true>(sh, vals, v0, v1, max(floor_key, nu.lo), nu.hi, above, goal);
+    }
+    if (!found && !r.ok) {
+      split = INFINITY;
+      r = select<Raw, true>(sh, vals, v0, v1, floor_key, sh.row.kmax, 0, goal);
+    }
+    if (r.ok) {  // else everything with weight is kept
       const unsigned long long w = weight_of(sh, K::value(r.key));
-      const unsigned long long n = (r.goal - r.above + w - 1) / w;
-      if (pass == 0) {
-        const double first = ceil(((double)r.goal - e - (double)r.above) / (double)w);
-        const double last = ceil(((double)r.goal + e - (double)r.above) / (double)w);
-        if (!(first == (double)n && last == (double)n && n <= r.count)) continue;  // too near a border
-      }
       tau = K::value(r.key);
-      quota = (uint32_t)min(n, (unsigned long long)r.count);
-      kept_bound = (double)r.goal / (double)w;
-      break;
+      quota = (uint32_t)min((goal - r.above + w - 1) / w, (unsigned long long)r.count);
     }
   }
   if (use_m) {
@@ -1105,114 +1111,78 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
     if (below >= tau) {
       tau = below;
       quota = 0;
+      if (tau >= split) split = INFINITY;
     }
   }
 
   // ---- draw: the range in which the running sum passes u * S, then, by its
   // warp, the lane and the token
-  for (int pass = fast_ok && kept_bound > 4096.0 ? 0 : 1; pass < 2; ++pass) {
-    const bool fast = pass == 0;
-    const float one = fast ? (float)SMP_FAST_ONE : (float)SMP_ONE;
-    const unsigned long long wtau =
-        quota == 0 ? 0ull
-                   : (fast ? __float2ull_rn(ex2_approx(fmaf(tau, sh.row.fc, sh.row.fm)) * one) : weight_of(sh, tau));
-    sum_pass(fast);
-    if (warp == 0) {
-      const Found f = find_entry(sh.wsum, sh.wties, ranges, quota, wtau, sh.row.u);
-      if (f.entry >= 0) {
-        sh.at_range = f.entry;
-        sh.at_target = f.t;
-        sh.at_ties = f.quota;
-        sh.total = f.total;
-      }
+  const float from = above_of(tau);
+  const unsigned long long wtau = quota > 0 ? weight_of(sh, tau) : 0ull;
+  sum_pass(from, split, false);
+  if (warp == 0) {
+    if (split != INFINITY) {
+      for (int i = lane; i < ranges; i += 32) sh.wsum[i] += sh.whigh[i];
+      __syncwarp();
     }
-    __syncthreads();
-    if (sh.at_range == rank * SMP_WARPS + warp) {
-      unsigned long long t = sh.at_target;
-      uint32_t left = sh.at_ties;
-      const float from = above_tau(fast);
-      for (int vb = v0; vb < v1; vb += 32) {
-        const int v = vb + lane;
-        const uint4 q = v < v1 ? vals[v] : make_uint4(K::kFill, K::kFill, K::kFill, K::kFill);
-        float wf[PV], err = 0.f, x[PV];
-        unsigned long long s = 0;
-        uint32_t ties = 0;
-        K::unpack(q, x);
-        if (fast) {
-          s = __float2ull_rn(fast_vector<Raw>(q, sh.row.fc, sh.row.fm, from, wf, err) * one);
-        } else {
-#pragma unroll
-          for (int i = 0; i < PV; ++i) s += weight_from(x[i], from, sh.row.xmax, sh.row.k1, sh.exp2_table);
-        }
-        uint32_t mine = 0, after = 0;  // ties this lane may keep; left after this step
-        if (quota > 0) {
-#pragma unroll
-          for (int i = 0; i < PV; ++i) ties += x[i] == tau;
-          const uint32_t tinc = warp_inclusive(ties, lane);
-          mine = left > tinc - ties ? left - (tinc - ties) : 0;
-          const uint32_t all = __shfl_sync(0xffffffffu, tinc, 31);
-          after = left > all ? left - all : 0;
-          s += (unsigned long long)min(mine, ties) * wtau;
-        }
-        const unsigned long long inc = warp_inclusive(s, lane);
-        const unsigned long long all = __shfl_sync(0xffffffffu, inc, 31);
-        if (t < all) {
-          // how far an approximate running sum less u * S may be from the
-          // exact one: (1 - u) times the error before, u times the error
-          // after (the ties' weights: within 5e-6 of themselves and half a
-          // unit; the vector's own sum: 2^-20)
-          double margin = 0.0;
-          if (fast) {
-            float e0 = 0.f, e1 = 0.f;
-            for (int i = lane; i < ranges; i += 32) {
-              e0 += i <= sh.at_range ? sh.werr[i] : 0.f;
-              e1 += i >= sh.at_range ? sh.werr[i] : 0.f;
-            }
-            const double uc = fmin(fmax(sh.row.u, 0.0), 1.0);
-            margin = ((1.0 - uc) * (double)warp_sum(e0) + uc * (double)warp_sum(e1)) * (1.01 / 4194304.0 * SMP_FAST_ONE) +
-                     nvec + (double)quota * (5e-6 * (double)wtau + 1.0) + 2.0 + (double)s * 9.5367431640625e-7;
-          }
-          if (inc - s <= t && t < inc) {
-            unsigned long long run = inc - s, w_at = 0;
-            int at = -1;
-            float x_at = 0.f;
-#pragma unroll
-            for (int i = 0; i < PV; ++i) {
-              if (at < 0) {
-                unsigned long long w = 0;
-                if (x[i] >= from)
-                  w = fast ? __float2ull_rn(wf[i] * one) : exact_weight(x[i], sh.row.xmax, sh.row.k1, sh.exp2_table);
-                else if (mine > 0 && x[i] == tau) {
-                  w = wtau;
-                  --mine;
-                }
-                if (t < run + w) {
-                  at = i;
-                  x_at = x[i];
-                  w_at = w;
-                } else {
-                  run += w;
-                }
-              }
-            }
-            if (!fast || (at >= 0 && (double)(t - run) > margin && (double)(run + w_at - t) > margin)) {
-              p.out[row] = token0 + v * PV + at;
-              if (p.logprob)
-                p.logprob[row] =
-                    log_share(sh.row, x_at, (double)sh.total / (double)one * (fast ? sh.row.shift : 1.0));
-            } else {
-              for (int c = 0; c < cs; ++c) *cluster.map_shared_rank(&sh.redo, c) = 2;
-            }
-          }
-          break;
-        }
-        t -= all;
-        left = after;
-      }
+    const Found f = find_entry(sh.wsum, sh.wties, ranges, quota, wtau, sh.row.u);
+    if (f.entry >= 0) {
+      sh.at_range = f.entry;
+      sh.at_target = f.t;
+      sh.at_ties = f.quota;
+      sh.total = f.total;
     }
-    if (!fast) return;
-    cluster.sync();
-    if (sh.redo != 2) return;
+  }
+  __syncthreads();
+  if (sh.at_range != rank * SMP_WARPS + warp) return;
+  unsigned long long t = sh.at_target;
+  uint32_t left = sh.at_ties;
+  for (int vb = v0; vb < v1; vb += 32) {
+    const int v = vb + lane;
+    const uint4 q = v < v1 ? vals[v] : make_uint4(K::kFill, K::kFill, K::kFill, K::kFill);
+    float x[PV];
+    unsigned long long s = 0;
+    uint32_t ties = 0, mine = 0;  // ties, and how many of them this lane may keep
+    K::unpack(q, x);
+#pragma unroll
+    for (int i = 0; i < PV; ++i) s += weight_from(x[i], from, sh.row.xmax, sh.row.k1, sh.exp2_table);
+    if (quota > 0) {
+#pragma unroll
+      for (int i = 0; i < PV; ++i) ties += x[i] == tau;
+      const uint32_t tinc = warp_inclusive(ties, lane);
+      mine = left > tinc - ties ? left - (tinc - ties) : 0;
+      const uint32_t all = __shfl_sync(0xffffffffu, tinc, 31);
+      left = left > all ? left - all : 0;
+      s += (unsigned long long)min(mine, ties) * wtau;
+    }
+    const unsigned long long inc = warp_inclusive(s, lane);
+    const unsigned long long all = __shfl_sync(0xffffffffu, inc, 31);
+    if (t < all) {
+      if (inc - s <= t && t < inc) {
+        unsigned long long run = inc - s;
+        int at = -1;
+        float x_at = 0.f;
+#pragma unroll
+        for (int i = 0; i < PV; ++i) {
+          if (at < 0) {
+            unsigned long long w = weight_from(x[i], from, sh.row.xmax, sh.row.k1, sh.exp2_table);
+            if (mine > 0 && x[i] == tau) {
+              w = wtau;
+              --mine;
+            }
+            if (t < run + w) {
+              at = i;
+              x_at = x[i];
+            }
+            run += w;
+          }
+        }
+        p.out[row] = token0 + v * PV + at;
+        if (p.logprob) p.logprob[row] = log_share(sh.row, x_at, (double)sh.total / SMP_ONE);
+      }
+      return;
+    }
+    t -= all;
   }
 }
 
