@@ -73,14 +73,21 @@ __global__ void __launch_bounds__(128, 2)
 
   // which rows and which adapter: the same for every CTA of the cluster
   const int planes = lo.tile_ptr[lo.tiles];
-  if (plane >= planes) return;
+  if (plane >= planes) {
+    pdl_wait();  // with no plane at all, this grid's end must still mean the previous one's
+    return;
+  }
   const int t = lo.plane_tile[plane], adapter = lo.plane_adapter[plane];
   const int m0 = t * lo.tile_rows + blockIdx.y * LOW_BM;
   if (planes > lo.max_planes || t < 0 || t >= lo.tiles || adapter < 0 || adapter >= lo.adapters) {
     if (tid == 0) record_error(err, kErrBadIndex);
+    pdl_wait();
     return;
   }
-  if (m0 >= M) return;
+  if (m0 >= M) {
+    pdl_wait();
+    return;
+  }
   const int rows = min(LOW_BM, M - m0), slot = plane - lo.tile_ptr[t];
   const bool mine = tid < rows && lo.row_slot[m0 + tid] == slot;
   bf16* low = lo.low + ((size_t)plane * 2 * lo.tile_rows + blockIdx.y * LOW_BM) * lo.rank;
@@ -428,6 +435,17 @@ __global__ void __launch_bounds__(192, 2)
   if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);
 }
 
+// A load that stays behind pdl_wait(): one through a __restrict__ pointer to
+// const may be moved above it, since nothing in the kernel writes there.
+__device__ __forceinline__ uint4 ld_after_wait(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // Few rows (decode): dot products, `ks` warps of a CTA to each (row, rank),
 // every warp with its share of the adapter's row in registers before the wait
 // for x.  No shared tiles, so these CTAs fit beside the product's, which are
@@ -435,7 +453,7 @@ __global__ void __launch_bounds__(192, 2)
 // value: 2-3 us, against 5-6 for the tensor-core kernel's chain (tiles, TMEM,
 // partials, cluster).  A is read once per row here, from L2 where rows share it.
 constexpr int ROWS_VEC = 8;  // 16-byte vectors a lane holds: 2048 elements of K a warp
-__global__ void __launch_bounds__(256, 2) lora_low_rows_kernel(const bf16* __restrict__ x, int64_t ldx, int M, int K,
+__global__ void __launch_bounds__(256, 2) lora_low_rows_kernel(const bf16* x, int64_t ldx, int M, int K,
                                                                const __grid_constant__ LLLora lo, int ks, int* err) {
   __shared__ float parts[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -446,6 +464,7 @@ __global__ void __launch_bounds__(256, 2) lora_low_rows_kernel(const bf16* __res
   const int p0 = lo.tile_ptr[t], np = lo.tile_ptr[t + 1] - p0, slot = lo.row_slot[m];
   if (p0 < 0 || np < 0 || p0 + np > lo.max_planes || slot >= np) {
     if (threadIdx.x == 0) record_error(err, kErrBadIndex);
+    pdl_wait();
     return;
   }
   int a = slot >= 0 ? lo.plane_adapter[p0 + slot] : -1;
@@ -471,7 +490,7 @@ __global__ void __launch_bounds__(256, 2) lora_low_rows_kernel(const bf16* __res
 #pragma unroll
       for (int i = 0; i < ROWS_VEC; ++i) {
         const int j = b + lane + 32 * i;
-        xv[i] = j < v1 ? xr[j] : make_uint4(0, 0, 0, 0);
+        xv[i] = j < v1 ? ld_after_wait(xr + j) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < ROWS_VEC; ++i) {

@@ -227,6 +227,40 @@ def test_captured_and_replayed_with_other_adapters(M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["mixed", "none"])
+@pytest.mark.parametrize("M,R", [(1, 16), (4, 16), (100, 64), (128, 256), (300, 16)])
+def test_a_chain_of_products_in_a_graph(M, R, rows):
+    """Each reads what the one before wrote, with no host between them: a
+    kernel that looks at its rows before they are there shows here."""
+    H, inter, n = 1024, 2048, 3
+    up = make(M, H, 2 * inter, R, n, rows, seed=M, device="cuda")
+    down = make(M, inter, H, R, n, rows, seed=M + 1, device="cuda")
+    su, sd = (ops.LoraStack(t["a"], t["b"], t["scale"]) for t in (up, down))
+    plan = ops.lora_plan(up["ids"], "cuda")
+
+    def chain(wait):
+        x, outs = up["x"], []
+        for _ in range(4):
+            m = ops.linear_lora(x, up["w"], up["bias"], su, plan, swiglu_epilogue=True)
+            wait()
+            x = ops.linear_lora(m, down["w"], down["bias"], sd, plan)
+            x = (x / x.float().norm(dim=1, keepdim=True) * H ** 0.5).to(BF)
+            wait()
+            outs += [m, x]
+        return outs
+
+    want = chain(torch.cuda.synchronize)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(lambda: None)
+    for _ in range(5):
+        for t in got:
+            t.fill_(float("nan"))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_two_streams_share_a_stack_and_a_plan():
     t = make(16, 3584, 4608, 16, 5, "mixed", seed=5, device="cuda")
     stack, plan = ops.LoraStack(t["a"], t["b"], t["scale"]), ops.lora_plan(t["ids"], "cuda")
