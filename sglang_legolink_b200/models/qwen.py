@@ -45,6 +45,7 @@ class ForwardBatch:
     logit_rows: Optional[torch.Tensor] = None  # [R] int64 rows whose logits are returned
     tiles: Optional[torch.Tensor] = None  # prefill attention work list
     tiles_nsplit: int = 1  # its key-range split count (ops.tiles_split_count)
+    lora: Optional["ops.LoraPlan"] = None  # the rows' adapters (QwenModel.add_adapter); None: no row has one
     decode_nsplit: Optional[int] = None
     # grouped execution rows of one extend forward (row-wise repair compute):
     # {"batch_execution_unit_size": n, "repair_ranges": [{"start", "end"}], ...}
@@ -83,6 +84,9 @@ class QwenModel:
         self.lm_head: Optional[torch.Tensor] = None
         self.cos_sin: Optional[torch.Tensor] = None
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
+        self.adapter_names: list[str] = []  # adapter i of a batch's plan
+        self._adapters: list = []
+        self._layer_adapters: list = []
         self._bufs: dict = {}
         self.buf_generation = 0  # bumped whenever a scratch buffer is replaced by a larger one
 
@@ -221,6 +225,35 @@ class QwenModel:
     def save_pretrained(self, path: str, state: dict) -> None:
         save_safetensors_checkpoint(path, self.cfg, state)
 
+    # ------------------------------------------------------------- adapters
+    def add_adapter(self, name: str, adapter) -> int:
+        """Adds a low-rank adapter (:class:`~.adapters.Adapter`); rows whose
+        plan (``ForwardBatch.lora``) names its index, the return value, run
+        with it.  The stacks of all adapters are rebuilt, so captured graphs
+        are dropped; a name is never given to other weights."""
+        from .adapters import LayerAdapters
+
+        if self.tp_size > 1:
+            raise ValueError("adapters are not supported with tensor parallelism")
+        if name in self.adapter_names:
+            raise ValueError(f"adapter '{name}' is loaded already")
+        bad = sorted({layer for layer, _ in adapter.mats if not 0 <= layer < self.cfg.num_layers})
+        if bad or not adapter.mats:
+            raise ValueError(f"adapter '{name}' names layers {bad} of a {self.cfg.num_layers}-layer model"
+                             if bad else f"adapter '{name}' has no matrices")
+        adapters = self._adapters + [adapter]
+        stacks = [LayerAdapters(self.cfg, adapters, i, self.device, self.dtype) for i in range(self.cfg.num_layers)]
+        self._adapters, self._layer_adapters = adapters, stacks
+        self.adapter_names = self.adapter_names + [name]
+        self.buf_generation += 1
+        return len(adapters) - 1
+
+    def _proj(self, x, w, bias, stack, fb: ForwardBatch, out, swiglu: bool = False):
+        """A projection of the generic forward, with the rows' adapters."""
+        if fb.lora is None or stack is None:
+            return ops.linear(x, w, bias, out=out, swiglu_epilogue=swiglu)
+        return ops.linear_lora(x, w, bias, stack, fb.lora, out=out, swiglu_epilogue=swiglu)
+
     # -------------------------------------------------------------- buffers
     def _buf(self, name, shape, dtype=None):
         dtype = dtype or self.dtype
@@ -246,7 +279,9 @@ class QwenModel:
         if (fb.mode == "extend" and getattr(self.comm, "name", "") == "fused" and fb.input_ids.is_cuda
                 and self.comm.use_fused(T)):
             return self._forward_fused_tp(fb, kv, return_hidden)
-        if fb.mode == "decode" and not return_hidden and self._decode_fusable(T):
+        # rows with adapters take the generic path: the fused decode epilogues
+        # write K/V and the residual before an adapter's term could join
+        if fb.mode == "decode" and not return_hidden and fb.lora is None and self._decode_fusable(T):
             return self._forward_decode_fused(fb, kv)
         if (fb.mode == "decode" and not return_hidden and getattr(self.comm, "name", "") == "fused"
                 and fb.input_ids.is_cuda and self.comm.decode_fusable(T)):
@@ -272,6 +307,8 @@ class QwenModel:
 
             rw_o = rowwise_slices(fb.repair_meta, T, "output_projection")
             rw_ffn = rowwise_slices(fb.repair_meta, T, "ffn")
+            if fb.lora is not None and (rw_o or rw_ffn):
+                raise ValueError("row-wise repair compute does not run rows with adapters")
         cap = self.capture if fb.mode == "extend" else None
         mk = self.markers
         cmp_attn = False
@@ -284,7 +321,8 @@ class QwenModel:
                 ops.fused_add_rmsnorm(h, residual, lw.in_norm, c.rms_norm_eps)
             if cap is not None and cap.wants(li):
                 cap.on_component(li, "pre_attention_norm", hidden=h, residual=residual)
-            ops.linear(h, lw.qkv_w, lw.qkv_b, out=qkv)
+            la = self._layer_adapters[li] if fb.lora is not None else None
+            self._proj(h, lw.qkv_w, lw.qkv_b, la and la.qkv, fb, qkv)
             ops.rope_qkv_write(qkv, fb.positions, fb.slots, self.cos_sin, q, kv.k[li], kv.v[li], self.hq, self.hkv,
                                D, lw.q_norm, lw.k_norm, c.rms_norm_eps)
             if cap is not None and cap.wants(li):
@@ -307,8 +345,11 @@ class QwenModel:
                             fb.repair_meta.setdefault("native_operator_comparisons", []).append(row)
                         emit_trace("repair_attention_compare", **row)
             # row-wise: each grouped row with the shapes it has alone
-            for sl in rw_o or (slice(None),):
-                self._row_parallel(attn[sl], lw.o_w, o[sl])
+            if la is not None:
+                self._proj(attn, lw.o_w, None, la.o, fb, o)
+            else:
+                for sl in rw_o or (slice(None),):
+                    self._row_parallel(attn[sl], lw.o_w, o[sl])
             if cap is not None and cap.wants(li):
                 cap.on_component(li, "attention", attention_output=attn)
                 cap.on_component(li, "output_projection", projected_output=o)
@@ -316,9 +357,13 @@ class QwenModel:
             if cap is not None and cap.wants(li):
                 cap.on_component(li, "post_attention_norm", hidden=o, residual=residual)
             with mk.region("FFN", li, hidden=o):
-                for sl in rw_ffn or (slice(None),):
-                    ops.linear(o[sl], lw.gu_w, out=mlp[sl], swiglu_epilogue=True)
-                    self._row_parallel(mlp[sl], lw.down_w, h[sl])
+                if la is not None:
+                    self._proj(o, lw.gu_w, None, la.gu, fb, mlp, swiglu=True)
+                    self._proj(mlp, lw.down_w, None, la.down, fb, h)
+                else:
+                    for sl in rw_ffn or (slice(None),):
+                        ops.linear(o[sl], lw.gu_w, out=mlp[sl], swiglu_epilogue=True)
+                        self._row_parallel(mlp[sl], lw.down_w, h[sl])
             if cap is not None:
                 if cap.wants(li):
                     cap.on_component(li, "mlp", mlp_output=h)

@@ -310,6 +310,7 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
         raise ValueError(f"the plan is for {plan.rows} rows, x has {M}")
     if plan.top_adapter >= lora.count:
         raise ValueError(f"the plan names adapter {plan.top_adapter}, the stack has {lora.count}")
+    plan.limit = min(plan.limit, lora.count)
     if M == 0 or not x.is_cuda:
         y = ref.linear_lora(x, w, bias, lora.a, lora.b, lora.scale, plan.row_adapters)
         y = (ref_swiglu_interleaved(y) if swiglu_epilogue else y).to(x.dtype)

@@ -63,6 +63,7 @@ class LoraPlan:
         self.tile_rows = 128 if self.rows <= 128 else 256
         self.tiles = -(-self.rows // self.tile_rows)
         self.device = torch.device(device)
+        self.limit = 1 << 31  # the smallest stack that the plan has been used with
         host, planes = self._build(ids)
         self.max_planes = max(1, planes if max_planes is None else int(max_planes))
         if planes > self.max_planes:
@@ -104,6 +105,8 @@ class LoraPlan:
         host, planes = self._build(ids)
         if planes > self.max_planes:
             raise ValueError(f"the rows need {planes} planes, the plan holds {self.max_planes}")
+        if ids.size and ids.max() >= self.limit:  # a captured call would read behind its stack
+            raise ValueError(f"adapter {int(ids.max())}: the plan was used with a stack of {self.limit}")
         self._store(ids, host)
         return self
 

@@ -38,7 +38,7 @@ from ..utils import launch_count
 from ..utils.trace import emit_trace, CudaTimer
 from .link_plan import ResolvedLinkPlan, resolve_link_plan
 from .repair_diagnostics import compare_enabled, compare_kv_link
-from .sampling import GREEDY, SamplingParams, make_generator, sample_rows
+from .sampling import GREEDY, SamplingParams, draw_rows, make_generator, sample_rows
 
 
 class RuntimeErrorAbort(RuntimeError):
@@ -78,6 +78,7 @@ class Sequence_:
     sampling: SamplingParams = GREEDY
     generator: Optional[torch.Generator] = None
     promotion: Optional[dict] = None  # record of an experimental group promotion
+    adapter: int = -1  # index of the model's adapter it runs with
 
 
 @dataclass
@@ -157,7 +158,12 @@ class Engine:
                  mem_fraction: float = 0.85, max_blocks: Optional[int] = None, max_context: int = 32768,
                  use_cuda_graphs: bool = True, residency: Optional[int] = None, legolink_only: bool = False,
                  compat_overrides: Optional[dict] = None, kv_pool: Optional[KVPool] = None,
-                 directory=None, replica_rank: int = 0, peer_pools: Optional[dict] = None):
+                 directory=None, replica_rank: int = 0, peer_pools: Optional[dict] = None,
+                 sampler: str = "torch"):
+        if sampler not in ("torch", "kernel"):
+            raise ValueError("sampler must be 'torch' (per-row torch ops) or 'kernel' (one launch a batch)")
+        self.sampler = sampler
+        self._adapter_labels: set = set()  # adapter ids that blocks were compiled under without an adapter
         self.model = model
         self.cfg = model.cfg
         self.device = model.device
@@ -251,6 +257,36 @@ class Engine:
         c["legolink_policy_version"] = str(legolink_policy_version or LEGOLINK_POLICY_VERSION)
         return "|".join(f"{k}={c[k]}" for k in sorted(c))
 
+    # -------------------------------------------------------------- adapters
+    def load_adapter(self, name: str, source) -> None:
+        """Loads a low-rank adapter: a PEFT checkpoint directory or a
+        :class:`~sglang_legolink_b200.models.adapters.Adapter`.  From then on
+        a Compile, Link or plain request whose ``adapter_id`` is ``name`` runs
+        with it (an id that names no loaded adapter stays what it was: part of
+        the blocks' compatibility key).  A name keeps its weights for the
+        engine's life, since registered blocks hold K/V computed with them."""
+        from ..models.adapters import Adapter
+
+        with self._lock:
+            if str(name) in self._adapter_labels:
+                raise ValueError(f"blocks were compiled under adapter_id '{name}' without an adapter")
+            self.model.add_adapter(str(name), source if isinstance(source, Adapter) else Adapter.from_pretrained(source))
+
+    @property
+    def adapters(self) -> list[str]:
+        return list(self.model.adapter_names)
+
+    def _adapter(self, adapter_id) -> int:
+        names = self.model.adapter_names
+        return names.index(str(adapter_id)) if adapter_id is not None and str(adapter_id) in names else -1
+
+    def _rows_plan(self, adapters: Sequence[int], counts: Sequence[int], max_planes: Optional[int] = None):
+        """Plan of a batch's rows (``counts[i]`` rows of adapter
+        ``adapters[i]``); None when no row has one."""
+        if all(a < 0 for a in adapters):
+            return None
+        return ops.lora_plan(np.repeat(np.asarray(adapters, dtype=np.int64), counts), self.device, max_planes)
+
     def next_rid(self, prefix="req") -> str:
         self._rid += 1
         return f"{prefix}-{self._rid}"
@@ -319,8 +355,9 @@ class Engine:
 
     # ----------------------------------------------------------- batch build
     def _extend_batch(self, items: list[tuple[list[int], list[int], list[int], int]],
-                      logits_last_only=True) -> ForwardBatch:
-        """items: (token_ids_of_rows, positions_of_rows, pages, kv_len).
+                      logits_last_only=True, adapters: Optional[Sequence[int]] = None) -> ForwardBatch:
+        """items: (token_ids_of_rows, positions_of_rows, pages, kv_len);
+        ``adapters``: each item's adapter index (-1: none).
         The batch's int32 arrays travel in one host->device copy and its
         int64 arrays in another (numpy on the host, views on the device)."""
         ps = self.page_size
@@ -376,6 +413,7 @@ class Engine:
             logit_rows=d64[off64:],
             tiles=view[5].view(-1, 4) if self.is_cuda else None,
             tiles_nsplit=tiles_nsplit,
+            lora=self._rows_plan(adapters, counts) if adapters is not None else None,
         )
 
     def _kernel_check(self, what: str) -> None:
@@ -402,14 +440,28 @@ class Engine:
         if not any(not p.greedy for p in params):
             return ids
         full = self.model.full_logits(logits[: len(params)])
+        if self.sampler == "kernel":
+            copy = (lambda a: _pinned_copy(a, self.device)) if self.is_cuda else torch.from_numpy
+            drawn = draw_rows(full, list(params), list(gens) or None, copy)
+            if any(p.greedy for p in params):  # these keep the argmax kernel's token
+                greedy_rows = copy(np.asarray([p.greedy for p in params]))
+                drawn = torch.where(greedy_rows, ids[: len(params)].to(drawn.dtype), drawn)
+            return drawn
         drawn = sample_rows(full, list(params), list(gens) or None)
         ids = ids.clone()
         ids[: len(params)] = drawn.to(ids.device)
         return ids
 
+    def _tokens(self, ids: torch.Tensor) -> list[int]:
+        """Sampled ids on the host; a sampled row with nothing to draw is an error."""
+        out = ids.tolist()
+        if self.sampler == "kernel" and min(out, default=0) < 0:
+            raise KernelFault("sampling: a row of logits holds no number above -inf")
+        return out
+
     def _new_sampling(self, sampling: Optional[SamplingParams]):
         sp = sampling or GREEDY
-        return sp, make_generator(sp, self.device)
+        return sp, make_generator(sp, "cpu" if self.sampler == "kernel" else self.device)
 
     # --------------------------------------------------------------- compile
     def compile(self, token_ids: Sequence[int], cache_key: str, *, sub_context: Optional[dict] = None,
@@ -457,6 +509,8 @@ class Engine:
             raise ContractError("Compile requires a non-empty sub-context.")
         ckey = self.compat_key(sc.get("adapter_id"), sc.get("segmentation_policy_version"),
                                sc.get("legolink_policy_version"))
+        if sc.get("adapter_id") is not None and self._adapter(sc["adapter_id"]) < 0:
+            self._adapter_labels.add(str(sc["adapter_id"]))
         return toks, ckey, str(block_id or sc.get("semantic_block_id") or cache_key)
 
     def _clone_pages(self, pages: list[int]) -> list[int]:
@@ -714,8 +768,10 @@ class Engine:
                 if works:
                     with timer.span("kv_link"):
                         self._run_kv_links([w for _, w in works], timer)
-                items, params, gens = [], [], []
-                for _, toks, _, _, _, pages in prepared:
+                items, params, gens, adapters = [], [], [], []
+                for i, toks, _, _, _, pages in prepared:
+                    sc = compiles[i][2] if len(compiles[i]) > 2 else None
+                    adapters.append(self._adapter((sc or {}).get("adapter_id")))
                     items.append((toks, list(range(len(toks))), pages, len(toks)))
                     params.append(GREEDY)
                     gens.append(None)
@@ -725,8 +781,9 @@ class Engine:
                                   w.resolved.total_token_count))
                     params.append(w.sampling)
                     gens.append(w.generator)
+                    adapters.append(self._adapter(w.plan.get("adapter_id")))
                 with timer.span("sparse_repair"):
-                    fb = self._extend_batch(items)
+                    fb = self._extend_batch(items, adapters=adapters)
                     if len(prepared) > 1 and not works:  # grouped execution rows (row-wise compute when enabled)
                         o, ranges = 0, []
                         for _, toks, *_ in prepared:
@@ -734,7 +791,7 @@ class Engine:
                             o += len(toks)
                         fb.repair_meta = {"batch_execution_unit_size": len(prepared), "repair_ranges": ranges}
                     logits = self.model.forward(fb, self.kv)
-                    firsts = self._sample(logits, params, gens).tolist()
+                    firsts = self._tokens(self._sample(logits, params, gens))
                 self._kernel_check("link" if works else "compile")
             except Exception as e:
                 for i, *_rest, pages in prepared:
@@ -761,7 +818,8 @@ class Engine:
                 self._link_close(w, ok=True)
                 seq = Sequence_(rid=w.rid, token_ids=list(w.resolved.linked_token_ids), pages=w.pages,
                                 length=w.resolved.total_token_count, output_ids=[int(first)], kind="link",
-                                link_plan=w.resolved, sampling=w.sampling, generator=w.generator)
+                                link_plan=w.resolved, sampling=w.sampling, generator=w.generator,
+                                adapter=self._adapter(w.plan.get("adapter_id")))
                 emit_trace("model_link_complete", rid=w.rid, total_token_count=w.resolved.total_token_count,
                            recompute_rows=len(w.resolved.recompute_positions), linked_rows=w.linked_rows,
                            batch_links=len(works))
@@ -899,9 +957,16 @@ class Engine:
 
     # --------------------------------------------------------------- prefill
     def prefill(self, token_ids: Sequence[int], *, rid: Optional[str] = None, namespace: Optional[str] = None,
-                use_prefix_cache: bool = False, sampling: Optional[SamplingParams] = None) -> Sequence_:
-        """Full prefill of a plain prompt (the baseline of a Link)."""
+                use_prefix_cache: bool = False, sampling: Optional[SamplingParams] = None,
+                adapter: Optional[str] = None) -> Sequence_:
+        """Full prefill of a plain prompt (the baseline of a Link), with a
+        loaded ``adapter``'s weights if one is named."""
         with self._lock:
+            ad = self._adapter(adapter)
+            if adapter is not None and ad < 0:
+                raise ValueError(f"adapter '{adapter}' is not loaded")
+            if adapter is not None:  # its K/V is its own
+                namespace = f"{namespace or ''}\0adapter={adapter}"
             toks = [int(t) for t in token_ids]
             n = len(toks)
             rid = rid or self.next_rid("prefill")
@@ -922,9 +987,9 @@ class Engine:
                 raise
             try:
                 sp, gen = self._new_sampling(sampling)
-                fb = self._extend_batch([(toks[start:], list(range(start, n)), pages, n)])
+                fb = self._extend_batch([(toks[start:], list(range(start, n)), pages, n)], adapters=[ad])
                 logits = self.model.forward(fb, self.kv)
-                first = int(self._sample(logits, [sp], [gen])[0].item())
+                first = self._tokens(self._sample(logits, [sp], [gen])[:1])[0]
                 self._kernel_check("prefill")
             except Exception:
                 self.alloc.release(pages)
@@ -933,7 +998,7 @@ class Engine:
                 self.radix.insert(namespace or "", toks, pages)
             self.stats["prefills"] += 1
             return Sequence_(rid=rid, token_ids=toks, pages=pages, length=n, output_ids=[first], kind="plain",
-                             sampling=sp, generator=gen)
+                             sampling=sp, generator=gen, adapter=ad)
 
     # ---------------------------------------------------------------- decode
     def decode(self, seqs: list[Sequence_], steps: int, stop_ids: Sequence[int] = ()) -> None:
@@ -1080,9 +1145,9 @@ class Engine:
         dev = self.device
         fb = ForwardBatch(mode="decode", input_ids=ids.to(dev), positions=pos.to(dev), slots=slots.to(dev),
                           q_indptr=torch.arange(B + 1, dtype=torch.int32).to(dev), page_table=pt.to(dev),
-                          kv_lens=kvl.to(dev), logit_rows=None)
+                          kv_lens=kvl.to(dev), logit_rows=None, lora=self._rows_plan([s.adapter for s in seqs], 1))
         logits = self.model.forward(fb, self.kv)
-        out = self._sample(logits, [s.sampling for s in seqs], [s.generator for s in seqs]).tolist()
+        out = self._tokens(self._sample(logits, [s.sampling for s in seqs], [s.generator for s in seqs]))
         self._kernel_check("decode")
         return out
 
@@ -1106,32 +1171,40 @@ class Engine:
         g["graph"].replay()
         launch_count.add(g["launches"])
         if any(not s.sampling.greedy for s in seqs):
-            out = self._sample(g["logits"][:B], [s.sampling for s in seqs], [s.generator for s in seqs],
-                               greedy=g["out"][:B]).tolist()
+            out = self._tokens(self._sample(g["logits"][:B], [s.sampling for s in seqs], [s.generator for s in seqs],
+                                            greedy=g["out"][:B]))
         else:
             out = g["out"][:B].tolist()
         self._kernel_check("decode")
         return out
 
     def _graph(self, bucket: int, max_pages: int, seqs) -> dict:
-        """The decode graph of ``bucket`` rows, captured on first use.  The
-        graphs point into the model's scratch buffers; when a larger forward
+        """The decode graph of ``bucket`` rows, captured on first use; rows
+        with adapters have one of their own, whose plan is set to ``seqs``
+        here.  The graphs point into the model's scratch buffers; when a larger forward
         has since regrown one of them (the old memory is freed), every graph
         is dropped and captured again before it could replay."""
         gen = self.model.buf_generation
         if gen != self._graphs_gen:
             self._graphs.clear()
             self._graphs_gen = gen
-        g = self._graphs.get(bucket)
+        adapters = [s.adapter for s in seqs] + [-1] * (bucket - len(seqs))
+        lora = any(a >= 0 for a in adapters)
+        key = ("adapters", bucket) if lora else bucket
+        g = self._graphs.get(key)
         if g is None:
-            g = self._capture(bucket, max_pages, seqs)
+            g = self._capture(bucket, max_pages, seqs, self._rows_plan(adapters, 1, max_planes=bucket))
+            g["adapters"] = adapters
             if self.model.buf_generation != gen:  # the capture's warm-up regrew a buffer
                 self._graphs.clear()
-            self._graphs[bucket] = g
+            self._graphs[key] = g
             self._graphs_gen = self.model.buf_generation
+        elif lora and g["adapters"] != adapters:
+            g["fb"].lora.update(adapters)
+            g["adapters"] = adapters
         return g
 
-    def _capture(self, bucket: int, max_pages: int, seqs) -> dict:
+    def _capture(self, bucket: int, max_pages: int, seqs, lora=None) -> dict:
         dev = self.device
         ids, pos, slots, pt, kvl = self._decode_inputs(seqs, bucket, max_pages)
         st = {"ids": ids.to(dev), "pos": pos.to(dev), "slots": slots.to(dev), "pt": pt.to(dev),
@@ -1140,7 +1213,7 @@ class Engine:
         ops.workspace(dev).reserve_decode(bucket * self.model.hq, nsplit, self.cfg.head_dim)
         fb = ForwardBatch(mode="decode", input_ids=st["ids"], positions=st["pos"], slots=st["slots"],
                           q_indptr=torch.arange(bucket + 1, dtype=torch.int32, device=dev), page_table=st["pt"],
-                          kv_lens=st["kvl"], logit_rows=None, decode_nsplit=nsplit)
+                          kv_lens=st["kvl"], logit_rows=None, decode_nsplit=nsplit, lora=lora)
         out = torch.zeros(bucket, dtype=torch.int32, device=dev)
         # warm-up (allocates the model's scratch buffers outside the graph).
         # Row 0's writes land on the slot it is about to fill, so the real

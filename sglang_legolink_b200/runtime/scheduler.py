@@ -135,6 +135,7 @@ class Request:
     ttft_s: Optional[float] = None
     sampling: SamplingParams = GREEDY
     resume: Optional[list] = None  # tokens generated before a retraction (plain requests)
+    adapter: Optional[str] = None  # plain requests: the adapter to run with, if the engine has loaded it
 
 
 class Scheduler:
@@ -366,6 +367,9 @@ class Scheduler:
 
     def _admit(self, req: Request) -> None:
         eng = self.engine
+        # an adapter_id was ignored here before adapters could be loaded, and
+        # still is without one; beside loaded ones an unknown name is an error
+        adapter = {"adapter": req.adapter} if req.adapter is not None and getattr(eng, "adapters", ()) else {}
         try:
             if req.kind == "compile":
                 sc = req.sub_context or {}
@@ -384,10 +388,11 @@ class Scheduler:
                     eng.free(seq)
                     raise RequestRejected("overlength Link (total tokens + max_tokens exceeds the context window)")
             elif req.resume is not None:  # re-admitted after a retraction
-                seq = eng.prefill(list(req.input_ids) + list(req.resume), rid=req.rid, sampling=req.sampling)
+                seq = eng.prefill(list(req.input_ids) + list(req.resume), rid=req.rid, sampling=req.sampling,
+                                  **adapter)
                 seq.output_ids[:0] = req.resume
             else:
-                seq = eng.prefill(req.input_ids, rid=req.rid, sampling=req.sampling)
+                seq = eng.prefill(req.input_ids, rid=req.rid, sampling=req.sampling, **adapter)
             self._start(req, seq)
         except (ContractError, RuntimeErrorAbort, RequestRejected, ValueError, KeyError) as e:
             emit_trace("legolink_request_failed_closed", rid=req.rid, kind=req.kind, reason=str(e)[:500])

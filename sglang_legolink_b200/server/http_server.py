@@ -113,7 +113,9 @@ class RuntimeService:
             ids = list(p) if isinstance(p, list) else list(self.tokenizer.tokenize(str(p)))
         else:
             ids = _prompt_ids(self.tokenizer, payload)
-        return Request("plain", rid, ids, max_new, stop, sampling=sampling)
+        adapter = payload.get("adapter_id")
+        return Request("plain", rid, ids, max_new, stop, sampling=sampling,
+                       adapter=None if adapter is None else str(adapter))
 
     def complete(self, payload: dict) -> dict:
         req = self.build_request(payload)
@@ -281,7 +283,8 @@ def serve(svc: RuntimeService, host: str = "127.0.0.1", port: int = 30000) -> Th
 
 def build_service(model: str = "tiny-qwen2", *, device: str = "cpu", tokenizer: Optional[str] = None,
                   legolink_only: Optional[bool] = True, page_size: int = 16, num_pages: Optional[int] = None,
-                  max_context: int = 32768, seed: int = 0, layerwise_markers: bool = False) -> RuntimeService:
+                  max_context: int = 32768, seed: int = 0, layerwise_markers: bool = False,
+                  sampler: str = "torch", adapters=()) -> RuntimeService:
     import torch
 
     from ..host.tokenizer import HashTokenizer, HFTokenizer
@@ -299,10 +302,19 @@ def build_service(model: str = "tiny-qwen2", *, device: str = "cpu", tokenizer: 
 
         m.markers = LayerMarkers(True)
     tok = HFTokenizer(tokenizer) if tokenizer else HashTokenizer(m.cfg.vocab_size, name=m.cfg.name)
-    eng = Engine(m, page_size=page_size, num_pages=num_pages, max_context=max_context)
+    eng = Engine(m, page_size=page_size, num_pages=num_pages, max_context=max_context, sampler=sampler)
+    for name, path in adapters:
+        eng.load_adapter(name, path)
     sch = Scheduler(eng, legolink_only=legolink_only)
     sch.start()
     return RuntimeService(sch, tok, model_name=m.cfg.name)
+
+
+def adapter_arg(text: str) -> tuple[str, str]:
+    name, eq, path = text.partition("=")
+    if not (name and eq and path):
+        raise argparse.ArgumentTypeError(f"'{text}' is not NAME=PATH")
+    return name, path
 
 
 def main(argv=None) -> None:
@@ -327,7 +339,13 @@ def main(argv=None) -> None:
     ap.add_argument("--dp-base-port", type=int, default=0, help="replica r > 0 listens on this + r (default --port)")
     ap.add_argument("--dist-timeout", type=int, default=600, help="process-group timeout, seconds")
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--sampler", choices=("torch", "kernel"), default="torch",
+                    help="sampled rows: per-row torch ops, or one launch for the batch (other seeded draws)")
+    ap.add_argument("--adapter", action="append", default=[], type=adapter_arg, metavar="NAME=PATH",
+                    help="load a PEFT low-rank adapter; requests choose it with adapter_id (repeatable)")
     a = ap.parse_args(argv)
+    if a.adapter and a.tp_size > 1:
+        ap.error("--adapter is not supported with --tp-size")
     if a.tp_size > 1 or a.dp_size > 1 or a.pp_size != 1:
         from .launch import launch
 
@@ -335,7 +353,8 @@ def main(argv=None) -> None:
         return
     svc = build_service(a.model, device=a.device, tokenizer=a.tokenizer,
                         legolink_only=False if a.allow_plain_generation else None, page_size=a.page_size,
-                        max_context=a.context_length, layerwise_markers=a.enable_layerwise_nvtx_marker)
+                        max_context=a.context_length, layerwise_markers=a.enable_layerwise_nvtx_marker,
+                        sampler=a.sampler, adapters=a.adapter)
     if not a.skip_warmup and os.getenv("SGLANG_PIC_WARMUP", "1") != "0":
         print("warmup", svc.warmup(int(os.getenv("SGLANG_PIC_WARMUP_BLOCK_TOKENS", "256")),
                                    int(os.getenv("SGLANG_PIC_WARMUP_LEGOLINK_K", "16"))), flush=True)

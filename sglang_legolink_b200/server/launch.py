@@ -262,7 +262,9 @@ def _build_rank(a, rank: int, world: int, local: int, ctrl=None):
             pool = SharedKVPool(m.cfg.num_layers, pages, m.hkv, a.page_size, m.cfg.head_dim, dtype, dev)
             kw.update(kv_pool=pool, peer_pools={r: pool.peer(r) for r in range(world) if r != rank})
     eng = Engine(m, page_size=a.page_size, max_context=a.context_length,
-                 legolink_only=not a.allow_plain_generation, **kw)
+                 legolink_only=not a.allow_plain_generation, sampler=getattr(a, "sampler", "torch"), **kw)
+    for name, path in getattr(a, "adapter", ()):
+        eng.load_adapter(name, path)
     tok = HFTokenizer(a.tokenizer) if a.tokenizer else HashTokenizer(m.cfg.vocab_size, name=m.cfg.name)
     return eng, tok, m.cfg.name, directory
 
