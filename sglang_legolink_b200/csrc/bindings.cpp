@@ -362,7 +362,7 @@ void gemm_small_m_epi(const at::Tensor& a, const at::Tensor& w, const c10::optio
 at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
                        const c10::optional<at::Tensor>& out_, const at::Tensor& a, const at::Tensor& b,
                        const at::Tensor& scale, const at::Tensor& plan, int64_t tile_rows, int64_t max_planes,
-                       bool small_m, bool swiglu, const at::Tensor& err) {
+                       bool split_k, bool swiglu, const at::Tensor& err) {
   CHECK_CUDA(x); CHECK_BF16(x); CHECK_BF16(w); CHECK_BF16(a); CHECK_BF16(b); CHECK_F32(scale);
   CHECK_I32(plan); CHECK_I32(err); CHECK_CONTIG(w); CHECK_CONTIG(a); CHECK_CONTIG(b); CHECK_CONTIG(scale);
   CHECK_CONTIG(plan); CHECK_ALIGN16(x); CHECK_ALIGN16(w); CHECK_ALIGN16(a); CHECK_ALIGN16(b);
@@ -392,7 +392,6 @@ at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::opti
   TORCH_CHECK(tile_rows == (M <= 128 ? 128 : 256) && max_planes >= 1, "bad plan");
   TORCH_CHECK(plan.numel() == M + tiles + 1 + 2 * max_planes, "the plan is for another batch");
   TORCH_CHECK(max_planes <= 65535, "too many adapters per tile of rows");
-  TORCH_CHECK(!small_m || M <= 128, "the small-M kernel takes at most 128 rows");
   auto low = at::empty({max_planes * 2 * tile_rows, R}, x.options());
   LLLora lo{};
   lo.a = bp(a);
@@ -409,7 +408,7 @@ at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::opti
   lo.tile_rows = (int)tile_rows;
   lo.max_planes = (int)max_planes;
   check_rc(ll_lora_low(bp(x), x.stride(0), (int)M, (int)K, &lo, err.data_ptr<int>(), cur_stream()), "ll_lora_low");
-  if (small_m) {
+  if (split_k) {
     check_rc(ll_lora_gemv(bp(x), x.stride(0), bp(w), bp(out), out.stride(0), bp_opt(bias), (int)M, (int)N, (int)K,
                           swiglu ? 1 : 0, &lo, err.data_ptr<int>(), cur_stream()),
              "ll_lora_gemv");

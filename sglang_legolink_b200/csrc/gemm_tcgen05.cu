@@ -1351,6 +1351,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
 #pragma unroll 1
         for (int c = 0; c < BN; c += STEP) {
           const int col0 = nb * BN + c;
+          if (col0 >= N || row0w >= M) continue;  // warp-uniform: the box is wholly outside C
           uint32_t v[16];
           if constexpr (EPI == kEpiSwiGLU) {
 #pragma unroll
@@ -1361,7 +1362,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
               const int cb = col0 + 32 * hh;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                float g0 = __uint_as_float(r[2 * i]), g1 = __uint_as_float(r[2 * i + 1]);
+                // rows past M are zero, and the division of a zero takes a
+                // slow path that holds the whole warp up (362 rows, N = 12800,
+                // K = 344: 55 us, 27 without); they are clipped by the store
+                float g0 = row < M ? __uint_as_float(r[2 * i]) : 1.f;
+                float g1 = row < M ? __uint_as_float(r[2 * i + 1]) : 1.f;
                 float u0 = __uint_as_float(r[16 + 2 * i]), u1 = __uint_as_float(r[16 + 2 * i + 1]);
                 if (bias != nullptr && cb < N) {  // N % 32 == 0: a 32-column group is wholly in or out
                   g0 += __bfloat162float(bias[cb + 2 * i]);
@@ -1386,7 +1391,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
               v[i] = pack_bf16x2(a0, a1);
             }
           }
-          if (col0 >= N || row0w >= M) continue;  // warp-uniform: the box is wholly outside C
           uint8_t* box = boxes + (nbox & 1) * 2048;
           if (nbox >= 2 && lane == 0) bulk_wait_group_read1();
           __syncwarp();

@@ -25,7 +25,6 @@ constexpr int LOW_BM = 128;
 constexpr int LOW_BK = 64;
 constexpr int LOW_MAX_CLUSTER = 8;
 constexpr int LOW_RING = 96 * 1024;
-constexpr int64_t LOW_ROWS_BYTES = 24 << 20;
 
 struct LowShape {
   int npad;      // ranks rounded up to the MMA's multiple of 16
@@ -232,9 +231,10 @@ __global__ void __launch_bounds__(128, 2)
 }
 
 // ---------------------------------------------------------------------------
-// The product for up to 128 rows (decode): as the small-M GEMM, the weight
-// tile is the M = 128 side of the MMA and the rows are the N side, and K is
-// split so that every SM streams weights.  Here the splits of a feature tile
+// The product for up to 128 rows (decode), and for more where 128 x 128 tiles
+// leave SMs free: as the small-M GEMM, the weight tile is the M = 128 side of
+// the MMA and the rows (128 a CTA at most) are the N side, and K is split so
+// that every SM streams weights.  Here the splits of a feature tile
 // are a cluster: their fp32 partials stay in shared memory and each CTA sums,
 // in split order, and stores its share of the rows.  Nothing goes through
 // global memory and no CTA waits for a last one to add up 128 features x M
@@ -269,7 +269,7 @@ __device__ __forceinline__ float gemv_silu(float x) { return x / (1.0f + __expf(
 template <int BNX, bool SWIGLU>
 __global__ void __launch_bounds__(192, 2)
     lora_gemv_kernel(const __grid_constant__ GemvMaps tm, bf16* __restrict__ C, int64_t ldc,
-                     const bf16* __restrict__ bias, int M, int N, int K, const __grid_constant__ LLLora lo,
+                     const bf16* __restrict__ bias, int rows, int N, int K, const __grid_constant__ LLLora lo,
                      int* err) {
   using Cfg = GemvCfg<BNX>;
   constexpr int STAGES = Cfg::STAGES;
@@ -285,7 +285,10 @@ __global__ void __launch_bounds__(192, 2)
   const int cs = gridDim.x, crank = blockIdx.x, nb = blockIdx.y;
   const int num_kb = (K + LOW_BK - 1) / LOW_BK;
   const int rank_blocks = (lo.rank + LOW_BK - 1) / LOW_BK;
-  const int num_extra = min(lo.tile_ptr[1], lo.max_planes) * 2 * rank_blocks;
+  const int m0 = blockIdx.z * BNX, M = min(BNX, rows - m0);  // this CTA's rows
+  const int t = m0 / lo.tile_rows, p0 = max(0, lo.tile_ptr[t]);
+  const int num_extra = max(0, min(lo.tile_ptr[t + 1], lo.max_planes) - p0) * 2 * rank_blocks;
+  C += m0 * ldc;
   const int per = (num_kb + cs - 1) / cs, eper = (num_extra + cs - 1) / cs;
   const int kb0 = min(num_kb, crank * per), kb1 = min(num_kb, kb0 + per);
   const int e0 = min(num_extra, crank * eper), e1 = min(num_extra, e0 + eper);
@@ -328,14 +331,14 @@ __global__ void __launch_bounds__(192, 2)
         }
         if (kb < kb1) {
           if (i >= pre) tma_load_2d(sW + stage * Cfg::W_BYTES, &tm.w, &full[stage], kb * LOW_BK, nb * 128);
-          tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.x, &full[stage], kb * LOW_BK, 0);
+          tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.x, &full[stage], kb * LOW_BK, m0);
         } else {
           const int e = e0 + kb - kb1;
-          const int plane = (e >> 1) / rank_blocks, rb = (e >> 1) % rank_blocks;
+          const int plane = p0 + (e >> 1) / rank_blocks, rb = (e >> 1) % rank_blocks;
           tma_load_3d(sW + stage * Cfg::W_BYTES, &tm.b, &full[stage], rb * LOW_BK, nb * 128,
                       lo.plane_adapter[plane]);
           tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.low, &full[stage], rb * LOW_BK,
-                      (2 * plane + (e & 1)) * lo.tile_rows);
+                      (2 * plane + (e & 1)) * lo.tile_rows + m0 % lo.tile_rows);
         }
         if (++stage == STAGES) {
           stage = 0;
@@ -452,6 +455,12 @@ __device__ __forceinline__ uint4 ld_after_wait(const uint4* p) {
 // loading weights meanwhile; what counts is the time from x to the stored
 // value: 2-3 us, against 5-6 for the tensor-core kernel's chain (tiles, TMEM,
 // partials, cluster).  A is read once per row here, from L2 where rows share it.
+// Each (row, rank) is a CTA's share, two CTAs a SM: used up to one and a half
+// rounds of the 296 places, two where K is long.  us a call with this kernel /
+// the tensor cores': 64 rows, rank 32, K = 1024 (256 CTAs) 8.0 / 9.3; 64, 64,
+// 1024 (512) 9.9 / 9.4; 64, 32, 4096 (512) 12.4 / 12.8; 600, 16, 128 (1200)
+// 17.0 / 11.9; 2500, 16, 128 (5000) 42.7 / 12.0.
+constexpr int ROWS_SHORT = 444, ROWS_LONG = 592;
 constexpr int ROWS_VEC = 8;  // 16-byte vectors a lane holds: 2048 elements of K a warp
 __global__ void __launch_bounds__(256, 2) lora_low_rows_kernel(const bf16* x, int64_t ldx, int M, int K,
                                                                const __grid_constant__ LLLora lo, int ks, int* err) {
@@ -561,11 +570,10 @@ extern "C" int ll_lora_low(const bf16* x, int64_t ldx, int M, int K, const LLLor
   if (M <= 0) return 0;
   if ((K % 8) || (ldx % 8) || lo->rank <= 0 || lo->rank > LL_LORA_MAX_RANK || (lo->rank % 8)) return -3;
   if (lo->max_planes < 1 || lo->max_planes > 65535) return -3;
-  // one A row per row and rank through L2, up to this many bytes
-  if ((int64_t)M * lo->rank * K * 2 <= LOW_ROWS_BYTES) {
-    int ks = 1;
-    while (ks < 8 && ks * ROWS_VEC * 256 < K) ks *= 2;
-    const dim3 grid(M, (lo->rank + 8 / ks - 1) / (8 / ks));
+  int ks = 1;  // warps of a row and rank
+  while (ks < 8 && ks * ROWS_VEC * 256 < K) ks *= 2;
+  const dim3 grid(M, (lo->rank + 8 / ks - 1) / (8 / ks));
+  if ((int64_t)grid.x * grid.y <= (ks > 1 ? ROWS_LONG : ROWS_SHORT)) {
     const cudaError_t e =
         launch_pdl(lora_low_rows_kernel, grid, dim3(256), 0, stream, x, ldx, M, K, *lo, ks, err);
     return e == cudaSuccess ? 0 : -5;
@@ -616,12 +624,12 @@ extern "C" int ll_lora_low(const bf16* x, int64_t ldx, int M, int K, const LLLor
   return cudaLaunchKernelEx(&cfg, lora_low_kernel, tmX, tmA, M, K, *lo, shp, err) == cudaSuccess ? 0 : -5;
 }
 
-// One to 128 rows, one row tile.  N a multiple of 8 (32 with SwiGLU); out and
+// Any number of rows, 128 a CTA.  N a multiple of 8 (32 with SwiGLU); out and
 // bias on 8-byte boundaries.  K splits: as many CTAs (two a SM) as the feature
 // tiles leave room for, up to a cluster of 6.
 extern "C" int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, int64_t ldc, const bf16* bias, int M,
                             int N, int K, int swiglu, const LLLora* lo, int* err, cudaStream_t stream) {
-  if (M <= 0 || M > 128 || lo->tiles != 1 || lo->tile_rows != 128) return -3;
+  if (M <= 0 || lo->tile_rows != (M <= 128 ? 128 : 256)) return -3;
   if ((K % 8) || (N % 8) || (swiglu && (N % 32)) || (ldx % 8) || (ldc % 4)) return -3;
   const int bnx = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
   GemvMaps tm;
@@ -635,14 +643,16 @@ extern "C" int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, 
   if (!low_tmap(&tm.w, w, 2, dw, sw, box2w) || !low_tmap(&tm.x, x, 2, dx, sx, box2x) ||
       !low_tmap(&tm.low, lo->low, 2, dl, sl, box2x) || !low_tmap(&tm.b, lo->b, 3, db, sb, box3))
     return -2;
-  const int ntiles = (N + 127) / 128, num_kb = (K + LOW_BK - 1) / LOW_BK;
-  if (ntiles > 65535) return -3;
-  int cs = GEMV_PLACES / ntiles;
+  const int ntiles = (N + 127) / 128, mtiles = (M + bnx - 1) / bnx, num_kb = (K + LOW_BK - 1) / LOW_BK;
+  if (ntiles > 65535 || mtiles > 65535) return -3;
+  int cs = GEMV_PLACES / (ntiles * mtiles);
   if (cs > GEMV_MAX_CLUSTER) cs = GEMV_MAX_CLUSTER;
-  if (cs > (num_kb + 1) / 2) cs = (num_kb + 1) / 2;
+  // at least two k-blocks a CTA, the adapters' (at most that many) among them
+  const int64_t blocks = num_kb + (int64_t)(mtiles == 1 ? lo->max_planes : 1) * 2 * ((lo->rank + LOW_BK - 1) / LOW_BK);
+  if (cs > (blocks + 1) / 2) cs = (int)((blocks + 1) / 2);
   if (cs < 1) cs = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cs, ntiles);
+  cfg.gridDim = dim3(cs, ntiles, mtiles);
   cfg.blockDim = dim3(192);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];

@@ -315,9 +315,16 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
         y = ref.linear_lora(x, w, bias, lora.a, lora.b, lora.scale, plan.row_adapters)
         y = (ref_swiglu_interleaved(y) if swiglu_epilogue else y).to(x.dtype)
         return y if out is None else out.copy_(y)
-    small = M <= SMALL_M_MAX and not (M > 64 and N >= 148 * 256)  # as linear()
+    if M <= SMALL_M_MAX:
+        split = not (M > 64 and N >= 148 * 256)  # as linear()
+    else:
+        # 128 x 128 tiles with K split, while two CTAs or more have room for
+        # each; else linear()'s tiles.  us a call, split / not: 512 rows, K =
+        # 4096, N = 2048 (64 tiles) 23.7 / 33.3; 300, 4096, 4096 (96) 27.1 /
+        # 34.2; 512, 4096, 4096 (128) 41.7 / 35.2
+        split = -(-M // 128) * -(-N // 128) <= 124
     return _cuda().lora_linear(x, w, bias, out, lora.a, lora.b, lora.scale, plan.buf, plan.tile_rows, plan.max_planes,
-                               small, swiglu_epilogue, workspace(x.device).err)
+                               split, swiglu_epilogue, workspace(x.device).err)
 
 
 def ref_swiglu_interleaved(gu: torch.Tensor) -> torch.Tensor:

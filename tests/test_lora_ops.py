@@ -161,6 +161,15 @@ CASES = [  # M, K, N, R, adapters, rows, swiglu
     (1000, 512, 2048, 16, 300, "mixed", False),
     (5, 512, 1024, 16, 2, "none", False),
     (600, 512, 1024, 16, 2, "none", True),
+    (255, 1032, 1920, 24, 5, "mixed", False),  # K split past 128 rows
+    (513, 264, 1024, 136, 7, "runs", True),
+    (1920, 2048, 120, 16, 9, "runs", False),
+    (1100, 512, 1920, 16, 6, "runs", False),  # and not: 128 x 128,
+    (1100, 520, 1920, 88, 5, "mixed", True),
+    (200, 512, 8192, 16, 6, "mixed", False),  # 128 x 256
+    (200, 72, 8224, 24, 6, "runs", True),
+    (400, 200, 4104, 16, 6, "runs", False),  # and 256 x 256 tiles
+    (520, 136, 4096, 104, 6, "mixed", True),
 ]
 
 
@@ -171,9 +180,9 @@ def test_against_64_bits(M, K, N, R, n, rows, swiglu):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N", [(200, 1024), (200, 2048), (400, 2048)])
+@pytest.mark.parametrize("M,N", [(1100, 1920), (200, 8192), (400, 4096)])
 def test_a_batch_without_adapters_equals_linear_bit_for_bit(M, N):
-    """Past 128 rows the tiles and their k-blocks are those of linear()."""
+    """Where K is not split the tiles and their k-blocks are those of linear()."""
     t = make(M, 512, N, 16, 2, "none", seed=M, device="cuda")
     y = check(t)
     assert torch.equal(y, ops.linear(t["x"], t["w"], t["bias"]))
@@ -228,7 +237,7 @@ def test_captured_and_replayed_with_other_adapters(M):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", ["mixed", "none"])
-@pytest.mark.parametrize("M,R", [(1, 16), (4, 16), (100, 64), (128, 256), (300, 16)])
+@pytest.mark.parametrize("M,R", [(1, 16), (4, 16), (100, 64), (128, 256), (300, 16), (1100, 16)])
 def test_a_chain_of_products_in_a_graph(M, R, rows):
     """Each reads what the one before wrote, with no host between them: a
     kernel that looks at its rows before they are there shows here."""
