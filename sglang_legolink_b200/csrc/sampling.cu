@@ -18,19 +18,24 @@
 // counts (top-k) or weights (top-p) summed per bin; top-p selects within the
 // power of two that its cut falls in.
 //
-// Weights are integers: w in units of 2^-44, computed in double.  Integer sums
-// do not depend on their order, so a row gives the same token whatever batch,
-// cluster size or device it is drawn on, and the sums over a whole vocabulary
-// (2^19 tokens at most: 2^63) are exact to 2^-45 of the largest weight per
-// token.  A token below 2^-45 of it has weight 0 and is never drawn.
+// Weights are integers: w in units of 2^-44, computed in double to 1.2e-12 of
+// itself and rounded.  Integer sums do not depend on their order, so a row
+// gives the same token whatever batch, cluster size or device it is drawn on,
+// and the sums over a whole vocabulary (2^19 tokens at most: 2^63) are exact.
+// A token below 2^-45 of the largest has weight 0 and is never drawn.
 //
 // A cluster of CTAs owns a row and holds it in shared memory, so the logits
 // are read from memory once; the passes over the row run on shared memory and
 // exchange their sums through it (distributed shared memory).  The passes are
 // functions of their own, not inlined: two CTAs of 512 threads a SM leave 64
 // registers, and what the rest of the kernel keeps alive would spill inside
-// their loops, to memory that has no L1 left (an exact sum took 110 cycles a
-// warp and logit that way, 15 without).
+// their loops, to memory that has no L1 left.
+//
+// What bounds it: one row, the chain of some ten block and cluster steps of
+// 0.5 to 2 us (11.7 us for one row of 152064 tokens with top-k and top-p); a
+// batch of flat rows, the double operations of the exact sums (256 rows with
+// temperature alone 91 us, of which reading the logits is 12; 64 rows with
+// top-p 74 us, with three passes that evaluate every token).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -300,6 +305,30 @@ __device__ __noinline__ ExactSum exact_sum(const uint4* vals, int a, int b, floa
   return ExactSum{s - zero, high - (BOTH ? zero : 0ull)};
 }
 
+// The same where [from, upto] holds few of the tokens: over the set bits of a
+// mask, as many rounds as the fullest lane has, not over all of the vector's
+// elements (64 flat rows of 152064 tokens: 74 us a call, 78 without).
+template <typename Raw>
+__device__ __noinline__ unsigned long long exact_sum_of_few(const uint4* vals, int a, int b, float from, float upto,
+                                                            double xmax, double k1, const double* table) {
+  using K = Key<Raw>;
+  unsigned long long s = 0;
+  for (int v = a + (threadIdx.x & 31); v < b; v += 32) {
+    const uint4 q = vals[v];
+    if (K::largest(q) < from) continue;
+    float x[K::kPerVec];
+    K::unpack(q, x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < K::kPerVec; ++i) m |= (x[i] >= from && x[i] <= upto ? 1u : 0u) << i;
+    for (; m != 0; m &= m - 1) {
+      const Raw b = reinterpret_cast<const Raw*>(vals)[v * K::kPerVec + __ffs(m) - 1];
+      s += exact_weight(__uint_as_float((uint32_t)b << (32 - 8 * sizeof(Raw))), xmax, k1, table);
+    }
+  }
+  return s;
+}
+
 template <typename Raw>
 __device__ __noinline__ uint32_t count_equal(const uint4* vals, int a, int b, float tau) {
   using K = Key<Raw>;
@@ -360,8 +389,8 @@ __device__ __noinline__ void refine_sums(const uint4* vals, int a, int b, float 
   }
 }
 
-// Tokens per bin of (key - lo) >> shift, keys in [lo, hi]; with shift > 0 and
-// table, their weights too.
+// Tokens per bin of (key - lo) >> shift, keys in [lo, hi]; given `weight`,
+// their weights too.
 template <typename Raw>
 __device__ __noinline__ void histogram(const uint4* vals, int a, int b, float flo, float fhi, uint32_t lo, int shift,
                                        uint32_t* count, unsigned long long* weight, double xmax, double k1,
@@ -370,16 +399,16 @@ __device__ __noinline__ void histogram(const uint4* vals, int a, int b, float fl
   for (int v = a + (threadIdx.x & 31); v < b; v += 32) {
     const uint4 q = vals[v];
     if (K::largest(q) < flo) continue;
+    auto add = [&](float x) {
+      const uint32_t bin = (K::of(x) - lo) >> shift;
+      atomicAdd(&count[bin], 1u);
+      if (weight != nullptr) atomicAdd(&weight[bin], exact_weight(x, xmax, k1, table));
+    };
     float x[K::kPerVec];
     K::unpack(q, x);
 #pragma unroll
-    for (int i = 0; i < K::kPerVec; ++i) {
-      const uint32_t bin = (K::of(x[i]) - lo) >> shift;
-      if (x[i] >= flo && x[i] <= fhi) {
-        atomicAdd(&count[bin], 1u);
-        if (weight != nullptr) atomicAdd(&weight[bin], exact_weight(x[i], xmax, k1, table));
-      }
-    }
+    for (int i = 0; i < K::kPerVec; ++i)
+      if (x[i] >= flo && x[i] <= fhi) add(x[i]);
   }
 }
 
@@ -666,11 +695,9 @@ __device__ __noinline__ Nucleus find_nucleus(SampleShared& sh, const uint4* vals
     __syncthreads();
     r.lo = sh.edge[0];
     r.hi = sh.edge[1] - 1;
-    // (a bin per key takes 32-bit counts: cheaper than another level up to more tokens)
     r.inside = in / (double)ex2_approx(fmaf(K::value(r.lo), fc, fm)) * 1.001 + 1.0;
-    if (r.tokens <= SMP_FEW || r.inside <= (r.hi - r.lo < SMP_BINS ? 8192.0 : (double)SMP_FEW) || r.lo >= r.hi ||
-        level == 3)
-      break;
+    // keys that have a bin each are counted, however many tokens they are
+    if (r.tokens <= SMP_FEW || r.inside <= SMP_FEW || r.hi - r.lo < SMP_BINS || r.lo >= r.hi || level == 3) break;
     __syncthreads();  // the edges are read
   }
   return r;
@@ -967,7 +994,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
   const bool use_p = top_p < 1.f, use_m = min_p > 0.f;
   // approximate masses: where their arguments neither overflow nor cancel, fm
   // rounded to 2^-12 at most
-  const bool nucleus = use_p && k_of == 0 && T >= 1e-3f && T <= 1e4f && fabsf(xmax) / T * 1.4427f <= 4000.f;
+  const bool nucleus = use_p && k_of == 0 && V > SMP_FEW && T >= 1e-3f && T <= 1e4f && fabsf(xmax) / T * 1.4427f <= 4000.f;
   Nucleus nu{K::kNegInf + 1, sh.row.kmax, 1e30, 1e30, -1.0, 0.0};
   if (nucleus) nu = find_nucleus<Raw>(sh, vals, v0, v1, V, T);
 
@@ -1005,7 +1032,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
       }
     }
   } else if (use_p) {
-    if (nu.tokens <= SMP_FEW) xlo = K::value(nu.lo);
+    if (V <= SMP_FEW) xlo = SMP_LOWEST;  // all of them: sorting beats finding out which
+    else if (nu.tokens <= SMP_FEW) xlo = K::value(nu.lo);
   } else if (min_p >= 1e-4f) {
     // a little below max + T log(min_p)
     xlo = __double2float_rd(sh.row.xmax + (double)T * (log(sh.row.min_w) - 1e-6) - 1e-6 * fabs(sh.row.xmax));
@@ -1036,8 +1064,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
   // Weight within [from, upto] and tokens at tau per warp range, to every CTA;
   // `both`: and the weight above upto.
   auto sum_pass = [&](float from, float upto, bool both) {
-    const ExactSum e = both ? exact_sum<Raw, true>(vals, v0, v1, from, upto, sh.row.xmax, sh.row.k1, sh.exp2_table)
-                            : exact_sum<Raw, false>(vals, v0, v1, from, upto, sh.row.xmax, sh.row.k1, sh.exp2_table);
+    ExactSum e{0, 0};
+    if (both) e = exact_sum<Raw, true>(vals, v0, v1, from, upto, sh.row.xmax, sh.row.k1, sh.exp2_table);
+    else if (upto == INFINITY)
+      e = exact_sum<Raw, false>(vals, v0, v1, from, upto, sh.row.xmax, sh.row.k1, sh.exp2_table);
+    else e.s = exact_sum_of_few<Raw>(vals, v0, v1, from, upto, sh.row.xmax, sh.row.k1, sh.exp2_table);
     const unsigned long long s = warp_add(e.s), high = both ? warp_add(e.high) : 0ull;
     const uint32_t ties = quota > 0 ? __reduce_add_sync(0xffffffffu, count_equal<Raw>(vals, v0, v1, tau)) : 0u;
     if (lane < cs) {
@@ -1077,7 +1108,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
     const uint32_t floor_key = max(K::of(fmaxf(fmaxf(tau, SMP_LOWEST), sh.row.zero)), K::kNegInf + 1);
     Selected r{false, 0, 0, 0};
     bool found = false;
-    if (split != INFINITY && nu.inside <= SMP_FEW) {
+    if (split != INFINITY && nu.inside <= SMP_FEW && nu.hi - nu.lo >= SMP_BINS) {
       const uint32_t n = collect_all<Raw>(sh, vals, v0, v1, token0, K::value(max(floor_key, nu.lo)), split);
       if (n <= SMP_FEW) {
         if (rank == 0) cut_in_list<Raw>(sh, cs, n, above, goal);
