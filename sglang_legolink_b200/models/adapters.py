@@ -11,6 +11,7 @@ an adapter of rank r takes 3r there and 2r here, at most 256.
 
 from __future__ import annotations
 
+import hashlib
 import json
 import os
 import re
@@ -31,6 +32,17 @@ class Adapter:
     def __init__(self, mats: dict, scale: float):
         self.mats, self.scale = mats, float(scale)
 
+    def digest(self) -> str:
+        """Names the weights: blocks compiled with an adapter link only where
+        the adapter of that name has the same ones."""
+        h = hashlib.blake2b(repr(self.scale).encode(), digest_size=8)
+        for k in sorted(self.mats):
+            for t in self.mats[k]:
+                t = t.detach().float().cpu().contiguous()
+                h.update(repr((k, tuple(t.shape))).encode())
+                h.update(t.numpy().tobytes())
+        return h.hexdigest()
+
     @classmethod
     def from_state(cls, state: dict, alpha: float, rank: int, rslora: bool = False) -> "Adapter":
         """From PEFT tensor names (``...layers.N.self_attn.q_proj.lora_A.weight``)."""
@@ -41,8 +53,9 @@ class Adapter:
                 raise ValueError(f"adapter tensor '{name}' is not a low-rank matrix of a projection")
             half.setdefault((int(m[1]), m[2]), {})[m[3]] = t
         for k, ab in half.items():
-            if set(ab) != {"A", "B"} or ab["A"].shape[0] != ab["B"].shape[1]:
-                raise ValueError(f"adapter matrices of layer {k[0]} {k[1]} do not match")
+            if set(ab) != {"A", "B"} or any(t.dim() != 2 for t in ab.values()) \
+                    or not ab["A"].shape[0] == ab["B"].shape[1] == rank:
+                raise ValueError(f"adapter matrices of layer {k[0]} {k[1]} do not match each other and rank {rank}")
         return cls({k: (ab["A"], ab["B"]) for k, ab in half.items()},
                    alpha / (rank ** 0.5 if rslora else rank))
 

@@ -85,6 +85,7 @@ class QwenModel:
         self.cos_sin: Optional[torch.Tensor] = None
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
         self.adapter_names: list[str] = []  # adapter i of a batch's plan
+        self.adapter_digests: list[str] = []
         self._adapters: list = []
         self._layer_adapters: list = []
         self._bufs: dict = {}
@@ -243,6 +244,7 @@ class QwenModel:
                              if bad else f"adapter '{name}' has no matrices")
         adapters = self._adapters + [adapter]
         stacks = [LayerAdapters(self.cfg, adapters, i, self.device, self.dtype) for i in range(self.cfg.num_layers)]
+        self.adapter_digests = self.adapter_digests + [adapter.digest()]
         self._adapters, self._layer_adapters = adapters, stacks
         self.adapter_names = self.adapter_names + [name]
         self.buf_generation += 1

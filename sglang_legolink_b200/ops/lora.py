@@ -96,7 +96,8 @@ class LoraPlan:
 
     def update(self, row_adapters) -> "LoraPlan":
         """Gives the same rows other adapters, in the same device buffer: a
-        CUDA graph captured with this plan replays with the new ones.  Build
+        CUDA graph captured with this plan replays with the new ones.  The
+        copy is made on the current stream: the one the plan is used on.  Build
         the plan with ``max_planes`` = the most adapters it may ever hold
         (times the row tiles); more than that is refused."""
         ids = _host_ids(row_adapters)

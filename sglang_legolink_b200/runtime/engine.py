@@ -163,7 +163,6 @@ class Engine:
         if sampler not in ("torch", "kernel"):
             raise ValueError("sampler must be 'torch' (per-row torch ops) or 'kernel' (one launch a batch)")
         self.sampler = sampler
-        self._adapter_labels: set = set()  # adapter ids that blocks were compiled under without an adapter
         self.model = model
         self.cfg = model.cfg
         self.device = model.device
@@ -253,6 +252,8 @@ class Engine:
     def compat_key(self, adapter_id=None, segmentation_policy_version=None, legolink_policy_version=None) -> str:
         c = dict(self.compat)
         c["adapter_id"] = str(adapter_id or "none")
+        if self._adapter(adapter_id) >= 0:
+            c["adapter_id"] += "#" + self.model.adapter_digests[self._adapter(adapter_id)]
         c["segmentation_policy_version"] = str(segmentation_policy_version or "field-first-v1")
         c["legolink_policy_version"] = str(legolink_policy_version or LEGOLINK_POLICY_VERSION)
         return "|".join(f"{k}={c[k]}" for k in sorted(c))
@@ -262,15 +263,17 @@ class Engine:
         """Loads a low-rank adapter: a PEFT checkpoint directory or a
         :class:`~sglang_legolink_b200.models.adapters.Adapter`.  From then on
         a Compile, Link or plain request whose ``adapter_id`` is ``name`` runs
-        with it (an id that names no loaded adapter stays what it was: part of
-        the blocks' compatibility key).  A name keeps its weights for the
-        engine's life, since registered blocks hold K/V computed with them."""
+        with it.  An id that names no loaded adapter stays what it was: a
+        label in the blocks' compatibility key; blocks compiled under it before
+        its adapter was loaded, or on a replica whose adapter of that name has
+        other weights, are incompatible, not linked."""
         from ..models.adapters import Adapter
 
         with self._lock:
-            if str(name) in self._adapter_labels:
-                raise ValueError(f"blocks were compiled under adapter_id '{name}' without an adapter")
-            self.model.add_adapter(str(name), source if isinstance(source, Adapter) else Adapter.from_pretrained(source))
+            name = str(name)
+            if not name:
+                raise ValueError("an adapter needs a name")
+            self.model.add_adapter(name, source if isinstance(source, Adapter) else Adapter.from_pretrained(source))
 
     @property
     def adapters(self) -> list[str]:
@@ -443,10 +446,13 @@ class Engine:
         if self.sampler == "kernel":
             copy = (lambda a: _pinned_copy(a, self.device)) if self.is_cuda else torch.from_numpy
             drawn = draw_rows(full, list(params), list(gens) or None, copy)
+            ids = ids.clone()
+            here = ids[: len(params)]
             if any(p.greedy for p in params):  # these keep the argmax kernel's token
                 greedy_rows = copy(np.asarray([p.greedy for p in params]))
-                drawn = torch.where(greedy_rows, ids[: len(params)].to(drawn.dtype), drawn)
-            return drawn
+                drawn = torch.where(greedy_rows, here.to(drawn.dtype), drawn)
+            here.copy_(drawn)
+            return ids
         drawn = sample_rows(full, list(params), list(gens) or None)
         ids = ids.clone()
         ids[: len(params)] = drawn.to(ids.device)
@@ -509,8 +515,6 @@ class Engine:
             raise ContractError("Compile requires a non-empty sub-context.")
         ckey = self.compat_key(sc.get("adapter_id"), sc.get("segmentation_policy_version"),
                                sc.get("legolink_policy_version"))
-        if sc.get("adapter_id") is not None and self._adapter(sc["adapter_id"]) < 0:
-            self._adapter_labels.add(str(sc["adapter_id"]))
         return toks, ckey, str(block_id or sc.get("semantic_block_id") or cache_key)
 
     def _clone_pages(self, pages: list[int]) -> list[int]:

@@ -164,11 +164,29 @@ def test_a_label_that_names_no_adapter_stays_a_label():
     b = toks(32, 9)
     eng.compile(b, "x", sub_context={"adapter_id": "legal"})
     plan = {"cache_keys": ["x"], "recompute_tokens_per_block": [32], "adapter_id": "legal"}
-    s, f = eng.link(plan, [1, 2]), eng.prefill(b + [1, 2])
+    s, f = eng.link(dict(plan), [1, 2]), eng.prefill(b + [1, 2])
     eng.decode([s, f], 4)
     assert s.output_ids == f.output_ids
-    with pytest.raises(ValueError, match="compiled under"):
-        eng.load_adapter("legal", ads["two"])
+    # once an adapter of that name is loaded, its blocks are other blocks
+    eng.load_adapter("legal", ads["two"])
+    with pytest.raises(LinkSourceUnavailable):
+        eng.link(dict(plan), [1, 2])
+    eng.compile(b, "y", sub_context={"adapter_id": "legal"})
+    s = eng.link({**plan, "cache_keys": ["y"]}, [1, 2])
+    f = eng.prefill(b + [1, 2], adapter="legal")
+    eng.decode([s, f], 4)
+    assert s.output_ids == f.output_ids
+
+
+def test_the_compatibility_key_names_the_adapters_weights():
+    a, _ = engine(load=("one",))
+    b, ads = engine(load=())
+    plain = b.compat_key("one")
+    b.load_adapter("one", ads["two"])
+    c, _ = engine(load=("one", "two"))
+    assert a.compat_key() == b.compat_key() == c.compat_key() and a.compat_key("x") == b.compat_key("x")
+    assert a.compat_key("one") == c.compat_key("one")
+    assert len({a.compat_key("one"), b.compat_key("one"), plain}) == 3
 
 
 def test_requests_reach_their_adapter():
@@ -217,6 +235,10 @@ def test_adapter_refusals(world):
     del half[next(k for k in half if "lora_B" in k)]
     with pytest.raises(ValueError, match="do not match"):
         Adapter.from_state(half, 8, 8)
+    with pytest.raises(ValueError, match="do not match"):
+        Adapter.from_state(st, 8, 16)
+    with pytest.raises(ValueError, match="needs a name"):
+        eng.load_adapter("", ads["two"])
     with pytest.raises(ValueError, match="exceeds 256"):
         eng.load_adapter("wide", Adapter.from_state(state_of(cfg, 88, 4, ("q_proj", "k_proj", "v_proj")), 8, 88))
     with pytest.raises(ValueError, match="names layers"):
