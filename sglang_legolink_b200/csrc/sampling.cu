@@ -32,7 +32,7 @@
 // their loops, to memory that has no L1 left.
 //
 // What bounds it: one row, the chain of some ten block and cluster steps of
-// 0.5 to 2 us (11.7 us for one row of 152064 tokens with top-k and top-p); a
+// 0.5 to 2 us (10.3 us for one row of 152064 tokens with top-k and top-p); a
 // batch of flat rows, the double operations of the exact sums (256 rows with
 // temperature alone 91 us, of which reading the logits is 12; 64 rows with
 // top-p 74 us, with three passes that evaluate every token).
@@ -144,7 +144,7 @@ struct Row {
 
 struct SampleShared {
   Row row;
-  float wmax[SMP_RANGES];                // largest logit of each warp range
+  alignas(16) float wmax[SMP_RANGES];    // largest logit of each warp range
   float wkth[SMP_RANGES];                // the r-th largest of its lanes' largest
   unsigned long long wsum[SMP_RANGES];   // kept weight of each range
   uint32_t wties[SMP_RANGES];            // its tokens equal to tau
@@ -174,7 +174,9 @@ struct SampleShared {
     uint32_t mine[SMP_OCTAVES][SMP_THREADS];  // each thread's mass per bin
   };
 };
-static_assert(offsetof(SampleShared, count) % 16 == 0 && offsetof(SampleShared, weight) % 16 == 0, "vector reads");
+static_assert(offsetof(SampleShared, wmax) % 16 == 0 && offsetof(SampleShared, count) % 16 == 0 &&
+                  offsetof(SampleShared, weight) % 16 == 0,
+              "vector reads");
 
 // w of a logit, in units of 2^-44, with w = 2^(t / 32), t = (x - max) 32 / (T ln 2):
 // t = n + f, n whole and |f| <= 1/2;  2^(f / 32) by its Taylor polynomial of
@@ -384,7 +386,8 @@ __device__ __noinline__ void refine_sums(const uint4* vals, int a, int b, float 
       const bool in = x[i] >= flo && x[i] <= fhi;
       const uint32_t bin = __float_as_uint(bin_of(x[i], a1, sc)) - 0x4B000000u;
       // of the heaviest within the keys: at most 2^23
-      mine[bin * SMP_THREADS] += (uint32_t)ex2_approx(in ? fmaf(x[i] - fhi, k, 23.f) : -INFINITY);
+      mine[bin * SMP_THREADS] +=
+          __float_as_uint(ex2_approx(in ? fmaf(x[i] - fhi, k, 23.f) : -INFINITY) + 8388608.f) - 0x4B000000u;
     }
   }
 }
@@ -770,6 +773,119 @@ __device__ __noinline__ void cut_in_list(SampleShared& sh, int cs, uint32_t n, u
   }
 }
 
+// Bitonic sort, largest first, of `size` (a power of two, 4 to 128) values of
+// one warp: lane l holds values 4 l to 4 l + 3.
+__device__ __forceinline__ void order_pair(unsigned long long& a, unsigned long long& b, bool down) {
+  const bool swap = (a < b) == down;
+  const unsigned long long x = swap ? b : a, y = swap ? a : b;
+  a = x;
+  b = y;
+}
+__device__ __forceinline__ void warp_sort_descending(unsigned long long (&c)[4], uint32_t size) {
+  const uint32_t lane = threadIdx.x & 31;
+  order_pair(c[0], c[1], true);
+  order_pair(c[2], c[3], false);
+  for (uint32_t k = 4; k <= size; k *= 2) {
+    const bool down = (4 * lane & k) == 0;
+    for (uint32_t j = k / 8; j > 0; j /= 2) {  // between lanes
+      const bool large = down == ((lane & j) == 0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned long long o = __shfl_xor_sync(0xffffffffu, c[q], j);
+        c[q] = large == (o > c[q]) ? o : c[q];
+      }
+    }
+    order_pair(c[0], c[2], down);
+    order_pair(c[1], c[3], down);
+    order_pair(c[0], c[1], down);
+    order_pair(c[2], c[3], down);
+  }
+}
+
+// finish_list by one warp, without a barrier: for as many candidates as a
+// usual top-k leaves (top-k 50 of 152064 tokens: one row 10.3 us a call, 11.9
+// by the whole CTA; 64 rows 13.2 and 17.7).
+constexpr int SMP_WARP_FEW = 128;
+template <typename Raw>
+__device__ __noinline__ bool finish_in_warp(SampleShared& sh, const LLSample& p, int64_t row, int cs, uint32_t n,
+                                            uint32_t limit, bool use_p, bool use_m, double below, double err) {
+  using K = Key<Raw>;
+  const uint32_t lane = threadIdx.x, segment = SMP_LIST / cs;
+  unsigned long long c[4] = {0, 0, 0, 0}, w[4];
+  uint32_t base = 0, size = 4;
+  for (int r = 0; r < cs; ++r) {
+    const uint32_t m = sh.listed[r];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t i = 4 * lane + q - base;  // wraps before the segment
+      if (i < m) c[q] = sh.list[r * segment + i];
+    }
+    base += m;
+  }
+  while (size < n) size *= 2;
+  warp_sort_descending(c, size);
+  limit = min(limit, n);
+  auto weigh = [&](uint32_t count, bool high_half) {  // weights of the first `count`, what is before this lane's, all
+    unsigned long long mine = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float x = K::value((uint32_t)(high_half ? c[q] >> 32 : c[q]));
+      w[q] = 4 * lane + q < count ? weight_from(x, sh.row.zero, sh.row.xmax, sh.row.k1, sh.exp2_table) : 0ull;
+      mine += w[q];
+    }
+    const unsigned long long inc = warp_inclusive(mine, (int)lane);
+    return make_ulonglong2(inc - mine, __shfl_sync(0xffffffffu, inc, 31));
+  };
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (4 * lane + q >= limit) c[q] = 0;
+  if (use_p) {
+    const ulonglong2 ex = weigh(limit, true);
+    const double scale = below >= 0.0 ? sh.row.shift * SMP_ONE : 0.0;
+    const double goal = fmax(1.0, ceil(sh.row.top_p * ((double)ex.y + below * scale)));
+    const double e = sh.row.top_p * err * scale + 2.0;
+    bool near = (double)ex.y < goal + e;
+    unsigned long long run = ex.x;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool first = lane == 0 && q == 0;
+      near = near || (c[q] != 0 && !first && fabs((double)run - goal) <= e);
+      if ((double)run >= goal && !first) c[q] = 0;
+      run += w[q];
+    }
+    if (below >= 0.0 && __any_sync(0xffffffffu, near)) return false;
+  }
+  if (use_m) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (c[q] != 0 && !heavy(sh.row, K::value((uint32_t)(c[q] >> 32)))) c[q] = 0;
+  }
+  uint32_t kept = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    kept += c[q] != 0;
+    c[q] = c[q] << 32 | c[q] >> 32;
+  }
+  kept = __reduce_add_sync(0xffffffffu, kept);
+  size = 4;
+  while (size < kept) size *= 2;
+  warp_sort_descending(c, size);
+  const ulonglong2 ex = weigh(kept, false);
+  const double u = sh.row.u;
+  unsigned long long t = u > 0.0 ? (u < 1.0 ? (unsigned long long)(u * (double)ex.y) : ex.y - 1) : 0ull;
+  if (t >= ex.y) t = ex.y - 1;
+  unsigned long long run = ex.x;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (run <= t && t < run + w[q]) {
+      p.out[row] = (int)(0xFFFFFFFFu - (uint32_t)(c[q] >> 32));
+      if (p.logprob) p.logprob[row] = log_share(sh.row, K::value((uint32_t)c[q]), (double)ex.y / SMP_ONE);
+    }
+    run += w[q];
+  }
+  return true;
+}
+
 // The few candidates in sh.list, in segments of one CTA each: filters, draw.
 // `below`, `err`: mass (units of 1) of the row's other tokens and its error,
 // for a top-p over the whole row; else -1.  False: too near a border.
@@ -778,6 +894,10 @@ __device__ __noinline__ bool finish_list(SampleShared& sh, const LLSample& p, in
                                          uint32_t limit, bool use_p, bool use_m, double below, double err) {
   using K = Key<Raw>;
   const int tid = threadIdx.x;
+  if (n <= SMP_WARP_FEW) {
+    const bool ok = tid >= 32 || finish_in_warp<Raw>(sh, p, row, cs, n, limit, use_p, use_m, below, err);
+    return below < 0.0 || !__syncthreads_or(!ok);
+  }
   // two tokens a thread, in the order: weights and what is before them
   ulonglong2 c = sorted_list(sh, cs, n);
   limit = min(limit, n);
@@ -1009,10 +1129,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
     if (tid < ranges) {
       const float mine = sh.wmax[tid];
       int larger = 0;
-#pragma unroll 8
-      for (int i = 0; i < ranges; ++i) {
-        const float o = sh.wmax[i];
-        larger += o > mine || (o == mine && i < tid);
+#pragma unroll 4
+      for (int i = 0; i < ranges; i += 4) {
+        const float4 o = *reinterpret_cast<const float4*>(&sh.wmax[i]);
+        larger += (o.x > mine || (o.x == mine && i < tid)) + (o.y > mine || (o.y == mine && i + 1 < tid)) +
+                  (o.z > mine || (o.z == mine && i + 2 < tid)) + (o.w > mine || (o.w == mine && i + 3 < tid));
       }
       if (larger == k_of - 1) sh.bound = mine;
     }
