@@ -392,7 +392,6 @@ at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::opti
   TORCH_CHECK(tile_rows == (M <= 128 ? 128 : 256) && max_planes >= 1, "bad plan");
   TORCH_CHECK(plan.numel() == M + tiles + 1 + 2 * max_planes, "the plan is for another batch");
   TORCH_CHECK(max_planes <= 65535, "too many adapters per tile of rows");
-  auto low = at::empty({max_planes * 2 * tile_rows, R}, x.options());
   LLLora lo{};
   lo.a = bp(a);
   lo.b = bp(b);
@@ -401,12 +400,13 @@ at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::opti
   lo.tile_ptr = lo.row_slot + M;
   lo.plane_adapter = lo.tile_ptr + tiles + 1;
   lo.plane_tile = lo.plane_adapter + max_planes;
-  lo.low = bp(low);
   lo.adapters = (int)n;
   lo.rank = (int)R;
   lo.tiles = (int)tiles;
   lo.tile_rows = (int)tile_rows;
   lo.max_planes = (int)max_planes;
+  auto low = at::empty({max_planes * lo.halves() * tile_rows, lo.ld()}, x.options());
+  lo.low = bp(low);
   check_rc(ll_lora_low(bp(x), x.stride(0), (int)M, (int)K, &lo, err.data_ptr<int>(), cur_stream()), "ll_lora_low");
   if (split_k) {
     check_rc(ll_lora_gemv(bp(x), x.stride(0), bp(w), bp(out), out.stride(0), bp_opt(bias), (int)M, (int)N, (int)K,

@@ -61,11 +61,12 @@ struct NoLora {
 };
 struct alignas(64) LoraBlocks {
   static constexpr bool on = true;
-  CUtensorMap tm_low;        // [planes * 2 (hi, lo) * tile_rows, rank]
+  CUtensorMap tm_low;        // [planes * halves * tile_rows, rank (packed: hi beside lo)]
   CUtensorMap tm_b;          // [adapters, N, rank]
   const int* tile_ptr;       // planes of row tile t: [tile_ptr[t], tile_ptr[t + 1])
   const int* plane_adapter;  // adapter of each plane
-  int rank_blocks;           // 64-rank blocks of an adapter
+  int steps, halves;         // k-blocks of a plane; 2 where hi and lo are blocks of rows, 1 packed
+  uint64_t again;            // packed: descriptor units back to B's first columns
   int tile_rows;             // rows of a plane
 };
 
@@ -178,16 +179,16 @@ __global__ void __launch_bounds__(192, 1)
         }
         if constexpr (Lora::on) {
           const int t0 = mb * GEMM_BM / lora.tile_rows, r0 = mb * GEMM_BM % lora.tile_rows;
-          const int p0 = lora.tile_ptr[t0], n_extra = (lora.tile_ptr[t0 + 1] - p0) * 2 * lora.rank_blocks;
+          const int p0 = lora.tile_ptr[t0], n_extra = (lora.tile_ptr[t0 + 1] - p0) * lora.steps;
           for (int e = 0; e < n_extra && ok; ++e) {
             if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
               ok = false;
               break;
             }
-            const int plane = p0 + (e >> 1) / lora.rank_blocks, rb = (e >> 1) % lora.rank_blocks;
+            const int plane = p0 + e / lora.steps, s = e % lora.steps, rb = s >> 1;
             mbar_arrive_expect_tx(&full[stage], Cfg::A_BYTES + Cfg::B_BYTES);
             tma_load_2d(sA + stage * Cfg::A_BYTES, &lora.tm_low, &full[stage], rb * GEMM_BK,
-                        (2 * plane + (e & 1)) * lora.tile_rows + r0);
+                        (plane * lora.halves + (s & 1)) * lora.tile_rows + r0);
             tma_load_3d(sB + stage * Cfg::B_BYTES, &lora.tm_b, &full[stage], rb * GEMM_BK, nb * BN,
                         lora.plane_adapter[plane]);
             if (++stage == STAGES) {
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(192, 1)
           int mb, nb;
           tile_coords(t, num_m, num_n, group_m, mb, nb);
           const int t0 = mb * GEMM_BM / lora.tile_rows;
-          num_kb_t += (lora.tile_ptr[t0 + 1] - lora.tile_ptr[t0]) * 2 * lora.rank_blocks;
+          num_kb_t += (lora.tile_ptr[t0 + 1] - lora.tile_ptr[t0]) * lora.steps;
         }
         for (int kb = 0; kb < num_kb_t; ++kb) {
           if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) {
@@ -229,9 +230,11 @@ __global__ void __launch_bounds__(192, 1)
           tc_fence_after();
           const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sA + stage * Cfg::A_BYTES));
           const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sB + stage * Cfg::B_BYTES));
+          uint64_t again = 0;  // from the third step on, B starts over
+          if constexpr (Lora::on) again = kb >= num_kb ? lora.again : 0;
 #pragma unroll
           for (int k = 0; k < GEMM_BK / 16; ++k) {
-            umma_bf16(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            umma_bf16(d_tmem, ad + 2 * k, bd + 2 * k - (k >= 2 ? again : 0), idesc, (kb | k) != 0 ? 1u : 0u);
           }
           umma_commit(&empty[stage]);
           if (++stage == STAGES) {
@@ -1210,17 +1213,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           }
         }
         if constexpr (Lora::on) {
-          const int p0 = lora.tile_ptr[mb], n_extra = (lora.tile_ptr[mb + 1] - p0) * 2 * lora.rank_blocks;
+          const int p0 = lora.tile_ptr[mb], n_extra = (lora.tile_ptr[mb + 1] - p0) * lora.steps;
           for (int e = 0; e < n_extra && ok; ++e) {
             if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
               ok = false;
               break;
             }
-            const int plane = p0 + (e >> 1) / lora.rank_blocks, rb = (e >> 1) % lora.rank_blocks;
+            const int plane = p0 + e / lora.steps, s = e % lora.steps, rb = s >> 1;
             const uint32_t leader_full = mapa_shared(smem_u32(&full[stage]), 0);
             if (crank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
             tma_load_2d_2sm(sA + stage * Cfg::A_BYTES, &lora.tm_low, leader_full, rb * GEMM_BK,
-                            (2 * plane + (e & 1)) * lora.tile_rows + (int)crank * GEMM_BM);
+                            (plane * lora.halves + (s & 1)) * lora.tile_rows + (int)crank * GEMM_BM);
             tma_load_3d_2sm(sB + stage * Cfg::B_BYTES, &lora.tm_b, leader_full, rb * GEMM_BK,
                             nb * BN + (int)crank * (BN / 2), lora.plane_adapter[plane]);
             if (++stage == STAGES) {
@@ -1250,7 +1253,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         if constexpr (Lora::on) {
           int mb, nb;
           tile_coords(t, num_m, num_n, group_m, mb, nb);
-          num_kb_t += (lora.tile_ptr[mb + 1] - lora.tile_ptr[mb]) * 2 * lora.rank_blocks;
+          num_kb_t += (lora.tile_ptr[mb + 1] - lora.tile_ptr[mb]) * lora.steps;
         }
         for (int kb = 0; kb < num_kb_t; ++kb) {
           if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) {
@@ -1260,9 +1263,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           tc_fence_after();
           const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sA + stage * Cfg::A_BYTES));
           const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sB + stage * Cfg::B_BYTES));
+          uint64_t again = 0;  // from the third step on, B starts over
+          if constexpr (Lora::on) again = kb >= num_kb ? lora.again : 0;
 #pragma unroll
           for (int k = 0; k < GEMM_BK / 16; ++k)
-            umma_bf16_2sm(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            umma_bf16_2sm(d_tmem, ad + 2 * k, bd + 2 * k - (k >= 2 ? again : 0), idesc, (kb | k) != 0 ? 1u : 0u);
           umma_commit_2sm_both(&empty[stage]);
           if (++stage == STAGES) {
             stage = 0;
@@ -1920,11 +1925,14 @@ static int make_tmap_lora_b(CUtensorMap* tm, const LLLora& lo, int N, int box_ro
 
 static int make_lora_blocks(LoraBlocks* lb, const LLLora& lo, int N, int b_box_rows) {
   if (lo.rank <= 0 || (lo.rank % 8) || lo.rank > LL_LORA_MAX_RANK || lo.adapters <= 0 || lo.tile_rows <= 0) return -3;
-  if (make_tmap_2d(&lb->tm_low, lo.low, lo.max_planes * 2 * lo.tile_rows, lo.rank, lo.rank, GEMM_BM)) return -2;
+  if (make_tmap_2d(&lb->tm_low, lo.low, lo.max_planes * lo.halves() * lo.tile_rows, lo.ld(), lo.ld(), GEMM_BM))
+    return -2;
   if (make_tmap_lora_b(&lb->tm_b, lo, N, b_box_rows)) return -2;
   lb->tile_ptr = lo.tile_ptr;
   lb->plane_adapter = lo.plane_adapter;
-  lb->rank_blocks = (lo.rank + GEMM_BK - 1) / GEMM_BK;
+  lb->steps = lo.steps();
+  lb->halves = lo.halves();
+  lb->again = lo.packed() ? 4 : 0;
   lb->tile_rows = lo.tile_rows;
   return 0;
 }

@@ -89,15 +89,16 @@ __global__ void __launch_bounds__(128, 2)
   }
   const int rows = min(LOW_BM, M - m0), slot = plane - lo.tile_ptr[t];
   const bool mine = tid < rows && lo.row_slot[m0 + tid] == slot;
-  bf16* low = lo.low + ((size_t)plane * 2 * lo.tile_rows + blockIdx.y * LOW_BM) * lo.rank;
-  const size_t lo_plane = (size_t)lo.tile_rows * lo.rank;
-  const int groups = lo.rank / 4;  // 4 ranks a thread
+  const int ld = lo.ld();
+  bf16* low = lo.low + ((size_t)plane * lo.halves() * lo.tile_rows + blockIdx.y * LOW_BM) * ld;
+  const size_t to_lo = lo.to_lo();
+  const int groups = (lo.packed() ? 32 : lo.rank) / 4;  // 4 columns a thread
   if (!__syncthreads_or(mine)) {   // no row of this half uses the adapter
     pdl_wait();
     for (int i = crank * 128 + tid; i < rows * groups; i += cs * 128) {
-      bf16* d = low + (size_t)(i / groups) * lo.rank + 4 * (i % groups);
+      bf16* d = low + (size_t)(i / groups) * ld + 4 * (i % groups);
       *reinterpret_cast<uint2*>(d) = make_uint2(0, 0);
-      *reinterpret_cast<uint2*>(d + lo_plane) = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(d + to_lo) = make_uint2(0, 0);
     }
     return;
   }
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(128, 2)
     for (int i = crank * 128 + tid; i < rows * groups; i += cs * 128) {
       const int row = i / groups, g = i % groups;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (lo.row_slot[m0 + row] == slot) {
+      if (4 * g < lo.rank && lo.row_slot[m0 + row] == slot) {
         for (int r = 0; r < cs; ++r) {
           const float4 p = ld_cluster_f32x4(low_mapa(base + (uint32_t)(row * shp.part_ld + 4 * g) * 4, r));
           v.x += p.x;
@@ -217,12 +218,12 @@ __global__ void __launch_bounds__(128, 2)
       }
       const uint32_t h0 = pack_bf16x2(v.x, v.y), h1 = pack_bf16x2(v.z, v.w);
       const float2 f0 = unpack_bf16x2(h0), f1 = unpack_bf16x2(h1);
-      bf16* d = low + (size_t)row * lo.rank + 4 * g;
+      bf16* d = low + (size_t)row * ld + 4 * g;
       *reinterpret_cast<uint2*>(d) = make_uint2(h0, h1);
       // an infinite value has no remainder
       const float r0 = v.x - f0.x, r1 = v.y - f0.y, r2 = v.z - f1.x, r3 = v.w - f1.y;
       auto rest = [](float r) { return r == r && fabsf(r) < 3.0e38f ? r : 0.f; };
-      *reinterpret_cast<uint2*>(d + lo_plane) =
+      *reinterpret_cast<uint2*>(d + to_lo) =
           make_uint2(pack_bf16x2(rest(r0), rest(r1)), pack_bf16x2(rest(r2), rest(r3)));
     }
   }
@@ -284,10 +285,10 @@ __global__ void __launch_bounds__(192, 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cs = gridDim.x, crank = blockIdx.x, nb = blockIdx.y;
   const int num_kb = (K + LOW_BK - 1) / LOW_BK;
-  const int rank_blocks = (lo.rank + LOW_BK - 1) / LOW_BK;
+  const int per_plane = lo.steps();
   const int m0 = blockIdx.z * BNX, M = min(BNX, rows - m0);  // this CTA's rows
   const int t = m0 / lo.tile_rows, p0 = max(0, lo.tile_ptr[t]);
-  const int num_extra = max(0, min(lo.tile_ptr[t + 1], lo.max_planes) - p0) * 2 * rank_blocks;
+  const int num_extra = max(0, min(lo.tile_ptr[t + 1], lo.max_planes) - p0) * per_plane;
   C += m0 * ldc;
   const int per = (num_kb + cs - 1) / cs, eper = (num_extra + cs - 1) / cs;
   const int kb0 = min(num_kb, crank * per), kb1 = min(num_kb, kb0 + per);
@@ -334,11 +335,11 @@ __global__ void __launch_bounds__(192, 2)
           tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.x, &full[stage], kb * LOW_BK, m0);
         } else {
           const int e = e0 + kb - kb1;
-          const int plane = p0 + (e >> 1) / rank_blocks, rb = (e >> 1) % rank_blocks;
+          const int plane = p0 + e / per_plane, s = e % per_plane, rb = s >> 1;
           tma_load_3d(sW + stage * Cfg::W_BYTES, &tm.b, &full[stage], rb * LOW_BK, nb * 128,
                       lo.plane_adapter[plane]);
           tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.low, &full[stage], rb * LOW_BK,
-                      (2 * plane + (e & 1)) * lo.tile_rows + m0 % lo.tile_rows);
+                      (plane * lo.halves() + (s & 1)) * lo.tile_rows + m0 % lo.tile_rows);
         }
         if (++stage == STAGES) {
           stage = 0;
@@ -361,8 +362,10 @@ __global__ void __launch_bounds__(192, 2)
         tc_fence_after();
         const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sW + stage * Cfg::W_BYTES));
         const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sX + stage * Cfg::X_BYTES));
+        const uint64_t again = lo.packed() && i >= kb1 - kb0 ? 4 : 0;  // lo meets B's first columns again
 #pragma unroll
-        for (int k = 0; k < LOW_BK / 16; ++k) umma_bf16(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0 ? 1u : 0u);
+        for (int k = 0; k < LOW_BK / 16; ++k)
+          umma_bf16(tmem, ad + 2 * k - (k >= 2 ? again : 0), bd + 2 * k, idesc, (i | k) != 0 ? 1u : 0u);
         umma_commit(&empty[stage]);
         if (++stage == STAGES) {
           stage = 0;
@@ -528,10 +531,13 @@ __global__ void __launch_bounds__(256, 2) lora_low_rows_kernel(const bf16* x, in
   const float rest = v - __bfloat162float(hi);
   const bf16 rem = __float2bfloat16(rest == rest && fabsf(rest) < 3.0e38f ? rest : 0.f);  // none of an infinite value
   const bf16 zero = __float2bfloat16(0.f);
+  const size_t to_lo = lo.to_lo();
   for (int j = lane; j < np; j += 32) {
-    bf16* d = lo.low + ((size_t)(p0 + j) * 2 * lo.tile_rows + m % lo.tile_rows) * lo.rank + r;
+    bf16* d = lo.low + ((size_t)(p0 + j) * lo.halves() * lo.tile_rows + m % lo.tile_rows) * lo.ld() + r;
     d[0] = j == slot ? hi : zero;
-    d[(size_t)lo.tile_rows * lo.rank] = j == slot ? rem : zero;
+    d[to_lo] = j == slot ? rem : zero;
+    if (lo.packed())
+      for (int z = lo.rank; r + z < 32; z += lo.rank) d[z] = d[z + 32] = zero;
   }
 }
 
@@ -636,8 +642,8 @@ extern "C" int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, 
   const cuuint32_t box2w[2] = {64, 128}, box2x[2] = {64, (cuuint32_t)bnx}, box3[3] = {64, 128, 1};
   const cuuint64_t dw[2] = {(cuuint64_t)K, (cuuint64_t)N}, sw[1] = {(cuuint64_t)K * 2};
   const cuuint64_t dx[2] = {(cuuint64_t)K, (cuuint64_t)M}, sx[1] = {(cuuint64_t)ldx * 2};
-  const cuuint64_t dl[2] = {(cuuint64_t)lo->rank, (cuuint64_t)lo->max_planes * 2 * lo->tile_rows};
-  const cuuint64_t sl[1] = {(cuuint64_t)lo->rank * 2};
+  const cuuint64_t dl[2] = {(cuuint64_t)lo->ld(), (cuuint64_t)lo->max_planes * lo->halves() * lo->tile_rows};
+  const cuuint64_t sl[1] = {(cuuint64_t)lo->ld() * 2};
   const cuuint64_t db[3] = {(cuuint64_t)lo->rank, (cuuint64_t)N, (cuuint64_t)lo->adapters};
   const cuuint64_t sb[2] = {(cuuint64_t)lo->rank * 2, (cuuint64_t)lo->rank * 2 * N};
   if (!low_tmap(&tm.w, w, 2, dw, sw, box2w) || !low_tmap(&tm.x, x, 2, dx, sx, box2x) ||
@@ -648,7 +654,7 @@ extern "C" int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, 
   int cs = GEMV_PLACES / (ntiles * mtiles);
   if (cs > GEMV_MAX_CLUSTER) cs = GEMV_MAX_CLUSTER;
   // at least two k-blocks a CTA, the adapters' (at most that many) among them
-  const int64_t blocks = num_kb + (int64_t)(mtiles == 1 ? lo->max_planes : 1) * 2 * ((lo->rank + LOW_BK - 1) / LOW_BK);
+  const int64_t blocks = num_kb + (int64_t)(mtiles == 1 ? lo->max_planes : 1) * lo->steps();
   if (cs > (blocks + 1) / 2) cs = (int)((blocks + 1) / 2);
   if (cs < 1) cs = 1;
   cudaLaunchConfig_t cfg = {};
