@@ -454,10 +454,13 @@ __device__ __forceinline__ uint4 ld_after_wait(const uint4* p) {
 
 // Few rows (decode): dot products, `ks` warps of a CTA to each (row, rank),
 // every warp with its share of the adapter's row in registers before the wait
-// for x.  No shared tiles, so these CTAs fit beside the product's, which are
-// loading weights meanwhile; what counts is the time from x to the stored
-// value: 2-3 us, against 5-6 for the tensor-core kernel's chain (tiles, TMEM,
-// partials, cluster).  A is read once per row here, from L2 where rows share it.
+// for x.  No shared tiles, and one of these CTAs a SM leaves registers for the
+// product's two, which load weights meanwhile; what counts is the time from x
+// to the stored value, 1.5 us less than the tensor-core kernel's chain (tiles,
+// TMEM, partials, cluster).  A is read once per row here, from L2 where rows
+// share it.  Fewer registers (4 vectors a lane, 62) and more CTAs a SM: 61 rows
+// 25.6 to 27.7 us a call for 26.8, one row 9.7 to 10.6 for 9.6.
+//
 // Each (row, rank) is a CTA's share, two CTAs a SM: used up to one and a half
 // rounds of the 296 places, two where K is long.  us a call with this kernel /
 // the tensor cores': 64 rows, rank 32, K = 1024 (256 CTAs) 8.0 / 9.3; 64, 64,
