@@ -223,6 +223,37 @@ def test_a_checkpoint_directory(tmp_path, world):
             Adapter.from_pretrained(str(tmp_path))
 
 
+def test_the_service_runs_requests_with_their_adapter(tmp_path):
+    from safetensors.torch import save_file
+
+    from sglang_legolink_b200.server.http_server import adapter_arg, build_service
+
+    save_file(state_of(PRESETS["tiny-qwen2"], 8, 1), str(tmp_path / "adapter_model.safetensors"))
+    (tmp_path / "adapter_config.json").write_text(json.dumps({"r": 8, "lora_alpha": 16}))
+    name, path = adapter_arg(f"legal={tmp_path}")
+    svc = build_service("tiny-qwen2", max_context=4096, legolink_only=False, sampler="kernel", adapters=[(name, path)])
+    try:
+        def ask(text, **kw):
+            return svc.complete({"messages": [{"role": "user", "content": text}], "max_tokens": 5, "ignore_eos": True,
+                                 **kw})["meta_info"]["output_ids"]
+
+        assert ask("a question", adapter_id="legal") != ask("a question")
+        sampled = {"temperature": 0.9, "top_p": 0.9, "min_p": 0.02, "seed": 5}
+        assert ask("a question", adapter_id="legal", **sampled) == ask("a question", adapter_id="legal", **sampled)
+        ask("a block of text " * 8, sub_context={"cache_key": "k", "adapter_id": "legal"})
+        linked = ask("and so?", pic_link={"cache_keys": ["k"], "recompute_initial_tokens": 4, "adapter_id": "legal"})
+        assert len(linked) == 5
+        with pytest.raises(Exception, match="noc_residency_recovery"):
+            ask("and so?", pic_link={"cache_keys": ["k"], "recompute_initial_tokens": 4})
+        with pytest.raises(Exception, match="not loaded"):
+            ask("a question", adapter_id="other")
+    finally:
+        svc.scheduler.stop()
+    for bad in ("legal", "=path", "legal="):
+        with pytest.raises(Exception, match="NAME=PATH"):
+            adapter_arg(bad)
+
+
 def test_adapter_refusals(world):
     eng, ads = world
     cfg = eng.cfg
