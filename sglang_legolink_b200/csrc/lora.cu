@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(128, 2)
       float* d = part + (size_t)tid * shp.part_ld + c;
 #pragma unroll
       for (int i = 0; i < 32; i += 4)
-        if (c + i < lo.rank)
+        if (c + i < lo.rank && tid < rows)  // the partials have `rows` rows, not the warp's 32
           *reinterpret_cast<float4*>(d + i) =
               kb1 > kb0 ? make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]),
                                       __uint_as_float(r[i + 3]))

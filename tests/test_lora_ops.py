@@ -155,6 +155,9 @@ CASES = [  # M, K, N, R, adapters, rows, swiglu
     (128, 512, 1024, 16, 128, "all", True),
     (100, 64, 37888, 16, 9, "mixed", False),
     (129, 512, 1024, 8, 2, "runs", False),
+    (97, 1024, 512, 256, 3, "mixed", False),  # partials of rows that are no multiple of 32, at large ranks
+    (100, 2048, 256, 200, 5, "mixed", True),
+    (65, 4096, 128, 256, 40, "all", False),
     (257, 520, 264, 80, 4, "mixed", False),
     (300, 512, 1024, 192, 3, "runs", True),
     (700, 8, 8, 8, 1, "runs", False),
