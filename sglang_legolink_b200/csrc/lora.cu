@@ -204,12 +204,17 @@ __global__ void __launch_bounds__(128, 2)
       const int row = i / groups, g = i % groups;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (4 * g < lo.rank && lo.row_slot[m0 + row] == slot) {
-        for (int r = 0; r < cs; ++r) {
-          const float4 p = ld_cluster_f32x4(low_mapa(base + (uint32_t)(row * shp.part_ld + 4 * g) * 4, r));
-          v.x += p.x;
-          v.y += p.y;
-          v.z += p.z;
-          v.w += p.w;
+        float4 p[LOW_MAX_CLUSTER];  // all of them in flight at once
+        const uint32_t at = base + (uint32_t)(row * shp.part_ld + 4 * g) * 4;
+#pragma unroll
+        for (int r = 0; r < LOW_MAX_CLUSTER; ++r)
+          p[r] = r < cs ? ld_cluster_f32x4(low_mapa(at, r)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < LOW_MAX_CLUSTER; ++r) {
+          v.x += p[r].x;
+          v.y += p[r].y;
+          v.z += p[r].z;
+          v.w += p[r].w;
         }
         v.x *= scale;
         v.y *= scale;
