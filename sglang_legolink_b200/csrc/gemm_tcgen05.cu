@@ -54,7 +54,8 @@ using TpArgs = LLTpArgs;
 // and its B matrix.  They accumulate into the same TMEM accumulator, so the adapters'
 // term joins the product in fp32, before the epilogue, and costs no pass over
 // the output: at 5087 rows x 4608 outputs a separate pass would read and write
-// 94 MB (14 us at HBM rate), the extra k-blocks add 2 to 56.
+// 94 MB (14 us at HBM rate), the extra k-blocks of a rank-48 adapter add 2 to
+// 56 (the whole product 136 us, 120 without adapters).
 // NoLora compiles the kernels without any of it.
 struct NoLora {
   static constexpr bool on = false;

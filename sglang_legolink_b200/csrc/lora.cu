@@ -7,12 +7,16 @@
 // rank 48), so what counts is bytes in flight: the cluster split puts up to
 // two CTAs with a ~96 KB ring on every SM whatever the number of row tiles.
 // The CTAs' fp32 partials meet in distributed shared memory and are summed in
-// CTA order, so a row's bits do not depend on timing.
+// CTA order, so a row's bits do not depend on timing.  That case takes 17 us
+// with cold caches: 4 until the last cluster has started, 1.5 to read the plan
+// and set up, 5 for the loads (8 TB/s, from L2 where two planes share rows), 4
+// for the partials.
 //
 // low is kept as two bf16 planes, hi = bf16(v) and lo = bf16(v - hi): the
 // product that reads them takes bf16 operands, and one bf16 would put 2^-9 of
 // every low-rank value into the result, as much again as rounding the result
-// itself; hi + lo holds 16 bits and costs one more k-block a plane.
+// itself; hi + lo holds 16 bits and costs one more k-block per 64 ranks of a
+// plane (none up to rank 32, lora.h).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -240,19 +244,20 @@ __global__ void __launch_bounds__(128, 2)
 // The product for up to 128 rows (decode), and for more where 128 x 128 tiles
 // leave SMs free: as the small-M GEMM, the weight tile is the M = 128 side of
 // the MMA and the rows (128 a CTA at most) are the N side, and K is split so
-// that every SM streams weights.  Here the splits of a feature tile
-// are a cluster: their fp32 partials stay in shared memory and each CTA sums,
-// in split order, and stores its share of the rows.  Nothing goes through
-// global memory and no CTA waits for a last one to add up 128 features x M
-// rows x all splits (at 61 rows x 5120 features, 7 splits, that fix-up alone
-// was 40 of 62 us).  Each split takes its share of the k-blocks of K, then its
-// share of the adapters'.  The first ring of weights is on its way before the
-// wait for the low-rank kernel.
+// that every SM streams weights.  Here the splits of a feature tile are a
+// cluster: their fp32 partials stay in shared memory and each CTA sums, in
+// split order, and stores its share of the rows.  Nothing goes through global
+// memory and no CTA waits for a last one to add up 128 features x M rows x all
+// splits (at 61 rows x 5120 features, 7 splits, that fix-up alone was 40 of 62
+// us).  Each split takes its share of the k-blocks of K, then its share of the
+// adapters'.  The first ring of weights is on its way before the wait for the
+// low-rank kernel.  Bound by reading weights: 16 rows, 3584 -> 37888 with
+// SwiGLU and 6 adapters of rank 32 in 48.4 us for both kernels, 6.1 TB/s.
 constexpr int GEMV_RING = 108 * 1024;
 // Clusters do not fill the SMs to the last place (two CTAs a SM, 296 places):
 // 36 clusters of 8 and 40 of 7 ran a second round.  us a call with 2 / 4 / 6 /
-// 8 (7) CTAs: 1 row x 4608 features 12.9 / 10.1 / 8.6 / 14.3, 61 rows x 5120
-// 43.2 / 31.1 / 27.9 / 38.7.
+// 8 (7) CTAs (hi and lo in blocks of their own): 1 row x 4608 features 12.9 /
+// 10.1 / 8.6 / 14.3, 61 rows x 5120 43.2 / 31.1 / 27.9 / 38.7.
 constexpr int GEMV_MAX_CLUSTER = 6;
 constexpr int GEMV_PLACES = 248;
 template <int BNX>
