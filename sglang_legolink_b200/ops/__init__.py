@@ -646,7 +646,7 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[t
            top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
            min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, return_logprobs: bool = False):
     """One token per row of ``logits`` [B, V] (bf16 or fp32, rows of any
-    stride, V <= 2^19), drawn with ``uniforms`` (float64 [B] in [0, 1)).
+    stride, V <= 2^19, of fp32 389,000), drawn with ``uniforms`` (float64 [B] in [0, 1)).
 
     Per row, each a [B] tensor or None: ``temperature`` (fp32; <= 0: the
     largest logit), ``top_k`` (int32; <= 0: off), ``top_p`` (fp32; >= 1: off)

@@ -228,6 +228,28 @@ def test_largest_vocabulary():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V,dtype", [(1 << 19, torch.bfloat16), (389000, torch.float32)])
+def test_longest_rows(V, dtype):
+    on_gpu(logits_of("tail", 3, V, seed=12, dtype=dtype), *settings(3, seed=13))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [1023, 1024, 1025, 2049])
+@pytest.mark.parametrize("k", [1, 2, 127, 128, 129, 1000, 1024, 1025])
+def test_numbers_of_candidates_at_which_the_way_changes(k, V):
+    """One warp, one CTA, the whole cluster; the row listed whole or not."""
+    B = 12
+    x = logits_of("coarse", B, V, seed=k, dtype=torch.bfloat16)
+    u = torch.rand(B, generator=torch.Generator().manual_seed(k + V), dtype=torch.float64)
+    kk = torch.full((B,), k, dtype=torch.int32)
+    p = torch.linspace(0.05, 1.0, B)
+    on_gpu(x, u, None, kk)
+    on_gpu(x, u, None, kk, p)
+    on_gpu(x, u, None, None, p)
+    on_gpu(x, u, None, kk, p, torch.full((B,), 1e-3))
+
+
+@pytest.mark.gpu
 def test_refusals():
     x, u = torch.zeros(2, 10, device="cuda"), torch.zeros(2, dtype=torch.float64, device="cuda")
     ops.sample(x, u)
