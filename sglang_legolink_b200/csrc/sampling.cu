@@ -240,35 +240,69 @@ __device__ __noinline__ ulonglong2 block_exclusive(unsigned long long v, unsigne
   return make_ulonglong2((warp > 0 ? before : 0ull) + inc - v, __shfl_sync(0xffffffffu, w, 31));
 }
 
-// Bitonic sort of n (a power of two, at most 2 SMP_THREADS) values, largest
-// first: thread t holds values 2t and 2t + 1.  Steps within a warp's 64 values
-// are shuffles, wider ones go through `buf`.
-__device__ __noinline__ ulonglong2 sort_descending(ulonglong2 c, unsigned long long* buf, uint32_t n) {
-  const uint32_t i = 2 * threadIdx.x;
-  for (uint32_t k = 2; k <= n; k *= 2)
-    for (uint32_t j = k / 2; j > 0; j /= 2) {
-      ulonglong2 o;  // the partners i ^ j, (i + 1) ^ j
-      if (j >= 64) {
-        __syncthreads();
-        buf[i] = c.x;
-        buf[i + 1] = c.y;
-        __syncthreads();
-        o.x = buf[i ^ j];
-        o.y = buf[(i ^ j) + 1];
-      } else if (j >= 2) {
-        o.x = __shfl_xor_sync(0xffffffffu, c.x, j / 2);
-        o.y = __shfl_xor_sync(0xffffffffu, c.y, j / 2);
-      } else {
-        o.x = c.y;
-        o.y = c.x;
+// Bitonic sort, largest first: thread t holds values 4 t to 4 t + 3.  The
+// steps of one round between lanes, then within the thread.
+__device__ __forceinline__ void order_pair(unsigned long long& a, unsigned long long& b, bool down) {
+  const bool swap = (a < b) == down;
+  const unsigned long long x = swap ? b : a, y = swap ? a : b;
+  a = x;
+  b = y;
+}
+__device__ __forceinline__ void take(unsigned long long& c, unsigned long long o, bool large) {
+  c = large == (o > c) ? o : c;
+}
+__device__ __forceinline__ void merge_in_warp(unsigned long long (&c)[4], uint32_t lanes, bool down) {
+  for (uint32_t j = lanes / 2; j > 0; j /= 2) {
+    const bool large = down == ((threadIdx.x & j) == 0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) take(c[q], __shfl_xor_sync(0xffffffffu, c[q], j), large);
+  }
+  order_pair(c[0], c[2], down);
+  order_pair(c[1], c[3], down);
+  order_pair(c[0], c[1], down);
+  order_pair(c[2], c[3], down);
+}
+// each warp's up to 128 values, in the directions of a longer sort
+__device__ __forceinline__ void warp_sort_descending(unsigned long long (&c)[4], uint32_t size) {
+  order_pair(c[0], c[1], true);
+  order_pair(c[2], c[3], false);
+  for (uint32_t k = 4; k <= size && k <= 128; k *= 2) merge_in_warp(c, k / 4, (4 * threadIdx.x & k) == 0);
+}
+// of n (a power of two, at most 2 SMP_THREADS) values, two a thread of the
+// CTA, through `buf`: 8 of its warps sort.  1024 values 2.4 us (two values a
+// thread and every step of more than 64 through shared memory: 5.3).
+__device__ __noinline__ ulonglong2 sort_descending(ulonglong2 v, unsigned long long* buf, uint32_t n) {
+  const uint32_t tid = threadIdx.x, i = 4 * tid;
+  ulonglong2* pairs = reinterpret_cast<ulonglong2*>(buf);
+  pairs[tid] = v;
+  __syncthreads();
+  if (i < 2 * SMP_THREADS) {
+    auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(SMP_THREADS / 2) : "memory"); };
+    const ulonglong2 a = pairs[2 * tid], b = pairs[2 * tid + 1];
+    unsigned long long c[4] = {a.x, a.y, b.x, b.y};
+    warp_sort_descending(c, n);
+    for (uint32_t k = 256; k <= n; k *= 2) {
+      const bool down = (i & k) == 0;
+      for (uint32_t j = k / 2; j >= 128; j /= 2) {  // between warps
+        sync();
+        pairs[2 * tid] = make_ulonglong2(c[0], c[1]);
+        pairs[2 * tid + 1] = make_ulonglong2(c[2], c[3]);
+        sync();
+        const bool large = down == ((i & j) == 0);
+        const ulonglong2 o = pairs[2 * (tid ^ (j / 4))], p = pairs[2 * (tid ^ (j / 4)) + 1];
+        take(c[0], o.x, large);
+        take(c[1], o.y, large);
+        take(c[2], p.x, large);
+        take(c[3], p.y, large);
       }
-      // the lower index of a pair keeps the larger value where (i & k) == 0
-      const bool down = (i & k) == 0, low = (i & j) == 0;
-      const bool large = down == low, large1 = j == 1 ? !large : large;
-      c.x = large == (o.x > c.x) ? o.x : c.x;
-      c.y = large1 == (o.y > c.y) ? o.y : c.y;
+      merge_in_warp(c, 32, down);
     }
-  return c;
+    sync();
+    pairs[2 * tid] = make_ulonglong2(c[0], c[1]);
+    pairs[2 * tid + 1] = make_ulonglong2(c[2], c[3]);
+  }
+  __syncthreads();
+  return pairs[tid];
 }
 
 // ---- passes over a warp's range [a, b) of vectors, results per lane
@@ -773,35 +807,6 @@ __device__ __noinline__ void cut_in_list(SampleShared& sh, int cs, uint32_t n, u
   }
 }
 
-// Bitonic sort, largest first, of `size` (a power of two, 4 to 128) values of
-// one warp: lane l holds values 4 l to 4 l + 3.
-__device__ __forceinline__ void order_pair(unsigned long long& a, unsigned long long& b, bool down) {
-  const bool swap = (a < b) == down;
-  const unsigned long long x = swap ? b : a, y = swap ? a : b;
-  a = x;
-  b = y;
-}
-__device__ __forceinline__ void warp_sort_descending(unsigned long long (&c)[4], uint32_t size) {
-  const uint32_t lane = threadIdx.x & 31;
-  order_pair(c[0], c[1], true);
-  order_pair(c[2], c[3], false);
-  for (uint32_t k = 4; k <= size; k *= 2) {
-    const bool down = (4 * lane & k) == 0;
-    for (uint32_t j = k / 8; j > 0; j /= 2) {  // between lanes
-      const bool large = down == ((lane & j) == 0);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const unsigned long long o = __shfl_xor_sync(0xffffffffu, c[q], j);
-        c[q] = large == (o > c[q]) ? o : c[q];
-      }
-    }
-    order_pair(c[0], c[2], down);
-    order_pair(c[1], c[3], down);
-    order_pair(c[0], c[1], down);
-    order_pair(c[2], c[3], down);
-  }
-}
-
 // finish_list by one warp, without a barrier: for as many candidates as a
 // usual top-k leaves (top-k 50 of 152064 tokens: one row 10.3 us a call, 11.9
 // by the whole CTA; 64 rows 13.2 and 17.7).
@@ -1255,7 +1260,15 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
   }
   if (use_m) {
     if (warp == 0) {
-      const uint32_t k = first_key(K::kNegInf + 1, sh.row.kmax, [&](uint32_t q) { return heavy(sh.row, K::value(q)); });
+      // at max + T log(min_p), up to roundings: searched a millionth around it
+      uint32_t lo = K::kNegInf + 1, hi = sh.row.kmax;
+      const double at = sh.row.xmax + (double)T * log(sh.row.min_w);
+      const double margin = 1e-6 * (fabs(at) + fabs(sh.row.xmax) + (double)T);
+      if (fabs(at) + margin < 3e38) {
+        lo = max(lo, K::of(__double2float_rd(at - margin)));
+        hi = min(hi, K::of(__double2float_ru(at + margin)) + 1);
+      }
+      const uint32_t k = first_key(lo, max(lo, hi), [&](uint32_t q) { return heavy(sh.row, K::value(q)); });
       if (lane == 0) sh.minp_key = k;
     }
     __syncthreads();
