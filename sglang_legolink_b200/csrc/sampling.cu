@@ -126,7 +126,7 @@ struct Key<uint32_t> {  // fp32
 };
 
 constexpr int SMP_RANGES = SMP_MAX_CLUSTER * SMP_WARPS;  // warp ranges of a row
-constexpr int SMP_OCTAVES = 16;            // powers of two of the weight, the last one open
+constexpr int SMP_OCTAVES = 16;            // bins of the weight, by powers of two (octave_start), the last one open
 constexpr int SMP_LIST = 2048;             // candidates, in one segment per CTA
 constexpr int SMP_FEW = 2 * SMP_THREADS;   // of them that one CTA sorts
 constexpr float SMP_LOWEST = -3.4028234663852886e38f;
@@ -378,8 +378,17 @@ __device__ __noinline__ uint32_t count_equal(const uint4* vals, int a, int b, fl
   return n;
 }
 
-// Approximate mass per bin floor(-log2 w) of all logits, to the thread's own
-// sums: w 2^(bin + 23) <= 2^23, rounded to a whole number.
+// Bins of a = -log2 w: eight of one octave, seven of two, the rest (a >= 22) in
+// the last.  A small nucleus wants narrow bins.  Of flat rows the largest
+// weight is far above most, and the cut falls at 15 to 20: with 16 bins of one
+// octave it was in the open one and took a pass more (64 flat rows 75 us, for 67; 16 of fp32 65, for 47).
+__host__ __device__ __forceinline__ constexpr int octave_start(int bin) { return bin < 8 ? bin : 2 * bin - 8; }
+__device__ __forceinline__ float octave_of(float a) {  // + 2^23
+  return __fadd_rd(fminf(fminf(a, fmaf(a, 0.5f, 4.f)), (float)(SMP_OCTAVES - 1)), 8388608.f);
+}
+
+// Approximate mass per bin of all logits, to the thread's own sums:
+// w 2^(octave_start + 23) <= 2^23, rounded to a whole number.
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -394,8 +403,9 @@ __device__ __noinline__ void octave_sums(const uint4* vals, int a, int b, float 
 #pragma unroll
     for (int i = 0; i < K::kPerVec; ++i) {
       const float arg = fmaf(x[i], fc, fm);  // < 0
-      const uint32_t bin = __float_as_uint(__fadd_rd(fminf(-arg, (float)(SMP_OCTAVES - 1)), 8388608.f)) - 0x4B000000u;
-      const float m = fmaf(ex2_approx(arg), __uint_as_float((127u + 23u + bin) << 23), 8388608.f);
+      const uint32_t bin = __float_as_uint(octave_of(-arg)) - 0x4B000000u;
+      const float m = fmaf(ex2_approx(arg), __uint_as_float((127u + 23u + (uint32_t)max((int)bin, 2 * (int)bin - 8)) << 23),
+                           8388608.f);
       mine[bin * SMP_THREADS] += __float_as_uint(m) - 0x4B000000u;
     }
   }
@@ -652,9 +662,9 @@ __device__ __forceinline__ uint32_t first_key(uint32_t lo, uint32_t hi, In in) {
 }
 
 // top-p over the whole row: the keys within which its cut falls, from
-// approximate masses.  The mass per power of two of the weight (bins
-// floor(-log2 w), the last one open), then, while the bin of the cut holds
-// many tokens for one histogram, the mass of its sixteenths.  What is selected
+// approximate masses.  The mass per power or two of the weight (octave_of),
+// then, while the bin of the cut holds many tokens for one histogram, the mass
+// of its sixteenths.  What is selected
 // within the keys is checked against exact sums; the few tokens of a small
 // nucleus are enough with the mass below them and its error.
 struct Nucleus {
@@ -693,8 +703,8 @@ __device__ __noinline__ Nucleus find_nucleus(SampleShared& sh, const uint4* vals
     if (lane < SMP_OCTAVES) {
       unsigned long long m = 0;
       for (int c = 0; c < cs; ++c) m += sh.octave[level & 1][c][lane];
-      // units: of bin b 2^(9 - 23 - b); of a later level, the weight of hi 2^(9 - 23)
-      mass = (double)m * (level == 0 ? __hiloint2double((1023 - 14 - lane) << 20, 0)
+      // units: of a bin 2^(9 - 23 - octave_start); of a later level, the weight of hi 2^(9 - 23)
+      mass = (double)m * (level == 0 ? __hiloint2double((1023 - 14 - octave_start(lane)) << 20, 0)
                                      : (double)ex2_approx(fmaf(fhi, fc, fm)) * (1.0 / 16384.0));
     }
     const double upto = warp_inclusive(mass, lane), all = __shfl_sync(0xffffffffu, upto, 31);
@@ -705,14 +715,16 @@ __device__ __noinline__ Nucleus find_nucleus(SampleShared& sh, const uint4* vals
     goal -= here - in;
     if (level == 0) {
       // tokens: by the bins' smallest weights, and what the coarser units dropped
-      const double n = lane < SMP_OCTAVES - 1 ? mass * (double)(2u << lane) * 1.001 + 1.0 : 1e30;
+      const double n = lane < SMP_OCTAVES - 1 ? mass * (double)(1u << octave_start(lane + 1)) * 1.001 + 1.0 : 1e30;
       r.tokens = __shfl_sync(0xffffffffu, warp_inclusive(n, lane), at);
-      // error: 2^-22 (ex2) + 2^-23 (rounded to a whole) + 2 * 2^-24 |arg| ln 2
-      // (argument; the open bin: at most 46); its wholes, and the coarser units
+      // error: 2^-22 (ex2) + 2^-22 (rounded to a whole, of 2^21 or more) +
+      // 2 * 2^-24 |arg| ln 2 (argument; the open bin: at most 46); its wholes
+      // (half of 2^-45 a token), and the coarser units
       double err = lane < SMP_OCTAVES
-                       ? mass * ((1.5 + 0.35 * (lane == SMP_OCTAVES - 1 ? 46.0 : lane + 1.0)) * (1.01 / 4194304.0)) +
-                             (lane == SMP_OCTAVES - 1 ? (double)V : 0.0) * __hiloint2double((1023 - 39) << 20, 0) +
-                             cs * __hiloint2double((1023 - 14 - lane) << 20, 0)
+                       ? mass * ((2.0 + 0.35 * (lane == SMP_OCTAVES - 1 ? 46.0 : octave_start(lane + 1))) *
+                                 (1.01 / 4194304.0)) +
+                             (lane == SMP_OCTAVES - 1 ? (double)V : 0.0) * __hiloint2double((1023 - 46) << 20, 0) +
+                             cs * __hiloint2double((1023 - 14 - octave_start(lane)) << 20, 0)
                        : 0.0;
       err = warp_inclusive(err, lane);
       r.below = all - here;
@@ -725,7 +737,7 @@ __device__ __noinline__ Nucleus find_nucleus(SampleShared& sh, const uint4* vals
       if (warp == 0 ? at < SMP_OCTAVES - 1 : at > 0)
         k = first_key(r.lo, r.hi, [&](uint32_t q) {
           const float x = K::value(q);
-          return level == 0 ? fmaf(x, fc, fm) > -(float)b : bin_of(x, fhi, sc) < 8388608.f + (float)b;
+          return (level == 0 ? octave_of(-fmaf(x, fc, fm)) : bin_of(x, fhi, sc)) < 8388608.f + (float)b;
         });
       if (lane == 0) sh.edge[warp] = k;
     }
