@@ -35,7 +35,7 @@
 // 0.5 to 2 us (10.3 us for one row of 152064 tokens with top-k and top-p); a
 // batch of flat rows, the double operations of the exact sums (256 rows with
 // temperature alone 91 us, of which reading the logits is 12; 64 rows with
-// top-p 74 us, with three passes that evaluate every token).
+// top-p 67 us, with three passes that evaluate every token).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -343,7 +343,7 @@ __device__ __noinline__ ExactSum exact_sum(const uint4* vals, int a, int b, floa
 
 // The same where [from, upto] holds few of the tokens: over the set bits of a
 // mask, as many rounds as the fullest lane has, not over all of the vector's
-// elements (64 flat rows of 152064 tokens: 74 us a call, 78 without).
+// elements (64 flat rows of 152064 tokens: 66.7 us a call, 68.6 without).
 template <typename Raw>
 __device__ __noinline__ unsigned long long exact_sum_of_few(const uint4* vals, int a, int b, float from, float upto,
                                                             double xmax, double k1, const double* table) {
@@ -378,13 +378,15 @@ __device__ __noinline__ uint32_t count_equal(const uint4* vals, int a, int b, fl
   return n;
 }
 
-// Bins of a = -log2 w: eight of one octave, seven of two, the rest (a >= 22) in
-// the last.  A small nucleus wants narrow bins.  Of flat rows the largest
-// weight is far above most, and the cut falls at 15 to 20: with 16 bins of one
-// octave it was in the open one and took a pass more (64 flat rows 75 us, for 67; 16 of fp32 65, for 47).
-__host__ __device__ __forceinline__ constexpr int octave_start(int bin) { return bin < 8 ? bin : 2 * bin - 8; }
+// Bins of a = -log2 w: fifteen of two octaves, the rest (a >= 30) in the last.
+// Of a flat row the largest weight is far above most, and top-p's cut falls at
+// 15 to 20: with bins of one octave it was in the open one and took a pass
+// more (64 such rows 75 us, 67 now; 16 of fp32 65, 47).  Eight bins of one
+// octave before wider ones cost more to tell apart than their shorter lists
+// of a small nucleus save (68).
+__host__ __device__ __forceinline__ constexpr int octave_start(int bin) { return 2 * bin; }
 __device__ __forceinline__ float octave_of(float a) {  // + 2^23
-  return __fadd_rd(fminf(fminf(a, fmaf(a, 0.5f, 4.f)), (float)(SMP_OCTAVES - 1)), 8388608.f);
+  return __fadd_rd(fminf(a * 0.5f, (float)(SMP_OCTAVES - 1)), 8388608.f);
 }
 
 // Approximate mass per bin of all logits, to the thread's own sums:
@@ -404,7 +406,7 @@ __device__ __noinline__ void octave_sums(const uint4* vals, int a, int b, float 
     for (int i = 0; i < K::kPerVec; ++i) {
       const float arg = fmaf(x[i], fc, fm);  // < 0
       const uint32_t bin = __float_as_uint(octave_of(-arg)) - 0x4B000000u;
-      const float m = fmaf(ex2_approx(arg), __uint_as_float((127u + 23u + (uint32_t)max((int)bin, 2 * (int)bin - 8)) << 23),
+      const float m = fmaf(ex2_approx(arg), __uint_as_float((127u + 23u + 2u * bin) << 23),
                            8388608.f);
       mine[bin * SMP_THREADS] += __float_as_uint(m) - 0x4B000000u;
     }
@@ -719,11 +721,11 @@ __device__ __noinline__ Nucleus find_nucleus(SampleShared& sh, const uint4* vals
       r.tokens = __shfl_sync(0xffffffffu, warp_inclusive(n, lane), at);
       // error: 2^-22 (ex2) + 2^-22 (rounded to a whole, of 2^21 or more) +
       // 2 * 2^-24 |arg| ln 2 (argument; the open bin: at most 46); its wholes
-      // (half of 2^-45 a token), and the coarser units
+      // (half of 2^-53 a token), and the coarser units
       double err = lane < SMP_OCTAVES
                        ? mass * ((2.0 + 0.35 * (lane == SMP_OCTAVES - 1 ? 46.0 : octave_start(lane + 1))) *
                                  (1.01 / 4194304.0)) +
-                             (lane == SMP_OCTAVES - 1 ? (double)V : 0.0) * __hiloint2double((1023 - 46) << 20, 0) +
+                             (lane == SMP_OCTAVES - 1 ? (double)V : 0.0) * __hiloint2double((1023 - 54) << 20, 0) +
                              cs * __hiloint2double((1023 - 14 - octave_start(lane)) << 20, 0)
                        : 0.0;
       err = warp_inclusive(err, lane);
