@@ -242,6 +242,62 @@ def bench_tp_reduce(pk, with_torch):
     return rows
 
 
+def bench_lora(pk, with_torch):
+    """A projection with each row's low-rank adapter; the fraction is of the
+    longer of its bytes at HBM rate and its operations at the GEMM rate."""
+    rows = []
+    for M, N, K, R, n, swiglu in [(1, 4608, 3584, 48, 1, False), (16, 37888, 3584, 32, 8, True),
+                                  (61, 5120, 8192, 16, 32, False), (300, 4608, 3584, 48, 3, False),
+                                  (5087, 4608, 3584, 48, 4, False), (2048, 37888, 3584, 32, 6, True)]:
+        x = torch.randn(M, K, device="cuda", dtype=torch.bfloat16)
+        w = torch.randn(N, K, device="cuda", dtype=torch.bfloat16) * K ** -0.5
+        a = torch.randn(n, R, K, device="cuda", dtype=torch.bfloat16) * K ** -0.5
+        b = torch.randn(n, N, R, device="cuda", dtype=torch.bfloat16) * 0.05
+        stack = ops.LoraStack(a, b, torch.ones(n, device="cuda"))
+        plan = ops.lora_plan(torch.arange(M) % n if M <= 128 else torch.arange(M) * n // M, "cuda")
+        out = torch.empty(M, N // 2 if swiglu else N, device="cuda", dtype=torch.bfloat16)
+        ms = time_fn(lambda: ops.linear_lora(x, w, None, stack, plan, out=out, swiglu_epilogue=swiglu))
+        byts = 2 * (x.numel() + w.numel() + a.numel() + b.numel() + out.numel())
+        floor = max(byts / pk["hbm_gbs"] / 1e6, 2 * M * (N * K + R * (N + K)) / pk["bf16_tflops"] / 1e9)
+        row = {"op": f"linear_lora[M{M},N{N},K{K},rank{R},{n} adapters{',swiglu' if swiglu else ''}]",
+               "ms": round(ms, 4), "frac_of_floor": round(floor / ms, 3)}
+        if with_torch:  # the projection alone
+            row["torch_linear_ms"] = round(time_fn(lambda: x @ w.t()), 4)
+        rows.append(row)
+    return rows
+
+
+def bench_sample(pk, with_torch):
+    """A batch of rows drawn in one launch, against reading the logits once."""
+    rows = []
+    V = 152064
+    for B, kind in [(1, "top_k"), (16, "top_k"), (64, "top_k"), (16, "top_p"), (64, "top_p"), (64, "temperature"),
+                    (256, "temperature")]:
+        x = (torch.randn(B, V, device="cuda") * 2).to(torch.bfloat16)
+        u = torch.rand(B, device="cuda", dtype=torch.float64)
+        t = torch.full((B,), 0.8, device="cuda")
+        k = torch.full((B,), 50, device="cuda", dtype=torch.int32) if kind == "top_k" else None
+        p = torch.full((B,), 0.9, device="cuda") if kind != "temperature" else None
+        ms = time_fn(lambda: ops.sample(x, u, t, k, p))
+        gbs = B * V * 2 / ms / 1e6
+        row = {"op": f"sample[{B} rows x {V},{kind}]", "ms": round(ms, 4), "gbs": round(gbs, 1),
+               "frac_of_hbm": round(gbs / pk["hbm_gbs"], 3)}
+        if with_torch:
+            def plain():
+                y = x.float() / 0.8
+                if k is not None:
+                    y = torch.where(y < torch.topk(y, 50).values[:, -1:], -math.inf, y)
+                q = torch.softmax(y, -1)
+                if p is not None:
+                    s, i = torch.sort(q, dim=-1, descending=True)
+                    q = torch.zeros_like(q).scatter_(-1, i, torch.where(s.cumsum(-1) - s < 0.9, s, 0.0))
+                return torch.multinomial(q, 1)
+
+            row["torch_ms"] = round(time_fn(plain), 4)
+        rows.append(row)
+    return rows
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--only", default="gemm,small_m,attn,kv_link")
@@ -249,7 +305,8 @@ def main():
     a = ap.parse_args()
     pk = peaks()
     fns = {"gemm": bench_gemm, "small_m": bench_small_m, "attn": bench_attention, "kv_link": bench_kv_link,
-           "attn_variants": bench_attention_variants, "tp_reduce": bench_tp_reduce}
+           "attn_variants": bench_attention_variants, "tp_reduce": bench_tp_reduce, "lora": bench_lora,
+           "sample": bench_sample}
     for name in a.only.split(","):
         for r in fns[name](pk, a.torch):
             r["peaks"] = pk["src"]
