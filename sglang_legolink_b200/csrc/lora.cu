@@ -72,8 +72,6 @@ __global__ void __launch_bounds__(128, 2)
   const int cs = gridDim.x, crank = blockIdx.x;
   const int plane = blockIdx.z;
 
-  pdl_trigger();
-
   // which rows and which adapter: the same for every CTA of the cluster
   const int planes = lo.tile_ptr[lo.tiles];
   if (plane >= planes) {
@@ -99,6 +97,7 @@ __global__ void __launch_bounds__(128, 2)
   const int groups = (lo.packed() ? 32 : lo.rank) / 4;  // 4 columns a thread
   if (!__syncthreads_or(mine)) {   // no row of this half uses the adapter
     pdl_wait();
+    pdl_trigger();
     for (int i = crank * 128 + tid; i < rows * groups; i += cs * 128) {
       bf16* d = low + (size_t)(i / groups) * ld + 4 * (i % groups);
       *reinterpret_cast<uint2*>(d) = make_uint2(0, 0);
@@ -135,6 +134,9 @@ __global__ void __launch_bounds__(128, 2)
       tma_load_3d(sA + i * a_bytes, &tmA, &full[i], (kb0 + i) * LOW_BK, 0, adapter);
     }
     pdl_wait();
+    // only now: every CTA that lets the product start has seen x complete, so
+    // the product may read x at once (lora_gemv_kernel, `x_ready`)
+    pdl_trigger();
     for (int i = 0; i < pre; ++i)
       tma_load_2d(sX + i * LOW_BM * LOW_BK * 2, &tmX, &full[i], (kb0 + i) * LOW_BK, m0);
     int stage = pre % shp.stages;
@@ -250,8 +252,16 @@ __global__ void __launch_bounds__(128, 2)
 // memory and no CTA waits for a last one to add up 128 features x M rows x all
 // splits (at 61 rows x 5120 features, 7 splits, that fix-up alone was 40 of 62
 // us).  Each split takes its share of the k-blocks of K, then its share of the
-// adapters'.  The first ring of weights is on its way before the wait for the
-// low-rank kernel.  Bound by reading weights: 16 rows, 3584 -> 37888 with
+// adapters'.
+//
+// Behind the few-row kernel (2 to 5 us) the first ring of weights is on its way
+// while that one waits for x and runs.  Behind the tensor-core kernel (10 us
+// and more) this one starts when x is there (`x_ready`) and runs the k-blocks
+// of K beside it; the wait comes before the adapters' k-blocks: 300 rows, 3584
+// -> 4608, rank 48, 27.9 -> 22.2 us, 300 x 3584 x 18944 84.7 -> 66.8.  (The same
+// behind the few-row kernel: 16 rows, 3584 -> 37888, 48.4 -> 50.0.)
+//
+// Bound by reading weights: 16 rows, 3584 -> 37888 with
 // SwiGLU and 6 adapters of rank 32 in 48.4 us for both kernels, 6.1 TB/s.
 constexpr int GEMV_RING = 108 * 1024;
 // Clusters do not fill the SMs to the last place (two CTAs a SM, 296 places):
@@ -281,7 +291,7 @@ template <int BNX, bool SWIGLU>
 __global__ void __launch_bounds__(192, 2)
     lora_gemv_kernel(const __grid_constant__ GemvMaps tm, bf16* __restrict__ C, int64_t ldc,
                      const bf16* __restrict__ bias, int rows, int N, int K, const __grid_constant__ LLLora lo,
-                     int* err) {
+                     bool x_ready, int* err) {
   using Cfg = GemvCfg<BNX>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -330,7 +340,8 @@ __global__ void __launch_bounds__(192, 2)
         mbar_arrive_expect_tx(&full[i], Cfg::W_BYTES + Cfg::X_BYTES);
         tma_load_2d(sW + i * Cfg::W_BYTES, &tm.w, &full[i], (kb0 + i) * LOW_BK, nb * 128);
       }
-      pdl_wait();
+      bool waited = !x_ready;
+      if (waited) pdl_wait();
       for (int i = 0; i < steps; ++i) {
         const int kb = kb0 + i;
         if (i >= pre) {
@@ -344,6 +355,8 @@ __global__ void __launch_bounds__(192, 2)
           if (i >= pre) tma_load_2d(sW + stage * Cfg::W_BYTES, &tm.w, &full[stage], kb * LOW_BK, nb * 128);
           tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.x, &full[stage], kb * LOW_BK, m0);
         } else {
+          if (!waited) pdl_wait();
+          waited = true;
           const int e = e0 + kb - kb1;
           const int plane = p0 + e / per_plane, s = e % per_plane, rb = s >> 1;
           tma_load_3d(sW + stage * Cfg::W_BYTES, &tm.b, &full[stage], rb * LOW_BK, nb * 128,
@@ -585,14 +598,25 @@ static bool low_tmap(CUtensorMap* tm, const void* ptr, int rank, const cuuint64_
 
 using namespace ll;
 
+// The few-row kernel's grid, and whether it is the one to take.
+static dim3 rows_grid(int M, int K, int rank, int* ks) {
+  *ks = 1;  // warps of a row and rank
+  while (*ks < 8 && *ks * ROWS_VEC * 256 < K) *ks *= 2;
+  return dim3(M, (rank + 8 / *ks - 1) / (8 / *ks));
+}
+static bool by_rows(int M, int K, int rank) {
+  int ks;
+  const dim3 g = rows_grid(M, K, rank, &ks);
+  return (int64_t)g.x * g.y <= (ks > 1 ? ROWS_LONG : ROWS_SHORT);
+}
+
 extern "C" int ll_lora_low(const bf16* x, int64_t ldx, int M, int K, const LLLora* lo, int* err, cudaStream_t stream) {
   if (M <= 0) return 0;
   if ((K % 8) || (ldx % 8) || lo->rank <= 0 || lo->rank > LL_LORA_MAX_RANK || (lo->rank % 8)) return -3;
   if (lo->max_planes < 1 || lo->max_planes > 65535) return -3;
-  int ks = 1;  // warps of a row and rank
-  while (ks < 8 && ks * ROWS_VEC * 256 < K) ks *= 2;
-  const dim3 grid(M, (lo->rank + 8 / ks - 1) / (8 / ks));
-  if ((int64_t)grid.x * grid.y <= (ks > 1 ? ROWS_LONG : ROWS_SHORT)) {
+  if (by_rows(M, K, lo->rank)) {
+    int ks;
+    const dim3 grid = rows_grid(M, K, lo->rank, &ks);
     const cudaError_t e =
         launch_pdl(lora_low_rows_kernel, grid, dim3(256), 0, stream, x, ldx, M, K, *lo, ks, err);
     return e == cudaSuccess ? 0 : -5;
@@ -681,6 +705,7 @@ extern "C" int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const bool x_ready = !by_rows(M, K, lo->rank);
   cudaError_t e;
 #define LL_GEMV(BNX_, SW_)                                                                      \
   do {                                                                                          \
@@ -688,7 +713,7 @@ extern "C" int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, 
     static unsigned long long done = 0;                                                         \
     if (!smem_on_device(kern, GemvCfg<BNX_>::SMEM, done)) return -7;                            \
     cfg.dynamicSmemBytes = GemvCfg<BNX_>::SMEM;                                                 \
-    e = cudaLaunchKernelEx(&cfg, kern, tm, C, ldc, bias, M, N, K, *lo, err);                    \
+    e = cudaLaunchKernelEx(&cfg, kern, tm, C, ldc, bias, M, N, K, *lo, x_ready, err);                    \
   } while (0)
 #define LL_GEMV_SW(BNX_)              \
   do {                                \
