@@ -484,12 +484,15 @@ __device__ __forceinline__ uint4 ld_after_wait(const uint4* p) {
 // share it.  Fewer registers (4 vectors a lane, 62) and more CTAs a SM: 61 rows
 // 25.6 to 27.7 us a call for 26.8, one row 9.7 to 10.6 for 9.6.
 //
-// Each (row, rank) is a CTA's share, two CTAs a SM: used up to one and a half
-// rounds of the 296 places, two where K is long.  us a call with this kernel /
-// the tensor cores': 64 rows, rank 32, K = 1024 (256 CTAs) 8.0 / 9.3; 64, 64,
-// 1024 (512) 9.9 / 9.4; 64, 32, 4096 (512) 12.4 / 12.8; 600, 16, 128 (1200)
-// 17.0 / 11.9; 2500, 16, 128 (5000) 42.7 / 12.0.
-constexpr int ROWS_SHORT = 444, ROWS_LONG = 592;
+// Each (row, rank) is a CTA's share, two CTAs a SM: used up to one round of the
+// 296 places, two (one and a half where K is short) where a tile has many
+// planes, each of which costs the tensor-core kernel CTAs and loads.  us a call
+// with this kernel / the tensor cores', 4608 features: 48 rows, K = 3584, rank
+// 16 (192 CTAs) 11.4 / 12.7; 64, 1024, 32 (256) 10.3 / 11.0; 48, 3584, 32 (384)
+// 13.6 / 12.8; 96, 3584, 16 (384) with 6 planes 16.0 / 14.8, with 57 24.8 /
+// 27.2; 61, 8192, 16 (488) with 26 planes 26.0 / 27.7; 64, 3584, 48 (768) with 6
+// planes 17.7 / 14.3.
+constexpr int ROWS_PLACES = 296, ROWS_SHORT = 444, ROWS_LONG = 592, ROWS_PLANES = 8;
 constexpr int ROWS_VEC = 8;  // 16-byte vectors a lane holds: 2048 elements of K a warp
 __global__ void __launch_bounds__(256, 2) lora_low_rows_kernel(const bf16* x, int64_t ldx, int M, int K,
                                                                const __grid_constant__ LLLora lo, int ks, int* err) {
@@ -604,17 +607,17 @@ static dim3 rows_grid(int M, int K, int rank, int* ks) {
   while (*ks < 8 && *ks * ROWS_VEC * 256 < K) *ks *= 2;
   return dim3(M, (rank + 8 / *ks - 1) / (8 / *ks));
 }
-static bool by_rows(int M, int K, int rank) {
+static bool by_rows(int M, int K, const LLLora& lo) {
   int ks;
-  const dim3 g = rows_grid(M, K, rank, &ks);
-  return (int64_t)g.x * g.y <= (ks > 1 ? ROWS_LONG : ROWS_SHORT);
+  const dim3 g = rows_grid(M, K, lo.rank, &ks);
+  return (int64_t)g.x * g.y <= (lo.max_planes <= ROWS_PLANES ? ROWS_PLACES : (ks > 1 ? ROWS_LONG : ROWS_SHORT));
 }
 
 extern "C" int ll_lora_low(const bf16* x, int64_t ldx, int M, int K, const LLLora* lo, int* err, cudaStream_t stream) {
   if (M <= 0) return 0;
   if ((K % 8) || (ldx % 8) || lo->rank <= 0 || lo->rank > LL_LORA_MAX_RANK || (lo->rank % 8)) return -3;
   if (lo->max_planes < 1 || lo->max_planes > 65535) return -3;
-  if (by_rows(M, K, lo->rank)) {
+  if (by_rows(M, K, *lo)) {
     int ks;
     const dim3 grid = rows_grid(M, K, lo->rank, &ks);
     const cudaError_t e =
@@ -705,7 +708,7 @@ extern "C" int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  const bool x_ready = !by_rows(M, K, lo->rank);
+  const bool x_ready = !by_rows(M, K, *lo);
   cudaError_t e;
 #define LL_GEMV(BNX_, SW_)                                                                      \
   do {                                                                                          \
