@@ -41,6 +41,7 @@
 
 #include <climits>
 #include <cstddef>
+#include <utility>
 
 #include "common.cuh"
 #include "sampling.h"
@@ -977,6 +978,9 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int V = p.V, ranges = cs * SMP_WARPS;
 
+  // another CTA's shared memory may be written once that CTA has started: every
+  // CTA says so here, and the wait is where the load is done
+  auto started = cluster.barrier_arrive();
   pdl_trigger();
   if (tid == 0) sh.redo = 0;
   if (tid < 32) sh.exp2_table[tid] = exp2((double)tid / 32.0);
@@ -1045,6 +1049,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
       kth = __shfl_sync(0xffffffffu, mine, __ffs(at) - 1);
     }
     const float wmax = warp_max(mine);
+    cluster.barrier_wait(std::move(started));
     if (lane < cs) {
       cluster.map_shared_rank(sh.wmax, lane)[rank * SMP_WARPS + warp] = wmax;
       cluster.map_shared_rank(sh.wkth, lane)[rank * SMP_WARPS + warp] = kth;
