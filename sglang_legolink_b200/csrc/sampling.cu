@@ -440,12 +440,14 @@ __device__ __noinline__ void refine_sums(const uint4* vals, int a, int b, float 
 }
 
 // Tokens per bin of (key - lo) >> shift, keys in [lo, hi]; given `weight`,
-// their weights too.
+// their weights too.  The key below that of 0 would be -0's and is no value's:
+// a range that ends there ends at the one before, since +0 <= -0.
 template <typename Raw>
-__device__ __noinline__ void histogram(const uint4* vals, int a, int b, float flo, float fhi, uint32_t lo, int shift,
+__device__ __noinline__ void histogram(const uint4* vals, int a, int b, uint32_t lo, uint32_t hi, int shift,
                                        uint32_t* count, unsigned long long* weight, double xmax, double k1,
                                        const double* table) {
   using K = Key<Raw>;
+  const float flo = K::value(lo), fhi = K::value(hi == K::of(0.f) - 1 ? hi - 1 : hi);
   for (int v = a + (threadIdx.x & 31); v < b; v += 32) {
     const uint4 q = vals[v];
     if (K::largest(q) < flo) continue;
@@ -576,8 +578,8 @@ __device__ __noinline__ Selected select(SampleShared& sh, const uint4* vals, int
       if (weighted) sh.weight[i] = 0;
     }
     __syncthreads();
-    histogram<Raw>(vals, v0, v1, K::value(lo), K::value(hi), lo, shift, sh.count, weighted ? sh.weight : nullptr,
-                   sh.row.xmax, sh.row.k1, sh.exp2_table);
+    histogram<Raw>(vals, v0, v1, lo, hi, shift, sh.count, weighted ? sh.weight : nullptr, sh.row.xmax, sh.row.k1,
+                   sh.exp2_table);
     cluster.sync();
     // thread t merges four bins, thread 0 the largest keys; every CTA's at once
     uint32_t cnt[PER] = {};
