@@ -250,12 +250,15 @@ class Engine:
         return d
 
     def compat_key(self, adapter_id=None, segmentation_policy_version=None, legolink_policy_version=None) -> str:
+        def text(v) -> str:  # the request's own: "|" parts the fields, "#" an adapter from its weights
+            return str(v).replace("%", "%25").replace("|", "%7C").replace("#", "%23")
+
         c = dict(self.compat)
-        c["adapter_id"] = str(adapter_id or "none")
+        c["adapter_id"] = text(adapter_id or "none")
         if self._adapter(adapter_id) >= 0:
             c["adapter_id"] += "#" + self.model.adapter_digests[self._adapter(adapter_id)]
-        c["segmentation_policy_version"] = str(segmentation_policy_version or "field-first-v1")
-        c["legolink_policy_version"] = str(legolink_policy_version or LEGOLINK_POLICY_VERSION)
+        c["segmentation_policy_version"] = text(segmentation_policy_version or "field-first-v1")
+        c["legolink_policy_version"] = text(legolink_policy_version or LEGOLINK_POLICY_VERSION)
         return "|".join(f"{k}={c[k]}" for k in sorted(c))
 
     # -------------------------------------------------------------- adapters
