@@ -79,6 +79,7 @@ class Sequence_:
     generator: Optional[torch.Generator] = None
     promotion: Optional[dict] = None  # record of an experimental group promotion
     adapter: int = -1  # index of the model's adapter it runs with
+    error: Optional[Exception] = None  # it failed alone in a batch; it decodes no further
 
 
 @dataclass
@@ -461,12 +462,11 @@ class Engine:
         ids[: len(params)] = drawn.to(ids.device)
         return ids
 
-    def _tokens(self, ids: torch.Tensor) -> list[int]:
-        """Sampled ids on the host; a sampled row with nothing to draw is an error."""
-        out = ids.tolist()
-        if self.sampler == "kernel" and min(out, default=0) < 0:
-            raise KernelFault("sampling: a row of logits holds no number above -inf")
-        return out
+    @staticmethod
+    def _no_token() -> KernelFault:
+        """The error of a sampled row with nothing to draw, id -1 (the
+        one-launch sampler's answer); it is that row's alone."""
+        return KernelFault("sampling: a row of logits holds no number above -inf")
 
     def _new_sampling(self, sampling: Optional[SamplingParams]):
         sp = sampling or GREEDY
@@ -798,7 +798,7 @@ class Engine:
                             o += len(toks)
                         fb.repair_meta = {"batch_execution_unit_size": len(prepared), "repair_ranges": ranges}
                     logits = self.model.forward(fb, self.kv)
-                    firsts = self._tokens(self._sample(logits, params, gens))
+                    firsts = self._sample(logits, params, gens).tolist()
                 self._kernel_check("link" if works else "compile")
             except Exception as e:
                 for i, *_rest, pages in prepared:
@@ -822,7 +822,10 @@ class Engine:
                     c_out[i] = e
             # ---- Links: close reservations, account, build sequences
             for (i, w), first in zip(works, firsts[len(prepared):]):
-                self._link_close(w, ok=True)
+                self._link_close(w, ok=first >= 0)
+                if first < 0:
+                    l_out[i] = self._no_token()
+                    continue
                 seq = Sequence_(rid=w.rid, token_ids=list(w.resolved.linked_token_ids), pages=w.pages,
                                 length=w.resolved.total_token_count, output_ids=[int(first)], kind="link",
                                 link_plan=w.resolved, sampling=w.sampling, generator=w.generator,
@@ -996,8 +999,10 @@ class Engine:
                 sp, gen = self._new_sampling(sampling)
                 fb = self._extend_batch([(toks[start:], list(range(start, n)), pages, n)], adapters=[ad])
                 logits = self.model.forward(fb, self.kv)
-                first = self._tokens(self._sample(logits, [sp], [gen])[:1])[0]
+                first = int(self._sample(logits, [sp], [gen])[0].item())
                 self._kernel_check("prefill")
+                if first < 0:
+                    raise self._no_token()
             except Exception:
                 self.alloc.release(pages)
                 raise
@@ -1010,9 +1015,12 @@ class Engine:
     # ---------------------------------------------------------------- decode
     def decode(self, seqs: list[Sequence_], steps: int, stop_ids: Sequence[int] = ()) -> None:
         """Greedy-decode ``steps`` tokens for every sequence (in place).  The
-        last output token of each sequence is fed as the next input."""
+        last output token of each sequence is fed as the next input.  A
+        sequence that fails alone (``error``) stops there; its error is raised
+        once the others are done."""
         stop = set(int(s) for s in stop_ids)
         done = 0
+        failed = None
         while done < steps:
             live = [s for s in seqs if not s.finished]
             if not live:
@@ -1025,9 +1033,14 @@ class Engine:
             nxt = self.decode_step(live)
             done += 1
             for s, t in zip(live, nxt):
+                if s.error is not None:
+                    failed = failed or s.error
+                    continue
                 s.output_ids.append(int(t))
                 if int(t) in stop:
                     s.finished = True
+        if failed is not None:
+            raise failed
 
     def warm_decode(self, seqs: list[Sequence_]) -> None:
         """Captures the CUDA graph that a greedy decode of ``seqs`` replays
@@ -1109,7 +1122,12 @@ class Engine:
             self.stats["decode_steps"] += steps
 
     def decode_step(self, seqs: list[Sequence_]) -> list[int]:
+        """One token for every sequence.  -1 for one whose row held nothing to
+        draw: its ``error`` is set, and a later step with it is refused."""
         with self._lock:
+            for s in seqs:
+                if s.error is not None:
+                    raise s.error
             B = len(seqs)
             for s in seqs:
                 self._ensure_capacity(s, s.length + 1)
@@ -1117,9 +1135,11 @@ class Engine:
                 out = self._graph_step(seqs)
             else:
                 out = self._eager_step(seqs)
-            for s in seqs:
+            for s, t in zip(seqs, out):
                 s.token_ids.append(s.output_ids[-1])
                 s.length += 1
+                if t < 0:
+                    s.error, s.finished = self._no_token(), True
             self.stats["decode_steps"] += 1
             return out
 
@@ -1154,7 +1174,7 @@ class Engine:
                           q_indptr=torch.arange(B + 1, dtype=torch.int32).to(dev), page_table=pt.to(dev),
                           kv_lens=kvl.to(dev), logit_rows=None, lora=self._rows_plan([s.adapter for s in seqs], 1))
         logits = self.model.forward(fb, self.kv)
-        out = self._tokens(self._sample(logits, [s.sampling for s in seqs], [s.generator for s in seqs]))
+        out = self._sample(logits, [s.sampling for s in seqs], [s.generator for s in seqs]).tolist()
         self._kernel_check("decode")
         return out
 
@@ -1178,8 +1198,8 @@ class Engine:
         g["graph"].replay()
         launch_count.add(g["launches"])
         if any(not s.sampling.greedy for s in seqs):
-            out = self._tokens(self._sample(g["logits"][:B], [s.sampling for s in seqs], [s.generator for s in seqs],
-                                            greedy=g["out"][:B]))
+            out = self._sample(g["logits"][:B], [s.sampling for s in seqs], [s.generator for s in seqs],
+                               greedy=g["out"][:B]).tolist()
         else:
             out = g["out"][:B].tolist()
         self._kernel_check("decode")

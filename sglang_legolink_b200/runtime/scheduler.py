@@ -481,6 +481,11 @@ class Scheduler:
         self.stats["decode_steps"] += 1
         still = []
         for r, t in zip(self.running, toks):
+            if r.seq.error is not None:  # its row alone; the others go on
+                emit_trace("legolink_request_failed_closed", rid=r.rid, kind=r.kind, reason=str(r.seq.error)[:500])
+                r.events.put(("error", f"decode failed: {r.seq.error!r}"))
+                eng.free(r.seq)
+                continue
             r.seq.output_ids.append(int(t))
             r.events.put(("token", int(t)))
             n = len(r.seq.output_ids)
