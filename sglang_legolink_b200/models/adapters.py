@@ -73,30 +73,51 @@ class Adapter:
         return cls.from_state(state, float(cfg["lora_alpha"]), int(cfg["r"]), bool(cfg.get("use_rslora")))
 
 
-def _merged(adapters: list, layer: int, parts: list, in_dim: int):
-    """The adapters' (a, per-part b) of a fused projection, its parts
-    ``(name, rows)`` stacked in the rank; None where no adapter has any."""
-    ranks = [sum(ad.mats[(layer, n)][0].shape[0] for n, _ in parts if (layer, n) in ad.mats) for ad in adapters]
-    if not any(ranks):
-        return None
-    rank = -(-max(ranks) // 8) * 8
-    if rank > ops.LORA_MAX_RANK:
-        raise ValueError(f"layer {layer} {'+'.join(n for n, _ in parts)}: rank {max(ranks)} of the fused projection "
-                         f"exceeds {ops.LORA_MAX_RANK}")
-    a = torch.zeros(len(adapters), rank, in_dim)
-    b = [torch.zeros(len(adapters), rows, rank) for _, rows in parts]
-    for i, ad in enumerate(adapters):
-        at = 0
-        for (name, rows), bp in zip(parts, b):
-            if (layer, name) not in ad.mats:
-                continue
-            ma, mb = ad.mats[(layer, name)]
-            r = ma.shape[0]
-            if tuple(ma.shape) != (r, in_dim) or tuple(mb.shape) != (rows, r):
-                raise ValueError(f"adapter of layer {layer} {name}: a {tuple(ma.shape)}, b {tuple(mb.shape)} do not "
-                                 f"fit a projection [{rows}, {in_dim}]")
-            a[i, at:at + r] = ma.float()
-            bp[i, :, at:at + r] = mb.float()
+# the projections of a layer's stacks: of each part its name and (in, out) sizes
+def _stacks(cfg) -> dict:
+    H, inter = cfg.hidden_size, cfg.intermediate_size
+    return {"qkv": (("q_proj", H, cfg.q_size), ("k_proj", H, cfg.kv_size), ("v_proj", H, cfg.kv_size)),
+            "o": (("o_proj", cfg.q_size, H),),
+            "gu": (("gate_proj", H, inter), ("up_proj", H, inter)),
+            "down": (("down_proj", inter, H),)}
+
+
+def check_adapter(cfg, adapter: Adapter, dtype) -> None:
+    """Raises ValueError where the adapter does not fit the model, before
+    anything of it is on the device."""
+    if not torch.isfinite(torch.tensor(adapter.scale, dtype=torch.float32)):
+        raise ValueError("adapter weights must be finite")
+    for parts in _stacks(cfg).values():
+        for layer in range(cfg.num_layers):
+            rank = 0
+            for name, in_dim, rows in parts:
+                if (layer, name) not in adapter.mats:
+                    continue
+                ma, mb = adapter.mats[(layer, name)]
+                r = ma.shape[0]
+                if tuple(ma.shape) != (r, in_dim) or tuple(mb.shape) != (rows, r):
+                    raise ValueError(f"adapter of layer {layer} {name}: a {tuple(ma.shape)}, b {tuple(mb.shape)} do not "
+                                     f"fit a projection [{rows}, {in_dim}]")
+                if not (torch.isfinite(ma.to(dtype)).all() and torch.isfinite(mb.to(dtype)).all()):
+                    raise ValueError("adapter weights must be finite")
+                rank += r
+            if rank > ops.LORA_MAX_RANK:
+                raise ValueError(f"layer {layer} {'+'.join(n for n, *_ in parts)}: rank {rank} of the fused projection "
+                                 f"exceeds {ops.LORA_MAX_RANK}")
+
+
+def _merged(adapter: Adapter, layer: int, parts):
+    """The adapter's (a, per-part b) of a fused projection, its parts stacked
+    in the rank."""
+    mats = [adapter.mats.get((layer, name)) for name, *_ in parts]
+    rank = sum(m[0].shape[0] for m in mats if m is not None)
+    a = torch.zeros(rank, parts[0][1])
+    b = [torch.zeros(rows, rank) for _, _, rows in parts]
+    at = 0
+    for m, bp in zip(mats, b):
+        if m is not None:
+            r = m[0].shape[0]
+            a[at:at + r], bp[:, at:at + r] = m[0].float(), m[1].float()
             at += r
     return a, b
 
@@ -106,23 +127,30 @@ class LayerAdapters:
 
     __slots__ = ("qkv", "o", "gu", "down")
 
-    def __init__(self, cfg, adapters: list, layer: int, device, dtype):
-        scale = torch.tensor([ad.scale for ad in adapters])
+    def __init__(self):
+        self.qkv: Optional[ops.LoraStack] = None
+        self.o: Optional[ops.LoraStack] = None
+        self.gu: Optional[ops.LoraStack] = None
+        self.down: Optional[ops.LoraStack] = None
 
-        def stack(parts, in_dim, join) -> Optional[ops.LoraStack]:
-            m = _merged(adapters, layer, parts, in_dim)
-            if m is None:
-                return None
-            a, b = m
-            return ops.LoraStack(a.to(device=device, dtype=dtype), join(b).to(device=device, dtype=dtype),
-                                 scale.to(device))
-
-        def interleaved(b):
-            return torch.stack([ops.interleave_gate_up(g, u) for g, u in zip(b[0], b[1])])
-
-        H, inter = cfg.hidden_size, cfg.intermediate_size
-        self.qkv = stack([("q_proj", cfg.q_size), ("k_proj", cfg.kv_size), ("v_proj", cfg.kv_size)], H,
-                         lambda b: torch.cat(b, 1))
-        self.o = stack([("o_proj", H)], cfg.q_size, lambda b: b[0])
-        self.gu = stack([("gate_proj", inter), ("up_proj", inter)], H, interleaved)
-        self.down = stack([("down_proj", H)], inter, lambda b: b[0])
+    def add(self, cfg, adapter: Adapter, layer: int, keep: int, device, dtype) -> None:
+        """Puts an adapter behind the first ``keep``, one projection after the
+        other, so that one at most exists twice."""
+        for slot, parts in _stacks(cfg).items():
+            old = getattr(self, slot)
+            a, b = _merged(adapter, layer, parts)
+            rank = a.shape[0]
+            if old is None and not rank:
+                continue
+            b = ops.interleave_gate_up(*b) if slot == "gu" and rank else torch.cat(b)
+            if old is None:  # the adapters before have none
+                padded = -(-rank // 8) * 8
+                na = torch.zeros(keep + 1, padded, a.shape[1], device=device, dtype=dtype)
+                nb = torch.zeros(keep + 1, b.shape[0], padded, device=device, dtype=dtype)
+                na[keep, :rank], nb[keep, :, :rank] = a.to(na), b.to(nb)
+                scale = torch.zeros(keep + 1, device=device)
+                scale[keep] = adapter.scale
+                new = ops.LoraStack(na, nb, scale)
+            else:
+                new = old.joined(a, b, adapter.scale, keep)
+            setattr(self, slot, new)

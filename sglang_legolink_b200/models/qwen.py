@@ -86,7 +86,6 @@ class QwenModel:
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
         self.adapter_names: list[str] = []  # adapter i of a batch's plan
         self.adapter_digests: list[str] = []
-        self._adapters: list = []
         self._layer_adapters: list = []
         self._bufs: dict = {}
         self.buf_generation = 0  # bumped whenever a scratch buffer is replaced by a larger one
@@ -230,9 +229,10 @@ class QwenModel:
     def add_adapter(self, name: str, adapter) -> int:
         """Adds a low-rank adapter (:class:`~.adapters.Adapter`); rows whose
         plan (``ForwardBatch.lora``) names its index, the return value, run
-        with it.  The stacks of all adapters are rebuilt, so captured graphs
-        are dropped; a name is never given to other weights."""
-        from .adapters import LayerAdapters
+        with it.  It joins the stacks of those loaded before, so captured
+        graphs are dropped; a name is never given to other weights.  One that
+        does not fit, or finds no memory, leaves the others as they are."""
+        from .adapters import LayerAdapters, check_adapter
 
         if self.tp_size > 1:
             raise ValueError("adapters are not supported with tensor parallelism")
@@ -242,13 +242,16 @@ class QwenModel:
         if bad or not adapter.mats:
             raise ValueError(f"adapter '{name}' names layers {bad} of a {self.cfg.num_layers}-layer model"
                              if bad else f"adapter '{name}' has no matrices")
-        adapters = self._adapters + [adapter]
-        stacks = [LayerAdapters(self.cfg, adapters, i, self.device, self.dtype) for i in range(self.cfg.num_layers)]
-        self.adapter_digests = self.adapter_digests + [adapter.digest()]
-        self._adapters, self._layer_adapters = adapters, stacks
+        check_adapter(self.cfg, adapter, self.dtype)
+        digest, n = adapter.digest(), len(self.adapter_names)
+        self.buf_generation += 1  # from here on a captured graph may point at a stack that is gone
+        if not self._layer_adapters:
+            self._layer_adapters = [LayerAdapters() for _ in range(self.cfg.num_layers)]
+        for i, la in enumerate(self._layer_adapters):
+            la.add(self.cfg, adapter, i, n, self.device, self.dtype)
+        self.adapter_digests = self.adapter_digests + [digest]
         self.adapter_names = self.adapter_names + [name]
-        self.buf_generation += 1
-        return len(adapters) - 1
+        return n
 
     def _proj(self, x, w, bias, stack, fb: ForwardBatch, out, swiglu: bool = False):
         """A projection of the generic forward, with the rows' adapters."""

@@ -28,7 +28,7 @@ class LoraStack:
     The weights must be finite: rows of other adapters in the same tile
     multiply ``b`` with zeros, which would turn an infinity into NaN."""
 
-    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor):
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, _checked: int = 0):
         if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
             raise ValueError(f"adapter shapes: a {tuple(a.shape)}, b {tuple(b.shape)}")
         n, rank, _ = a.shape
@@ -41,7 +41,7 @@ class LoraStack:
         self.a, self.b = a.contiguous(), b.contiguous()
         self.scale = scale.float().contiguous()
         self.count, self.rank = n, rank
-        if not bool(torch.isfinite(self.a).all() & torch.isfinite(self.b).all() & torch.isfinite(self.scale).all()):
+        if not bool(torch.stack([torch.isfinite(t[_checked:]).all() for t in (self.a, self.b, self.scale)]).all()):
             raise ValueError("adapter weights must be finite")
 
     @classmethod
@@ -51,6 +51,21 @@ class LoraStack:
         a = torch.stack([torch.nn.functional.pad(p[0], (0, 0, 0, rank - p[0].shape[0])) for p in pairs])
         b = torch.stack([torch.nn.functional.pad(p[1], (0, rank - p[1].shape[1])) for p in pairs])
         return cls(a, b, torch.tensor(list(scales), dtype=torch.float32, device=a.device))
+
+    def joined(self, a: torch.Tensor, b: torch.Tensor, scale: float, keep: Optional[int] = None) -> "LoraStack":
+        """A stack of this one's adapters (its first ``keep``) and one more,
+        ``a`` [r, K] and ``b`` [N, r], as the last; r = 0 for one that leaves
+        the projection as it is."""
+        n = self.count if keep is None else keep
+        r = a.shape[0]
+        rank = max(self.rank, -(-r // 8) * 8)
+        if a.shape[1:] != self.a.shape[2:] or tuple(b.shape) != (self.b.shape[1], r):
+            raise ValueError(f"adapter shapes: a {tuple(a.shape)}, b {tuple(b.shape)}")
+        na = self.a.new_zeros(n + 1, rank, self.a.shape[2])
+        nb = self.b.new_zeros(n + 1, self.b.shape[1], rank)
+        na[:n, : self.rank], nb[:n, :, : self.rank] = self.a[:n], self.b[:n]
+        na[n, :r], nb[n, :, :r] = a.to(na), b.to(nb)
+        return LoraStack(na, nb, torch.cat([self.scale[:n], self.scale.new_full((1,), scale)]), n)
 
 
 class LoraPlan:
