@@ -9,7 +9,7 @@ adapters, and multiply each plane with its adapter's B.
 
 from __future__ import annotations
 
-from typing import Optional, Sequence, Union
+from typing import Callable, Optional, Sequence, Union
 
 import numpy as np
 import torch
@@ -72,7 +72,8 @@ class LoraPlan:
     """Which adapter each row of a batch uses (:func:`lora_plan`).  One plan
     serves every projection of a forward, on any stream."""
 
-    def __init__(self, row_adapters, device, max_planes: Optional[int] = None):
+    def __init__(self, row_adapters, device, max_planes: Optional[int] = None,
+                 copy: Optional[Callable[[np.ndarray], torch.Tensor]] = None):
         ids = _host_ids(row_adapters)
         self.rows = len(ids)
         self.tile_rows = 128 if self.rows <= 128 else 256
@@ -83,7 +84,8 @@ class LoraPlan:
         self.max_planes = max(1, planes if max_planes is None else int(max_planes))
         if planes > self.max_planes:
             raise ValueError(f"the rows need {planes} planes, max_planes is {self.max_planes}")
-        self.buf = torch.empty(self.rows + self.tiles + 1 + 2 * self.max_planes, dtype=torch.int32, device=self.device)
+        self._copy = copy
+        self.buf: Optional[torch.Tensor] = None
         self._store(ids, host)
 
     def _build(self, ids: np.ndarray):
@@ -99,13 +101,16 @@ class LoraPlan:
 
     def _store(self, ids: np.ndarray, host) -> None:
         slot, ptr, keys = host
-        flat = np.zeros(self.buf.numel(), dtype=np.int32)
+        flat = np.zeros(self.rows + self.tiles + 1 + 2 * self.max_planes, dtype=np.int32)
         flat[: self.rows] = slot
         flat[self.rows : self.rows + self.tiles + 1] = ptr
         planes = flat[self.rows + self.tiles + 1 :].reshape(2, self.max_planes)
         planes[0, : len(keys)] = keys & 0xFFFFFFFF
         planes[1, : len(keys)] = keys >> 32
-        self.buf.copy_(torch.from_numpy(flat))
+        if self.buf is None:
+            self.buf = self._copy(flat) if self._copy else torch.from_numpy(flat).to(self.device)
+        else:
+            self.buf.copy_(self._copy(flat) if self._copy else torch.from_numpy(flat))
         self.top_adapter = int(ids.max()) if self.rows else -1
         self.row_adapters = torch.from_numpy(ids)
 
@@ -140,7 +145,10 @@ def _host_ids(row_adapters) -> np.ndarray:
 
 
 def lora_plan(row_adapters: Union[Sequence[int], np.ndarray, torch.Tensor], device,
-              max_planes: Optional[int] = None) -> LoraPlan:
+              max_planes: Optional[int] = None,
+              copy: Optional[Callable[[np.ndarray], torch.Tensor]] = None) -> LoraPlan:
     """Plan of a batch whose row m uses adapter ``row_adapters[m]`` (-1: none),
-    in any order; host values (a CUDA tensor is read back)."""
-    return LoraPlan(row_adapters, device, max_planes)
+    in any order; host values (a CUDA tensor is read back).  ``copy``: host
+    array -> new tensor on ``device``, in place of a copy that the host waits
+    for; the plan is then ready on the stream that ``copy`` used."""
+    return LoraPlan(row_adapters, device, max_planes, copy)

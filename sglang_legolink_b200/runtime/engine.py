@@ -105,11 +105,11 @@ def group_promotion_enabled() -> bool:
     return env_flag("SGLANG_PIC_EXPERIMENTAL_GROUP_PROMOTION")
 
 
-def _pinned_copy(host: np.ndarray, dev) -> torch.Tensor:
-    """One pinned staging buffer per dtype and device (grown on demand);
-    the copy is asynchronous, and the staging buffer is reused only after the
-    previous copy from it has finished."""
-    key = (str(host.dtype), str(dev))
+def _pinned_copy(host: np.ndarray, dev, use: str = "") -> torch.Tensor:
+    """One pinned staging buffer per dtype, device and ``use`` (grown on
+    demand); the copy is asynchronous, and the staging buffer is reused only
+    after the previous copy from it has finished."""
+    key = (str(host.dtype), str(dev), use)
     ent = _PINNED.get(key)
     if ent is None or ent[0].numel() < host.size:
         buf = torch.empty(max(host.size, 1 << 16), dtype=torch.from_numpy(host[:0]).dtype, pin_memory=True)
@@ -292,7 +292,10 @@ class Engine:
         ``adapters[i]``); None when no row has one."""
         if all(a < 0 for a in adapters):
             return None
-        return ops.lora_plan(np.repeat(np.asarray(adapters, dtype=np.int64), counts), self.device, max_planes)
+        # a staging buffer of its own: the batch's other arrays are still in
+        # theirs, behind the kernels that run ahead of this step
+        copy = (lambda a: _pinned_copy(a, self.device, "plan")) if self.is_cuda else None
+        return ops.lora_plan(np.repeat(np.asarray(adapters, dtype=np.int64), counts), self.device, max_planes, copy)
 
     def next_rid(self, prefix="req") -> str:
         self._rid += 1
