@@ -304,7 +304,12 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
     gate/up product.  bf16, row strides and K multiples of 8, N of 8 (of 32
     with SwiGLU); ``w`` row-major.  CUDA: two launches, the low-rank rows and
     the product; their scratch belongs to the call, so calls on several
-    streams may share a stack and a plan."""
+    streams may share a stack and a plan.
+
+    The same call gives the same bits.  A row's last bits may change with the
+    batch around it: the kernels and the splits of K, and with them the order
+    of its sums, go by the number of rows, the adapters that the others use and
+    the plan's ``max_planes``; the values of other rows never matter."""
     M, N = x.shape[0], w.shape[0]
     if plan.rows != M:
         raise ValueError(f"the plan is for {plan.rows} rows, x has {M}")
