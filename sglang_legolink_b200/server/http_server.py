@@ -113,7 +113,7 @@ class RuntimeService:
             ids = list(p) if isinstance(p, list) else list(self.tokenizer.tokenize(str(p)))
         else:
             ids = _prompt_ids(self.tokenizer, payload)
-        adapter = payload.get("adapter_id")
+        adapter = payload.get("adapter_id") or None  # empty: none, as in a Compile's or Link's
         return Request("plain", rid, ids, max_new, stop, sampling=sampling,
                        adapter=None if adapter is None else str(adapter))
 

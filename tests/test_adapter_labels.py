@@ -49,3 +49,28 @@ def test_a_block_compiled_under_a_look_alike_label_does_not_link_as_the_adapters
     with pytest.raises(LinkSourceUnavailable):
         e.link({"cache_keys": ["x"], "recompute_tokens_per_block": [4], "adapter_id": "one"}, [1, 2])
     e.free(e.link({"cache_keys": ["x"], "recompute_tokens_per_block": [4], "adapter_id": label}, [1, 2]))
+
+
+@pytest.mark.parametrize("none", ["", None])
+def test_an_empty_adapter_id_names_no_adapter_in_any_request(none, tmp_path):
+    """As in Compile and Link requests, whose key for it is that of no adapter."""
+    import json
+
+    from safetensors.torch import save_file
+
+    from sglang_legolink_b200.server.http_server import build_service
+
+    c = PRESETS["tiny-qwen2"]
+    pre = "base_model.model.model.layers.0.self_attn.q_proj"
+    save_file({f"{pre}.lora_A.weight": torch.randn(8, c.hidden_size), f"{pre}.lora_B.weight": torch.randn(c.q_size, 8)},
+              str(tmp_path / "adapter_model.safetensors"))
+    (tmp_path / "adapter_config.json").write_text(json.dumps({"r": 8, "lora_alpha": 16}))
+    svc = build_service("tiny-qwen2", max_context=1024, legolink_only=False, adapters=[("legal", str(tmp_path))])
+    try:
+        ask = {"messages": [{"role": "user", "content": "a question"}], "max_tokens": 4, "ignore_eos": True}
+        want = svc.complete(ask)["meta_info"]["output_ids"]
+        assert svc.complete({**ask, "adapter_id": none})["meta_info"]["output_ids"] == want
+        eng = svc.scheduler.engine
+        assert eng.compat_key(none) == eng.compat_key()
+    finally:
+        svc.scheduler.stop()
