@@ -181,7 +181,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     first ``top_k`` tokens; of those, the ones whose predecessors hold less
     than ``top_p`` of their mass; of those, the ones with ``w >= min_p``.  The
     token is the first kept one, in index order, whose running sum of w
-    exceeds ``u`` times the kept sum.  NaN counts as -inf; a row with nothing
+    exceeds ``u`` times the kept sum (``u`` taken to the nearer end of [0, 1],
+    NaN to 0: the first and the last kept one).  NaN counts as -inf; a row with nothing
     above -inf gives token -1; +inf logits share all of the mass."""
     B, V = logits.shape
     x = logits.double()
@@ -207,7 +208,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     wk = w * torch.zeros_like(keep).scatter_(1, order, keep)
     cum = torch.cumsum(wk, dim=1)
     total = cum[:, -1:]
-    uu = u.double()[:, None].clamp(0.0, 1.0)
+    uu = torch.nan_to_num(u.double(), nan=0.0)[:, None].clamp(0.0, 1.0)
     ids = ((cum > uu * total) & (wk > 0)).to(torch.uint8).argmax(dim=1, keepdim=True)
     last = torch.where(wk > 0, ar, torch.full_like(ar, -1)).max(dim=1, keepdim=True).values
     ids = torch.where(uu * total >= total, last.clamp(min=0), ids)
