@@ -354,6 +354,23 @@ void gemm_small_m_epi(const at::Tensor& a, const at::Tensor& w, const c10::optio
            "ll_gemm_bf16_small_m_epi");
 }
 
+// Whether two tensors have bytes in common; columns of one buffer's rows, side
+// by side, have none.
+bool share_memory(const at::Tensor& a, const at::Tensor& b) {
+  auto bytes = [](const at::Tensor& v) {
+    int64_t n = 1;
+    for (int64_t i = 0; i < v.dim(); ++i) n += (v.size(i) - 1) * v.stride(i);
+    return n * (int64_t)v.element_size();
+  };
+  const int64_t off = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr());
+  if (off >= bytes(a) || -off >= bytes(b)) return false;
+  if (a.dim() != 2 || b.dim() != 2 || a.stride(0) != b.stride(0) || a.stride(1) != 1 || b.stride(1) != 1) return true;
+  const int64_t pitch = a.stride(0) * (int64_t)a.element_size();
+  if (pitch <= 0 || a.element_size() != b.element_size()) return true;
+  const int64_t d = (off % pitch + pitch) % pitch;  // b's first column behind a's
+  return d < a.size(1) * (int64_t)a.element_size() || d + b.size(1) * (int64_t)b.element_size() > pitch;
+}
+
 // A projection with per-row low-rank adapters (lora.h): the low-rank rows,
 // then the shared product with the adapters' B as further k-blocks.  The
 // scratch is this call's own, so calls on different streams share nothing.
@@ -383,6 +400,10 @@ at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const c10::opti
   TORCH_CHECK(x.stride(0) % 8 == 0 && out.stride(0) % 8 == 0, "row strides must be multiples of 8");
   TORCH_CHECK(x.stride(0) < (1ll << 31) && out.stride(0) < (1ll << 31), "row strides must be below 2^31");
   TORCH_CHECK(out.size(0) == M && out.size(1) == (swiglu ? N / 2 : N), "bad output shape");
+  // CTAs store their tiles while others still read
+  TORCH_CHECK(M == 1 || out.stride(0) >= out.size(1), "rows of the output share memory");
+  for (const at::Tensor* t : {&x, &w, &a, &b})
+    TORCH_CHECK(!share_memory(out, *t), "the output shares memory with an input");
   if (bias.has_value()) {
     CHECK_BF16(*bias); CHECK_CONTIG(*bias);
     CHECK_ALIGN16(*bias);
