@@ -55,7 +55,8 @@ using TpArgs = LLTpArgs;
 // term joins the product in fp32, before the epilogue, and costs no pass over
 // the output: at 5087 rows x 4608 outputs a separate pass would read and write
 // 94 MB (14 us at HBM rate), the extra k-blocks of a rank-48 adapter add 2 to
-// 56 (the whole product 136 us, 120 without adapters).
+// 56 (back to back, under the power cap: 156 us with the low-rank rows, 139
+// without adapters).
 // NoLora compiles the kernels without any of it.
 struct NoLora {
   static constexpr bool on = false;
@@ -1942,7 +1943,7 @@ static int make_lora_blocks(LoraBlocks* lb, const LLLora& lo, int N, int b_box_r
 // 256 tiles past 256 rows and from N = 2048 on, else 128 x 256 or 128 x 128.
 // Launched as ll_lora_low's dependent, so that its set-up overlaps that kernel;
 // it waits for it before its first tile.  (Starting the k-blocks of K at once
-// was slower at 5087 rows, 163 us for 142: the pairs that got their SMs last
+// was slower at 5087 rows, 163 us for 142 in a graph: the pairs that got their SMs last
 // finished last.)
 extern "C" int ll_gemm_bf16_lora(const void* A_, int lda, const void* W_, int ldw, void* C_, int ldc,
                                  const void* bias_, int M, int N, int K, int epilogue, const LLLora* lo, int* err,

@@ -7,10 +7,10 @@
 // rank 48), so what counts is bytes in flight: the cluster split puts up to
 // two CTAs with a ~96 KB ring on every SM whatever the number of row tiles.
 // The CTAs' fp32 partials meet in distributed shared memory and are summed in
-// CTA order, so a row's bits do not depend on timing.  That case takes 17 us
-// with cold caches: 4 until the last cluster has started, 1.5 to read the plan
-// and set up, 5 for the loads (8 TB/s, from L2 where two planes share rows), 4
-// for the partials.
+// CTA order, so a row's bits do not depend on timing.  That case takes 18 us
+// with cold caches; warm about 14: 4 until the last cluster has started, 1.3 to
+// read the plan and set up, 5 for the loads (8 TB/s, from L2 where two planes
+// share rows), 4 for the partials.
 //
 // low is kept as two bf16 planes, hi = bf16(v) and lo = bf16(v - hi): the
 // product that reads them takes bf16 operands, and one bf16 would put 2^-9 of
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(128, 2)
 // -> 4608, rank 48, 27.9 -> 22.2 us, 300 x 3584 x 18944 84.7 -> 66.8.  (The same
 // behind the few-row kernel: 16 rows, 3584 -> 37888, 48.4 -> 50.0.)
 //
-// Bound by reading weights: 16 rows, 3584 -> 37888 with
-// SwiGLU and 6 adapters of rank 32 in 48.4 us for both kernels, 6.1 TB/s.
+// Bound by reading weights: 16 rows, 3584 -> 37888 with SwiGLU and 6 adapters of
+// rank 32 (288 MB) in 48.7 us for both kernels in a graph, 5.9 TB/s.
 constexpr int GEMV_RING = 108 * 1024;
 // Clusters do not fill the SMs to the last place (two CTAs a SM, 296 places):
 // 36 clusters of 8 and 40 of 7 ran a second round.  us a call with 2 / 4 / 6 /

@@ -13,9 +13,9 @@
 // A k-block is 64 columns.  Up to rank 32 a plane's hi and lo are the halves of
 // one block (low's rows are 64 wide, zero between), and the last two of the
 // block's four MMA steps read B's first 32 columns once more.  Else hi and lo
-// are blocks of their own.  At 61 rows of 32 adapters, rank 16, K = 8192,
-// N = 5120: 26.8 us packed, 28.4 not; 16 rows of 8, rank 32, K = 3584, N = 37888
-// with SwiGLU: 48.4 and 51.0.
+// are blocks of their own.  In a graph, 61 rows of 32 adapters, rank 16, K =
+// 8192, N = 5120: 26.8 us packed, 28.4 not; 16 rows of 8, rank 32, K = 3584, N =
+// 37888 with SwiGLU: 48.4 and 51.0.
 //
 // Rows are cut into tiles of `tile_rows`; the planes of tile t are
 // [tile_ptr[t], tile_ptr[t + 1]) and plane_adapter names their adapters.

@@ -6,7 +6,9 @@ harness sends temperature 0 / top_k 1, ``sglang_adapter.py:324-333``).
 Greedy rows use the fused argmax kernel; sampled rows use torch ops on the
 logits the decode graph already produced (a [B, vocab] softmax is tiny next to
 the GEMMs), or, with ``Engine(sampler="kernel")``, one launch for the batch
-(:func:`draw_rows`), whose seeded draws are other ones.
+(:func:`draw_rows`), whose seeded draws are other ones.  The two also differ
+where logits tie at the border of top-k: :func:`sample_rows` keeps all of the
+equal ones, :func:`draw_rows` k tokens in all, the first by index.
 """
 
 from __future__ import annotations

@@ -107,3 +107,13 @@ def test_the_scheduler_fails_one_request(monkeypatch):
     assert [k for k, _ in events] == ["token", "token", "error"] and "sampling" in events[2][1]
     assert all(t >= 0 for k, t in events if k == "token")
     assert eng.alloc.num_free == free and not sch.running
+
+
+def test_what_the_two_samplers_keep_where_logits_tie_at_the_border_of_top_k():
+    from sglang_legolink_b200.runtime.sampling import draw_rows, make_generator, sample_rows
+
+    x = torch.tensor([[3.0, 1.0, 2.0, 1.0, 1.0, 0.0]])
+    p = SamplingParams(temperature=1.0, top_k=3, seed=2)
+    for draw, kept in ((sample_rows, {0, 1, 2, 3, 4}), (draw_rows, {0, 1, 2})):
+        g = [make_generator(p, "cpu")]
+        assert {int(draw(x, [p], g)[0]) for _ in range(600)} == kept
