@@ -304,10 +304,10 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
     gate/up product.  bf16, row strides and K multiples of 8, N of 8 (of 32
     with SwiGLU); ``w`` row-major.  CUDA: two launches, the low-rank rows and
     the product; their scratch belongs to the call, so calls on several
-    streams may share a stack and a plan.  As :func:`linear`'s weights, ``w``,
-    the stack and the plan may be read while the stream's previous kernel still
-    runs, so none of them may be that kernel's output; ``out`` may share no
-    memory with ``x`` or a weight.
+    streams may share a stack and a plan.  ``w``, the stack and the plan may be
+    read while this package's kernels just ahead in the stream still run (as
+    :func:`linear`'s weights), so they may not be outputs of those; ``x`` may.
+    ``out`` may share no memory with ``x`` or a weight.
 
     The same call gives the same bits.  A row's last bits may change with the
     batch around it: the kernels and the splits of K, and with them the order
