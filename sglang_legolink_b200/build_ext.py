@@ -26,6 +26,8 @@ CUDA_SOURCES = [
     "gemm_tcgen05.cu",
     "elementwise.cu",
     "lora.cu",
+    "q8_rows.cu",
+    "gemm_q8.cu",
     "sampling.cu",
     "attention.cu",
     "attention_tc.cu",

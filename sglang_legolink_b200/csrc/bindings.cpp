@@ -10,6 +10,7 @@ using bf16 = __nv_bfloat16;
 
 #include "gemm_epi.h"
 #include "lora.h"
+#include "q8.h"
 #include "sampling.h"
 #include "tp_fused.h"
 
@@ -29,6 +30,8 @@ int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, int64_t ldc
 int ll_gemm_bf16_lora(const void* A, int lda, const void* W, int ldw, void* C, int ldc, const void* bias, int M,
                       int N, int K, int epilogue, const LLLora* lo, int* err, void* stream);
 int ll_sample(const LLSample* p, cudaStream_t stream);
+int ll_q8_rows(const LLQ8Rows* p, cudaStream_t stream);
+int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int cluster, int* err, cudaStream_t stream);
 int ll_rmsnorm(bf16* out, const bf16* x, bf16* residual, const bf16* w, int rows, int hidden, float eps,
                cudaStream_t stream);
 int ll_rope_qkv_write(const bf16* qkv, const int* positions, const int64_t* slots, const float* cos_sin, bf16* q_out,
@@ -480,6 +483,129 @@ void sample(const at::Tensor& logits, const at::Tensor& u, const c10::optional<a
   check_rc(rc, "ll_sample");
 }
 
+// Matrices in 8 bits (q8.h): e4m3 values [rows, K] with one fp32 scale a row.
+// Elements from a row to the next; of a single row it is never used.
+int64_t row_step(const at::Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
+
+void check_matrix(const at::Tensor& t, at::ScalarType type, const at::Device& dev, int64_t rows, int64_t cols,
+                  const char* name) {
+  TORCH_CHECK(t.device() == dev, name, " must be on ", dev.str());
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", c10::toString(type));
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name, " must be [", num(rows), ", ", num(cols), "]");
+  TORCH_CHECK(cols == 1 || t.stride(1) == 1, "a row of ", name, " must be contiguous");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_step(t) * t.element_size() % 16 == 0,
+              "rows of ", name, " must start on 16-byte boundaries");
+}
+void check_vector(const at::Tensor& t, at::ScalarType type, const at::Device& dev, int64_t n, const char* name,
+                  bool aligned = true) {
+  TORCH_CHECK(t.device() == dev, name, " must be on ", dev.str());
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", c10::toString(type));
+  TORCH_CHECK(t.numel() == n && t.is_contiguous(), name, " must be a contiguous [", num(n), "]");
+  TORCH_CHECK(!aligned || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name,
+              " must start on a 16-byte boundary");
+}
+// A written matrix: rows of its own, apart from `others`.
+void check_written(const at::Tensor& t, at::TensorList others, const char* name) {
+  TORCH_CHECK(row_step(t) >= t.size(1), "rows of ", name, " share memory");
+  for (const at::Tensor& o : others)
+    TORCH_CHECK(!share_memory(t, o), name, " shares memory with another argument");
+}
+bool same_place(const at::Tensor& a, const at::Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && row_step(a) == row_step(b);
+}
+
+// y = x (w null), rmsnorm(x) w, or rmsnorm(x + residual) w with the sum to `sum`.
+void q8_rows(const at::Tensor& x, const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& sum,
+             const c10::optional<at::Tensor>& w, double eps, const at::Tensor& q, const at::Tensor& scale) {
+  CHECK_CUDA(x);
+  TORCH_CHECK(x.dim() == 2, "x must be [rows, K]");
+  const int64_t rows = x.size(0), K = x.size(1);
+  TORCH_CHECK(rows > 0 && rows < (1ll << 31) && K > 0 && K % 16 == 0 && K <= LL_Q8_MAX_K,
+              "K must be a multiple of 16, at most ", num(LL_Q8_MAX_K), ", and rows below 2^31");
+  check_matrix(x, at::kBFloat16, x.device(), rows, K, "x");
+  check_matrix(q, at::kFloat8_e4m3fn, x.device(), rows, K, "the values");
+  check_vector(scale, at::kFloat, x.device(), rows, "the scales", false);
+  check_written(q, {x, scale}, "the values");
+  TORCH_CHECK(!share_memory(scale, x), "the scales share memory with x");
+  LLQ8Rows p{};
+  if (w.has_value()) {
+    check_vector(*w, at::kBFloat16, x.device(), K, "the norm's weight");
+    check_written(q, {*w}, "the values");
+    TORCH_CHECK(!share_memory(scale, *w), "the scales share memory with the norm's weight");
+    p.w = bp(*w);
+  }
+  if (residual.has_value()) {
+    TORCH_CHECK(sum.has_value() && w.has_value(), "a residual comes with its sum and a norm");
+    check_matrix(*residual, at::kBFloat16, x.device(), rows, K, "the residual");
+    check_matrix(*sum, at::kBFloat16, x.device(), rows, K, "the sum");
+    check_written(*sum, {x, q, scale, *w}, "the sum");
+    if (!same_place(*sum, *residual)) check_written(*sum, {*residual}, "the sum");
+    check_written(q, {*residual}, "the values");
+    TORCH_CHECK(!share_memory(scale, *residual), "the scales share memory with the residual");
+    p.residual = bp(*residual);
+    p.sum = bp(*sum);
+    p.ldr = row_step(*residual);
+    p.lds = row_step(*sum);
+  }
+  p.x = bp(x);
+  p.q = static_cast<uint8_t*>(q.data_ptr());
+  p.scale = scale.data_ptr<float>();
+  p.ldx = row_step(x);
+  p.ldq = row_step(q);
+  p.rows = (int)rows;
+  p.K = (int)K;
+  p.eps = (float)eps;
+  c10::cuda::CUDAGuard g(x.device());
+  check_rc(ll_q8_rows(&p, cur_stream()), "ll_q8_rows");
+}
+
+// out = act(xs ws (x . w^T) + bias) + residual.  `cluster` names a kernel (ll_q8_gemm), 0: by the sizes.
+void q8_gemm(const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, const at::Tensor& ws,
+             const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, const at::Tensor& out,
+             bool swiglu, int64_t cluster, const at::Tensor& err) {
+  CHECK_CUDA(x); CHECK_I32(err);
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x and w must be matrices");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0), cols = swiglu ? N / 2 : N;
+  TORCH_CHECK(M > 0 && M < (1 << 28) && N > 0 && N < (1 << 28) && K > 0 && K < (1ll << 31), "bad sizes");
+  TORCH_CHECK(K % 16 == 0 && N % 8 == 0 && (!swiglu || N % 32 == 0),
+              "K must be a multiple of 16 and N of 8 (of 32: SwiGLU)");
+  check_matrix(x, at::kFloat8_e4m3fn, x.device(), M, K, "x");
+  check_matrix(w, at::kFloat8_e4m3fn, x.device(), N, K, "w");
+  check_vector(xs, at::kFloat, x.device(), M, "the scales of x", false);
+  check_vector(ws, at::kFloat, x.device(), N, "the scales of w");
+  check_matrix(out, at::kBFloat16, x.device(), M, cols, "out");
+  TORCH_CHECK(err.device() == x.device(), "the error word must be on ", x.device().str());
+  TORCH_CHECK(row_step(x) >= K && row_step(w) >= K, "rows of x or w share memory");
+  TORCH_CHECK(row_step(x) < (1ll << 31) && row_step(w) < (1ll << 31) && row_step(out) < (1ll << 31),
+              "row strides must be below 2^31");
+  check_written(out, {x, xs, w, ws}, "out");
+  LLQ8Gemm p{};
+  if (bias.has_value()) {
+    check_vector(*bias, at::kBFloat16, x.device(), N, "bias");
+    check_written(out, {*bias}, "out");
+    p.bias = bp(*bias);
+  }
+  if (residual.has_value()) {
+    check_matrix(*residual, at::kBFloat16, x.device(), M, cols, "the residual");
+    if (!same_place(out, *residual)) check_written(out, {*residual}, "out");
+    p.residual = bp(*residual);
+    p.ldr = row_step(*residual);
+  }
+  p.x = static_cast<const uint8_t*>(x.data_ptr());
+  p.w = static_cast<const uint8_t*>(w.data_ptr());
+  p.xs = xs.data_ptr<float>();
+  p.ws = ws.data_ptr<float>();
+  p.C = bp(out);
+  p.ldx = row_step(x);
+  p.ldw = row_step(w);
+  p.ldc = row_step(out);
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  c10::cuda::CUDAGuard g(x.device());
+  check_rc(ll_q8_gemm(&p, swiglu ? 1 : 0, (int)cluster, err.data_ptr<int>(), cur_stream()), "ll_q8_gemm");
+}
+
 void rmsnorm(at::Tensor& out, const at::Tensor& x, const c10::optional<at::Tensor>& residual, const at::Tensor& w,
              double eps) {
   CHECK_CUDA(x); CHECK_BF16(x); CHECK_BF16(out); CHECK_BF16(w); CHECK_CONTIG(x); CHECK_CONTIG(out);
@@ -630,6 +756,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_small_m_epi", &gemm_small_m_epi);
   m.def("lora_linear", &lora_linear);
   m.def("sample", &sample);
+  m.def("q8_rows", &q8_rows);
+  m.def("q8_gemm", &q8_gemm);
   m.def("rmsnorm", &rmsnorm);
   m.def("rope_qkv_write", &rope_qkv_write);
   m.def("kv_link_rope", &kv_link_rope);

@@ -1,0 +1,681 @@
+// The product of two matrices in 8 bits (q8.h) on the 5th-generation tensor
+// cores,
+//
+//   C[m, n] = act(xs[m] ws[n] sum_k X[m, k] W[n, k] + bias[n]) + residual[m, n],
+//
+// with X and W in e4m3 and the sum in fp32 in tensor memory.  A scale belongs to
+// a whole row, so it leaves the sum and is one product per output; a 128-byte
+// swizzled row of an operand tile holds 128 values, and one tcgen05.mma of
+// kind::f8f6f4 takes 32 of them: the same bytes per instruction as in bf16, twice
+// the products.
+//
+// * q8_split_kernel -- few rows.  The weight tile is the M = 128 side, the rows
+//   (up to 128) are the N side, and K is split over the CTAs of a cluster, whose
+//   fp32 partials meet in distributed shared memory.
+// * q8_pair_kernel -- many rows.  Pairs of CTAs (cta_group::2) on 256 x 256
+//   tiles, persistent, two accumulators in tensor memory, so that the epilogue of
+//   a tile runs beside the main loop of the next.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "q8.h"
+
+namespace ll {
+namespace q8 {
+
+constexpr int BK = 128;  // values (bytes) of a k-block: one swizzled row
+
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Instruction descriptor of kind::f8f6f4: fp32 accumulator, both operands e4m3
+// (format 0) and K-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// Arrives on the barrier at this offset in both CTAs of the pair.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)0x3)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair_local(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void load_pair(void* dst, const void* tmap, uint32_t leader_bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(leader_bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void store_box(const void* tmap, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+// Brings a box into L2.  Unlike a load into shared memory it may run ahead of the
+// wait for the kernels before: L2 is where their writes are seen, so a box that
+// one of them still writes is not held stale.
+__device__ __forceinline__ void prefetch_box(const void* tmap, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(x), "r"(y)
+               : "memory");
+}
+
+__device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
+// Lets the copies in flight land before a CTA that gave up exits.
+__device__ __forceinline__ void linger() {
+  const unsigned long long t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 2000000ull) {
+  }
+}
+
+struct alignas(64) Maps {
+  CUtensorMap w, x, c;
+};
+
+// ---------------------------------------------------------------------------
+// Few rows: D[128 features, BNX rows] = W_tile . X_tile^T over a CTA's share of
+// the k-blocks.  Bound by reading W: every CTA's first ring of weights is on its
+// way to L2 before the wait for the kernel ahead.  grid (cluster, feature tiles, row tiles).
+constexpr int SPLIT_RING = 108 * 1024;  // two CTAs a SM
+constexpr int SPLIT_MAX_CLUSTER = 8;
+template <int BNX>
+struct SplitCfg {
+  static constexpr int W_BYTES = 128 * BK;
+  static constexpr int X_BYTES = BNX * BK;
+  static constexpr int STAGES = SPLIT_RING / (W_BYTES + X_BYTES);
+  static constexpr int TMEM_COLS = BNX < 32 ? 32 : BNX;
+  static constexpr int LD = 132;  // floats per row of the partials
+  static constexpr int SMEM = STAGES * (W_BYTES + X_BYTES) + 1024;
+  static_assert(BNX * LD * 4 <= STAGES * (W_BYTES + X_BYTES), "the partials overlay the ring");
+};
+
+template <int BNX, bool SWIGLU>
+__global__ void __launch_bounds__(192, 2)
+    q8_split_kernel(const __grid_constant__ Maps tm, const __grid_constant__ LLQ8Gemm p, int* err) {
+  using Cfg = SplitCfg<BNX>;
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sW = smem;
+  uint8_t* sX = smem + STAGES * Cfg::W_BYTES;
+  float* part = reinterpret_cast<float*>(smem);  // [rows][LD], over the ring, once the product is done
+  __shared__ uint64_t full[STAGES], empty[STAGES], tfull;
+  __shared__ uint32_t tmem_slot;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cs = gridDim.x, crank = blockIdx.x, nb = blockIdx.y;
+  const int num_kb = (p.K + BK - 1) / BK, per = (num_kb + cs - 1) / cs;
+  const int kb0 = min(num_kb, crank * per), kb1 = min(num_kb, kb0 + per);
+  const int m0 = blockIdx.z * BNX, rows = min(BNX, p.M - m0);
+  pdl_trigger();
+
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&tfull, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&tmem_slot, Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      // every input may be an output of the kernel ahead
+      for (int kb = kb0; kb < min(kb1, kb0 + STAGES); ++kb) prefetch_box(&tm.w, kb * BK, nb * 128);
+      pdl_wait();
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&full[stage], Cfg::W_BYTES + Cfg::X_BYTES);
+        tma_load_2d(sW + stage * Cfg::W_BYTES, &tm.w, &full[stage], kb * BK, nb * 128);
+        tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.x, &full[stage], kb * BK, m0);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) linger();
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(128, BNX);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) break;
+        tc_fence_after();
+        const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sW + stage * Cfg::W_BYTES));
+        const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sX + stage * Cfg::X_BYTES));
+#pragma unroll
+        for (int k = 0; k < BK / 32; ++k) mma(tmem, ad + 2 * k, bd + 2 * k, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+        umma_commit(&empty[stage]);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      umma_commit(&tfull);
+    }
+  }
+  __syncwarp();
+  pdl_wait();  // the scales and the residual are the previous kernel's; C may still be read by it
+  const bool ok = __syncthreads_and(mbar_wait(&tfull, 0, err, kErrTmemFullTimeout));
+  tc_fence_after();
+  if (warp >= 2) {  // TMEM lane quarter of this warp: features; columns: rows
+    const int f = (warp & 3) * 32 + lane;
+#pragma unroll 1
+    for (int c = 0; c < BNX && c < rows; c += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tmem + (uint32_t((warp & 3) * 32) << 16) + c, r);  // BNX 16: columns 16.. unused
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (c + i < rows && c + i < BNX) part[(c + i) * Cfg::LD + f] = kb1 > kb0 ? __uint_as_float(r[i]) : 0.f;
+    }
+  }
+  tc_fence_before();
+  cluster_barrier();
+  tc_fence_after();
+  if (ok) {
+    const uint32_t base = smem_u32(part);
+    // four features of a row: the partials in split order, scales, bias
+    auto sum4 = [&](int row, float xs, int f) {
+      float4 t[SPLIT_MAX_CLUSTER];
+      const uint32_t at = base + (uint32_t)(row * Cfg::LD + f) * 4;
+#pragma unroll
+      for (int r = 0; r < SPLIT_MAX_CLUSTER; ++r) t[r] = r < cs ? ld_cluster(mapa(at, r)) : make_float4(0, 0, 0, 0);
+      float4 v = t[0];
+#pragma unroll
+      for (int r = 1; r < SPLIT_MAX_CLUSTER; ++r) {
+        v.x += t[r].x;
+        v.y += t[r].y;
+        v.z += t[r].z;
+        v.w += t[r].w;
+      }
+      const float4 s = *reinterpret_cast<const float4*>(p.ws + nb * 128 + f);
+      v.x = v.x * xs * s.x;
+      v.y = v.y * xs * s.y;
+      v.z = v.z * xs * s.z;
+      v.w = v.w * xs * s.w;
+      if (p.bias != nullptr) {
+        const uint2 bv = *reinterpret_cast<const uint2*>(p.bias + nb * 128 + f);
+        const float2 b0 = unpack_bf16x2(bv.x), b1 = unpack_bf16x2(bv.y);
+        v.x += b0.x;
+        v.y += b0.y;
+        v.z += b1.x;
+        v.w += b1.y;
+      }
+      return v;
+    };
+    constexpr int GROUPS = SWIGLU ? 16 : 32;  // 4-feature groups a row
+    for (int i = crank * 192 + tid; i < rows * GROUPS; i += cs * 192) {
+      const int row = i / GROUPS, g = i % GROUPS;
+      const int64_t m = m0 + row;
+      const int f = SWIGLU ? (g >> 2) * 32 + (g & 3) * 4 : 4 * g;
+      if (nb * 128 + f >= p.N) continue;
+      const int col = SWIGLU ? nb * 64 + 4 * g : nb * 128 + f;
+      uint2 rv = make_uint2(0, 0);
+      if (p.residual != nullptr) rv = *reinterpret_cast<const uint2*>(p.residual + m * p.ldr + col);
+      const float xs = p.xs[m];
+      float4 v = sum4(row, xs, f);
+      if constexpr (SWIGLU) {  // 16 gate features, then the matching 16 up features
+        const float4 u = sum4(row, xs, f + 16);
+        v = make_float4(silu(v.x) * u.x, silu(v.y) * u.y, silu(v.z) * u.z, silu(v.w) * u.w);
+      }
+      if (p.residual != nullptr) {
+        const float2 r0 = unpack_bf16x2(rv.x), r1 = unpack_bf16x2(rv.y);
+        v.x += r0.x;
+        v.y += r0.y;
+        v.z += r1.x;
+        v.w += r1.y;
+      }
+      *reinterpret_cast<uint2*>(p.C + m * p.ldc + col) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    }
+  }
+  cluster_barrier();  // the partials live until every CTA has read them
+  if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: CTA r of a pair loads rows [128 r, +128) of the tile's 256 rows of X
+// and of its 256 rows of W; the leader issues the MMAs (M = 256, N = 256, K = 32),
+// which accumulate rows [128 r, +128) in CTA r's tensor memory.  Loads of both
+// complete on the leader's `full` barrier, commits arrive in both CTAs.
+constexpr int BN = 256;
+constexpr int PAIR_STAGES = 6;
+constexpr int PAIR_TILE = 128 * BK;  // a CTA's half of X's, and of W's, k-block
+constexpr int PAIR_BOX = 32 * 64;    // epilogue staging: 32 rows x 32 bf16 columns
+constexpr int PAIR_SMEM = PAIR_STAGES * 2 * PAIR_TILE + 4 * 2 * PAIR_BOX + 1024 + 256;
+constexpr int PAIR_TMEM = 2 * BN;
+
+// Groups of `group_m` row tiles, rows fastest inside a group: the tiles in flight
+// share few rows of X and of W, both from L2.
+__device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, int group_m, int& mb, int& nb) {
+  const int per_group = group_m * num_n;
+  const int first_m = (t / per_group) * group_m;
+  const int gm = min(num_m - first_m, group_m);
+  const int r = t % per_group;
+  mb = first_m + r % gm;
+  nb = r / gm;
+}
+
+template <bool SWIGLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+    q8_pair_kernel(const __grid_constant__ Maps tm, const __grid_constant__ LLQ8Gemm p, int group_m, int* err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sX = smem;
+  uint8_t* sW = smem + PAIR_STAGES * PAIR_TILE;
+  uint8_t* sEpi = sW + PAIR_STAGES * PAIR_TILE;  // [4 warps][2] boxes
+  uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + 4 * 2 * PAIR_BOX);
+  uint64_t* empty = full + PAIR_STAGES;
+  uint64_t* tfull = empty + PAIR_STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_rank();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const int num_m = (p.M + 255) / 256, num_n = (p.N + BN - 1) / BN;
+  const int ntiles = num_m * num_n, num_kb = (p.K + BK - 1) / BK;
+  pdl_trigger();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PAIR_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 8);  // 4 epilogue warps x 2 CTAs (used on the leader)
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"((uint32_t)PAIR_TMEM)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_barrier();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&tm.x);
+      prefetch_tmap(&tm.w);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < ntiles && ok; t += npairs) {
+        int mb, nb;
+        pair_tile(t, num_m, num_n, group_m, mb, nb);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
+            ok = false;
+            break;
+          }
+          const uint32_t leader_full = mapa(smem_u32(&full[stage]), 0);
+          if (crank == 0) mbar_arrive_expect_tx(&full[stage], 4 * PAIR_TILE);
+          load_pair(sX + stage * PAIR_TILE, &tm.x, leader_full, kb * BK, mb * 256 + (int)crank * 128);
+          load_pair(sW + stage * PAIR_TILE, &tm.w, leader_full, kb * BK, nb * BN + (int)crank * 128);
+          if (++stage == PAIR_STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) linger();
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && crank == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(256, BN);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, aphase = 0;
+      bool ok = true;
+      for (int t = pair; t < ntiles && ok; t += npairs) {
+        if (!mbar_wait(&tempty[acc], aphase ^ 1, err, kErrTmemEmptyTimeout)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sX + stage * PAIR_TILE));
+          const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sW + stage * PAIR_TILE));
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k) mma_pair(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          commit_pair(&empty[stage]);
+          if (++stage == PAIR_STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        commit_pair(&tfull[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          aphase ^= 1;
+        }
+      }
+      // every MMA issued is done before its accumulator is given back
+      commit_pair_local(drain);
+      mbar_wait(drain, 0, nullptr, 0);
+    }
+    __syncwarp();
+  } else {
+    // warp (w % 4) owns TMEM lanes [32 (w % 4), +32): lane = row
+    const int q = warp & 3;
+    const uint32_t leader_tempty0 = mapa(smem_u32(&tempty[0]), 0), leader_tempty1 = mapa(smem_u32(&tempty[1]), 0);
+    uint8_t* boxes = sEpi + q * 2 * PAIR_BOX;
+    int acc = 0, nbox = 0;
+    uint32_t aphase = 0;
+    for (int t = pair; t < ntiles; t += npairs) {
+      int mb, nb;
+      pair_tile(t, num_m, num_n, group_m, mb, nb);
+      const int row0 = mb * 256 + (int)crank * 128 + q * 32, row = row0 + lane;
+      const float xs = row < p.M ? p.xs[row] : 1.f;
+      if (!mbar_wait(&tfull[acc], aphase, err, kErrTmemFullTimeout)) break;
+      tc_fence_after();
+      const uint32_t tbase = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN);
+      // scales and bias of 32 accumulator columns, the same for every lane
+      auto scaled = [&](uint32_t (&r)[32], int col) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          if (col + i >= p.N) break;  // N % 8 == 0
+          const float4 s = __ldg(reinterpret_cast<const float4*>(p.ws + col + i));
+          const float sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r[i + j] = __float_as_uint(__uint_as_float(r[i + j]) * xs * sv[j]);
+        }
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            if (col + i >= p.N) break;
+            const uint4 b = __ldg(reinterpret_cast<const uint4*>(p.bias + col + i));
+            const uint32_t bu[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = unpack_bf16x2(bu[j]);
+              r[i + 2 * j] = __float_as_uint(__uint_as_float(r[i + 2 * j]) + f.x);
+              r[i + 2 * j + 1] = __float_as_uint(__uint_as_float(r[i + 2 * j + 1]) + f.y);
+            }
+          }
+        }
+      };
+      constexpr int STEP = SWIGLU ? 64 : 32;  // accumulator columns of a box of 32 output columns
+#pragma unroll 1
+      for (int c = 0; c < BN; c += STEP) {
+        const int col0 = nb * BN + c;
+        if (col0 >= p.N || row0 >= p.M) continue;  // the whole box is outside C
+        const int out0 = SWIGLU ? col0 / 2 : col0, out_n = SWIGLU ? p.N / 2 : p.N;
+        uint4 res[4];
+        if (p.residual != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            res[i] = row < p.M && out0 + 8 * i < out_n
+                         ? *reinterpret_cast<const uint4*>(p.residual + row * p.ldr + out0 + 8 * i)
+                         : make_uint4(0, 0, 0, 0);
+        }
+        float v[32];
+        if constexpr (SWIGLU) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(tbase + c + 32 * h, r);
+            tmem_ld_wait();
+            scaled(r, col0 + 32 * h);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              // rows past M are zero, and dividing a zero takes a slow path
+              const float g = row < p.M ? __uint_as_float(r[i]) : 1.f;
+              v[16 * h + i] = silu(g) * __uint_as_float(r[16 + i]);
+            }
+          }
+        } else {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tbase + c, r);
+          tmem_ld_wait();
+          scaled(r, col0);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        }
+        if (p.residual != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t ru[4] = {res[i].x, res[i].y, res[i].z, res[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = unpack_bf16x2(ru[j]);
+              v[8 * i + 2 * j] += f.x;
+              v[8 * i + 2 * j + 1] += f.y;
+            }
+          }
+        }
+        // 16-byte chunk k of row r goes to chunk k ^ ((r >> 1) & 3), the 64-byte
+        // swizzle of C's map; rows past M and columns past N are clipped there
+        uint8_t* box = boxes + (nbox & 1) * PAIR_BOX;
+        if (nbox >= 2 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
+        uint4* d = reinterpret_cast<uint4*>(box + lane * 64);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          d[k ^ ((lane >> 1) & 3)] =
+              make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                         pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          store_box(&tm.c, box, out0, row0);
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        ++nbox;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(acc == 0 ? leader_tempty0 : leader_tempty1);
+      if (++acc == 2) {
+        acc = 0;
+        aphase ^= 1;
+      }
+    }
+    if (lane == 0 && nbox > 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+
+  tc_fence_before();
+  cluster_barrier();
+  tc_fence_after();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)PAIR_TMEM)
+                 : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeFn>(f)
+               : nullptr;
+  }();
+  return fn;
+}
+
+// Row-major [rows, K] of e4m3: boxes of 128 values x box_rows, 128-byte swizzle, zeros out of bounds.
+static bool operand_map(CUtensorMap* tm, const void* ptr, int rows, int K, int64_t ld, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {BK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  const EncodeFn enc = encode_fn();
+  return enc != nullptr && enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// C for the bulk stores: boxes of 32 columns (64 bytes) x 32 rows, 64-byte swizzle.
+static bool output_map(CUtensorMap* tm, void* ptr, int rows, int cols, int64_t ld) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {32, 32}, estr[2] = {1, 1};
+  const EncodeFn enc = encode_fn();
+  return enc != nullptr && enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                               CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Kern>
+static int launch(Kern kern, dim3 grid, int smem, int cluster, cudaStream_t stream, unsigned long long& done,
+                  const Maps& tm, const LLQ8Gemm& p, int* err) {
+  if (!smem_on_device(kern, smem, done)) return -7;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, tm, p, err) == cudaSuccess ? 0 : -5;
+}
+
+// CTAs that share a feature tile's K: as many as have places, two a SM.
+constexpr int SPLIT_PLACES = 248;
+static int split_rule(int M, int N, int K, int bnx) {
+  const int tiles = ((N + 127) / 128) * ((M + bnx - 1) / bnx), num_kb = (K + BK - 1) / BK;
+  int cs = SPLIT_PLACES / tiles;
+  if (cs > SPLIT_MAX_CLUSTER) cs = SPLIT_MAX_CLUSTER;
+  if (cs > (num_kb + 1) / 2) cs = (num_kb + 1) / 2;
+  return cs < 1 ? 1 : cs;
+}
+
+template <bool SWIGLU>
+static int split_launch(const LLQ8Gemm& p, int cs, int* err, cudaStream_t stream) {
+  const int bnx = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
+  if (cs <= 0) cs = split_rule(p.M, p.N, p.K, bnx);
+  Maps tm;
+  if (!operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) || !operand_map(&tm.x, p.x, p.M, p.K, p.ldx, bnx)) return -2;
+  tm.c = tm.x;  // not read
+  const dim3 grid(cs, (p.N + 127) / 128, (p.M + bnx - 1) / bnx);
+  if (grid.y > 65535 || grid.z > 65535) return -3;
+  static unsigned long long done[4] = {0, 0, 0, 0};
+  switch (bnx) {
+    case 16: return launch(q8_split_kernel<16, SWIGLU>, grid, SplitCfg<16>::SMEM, cs, stream, done[0], tm, p, err);
+    case 32: return launch(q8_split_kernel<32, SWIGLU>, grid, SplitCfg<32>::SMEM, cs, stream, done[1], tm, p, err);
+    case 64: return launch(q8_split_kernel<64, SWIGLU>, grid, SplitCfg<64>::SMEM, cs, stream, done[2], tm, p, err);
+    default: return launch(q8_split_kernel<128, SWIGLU>, grid, SplitCfg<128>::SMEM, cs, stream, done[3], tm, p, err);
+  }
+}
+
+template <bool SWIGLU>
+static int pair_launch(const LLQ8Gemm& p, int* err, cudaStream_t stream) {
+  Maps tm;
+  if (!operand_map(&tm.x, p.x, p.M, p.K, p.ldx, 128) || !operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) ||
+      !output_map(&tm.c, p.C, p.M, SWIGLU ? p.N / 2 : p.N, p.ldc))
+    return -2;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return -5;
+  const int num_m = (p.M + 255) / 256;
+  const int64_t tiles = (int64_t)num_m * ((p.N + BN - 1) / BN);
+  if (tiles > (1ll << 30)) return -3;
+  const int pairs = tiles < sms / 2 ? (int)tiles : sms / 2;
+  // as many row tiles a group as keep their rows of X within 40 MB of L2
+  int64_t group = (40ll << 20) / ((int64_t)256 * p.K);
+  group = group < 8 ? 8 : group;
+  group = group > num_m ? num_m : group;
+  static unsigned long long done = 0;
+  auto kern = q8_pair_kernel<SWIGLU>;
+  if (!smem_on_device(kern, PAIR_SMEM, done)) return -7;
+  const cudaError_t e = launch_pdl(kern, dim3(2 * pairs), dim3(192), PAIR_SMEM, stream, tm, p, (int)group, err);
+  return e == cudaSuccess ? 0 : -5;
+}
+
+}  // namespace q8
+}  // namespace ll
+
+// `cluster`: 0 takes the kernel by the rule below, -1 the pair kernel, 1 to 8
+// the split kernel with that many CTAs to a feature tile.
+extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int cluster, int* err, cudaStream_t stream) {
+  using namespace ll::q8;
+  if (p->M <= 0) return 0;
+  if (p->N <= 0 || p->K <= 0 || (p->K % 16) || (p->N % 8) || (swiglu && (p->N % 32))) return -3;
+  if ((p->ldx % 16) || (p->ldw % 16) || (p->ldc % 8) || (p->ldr % 8) || cluster > SPLIT_MAX_CLUSTER) return -3;
+  const bool split = cluster > 0 || (cluster == 0 && p->M <= 128);
+  if (split) return swiglu ? split_launch<true>(*p, cluster, err, stream) : split_launch<false>(*p, cluster, err, stream);
+  return swiglu ? pair_launch<true>(*p, err, stream) : pair_launch<false>(*p, err, stream);
+}

@@ -1,0 +1,200 @@
+// Rows to 8 bits: e4m3 values with one fp32 scale a row,
+//
+//   scale = max(amax |y| / 448, 2^-126),  q = e4m3(y * (1 / scale)),
+//
+// of y = x, of y = rmsnorm(x) w, or of y = rmsnorm(x + residual) w with the sum
+// stored as well.  448 is e4m3's largest number.  The floor 2^-126 keeps the
+// scale and its reciprocal normal numbers: a row of zeros has zeros and that
+// scale.  y is never rounded to bf16 on the way: its one rounding is e4m3's.  A
+// row with an infinity or a NaN has the scale NaN (its magnitudes are compared
+// as integers, where a NaN is the largest), so every product of that row is NaN.
+//
+// Bound by memory: each value is read once, kept in registers through the
+// reductions, and written as one byte.
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "q8.h"
+
+namespace ll {
+
+constexpr float kE4m3Max = 448.f;
+constexpr float kQ8MinScale = 1.17549435e-38f;  // 2^-126
+
+enum Q8Mode : int { kQ8Quantize = 0, kQ8Norm = 1, kQ8AddNorm = 2 };
+
+__device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+// Sum over the row's threads: a warp's (WARP), else the CTA's.  The order is
+// fixed, so a row's bits depend on K alone.
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = warp_sum(v);
+  if constexpr (!WARP) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    v = warp_sum(lane < (blockDim.x >> 5) ? red[lane] : 0.f);
+    __syncthreads();  // red is free again
+  }
+  return v;
+}
+template <bool WARP>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
+  v = warp_max_u32(v);
+  if constexpr (!WARP) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    v = warp_max_u32(lane < (blockDim.x >> 5) ? red[lane] : 0u);
+  }
+  return v;
+}
+
+// WARP: a row a warp; else a row a CTA.  VPT vectors of 8 values a thread.
+template <int VPT, int MODE, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : (VPT <= 4 ? 1024 : 512))
+    q8_rows_kernel(const __grid_constant__ LLQ8Rows p) {
+  __shared__ uint32_t red[32];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = WARP ? (threadIdx.x & 31) : threadIdx.x, step = WARP ? 32 : blockDim.x;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && row >= p.rows) return;
+  const int nvec = p.K / 8;
+  const uint4* xr = reinterpret_cast<const uint4*>(p.x + row * p.ldx);
+  float v[VPT][8];
+  uint4 in[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = tid + i * step;
+    in[i] = j < nvec ? xr[j] : make_uint4(0, 0, 0, 0);
+  }
+  if constexpr (MODE == kQ8AddNorm) {
+    const uint4* rr = reinterpret_cast<const uint4*>(p.residual + row * p.ldr);
+    uint4* sr = reinterpret_cast<uint4*>(p.sum + row * p.lds);
+    uint4 add[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = tid + i * step;
+      add[i] = j < nvec ? rr[j] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const uint32_t a[4] = {in[i].x, in[i].y, in[i].z, in[i].w}, b[4] = {add[i].x, add[i].y, add[i].z, add[i].w};
+      uint32_t o[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 fa = unpack_bf16x2(a[c]), fb = unpack_bf16x2(b[c]);
+        v[i][2 * c] = fa.x + fb.x;
+        v[i][2 * c + 1] = fa.y + fb.y;
+        o[c] = pack_bf16x2(v[i][2 * c], v[i][2 * c + 1]);
+      }
+      const int j = tid + i * step;
+      if (j < nvec) sr[j] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const uint32_t a[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 fa = unpack_bf16x2(a[c]);
+        v[i][2 * c] = fa.x;
+        v[i][2 * c + 1] = fa.y;
+      }
+    }
+  }
+  if constexpr (MODE != kQ8Quantize) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) ss = fmaf(v[i][c], v[i][c], ss);
+    ss = row_sum<WARP>(ss, reinterpret_cast<float*>(red));
+    float rstd = rsqrtf(ss / (float)p.K + p.eps);
+    if (!(ss < INFINITY)) {  // squares past fp32's range, or a value that is not finite: the same 2^-80 smaller
+      float s2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float t = v[i][c] * 0x1p-80f;
+          s2 = fmaf(t, t, s2);
+        }
+      s2 = row_sum<WARP>(s2, reinterpret_cast<float*>(red));
+      rstd = rsqrtf(s2 / (float)p.K) * 0x1p-80f;
+    }
+    const uint4* wr = reinterpret_cast<const uint4*>(p.w);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = tid + i * step;
+      const uint4 wv = j < nvec ? wr[j] : make_uint4(0, 0, 0, 0);
+      const uint32_t wu[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 fw = unpack_bf16x2(wu[c]);
+        v[i][2 * c] = v[i][2 * c] * rstd * fw.x;
+        v[i][2 * c + 1] = v[i][2 * c + 1] * rstd * fw.y;
+      }
+    }
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) top = max(top, __float_as_uint(v[i][c]) & 0x7fffffffu);
+  top = row_max<WARP>(top, red);
+  const float amax = __uint_as_float(top);
+  const float scale = amax < INFINITY ? fmaxf(amax / kE4m3Max, kQ8MinScale) : __uint_as_float(0x7fffffffu);
+  const float inv = 1.f / scale;
+  uint2* qr = reinterpret_cast<uint2*>(p.q + row * p.ldq);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = tid + i * step;
+    if (j < nvec)
+      qr[j] = make_uint2(e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
+                         e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+  }
+  if (tid == 0) p.scale[row] = scale;
+}
+
+template <int VPT, bool WARP>
+static cudaError_t q8_rows_launch(const LLQ8Rows& p, int grid, int threads, cudaStream_t stream) {
+  if (p.w == nullptr) return launch_pdl(q8_rows_kernel<VPT, kQ8Quantize, WARP>, dim3(grid), dim3(threads), 0, stream, p);
+  if (p.residual == nullptr)
+    return launch_pdl(q8_rows_kernel<VPT, kQ8Norm, WARP>, dim3(grid), dim3(threads), 0, stream, p);
+  return launch_pdl(q8_rows_kernel<VPT, kQ8AddNorm, WARP>, dim3(grid), dim3(threads), 0, stream, p);
+}
+
+}  // namespace ll
+
+using namespace ll;
+
+extern "C" int ll_q8_rows(const LLQ8Rows* p, cudaStream_t stream) {
+  if (p->rows <= 0) return 0;
+  if (p->K <= 0 || (p->K % 16) || p->K > LL_Q8_MAX_K) return -3;
+  const int nvec = p->K / 8;
+  cudaError_t e;
+  if (nvec <= 128) {  // a warp holds a row
+    const int warps = p->rows < 8 ? p->rows : 8, grid = (p->rows + warps - 1) / warps;
+    if (nvec <= 32) e = q8_rows_launch<1, true>(*p, grid, 32 * warps, stream);
+    else if (nvec <= 64) e = q8_rows_launch<2, true>(*p, grid, 32 * warps, stream);
+    else e = q8_rows_launch<4, true>(*p, grid, 32 * warps, stream);
+  } else {
+    const int vpt = nvec <= 512 ? 1 : (nvec <= 1024 ? 2 : (nvec <= 2048 ? 4 : 8));
+    const int threads = ((nvec + vpt - 1) / vpt + 31) / 32 * 32;
+    if (vpt == 1) e = q8_rows_launch<1, false>(*p, p->rows, threads, stream);
+    else if (vpt == 2) e = q8_rows_launch<2, false>(*p, p->rows, threads, stream);
+    else if (vpt == 4) e = q8_rows_launch<4, false>(*p, p->rows, threads, stream);
+    else e = q8_rows_launch<8, false>(*p, p->rows, threads, stream);
+  }
+  return e == cudaSuccess ? 0 : -5;
+}

@@ -23,12 +23,14 @@ import torch
 from . import reference as ref
 from ._ext import ExtensionMissing, cuda as _cuda  # noqa: F401
 from .lora import LORA_MAX_RANK, LoraPlan, LoraStack, lora_plan  # noqa: F401
+from .q8 import Q8, Q8_MAX_K, check_q8, check_rows, empty_q8  # noqa: F401
 
 __all__ = [
     "ExtensionMissing", "linear", "rmsnorm", "fused_add_rmsnorm", "rope_qkv_write", "attention_prefill",
     "attention_decode", "swiglu", "embedding", "argmax", "kv_link_rope", "interleave_gate_up",
     "deinterleave_gate_up", "prefill_tiles", "workspace", "check_errors", "gemv_rownorm", "gemv_residual",
     "gemv_qkv_rope", "LoraStack", "LoraPlan", "lora_plan", "linear_lora", "sample",
+    "Q8", "quantize_q8", "rmsnorm_q8", "fused_add_rmsnorm_q8", "linear_q8",
 ]
 
 SMALL_M_MAX = 128
@@ -333,6 +335,99 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
         split = -(-M // 128) * -(-N // 128) <= 124
     return _cuda().lora_linear(x, w, bias, out, lora.a, lora.b, lora.scale, plan.buf, plan.tile_rows, plan.max_planes,
                                split, swiglu_epilogue, workspace(x.device).err)
+
+
+def _rows_q8(x: torch.Tensor, out: Optional[Q8], w: Optional[torch.Tensor] = None, eps: float = 0.0,
+             residual: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None) -> Q8:
+    check_rows(x)
+    if w is not None and tuple(w.shape) != (x.shape[1],):
+        raise ValueError(f"the norm's weight must be [{x.shape[1]}], got {tuple(w.shape)}")
+    for t, name in ((residual, "residual"), (residual_out, "residual_out")):
+        if t is not None and t.shape != x.shape:
+            raise ValueError(f"{name} must be {list(x.shape)}, got {list(t.shape)}")
+    if out is None:
+        out = empty_q8(x.shape[0], x.shape[1], x.device)
+    else:
+        check_q8(out, "out")
+        if out.values.shape != x.shape:
+            raise ValueError(f"out must be {list(x.shape)}, got {list(out.values.shape)}")
+    if x.shape[0] == 0:
+        return out
+    if x.is_cuda:
+        _cuda().q8_rows(x, residual, residual_out, w, eps, out.values, out.scale)
+        return out
+    y = x.float()
+    if residual is not None:
+        y = y + residual.float()
+        residual_out.copy_(y)
+    q, s = ref.quantize_q8(y) if w is None else ref.rmsnorm_q8(y, w, eps)
+    out.values.copy_(q)
+    out.scale.copy_(s)
+    return out
+
+
+def quantize_q8(x: torch.Tensor, out: Optional[Q8] = None) -> Q8:
+    """Rows of ``x`` [M, K] to 8 bits (:class:`Q8`): e4m3 values and one fp32
+    scale a row, ``max(amax |x[m]| / 448, 2^-126)``.  A row with an infinity
+    or a NaN has the scale NaN.  K a multiple of 16, at most 32768; on CUDA
+    bf16, rows on 16-byte boundaries.  One launch."""
+    return _rows_q8(x, out)
+
+
+def rmsnorm_q8(x: torch.Tensor, w: torch.Tensor, eps: float, out: Optional[Q8] = None) -> Q8:
+    """:func:`rmsnorm` to 8 bits (:func:`quantize_q8`) in one launch; the norm
+    is not rounded to bf16 in between."""
+    return _rows_q8(x, out, w, eps)
+
+
+def fused_add_rmsnorm_q8(x: torch.Tensor, residual: torch.Tensor, w: torch.Tensor, eps: float,
+                         residual_out: Optional[torch.Tensor] = None, out: Optional[Q8] = None) -> Q8:
+    """``residual_out = x + residual`` (None: in place of ``residual``) and the
+    sum's :func:`rmsnorm_q8`, which takes the sum as it is before it is
+    rounded to bf16."""
+    return _rows_q8(x, out, w, eps, residual, residual if residual_out is None else residual_out)
+
+
+def linear_q8(x: Q8, w: Q8, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, swiglu_epilogue: bool = False) -> torch.Tensor:
+    """:func:`linear` of an input and a weight in 8 bits (:func:`quantize_q8`):
+
+    ``y[m, n] = x.scale[m] * w.scale[n] * sum_k x.values[m, k] * w.values[n, k]
+    + bias[n]``; with ``swiglu_epilogue`` then ``silu(gate) * up`` of the
+    interleaved gate/up product (half width); with ``residual`` [M, N] (half
+    width, likewise) that is added last.  Sums in fp32, one rounding to bf16.
+
+    K a multiple of 16, N of 8 (of 32 with SwiGLU), rows on 16-byte
+    boundaries; ``out`` may be ``residual`` itself, and shares memory with no
+    other input.  One launch without scratch, so calls on several streams may
+    share everything but ``out``.  The same call gives the same bits; a row's
+    last bits may change with the number of rows, which chooses the kernel and
+    its split of K, never with the other rows' values."""
+    check_q8(x, "x")
+    check_q8(w, "w")
+    M, K = x.values.shape
+    N = w.values.shape[0]
+    if w.values.shape[1] != K:
+        raise ValueError(f"x has rows of {K} values, w of {w.values.shape[1]}")
+    if N < 1 or K < 16 or K % 16 or N % (32 if swiglu_epilogue else 8):
+        raise ValueError(f"K = {K}, N = {N}: K must be a multiple of 16 and N of 8 (of 32: SwiGLU)")
+    cols = N // 2 if swiglu_epilogue else N
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
+    for t, name in ((residual, "residual"), (out, "out")):
+        if t is not None and tuple(t.shape) != (M, cols):
+            raise ValueError(f"{name} must be [{M}, {cols}], got {tuple(t.shape)}")
+    if out is None:
+        out = torch.empty(M, cols, dtype=torch.bfloat16, device=x.values.device)
+    if M == 0:
+        return out
+    if x.values.is_cuda:
+        _cuda().q8_gemm(x.values, x.scale, w.values, w.scale, bias, residual, out, swiglu_epilogue, 0,
+                        workspace(out.device).err)
+        return out
+    y = ref.linear_q8(x.values, x.scale, w.values, w.scale, bias)
+    y = ref_swiglu_interleaved(y) if swiglu_epilogue else y
+    return out.copy_(y if residual is None else y + residual.float())
 
 
 def ref_swiglu_interleaved(gu: torch.Tensor) -> torch.Tensor:

@@ -172,6 +172,32 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
     return y
 
 
+def quantize_q8(y: torch.Tensor):
+    """Rows to 8 bits: e4m3 values [M, K] and one fp32 scale a row [M],
+    ``s = max(amax |y| / 448, 2^-126)``, ``q = e4m3(y * (1 / s))``; the scale
+    of a row with an infinity or a NaN is NaN."""
+    y = y.float()
+    amax = y.abs().amax(dim=1)
+    scale = (amax / 448.0).clamp(min=2.0 ** -126)
+    scale = torch.where(amax < math.inf, scale, torch.full_like(scale, math.nan))
+    v = y * (1.0 / scale)[:, None]
+    return torch.where(v.isnan(), v, v.clamp(-448.0, 448.0)).to(torch.float8_e4m3fn), scale
+
+
+def rmsnorm_q8(x: torch.Tensor, w: torch.Tensor, eps: float):
+    xf = x.float()
+    # squares in 64 bits: fp32 ones of values past 2^64 are infinite
+    rstd = torch.rsqrt(xf.double().pow(2).mean(-1, keepdim=True) + eps).float()
+    return quantize_q8(xf * rstd * w.float())
+
+
+def linear_q8(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
+              bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """fp32 ``xs[m] ws[n] sum_k xq[m, k] wq[n, k] + bias[n]``."""
+    y = (xq.float() @ wq.float().t()) * xs[:, None] * ws
+    return y if bias is None else y + bias.float()
+
+
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
            top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
            min_p: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
