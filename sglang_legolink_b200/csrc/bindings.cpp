@@ -30,7 +30,7 @@ int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, int64_t ldc
 int ll_gemm_bf16_lora(const void* A, int lda, const void* W, int ldw, void* C, int ldc, const void* bias, int M,
                       int N, int K, int epilogue, const LLLora* lo, int* err, void* stream);
 int ll_sample(const LLSample* p, cudaStream_t stream);
-int ll_q8_rows(const LLQ8Rows* p, cudaStream_t stream);
+int ll_q8_rows(const LLQ8Rows* p, int variant, cudaStream_t stream);
 int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int cluster, int* err, cudaStream_t stream);
 int ll_rmsnorm(bf16* out, const bf16* x, bf16* residual, const bf16* w, int rows, int hidden, float eps,
                cudaStream_t stream);
@@ -491,7 +491,8 @@ void check_matrix(const at::Tensor& t, at::ScalarType type, const at::Device& de
                   const char* name) {
   TORCH_CHECK(t.device() == dev, name, " must be on ", dev.str());
   TORCH_CHECK(t.scalar_type() == type, name, " must be ", c10::toString(type));
-  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name, " must be [", num(rows), ", ", num(cols), "]");
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name, " must be [", num(rows), ", ",
+                    num(cols), "]");
   TORCH_CHECK(cols == 1 || t.stride(1) == 1, "a row of ", name, " must be contiguous");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_step(t) * t.element_size() % 16 == 0,
               "rows of ", name, " must start on 16-byte boundaries");
@@ -500,7 +501,8 @@ void check_vector(const at::Tensor& t, at::ScalarType type, const at::Device& de
                   bool aligned = true) {
   TORCH_CHECK(t.device() == dev, name, " must be on ", dev.str());
   TORCH_CHECK(t.scalar_type() == type, name, " must be ", c10::toString(type));
-  TORCH_CHECK(t.numel() == n && t.is_contiguous(), name, " must be a contiguous [", num(n), "]");
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.numel() == n, name, " must be [", num(n), "]");
+  TORCH_CHECK(n < 2 || t.stride(0) == 1, name, " must be contiguous");
   TORCH_CHECK(!aligned || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name,
               " must start on a 16-byte boundary");
 }
@@ -515,38 +517,50 @@ bool same_place(const at::Tensor& a, const at::Tensor& b) {
 }
 
 // y = x (w null), rmsnorm(x) w, or rmsnorm(x + residual) w with the sum to `sum`.
-void q8_rows(const at::Tensor& x, const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& sum,
-             const c10::optional<at::Tensor>& w, double eps, const at::Tensor& q, const at::Tensor& scale) {
+// `variant` names a kernel (ll_q8_rows), 0: by the sizes.
+std::tuple<at::Tensor, at::Tensor> q8_rows(const at::Tensor& x, const c10::optional<at::Tensor>& residual,
+                                           const c10::optional<at::Tensor>& sum, const c10::optional<at::Tensor>& w,
+                                           double eps, const c10::optional<at::Tensor>& q_,
+                                           const c10::optional<at::Tensor>& scale_, int64_t variant) {
   CHECK_CUDA(x);
-  TORCH_CHECK(x.dim() == 2, "x must be [rows, K]");
+  TORCH_CHECK_VALUE(x.dim() == 2, "x must be [rows, K]");
   const int64_t rows = x.size(0), K = x.size(1);
-  TORCH_CHECK(rows > 0 && rows < (1ll << 31) && K > 0 && K % 16 == 0 && K <= LL_Q8_MAX_K,
-              "K must be a multiple of 16, at most ", num(LL_Q8_MAX_K), ", and rows below 2^31");
-  check_matrix(x, at::kBFloat16, x.device(), rows, K, "x");
-  check_matrix(q, at::kFloat8_e4m3fn, x.device(), rows, K, "the values");
-  check_vector(scale, at::kFloat, x.device(), rows, "the scales", false);
-  check_written(q, {x, scale}, "the values");
-  TORCH_CHECK(!share_memory(scale, x), "the scales share memory with x");
+  TORCH_CHECK_VALUE(K >= 16 && K % 16 == 0 && K <= LL_Q8_MAX_K, "K must be a multiple of 16, at most ",
+                    num(LL_Q8_MAX_K), ", got ", num(K));
+  TORCH_CHECK(rows < (1ll << 31), "too many rows");
+  const at::Device dev = x.device();
+  check_matrix(x, at::kBFloat16, dev, rows, K, "x");
+  c10::cuda::CUDAGuard g(dev);
+  at::Tensor q = q_.has_value() ? *q_ : at::empty({rows, K}, x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor scale = scale_.has_value() ? *scale_ : at::empty({rows}, x.options().dtype(at::kFloat));
   LLQ8Rows p{};
+  if (q_.has_value() || scale_.has_value()) {
+    check_matrix(q, at::kFloat8_e4m3fn, dev, rows, K, "the values");
+    check_vector(scale, at::kFloat, dev, rows, "the scales", false);
+    check_written(q, {x, scale}, "the values");
+    TORCH_CHECK(!share_memory(scale, x), "the scales share memory with x");
+  }
   if (w.has_value()) {
-    check_vector(*w, at::kBFloat16, x.device(), K, "the norm's weight");
-    check_written(q, {*w}, "the values");
-    TORCH_CHECK(!share_memory(scale, *w), "the scales share memory with the norm's weight");
+    check_vector(*w, at::kBFloat16, dev, K, "the norm's weight");
+    TORCH_CHECK(!share_memory(q, *w) && !share_memory(scale, *w), "the result shares memory with the norm's weight");
     p.w = bp(*w);
   }
   if (residual.has_value()) {
     TORCH_CHECK(sum.has_value() && w.has_value(), "a residual comes with its sum and a norm");
-    check_matrix(*residual, at::kBFloat16, x.device(), rows, K, "the residual");
-    check_matrix(*sum, at::kBFloat16, x.device(), rows, K, "the sum");
-    check_written(*sum, {x, q, scale, *w}, "the sum");
-    if (!same_place(*sum, *residual)) check_written(*sum, {*residual}, "the sum");
-    check_written(q, {*residual}, "the values");
-    TORCH_CHECK(!share_memory(scale, *residual), "the scales share memory with the residual");
+    check_matrix(*residual, at::kBFloat16, dev, rows, K, "residual");
+    check_matrix(*sum, at::kBFloat16, dev, rows, K, "residual_out");
+    check_written(*sum, {x, q, scale, *w}, "residual_out");
+    if (!same_place(*sum, *residual)) {
+      check_written(*sum, {*residual}, "residual_out");
+      TORCH_CHECK(!share_memory(q, *residual) && !share_memory(scale, *residual),
+                  "the result shares memory with residual");
+    }
     p.residual = bp(*residual);
     p.sum = bp(*sum);
     p.ldr = row_step(*residual);
     p.lds = row_step(*sum);
   }
+  if (rows == 0) return {q, scale};
   p.x = bp(x);
   p.q = static_cast<uint8_t*>(q.data_ptr());
   p.scale = scale.data_ptr<float>();
@@ -555,42 +569,51 @@ void q8_rows(const at::Tensor& x, const c10::optional<at::Tensor>& residual, con
   p.rows = (int)rows;
   p.K = (int)K;
   p.eps = (float)eps;
-  c10::cuda::CUDAGuard g(x.device());
-  check_rc(ll_q8_rows(&p, cur_stream()), "ll_q8_rows");
+  check_rc(ll_q8_rows(&p, (int)variant, cur_stream()), "ll_q8_rows");
+  return {q, scale};
 }
 
-// out = act(xs ws (x . w^T) + bias) + residual.  `cluster` names a kernel (ll_q8_gemm), 0: by the sizes.
-void q8_gemm(const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, const at::Tensor& ws,
-             const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, const at::Tensor& out,
-             bool swiglu, int64_t cluster, const at::Tensor& err) {
+// act(xs ws (x . w^T) + bias) + residual.  `cluster` names a kernel (ll_q8_gemm), 0: by the sizes.
+at::Tensor q8_linear(const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, const at::Tensor& ws,
+                     const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                     const c10::optional<at::Tensor>& out_, bool swiglu, int64_t cluster, const at::Tensor& err) {
   CHECK_CUDA(x); CHECK_I32(err);
-  TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x and w must be matrices");
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, "x and w must be matrices");
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0), cols = swiglu ? N / 2 : N;
-  TORCH_CHECK(M > 0 && M < (1 << 28) && N > 0 && N < (1 << 28) && K > 0 && K < (1ll << 31), "bad sizes");
-  TORCH_CHECK(K % 16 == 0 && N % 8 == 0 && (!swiglu || N % 32 == 0),
-              "K must be a multiple of 16 and N of 8 (of 32: SwiGLU)");
-  check_matrix(x, at::kFloat8_e4m3fn, x.device(), M, K, "x");
-  check_matrix(w, at::kFloat8_e4m3fn, x.device(), N, K, "w");
-  check_vector(xs, at::kFloat, x.device(), M, "the scales of x", false);
-  check_vector(ws, at::kFloat, x.device(), N, "the scales of w");
-  check_matrix(out, at::kBFloat16, x.device(), M, cols, "out");
-  TORCH_CHECK(err.device() == x.device(), "the error word must be on ", x.device().str());
+  TORCH_CHECK_VALUE(w.size(1) == K, "x has rows of ", num(K), " values, w of ", num(w.size(1)));
+  TORCH_CHECK_VALUE(K > 0 && K % 16 == 0 && N > 0 && N % (swiglu ? 32 : 8) == 0, "K = ", num(K), ", N = ", num(N),
+                    ": K must be a multiple of 16 and N of 8 (of 32: SwiGLU)");
+  TORCH_CHECK(M < (1 << 28) && N < (1 << 28) && K < (1ll << 31), "too large");
+  const at::Device dev = x.device();
+  check_matrix(x, at::kFloat8_e4m3fn, dev, M, K, "x");
+  check_matrix(w, at::kFloat8_e4m3fn, dev, N, K, "w");
+  check_vector(xs, at::kFloat, dev, M, "the scales of x", false);
+  check_vector(ws, at::kFloat, dev, N, "the scales of w");
+  TORCH_CHECK(err.device() == dev, "the error word must be on ", dev.str());
   TORCH_CHECK(row_step(x) >= K && row_step(w) >= K, "rows of x or w share memory");
-  TORCH_CHECK(row_step(x) < (1ll << 31) && row_step(w) < (1ll << 31) && row_step(out) < (1ll << 31),
-              "row strides must be below 2^31");
-  check_written(out, {x, xs, w, ws}, "out");
+  c10::cuda::CUDAGuard g(dev);
+  at::Tensor out = out_.has_value() ? *out_ : at::empty({M, cols}, x.options().dtype(at::kBFloat16));
   LLQ8Gemm p{};
+  if (out_.has_value()) {
+    check_matrix(out, at::kBFloat16, dev, M, cols, "out");
+    check_written(out, {x, xs, w, ws}, "out");
+  }
   if (bias.has_value()) {
-    check_vector(*bias, at::kBFloat16, x.device(), N, "bias");
-    check_written(out, {*bias}, "out");
+    check_vector(*bias, at::kBFloat16, dev, N, "bias");
+    TORCH_CHECK(!share_memory(out, *bias), "out shares memory with bias");
     p.bias = bp(*bias);
   }
   if (residual.has_value()) {
-    check_matrix(*residual, at::kBFloat16, x.device(), M, cols, "the residual");
-    if (!same_place(out, *residual)) check_written(out, {*residual}, "out");
+    check_matrix(*residual, at::kBFloat16, dev, M, cols, "residual");
+    if (!same_place(out, *residual)) TORCH_CHECK(!share_memory(out, *residual), "out shares memory with residual");
+    TORCH_CHECK(row_step(*residual) >= cols, "rows of residual share memory");
     p.residual = bp(*residual);
     p.ldr = row_step(*residual);
   }
+  TORCH_CHECK(row_step(x) < (1ll << 31) && row_step(w) < (1ll << 31) && row_step(out) < (1ll << 31) &&
+                  p.ldr < (1ll << 31),
+              "row strides must be below 2^31");
+  if (M == 0) return out;
   p.x = static_cast<const uint8_t*>(x.data_ptr());
   p.w = static_cast<const uint8_t*>(w.data_ptr());
   p.xs = xs.data_ptr<float>();
@@ -602,8 +625,8 @@ void q8_gemm(const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, con
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
-  c10::cuda::CUDAGuard g(x.device());
   check_rc(ll_q8_gemm(&p, swiglu ? 1 : 0, (int)cluster, err.data_ptr<int>(), cur_stream()), "ll_q8_gemm");
+  return out;
 }
 
 void rmsnorm(at::Tensor& out, const at::Tensor& x, const c10::optional<at::Tensor>& residual, const at::Tensor& w,
@@ -757,7 +780,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("lora_linear", &lora_linear);
   m.def("sample", &sample);
   m.def("q8_rows", &q8_rows);
-  m.def("q8_gemm", &q8_gemm);
+  m.def("q8_linear", &q8_linear);
   m.def("rmsnorm", &rmsnorm);
   m.def("rope_qkv_write", &rope_qkv_write);
   m.def("kv_link_rope", &kv_link_rope);

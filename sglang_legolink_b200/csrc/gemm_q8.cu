@@ -109,6 +109,9 @@ __device__ __forceinline__ void prefetch_box(const void* tmap, int x, int y) {
 }
 
 __device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
+// The approximate quotient (off by 2 ulp; 0 for a divisor past 2^126, where x is
+// below -87 and silu(x) below 1e-36).
+__device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 // Lets the copies in flight land before a CTA that gave up exits.
 __device__ __forceinline__ void linger() {
   const unsigned long long t0 = globaltimer_ns();
@@ -117,7 +120,7 @@ __device__ __forceinline__ void linger() {
 }
 
 struct alignas(64) Maps {
-  CUtensorMap w, x, c;
+  CUtensorMap w, x, c, r;
 };
 
 // ---------------------------------------------------------------------------
@@ -300,10 +303,15 @@ __global__ void __launch_bounds__(192, 2)
 // which accumulate rows [128 r, +128) in CTA r's tensor memory.  Loads of both
 // complete on the leader's `full` barrier, commits arrive in both CTAs.
 constexpr int BN = 256;
-constexpr int PAIR_STAGES = 6;
+constexpr int PAIR_STAGES = 5;
 constexpr int PAIR_TILE = 128 * BK;  // a CTA's half of X's, and of W's, k-block
+constexpr int PAIR_EPI_WARPS = 8;    // two to a quarter of TMEM's lanes, each with half of the tile's columns
+constexpr int PAIR_COLS = BN / 2;    // accumulator columns of an epilogue warp
+constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
 constexpr int PAIR_BOX = 32 * 64;    // epilogue staging: 32 rows x 32 bf16 columns
-constexpr int PAIR_SMEM = PAIR_STAGES * 2 * PAIR_TILE + 4 * 2 * PAIR_BOX + 1024 + 256;
+constexpr int PAIR_BOXES = 3;        // of a warp: one is stored, one worked on, one being filled with residual
+constexpr int PAIR_EPI_BYTES = PAIR_EPI_WARPS * (PAIR_BOXES * PAIR_BOX + 2 * PAIR_COLS * 4);  // boxes; scales and bias
+constexpr int PAIR_SMEM = PAIR_STAGES * 2 * PAIR_TILE + PAIR_EPI_BYTES + 1024 + 512;
 constexpr int PAIR_TMEM = 2 * BN;
 
 // Groups of `group_m` row tiles, rows fastest inside a group: the tiles in flight
@@ -318,19 +326,21 @@ __device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, int group
 }
 
 template <bool SWIGLU>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     q8_pair_kernel(const __grid_constant__ Maps tm, const __grid_constant__ LLQ8Gemm p, int group_m, int* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
   uint8_t* sW = smem + PAIR_STAGES * PAIR_TILE;
-  uint8_t* sEpi = sW + PAIR_STAGES * PAIR_TILE;  // [4 warps][2] boxes
-  uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + 4 * 2 * PAIR_BOX);
+  uint8_t* sBox = sW + PAIR_STAGES * PAIR_TILE;                                              // [warps][boxes]
+  float* sCol = reinterpret_cast<float*>(sBox + PAIR_EPI_WARPS * PAIR_BOXES * PAIR_BOX);  // [warps][scales, bias]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sCol + PAIR_EPI_WARPS * 2 * PAIR_COLS);
   uint64_t* empty = full + PAIR_STAGES;
   uint64_t* tfull = empty + PAIR_STAGES;
   uint64_t* tempty = tfull + 2;
   uint64_t* drain = tempty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* rfull = drain + 1;  // [warps][boxes]: residual has landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + PAIR_EPI_WARPS * PAIR_BOXES);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = cluster_rank();
@@ -346,9 +356,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 8);  // 4 epilogue warps x 2 CTAs (used on the leader)
+      mbar_init(&tempty[a], 2 * PAIR_EPI_WARPS);  // of both CTAs (used on the leader)
     }
     mbar_init(drain, 1);
+    for (int i = 0; i < PAIR_EPI_WARPS * PAIR_BOXES; ++i) mbar_init(&rfull[i], 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -429,59 +440,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     }
     __syncwarp();
   } else {
-    // warp (w % 4) owns TMEM lanes [32 (w % 4), +32): lane = row
-    const int q = warp & 3;
+    // warp w reads TMEM lanes [32 (w % 4), +32) (lane = row) of the tile's columns [128 half, +128)
+    const int q = warp & 3, e = warp - 2, half = e >> 2;
     const uint32_t leader_tempty0 = mapa(smem_u32(&tempty[0]), 0), leader_tempty1 = mapa(smem_u32(&tempty[1]), 0);
-    uint8_t* boxes = sEpi + q * 2 * PAIR_BOX;
-    int acc = 0, nbox = 0;
-    uint32_t aphase = 0;
+    uint8_t* boxes = sBox + e * PAIR_BOXES * PAIR_BOX;
+    uint64_t* rbar = rfull + e * PAIR_BOXES;
+    float* scol = sCol + e * 2 * PAIR_COLS;
+    float* sbias = scol + PAIR_COLS;
+    constexpr int STEP = SWIGLU ? 64 : 32;  // accumulator columns of a box of 32 output columns
+    int acc = 0, b = 0;  // the box that is next
+    uint32_t aphase = 0, bphase = 0;
     for (int t = pair; t < ntiles; t += npairs) {
       int mb, nb;
       pair_tile(t, num_m, num_n, group_m, mb, nb);
       const int row0 = mb * 256 + (int)crank * 128 + q * 32, row = row0 + lane;
+      const int colw = nb * BN + half * PAIR_COLS;  // this warp's first accumulator column
+      // what does not depend on the product, while it runs
       const float xs = row < p.M ? p.xs[row] : 1.f;
-      if (!mbar_wait(&tfull[acc], aphase, err, kErrTmemFullTimeout)) break;
-      tc_fence_after();
-      const uint32_t tbase = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN);
-      // scales and bias of 32 accumulator columns, the same for every lane
-      auto scaled = [&](uint32_t (&r)[32], int col) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          if (col + i >= p.N) break;  // N % 8 == 0
-          const float4 s = __ldg(reinterpret_cast<const float4*>(p.ws + col + i));
-          const float sv[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) r[i + j] = __float_as_uint(__uint_as_float(r[i + j]) * xs * sv[j]);
-        }
-        if (p.bias != nullptr) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            if (col + i >= p.N) break;
-            const uint4 b = __ldg(reinterpret_cast<const uint4*>(p.bias + col + i));
-            const uint32_t bu[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack_bf16x2(bu[j]);
-              r[i + 2 * j] = __float_as_uint(__uint_as_float(r[i + 2 * j]) + f.x);
-              r[i + 2 * j + 1] = __float_as_uint(__uint_as_float(r[i + 2 * j + 1]) + f.y);
-            }
-          }
-        }
+      const int cl = colw + 4 * lane;  // N % 8 == 0: four columns are all there or none is
+      const float4 ws4 = cl < p.N ? *reinterpret_cast<const float4*>(p.ws + cl) : make_float4(0, 0, 0, 0);
+      const uint2 bias4 = p.bias != nullptr && cl < p.N ? *reinterpret_cast<const uint2*>(p.bias + cl) : make_uint2(0, 0);
+      // fills box `at` with the residual of accumulator columns [c, c + STEP),
+      // once the store that last read the box is done with it
+      auto fetch_residual = [&](int at, int c) {
+        if (p.residual == nullptr || lane != 0 || c >= PAIR_COLS || colw + c >= p.N || row0 >= p.M) return;
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        mbar_arrive_expect_tx(&rbar[at], PAIR_BOX);
+        tma_load_2d(boxes + at * PAIR_BOX, &tm.r, &rbar[at], SWIGLU ? (colw + c) / 2 : colw + c, row0);
       };
-      constexpr int STEP = SWIGLU ? 64 : 32;  // accumulator columns of a box of 32 output columns
+      fetch_residual(b, 0);
+      __syncwarp();  // the tile before is read
+      *reinterpret_cast<float4*>(scol + 4 * lane) = ws4;
+      {
+        const float2 b0 = unpack_bf16x2(bias4.x), b1 = unpack_bf16x2(bias4.y);
+        *reinterpret_cast<float4*>(sbias + 4 * lane) = make_float4(b0.x, b0.y, b1.x, b1.y);
+      }
+      __syncwarp();
+      if (!mbar_wait(&tfull[acc], aphase, err, kErrTmemFullTimeout)) {
+        if (p.residual != nullptr) linger();
+        break;
+      }
+      tc_fence_after();
+      const uint32_t tbase = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN + half * PAIR_COLS);
+      // r[i] ws xs + bias of columns [c, c + 32); every lane reads the same of them
+      auto scaled = [&](const uint32_t (&r)[32], int c, int i) {
+        const float4 s = *reinterpret_cast<const float4*>(scol + c + i), b = *reinterpret_cast<const float4*>(sbias + c + i);
+        return make_float4(fmaf(__uint_as_float(r[i]) * xs, s.x, b.x), fmaf(__uint_as_float(r[i + 1]) * xs, s.y, b.y),
+                           fmaf(__uint_as_float(r[i + 2]) * xs, s.z, b.z), fmaf(__uint_as_float(r[i + 3]) * xs, s.w, b.w));
+      };
 #pragma unroll 1
-      for (int c = 0; c < BN; c += STEP) {
-        const int col0 = nb * BN + c;
-        if (col0 >= p.N || row0 >= p.M) continue;  // the whole box is outside C
-        const int out0 = SWIGLU ? col0 / 2 : col0, out_n = SWIGLU ? p.N / 2 : p.N;
-        uint4 res[4];
-        if (p.residual != nullptr) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            res[i] = row < p.M && out0 + 8 * i < out_n
-                         ? *reinterpret_cast<const uint4*>(p.residual + row * p.ldr + out0 + 8 * i)
-                         : make_uint4(0, 0, 0, 0);
-        }
+      for (int c = 0; c < PAIR_COLS; c += STEP) {
+        if (colw + c >= p.N || row0 >= p.M) break;  // the whole box is outside C
+        const int out0 = SWIGLU ? (colw + c) / 2 : colw + c;
         float v[32];
         if constexpr (SWIGLU) {
 #pragma unroll
@@ -489,52 +499,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
             uint32_t r[32];
             tmem_ld_32x32b_x32(tbase + c + 32 * h, r);
             tmem_ld_wait();
-            scaled(r, col0 + 32 * h);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              // rows past M are zero, and dividing a zero takes a slow path
-              const float g = row < p.M ? __uint_as_float(r[i]) : 1.f;
-              v[16 * h + i] = silu(g) * __uint_as_float(r[16 + i]);
+            for (int i = 0; i < 16; i += 4) {
+              const float4 g = scaled(r, c + 32 * h, i), u = scaled(r, c + 32 * h, i + 16);
+              v[16 * h + i] = silu_fast(g.x) * u.x;
+              v[16 * h + i + 1] = silu_fast(g.y) * u.y;
+              v[16 * h + i + 2] = silu_fast(g.z) * u.z;
+              v[16 * h + i + 3] = silu_fast(g.w) * u.w;
             }
           }
         } else {
           uint32_t r[32];
           tmem_ld_32x32b_x32(tbase + c, r);
           tmem_ld_wait();
-          scaled(r, col0);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+          for (int i = 0; i < 32; i += 4) {
+            const float4 y = scaled(r, c, i);
+            v[i] = y.x;
+            v[i + 1] = y.y;
+            v[i + 2] = y.z;
+            v[i + 3] = y.w;
+          }
         }
+        // 16-byte chunk k of row r is chunk k ^ ((r >> 1) & 3) of a box, the 64-byte
+        // swizzle of the maps; rows past M and columns past N are clipped there
+        uint4* d = reinterpret_cast<uint4*>(boxes + b * PAIR_BOX + lane * 64);
+        const int swz = (lane >> 1) & 3;
         if (p.residual != nullptr) {
+          fetch_residual(b == PAIR_BOXES - 1 ? 0 : b + 1, c + STEP);
+          if (!mbar_wait(&rbar[b], bphase, err, kErrTmaFullTimeout)) linger();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t ru[4] = {res[i].x, res[i].y, res[i].z, res[i].w};
+          for (int k = 0; k < 4; ++k) {
+            const uint4 rv = d[k ^ swz];
+            const uint32_t ru[4] = {rv.x, rv.y, rv.z, rv.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float2 f = unpack_bf16x2(ru[j]);
-              v[8 * i + 2 * j] += f.x;
-              v[8 * i + 2 * j + 1] += f.y;
+              v[8 * k + 2 * j] += f.x;
+              v[8 * k + 2 * j + 1] += f.y;
             }
           }
+        } else {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PAIR_BOXES - 1) : "memory");
+          __syncwarp();
         }
-        // 16-byte chunk k of row r goes to chunk k ^ ((r >> 1) & 3), the 64-byte
-        // swizzle of C's map; rows past M and columns past N are clipped there
-        uint8_t* box = boxes + (nbox & 1) * PAIR_BOX;
-        if (nbox >= 2 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        __syncwarp();
-        uint4* d = reinterpret_cast<uint4*>(box + lane * 64);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          d[k ^ ((lane >> 1) & 3)] =
-              make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                         pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+          d[k ^ swz] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                                  pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
-          store_box(&tm.c, box, out0, row0);
+          store_box(&tm.c, boxes + b * PAIR_BOX, out0, row0);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
-        ++nbox;
+        if (++b == PAIR_BOXES) {
+          b = 0;
+          bphase ^= 1;
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -544,7 +566,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         aphase ^= 1;
       }
     }
-    if (lane == 0 && nbox > 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   tc_fence_before();
@@ -583,12 +605,12 @@ static bool operand_map(CUtensorMap* tm, const void* ptr, int rows, int K, int64
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// C for the bulk stores: boxes of 32 columns (64 bytes) x 32 rows, 64-byte swizzle.
-static bool output_map(CUtensorMap* tm, void* ptr, int rows, int cols, int64_t ld) {
+// C, or the residual: boxes of 32 columns (64 bytes) x 32 rows, 64-byte swizzle.
+static bool output_map(CUtensorMap* tm, const void* ptr, int rows, int cols, int64_t ld) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
   const cuuint32_t box[2] = {32, 32}, estr[2] = {1, 1};
   const EncodeFn enc = encode_fn();
-  return enc != nullptr && enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, estr,
+  return enc != nullptr && enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
                                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -612,11 +634,13 @@ static int launch(Kern kern, dim3 grid, int smem, int cluster, cudaStream_t stre
   return cudaLaunchKernelEx(&cfg, kern, tm, p, err) == cudaSuccess ? 0 : -5;
 }
 
-// CTAs that share a feature tile's K: as many as have places, two a SM.
+// CTAs that share a feature tile's K: as many as have places, two a SM; larger
+// clusters than pairs do not fill the SMs to the last place.
 constexpr int SPLIT_PLACES = 248;
 static int split_rule(int M, int N, int K, int bnx) {
-  const int tiles = ((N + 127) / 128) * ((M + bnx - 1) / bnx), num_kb = (K + BK - 1) / BK;
-  int cs = SPLIT_PLACES / tiles;
+  const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + bnx - 1) / bnx);
+  const int num_kb = (K + BK - 1) / BK;
+  int cs = tiles <= 148 && tiles > SPLIT_PLACES / 2 ? 2 : (int)(SPLIT_PLACES / tiles);
   if (cs > SPLIT_MAX_CLUSTER) cs = SPLIT_MAX_CLUSTER;
   if (cs > (num_kb + 1) / 2) cs = (num_kb + 1) / 2;
   return cs < 1 ? 1 : cs;
@@ -628,7 +652,7 @@ static int split_launch(const LLQ8Gemm& p, int cs, int* err, cudaStream_t stream
   if (cs <= 0) cs = split_rule(p.M, p.N, p.K, bnx);
   Maps tm;
   if (!operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) || !operand_map(&tm.x, p.x, p.M, p.K, p.ldx, bnx)) return -2;
-  tm.c = tm.x;  // not read
+  tm.c = tm.r = tm.x;  // not read
   const dim3 grid(cs, (p.N + 127) / 128, (p.M + bnx - 1) / bnx);
   if (grid.y > 65535 || grid.z > 65535) return -3;
   static unsigned long long done[4] = {0, 0, 0, 0};
@@ -646,6 +670,8 @@ static int pair_launch(const LLQ8Gemm& p, int* err, cudaStream_t stream) {
   if (!operand_map(&tm.x, p.x, p.M, p.K, p.ldx, 128) || !operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) ||
       !output_map(&tm.c, p.C, p.M, SWIGLU ? p.N / 2 : p.N, p.ldc))
     return -2;
+  tm.r = tm.c;  // read with a residual only
+  if (p.residual != nullptr && !output_map(&tm.r, p.residual, p.M, SWIGLU ? p.N / 2 : p.N, p.ldr)) return -2;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -661,7 +687,7 @@ static int pair_launch(const LLQ8Gemm& p, int* err, cudaStream_t stream) {
   static unsigned long long done = 0;
   auto kern = q8_pair_kernel<SWIGLU>;
   if (!smem_on_device(kern, PAIR_SMEM, done)) return -7;
-  const cudaError_t e = launch_pdl(kern, dim3(2 * pairs), dim3(192), PAIR_SMEM, stream, tm, p, (int)group, err);
+  const cudaError_t e = launch_pdl(kern, dim3(2 * pairs), dim3(PAIR_THREADS), PAIR_SMEM, stream, tm, p, (int)group, err);
   return e == cudaSuccess ? 0 : -5;
 }
 
@@ -675,7 +701,8 @@ extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int cluster, int* err, 
   if (p->M <= 0) return 0;
   if (p->N <= 0 || p->K <= 0 || (p->K % 16) || (p->N % 8) || (swiglu && (p->N % 32))) return -3;
   if ((p->ldx % 16) || (p->ldw % 16) || (p->ldc % 8) || (p->ldr % 8) || cluster > SPLIT_MAX_CLUSTER) return -3;
-  const bool split = cluster > 0 || (cluster == 0 && p->M <= 128);
+  const int64_t tiles = (int64_t)((p->N + 127) / 128) * ((p->M + 127) / 128);
+  const bool split = cluster > 0 || (cluster == 0 && (p->M <= 128 || tiles <= 200));
   if (split) return swiglu ? split_launch<true>(*p, cluster, err, stream) : split_launch<false>(*p, cluster, err, stream);
   return swiglu ? pair_launch<true>(*p, err, stream) : pair_launch<false>(*p, err, stream);
 }

@@ -23,14 +23,14 @@ import torch
 from . import reference as ref
 from ._ext import ExtensionMissing, cuda as _cuda  # noqa: F401
 from .lora import LORA_MAX_RANK, LoraPlan, LoraStack, lora_plan  # noqa: F401
-from .q8 import Q8, Q8_MAX_K, check_q8, check_rows, empty_q8  # noqa: F401
+from .q8 import Q8, check_product, check_rows, empty_q8
 
 __all__ = [
     "ExtensionMissing", "linear", "rmsnorm", "fused_add_rmsnorm", "rope_qkv_write", "attention_prefill",
     "attention_decode", "swiglu", "embedding", "argmax", "kv_link_rope", "interleave_gate_up",
     "deinterleave_gate_up", "prefill_tiles", "workspace", "check_errors", "gemv_rownorm", "gemv_residual",
     "gemv_qkv_rope", "LoraStack", "LoraPlan", "lora_plan", "linear_lora", "sample",
-    "Q8", "quantize_q8", "rmsnorm_q8", "fused_add_rmsnorm_q8", "linear_q8",
+    "Q8", "empty_q8", "quantize_q8", "rmsnorm_q8", "fused_add_rmsnorm_q8", "linear_q8",
 ]
 
 SMALL_M_MAX = 128
@@ -339,22 +339,11 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
 
 def _rows_q8(x: torch.Tensor, out: Optional[Q8], w: Optional[torch.Tensor] = None, eps: float = 0.0,
              residual: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None) -> Q8:
-    check_rows(x)
-    if w is not None and tuple(w.shape) != (x.shape[1],):
-        raise ValueError(f"the norm's weight must be [{x.shape[1]}], got {tuple(w.shape)}")
-    for t, name in ((residual, "residual"), (residual_out, "residual_out")):
-        if t is not None and t.shape != x.shape:
-            raise ValueError(f"{name} must be {list(x.shape)}, got {list(t.shape)}")
-    if out is None:
-        out = empty_q8(x.shape[0], x.shape[1], x.device)
-    else:
-        check_q8(out, "out")
-        if out.values.shape != x.shape:
-            raise ValueError(f"out must be {list(x.shape)}, got {list(out.values.shape)}")
-    if x.shape[0] == 0:
-        return out
     if x.is_cuda:
-        _cuda().q8_rows(x, residual, residual_out, w, eps, out.values, out.scale)
+        q, s = (None, None) if out is None else out
+        return Q8(*_cuda().q8_rows(x, residual, residual_out, w, eps, q, s, 0))
+    out = check_rows(x, out, w, residual, residual_out)
+    if x.shape[0] == 0:
         return out
     y = x.float()
     if residual is not None:
@@ -403,28 +392,12 @@ def linear_q8(x: Q8, w: Q8, bias: Optional[torch.Tensor] = None, residual: Optio
     share everything but ``out``.  The same call gives the same bits; a row's
     last bits may change with the number of rows, which chooses the kernel and
     its split of K, never with the other rows' values."""
-    check_q8(x, "x")
-    check_q8(w, "w")
-    M, K = x.values.shape
-    N = w.values.shape[0]
-    if w.values.shape[1] != K:
-        raise ValueError(f"x has rows of {K} values, w of {w.values.shape[1]}")
-    if N < 1 or K < 16 or K % 16 or N % (32 if swiglu_epilogue else 8):
-        raise ValueError(f"K = {K}, N = {N}: K must be a multiple of 16 and N of 8 (of 32: SwiGLU)")
-    cols = N // 2 if swiglu_epilogue else N
-    if bias is not None and tuple(bias.shape) != (N,):
-        raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
-    for t, name in ((residual, "residual"), (out, "out")):
-        if t is not None and tuple(t.shape) != (M, cols):
-            raise ValueError(f"{name} must be [{M}, {cols}], got {tuple(t.shape)}")
-    if out is None:
-        out = torch.empty(M, cols, dtype=torch.bfloat16, device=x.values.device)
-    if M == 0:
-        return out
     if x.values.is_cuda:
-        _cuda().q8_gemm(x.values, x.scale, w.values, w.scale, bias, residual, out, swiglu_epilogue, 0,
-                        workspace(out.device).err)
-        return out
+        return _cuda().q8_linear(x.values, x.scale, w.values, w.scale, bias, residual, out, swiglu_epilogue, 0,
+                                 workspace(x.values.device).err)
+    cols = check_product(x, w, bias, residual, out, swiglu_epilogue)
+    if out is None:
+        out = torch.empty(x.values.shape[0], cols, dtype=torch.bfloat16)
     y = ref.linear_q8(x.values, x.scale, w.values, w.scale, bias)
     y = ref_swiglu_interleaved(y) if swiglu_epilogue else y
     return out.copy_(y if residual is None else y + residual.float())

@@ -248,8 +248,8 @@ def raw(x, w, bias=None, residual=None, swiglu=False, kernel=0):
     """The product by a named kernel (-1: pairs of CTAs; n: n CTAs to a feature tile)."""
     M, N = x.values.shape[0], w.values.shape[0]
     out = torch.full((M + 2, N // 2 if swiglu else N), 3.0, dtype=torch.bfloat16, device="cuda")
-    ops._cuda().q8_gemm(x.values, x.scale, w.values, w.scale, bias, residual, out[:M],
-                        swiglu, kernel, ops.workspace("cuda").err)
+    ops._cuda().q8_linear(x.values, x.scale, w.values, w.scale, bias, residual, out[:M], swiglu, kernel,
+                          ops.workspace("cuda").err)
     assert bool((out[M:] == 3).all())
     return out[:M]
 
