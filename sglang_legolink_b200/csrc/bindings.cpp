@@ -31,7 +31,7 @@ int ll_gemm_bf16_lora(const void* A, int lda, const void* W, int ldw, void* C, i
                       int N, int K, int epilogue, const LLLora* lo, int* err, void* stream);
 int ll_sample(const LLSample* p, cudaStream_t stream);
 int ll_q8_rows(const LLQ8Rows* p, int variant, cudaStream_t stream);
-int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int cluster, int* err, cudaStream_t stream);
+int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, cudaStream_t stream);
 int ll_rmsnorm(bf16* out, const bf16* x, bf16* residual, const bf16* w, int rows, int hidden, float eps,
                cudaStream_t stream);
 int ll_rope_qkv_write(const bf16* qkv, const int* positions, const int64_t* slots, const float* cos_sin, bf16* q_out,
@@ -573,10 +573,10 @@ std::tuple<at::Tensor, at::Tensor> q8_rows(const at::Tensor& x, const c10::optio
   return {q, scale};
 }
 
-// act(xs ws (x . w^T) + bias) + residual.  `cluster` names a kernel (ll_q8_gemm), 0: by the sizes.
+// act(xs ws (x . w^T) + bias) + residual.  `kernel` names one (ll_q8_gemm), 0: by the sizes.
 at::Tensor q8_linear(const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, const at::Tensor& ws,
                      const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
-                     const c10::optional<at::Tensor>& out_, bool swiglu, int64_t cluster, const at::Tensor& err) {
+                     const c10::optional<at::Tensor>& out_, bool swiglu, int64_t kernel, const at::Tensor& err) {
   CHECK_CUDA(x); CHECK_I32(err);
   TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, "x and w must be matrices");
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0), cols = swiglu ? N / 2 : N;
@@ -625,7 +625,7 @@ at::Tensor q8_linear(const at::Tensor& x, const at::Tensor& xs, const at::Tensor
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
-  check_rc(ll_q8_gemm(&p, swiglu ? 1 : 0, (int)cluster, err.data_ptr<int>(), cur_stream()), "ll_q8_gemm");
+  check_rc(ll_q8_gemm(&p, swiglu ? 1 : 0, (int)kernel, err.data_ptr<int>(), cur_stream()), "ll_q8_gemm");
   return out;
 }
 

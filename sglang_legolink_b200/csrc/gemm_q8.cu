@@ -108,10 +108,9 @@ __device__ __forceinline__ void prefetch_box(const void* tmap, int x, int y) {
                : "memory");
 }
 
-__device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
-// The approximate quotient (off by 2 ulp; 0 for a divisor past 2^126, where x is
-// below -87 and silu(x) below 1e-36).
-__device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+// The approximate quotient is off by 2 ulp, and 0 for a divisor past 2^126, where x
+// is below -87 and silu(x) below 1e-36.
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 // Lets the copies in flight land before a CTA that gave up exits.
 __device__ __forceinline__ void linger() {
   const unsigned long long t0 = globaltimer_ns();
@@ -152,6 +151,7 @@ __global__ void __launch_bounds__(192, 2)
   float* part = reinterpret_cast<float*>(smem);  // [rows][LD], over the ring, once the product is done
   __shared__ uint64_t full[STAGES], empty[STAGES], tfull;
   __shared__ uint32_t tmem_slot;
+  __shared__ float sxs[BNX];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cs = gridDim.x, crank = blockIdx.x, nb = blockIdx.y;
@@ -220,10 +220,37 @@ __global__ void __launch_bounds__(192, 2)
   }
   __syncwarp();
   pdl_wait();  // the scales and the residual are the previous kernel's; C may still be read by it
+  // A thread keeps its four features (with SwiGLU four gate features and the
+  // matching up features, 16 further on) over the rows of its share; what the
+  // epilogue reads of them, and its first row's residual, is on its way while the
+  // product runs.
+  constexpr int GROUPS = SWIGLU ? 16 : 32, PER = 192 / GROUPS;  // groups of four outputs a row, rows at once
+  const int g = tid % GROUPS, f = SWIGLU ? (g >> 2) * 32 + (g & 3) * 4 : 4 * g;
+  const int col = SWIGLU ? nb * 64 + 4 * g : nb * 128 + f;
+  const bool live = nb * 128 + f < p.N;
+  const int row0 = crank * PER + tid / GROUPS, row_step = cs * PER;
+  float4 ws[2] = {}, bias[2] = {};
+#pragma unroll
+  for (int h = 0; h < (SWIGLU ? 2 : 1); ++h) {
+    if (!live) break;
+    ws[h] = *reinterpret_cast<const float4*>(p.ws + nb * 128 + f + 16 * h);
+    if (p.bias != nullptr) {
+      const uint2 b = *reinterpret_cast<const uint2*>(p.bias + nb * 128 + f + 16 * h);
+      const float2 b0 = unpack_bf16x2(b.x), b1 = unpack_bf16x2(b.y);
+      bias[h] = make_float4(b0.x, b0.y, b1.x, b1.y);
+    }
+  }
+  auto residual_at = [&](int row) {
+    return p.residual != nullptr && live && row < rows
+               ? *reinterpret_cast<const uint2*>(p.residual + (m0 + row) * p.ldr + col)
+               : make_uint2(0, 0);
+  };
+  uint2 next = residual_at(row0);
+  if (tid < rows) sxs[tid] = p.xs[m0 + tid];
   const bool ok = __syncthreads_and(mbar_wait(&tfull, 0, err, kErrTmemFullTimeout));
   tc_fence_after();
   if (warp >= 2) {  // TMEM lane quarter of this warp: features; columns: rows
-    const int f = (warp & 3) * 32 + lane;
+    const int feat = (warp & 3) * 32 + lane;
 #pragma unroll 1
     for (int c = 0; c < BNX && c < rows; c += 32) {
       uint32_t r[32];
@@ -231,69 +258,53 @@ __global__ void __launch_bounds__(192, 2)
       tmem_ld_wait();
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (c + i < rows && c + i < BNX) part[(c + i) * Cfg::LD + f] = kb1 > kb0 ? __uint_as_float(r[i]) : 0.f;
+        if (c + i < rows && c + i < BNX) part[(c + i) * Cfg::LD + feat] = kb1 > kb0 ? __uint_as_float(r[i]) : 0.f;
     }
   }
   tc_fence_before();
-  cluster_barrier();
+  if (cs > 1) cluster_barrier();
+  else __syncthreads();
   tc_fence_after();
-  if (ok) {
+  if (ok && live) {
     const uint32_t base = smem_u32(part);
-    // four features of a row: the partials in split order, scales, bias
-    auto sum4 = [&](int row, float xs, int f) {
-      float4 t[SPLIT_MAX_CLUSTER];
-      const uint32_t at = base + (uint32_t)(row * Cfg::LD + f) * 4;
+    // the partials of four features in split order, scales, bias
+    auto sum4 = [&](int row, float xs, int h) {
+      const int at = row * Cfg::LD + f + 16 * h;
+      float4 v = *reinterpret_cast<const float4*>(part + at);
+      if (cs > 1) {
+        float4 t[SPLIT_MAX_CLUSTER];
 #pragma unroll
-      for (int r = 0; r < SPLIT_MAX_CLUSTER; ++r) t[r] = r < cs ? ld_cluster(mapa(at, r)) : make_float4(0, 0, 0, 0);
-      float4 v = t[0];
+        for (int r = 0; r < SPLIT_MAX_CLUSTER; ++r)
+          t[r] = r < cs ? ld_cluster(mapa(base + 4 * at, r)) : make_float4(0, 0, 0, 0);
+        v = t[0];
 #pragma unroll
-      for (int r = 1; r < SPLIT_MAX_CLUSTER; ++r) {
-        v.x += t[r].x;
-        v.y += t[r].y;
-        v.z += t[r].z;
-        v.w += t[r].w;
+        for (int r = 1; r < SPLIT_MAX_CLUSTER; ++r) {
+          v.x += t[r].x;
+          v.y += t[r].y;
+          v.z += t[r].z;
+          v.w += t[r].w;
+        }
       }
-      const float4 s = *reinterpret_cast<const float4*>(p.ws + nb * 128 + f);
-      v.x = v.x * xs * s.x;
-      v.y = v.y * xs * s.y;
-      v.z = v.z * xs * s.z;
-      v.w = v.w * xs * s.w;
-      if (p.bias != nullptr) {
-        const uint2 bv = *reinterpret_cast<const uint2*>(p.bias + nb * 128 + f);
-        const float2 b0 = unpack_bf16x2(bv.x), b1 = unpack_bf16x2(bv.y);
-        v.x += b0.x;
-        v.y += b0.y;
-        v.z += b1.x;
-        v.w += b1.y;
-      }
-      return v;
+      return make_float4(fmaf(v.x * xs, ws[h].x, bias[h].x), fmaf(v.y * xs, ws[h].y, bias[h].y),
+                         fmaf(v.z * xs, ws[h].z, bias[h].z), fmaf(v.w * xs, ws[h].w, bias[h].w));
     };
-    constexpr int GROUPS = SWIGLU ? 16 : 32;  // 4-feature groups a row
-    for (int i = crank * 192 + tid; i < rows * GROUPS; i += cs * 192) {
-      const int row = i / GROUPS, g = i % GROUPS;
-      const int64_t m = m0 + row;
-      const int f = SWIGLU ? (g >> 2) * 32 + (g & 3) * 4 : 4 * g;
-      if (nb * 128 + f >= p.N) continue;
-      const int col = SWIGLU ? nb * 64 + 4 * g : nb * 128 + f;
-      uint2 rv = make_uint2(0, 0);
-      if (p.residual != nullptr) rv = *reinterpret_cast<const uint2*>(p.residual + m * p.ldr + col);
-      const float xs = p.xs[m];
-      float4 v = sum4(row, xs, f);
-      if constexpr (SWIGLU) {  // 16 gate features, then the matching 16 up features
-        const float4 u = sum4(row, xs, f + 16);
+#pragma unroll 2
+    for (int row = row0; row < rows; row += row_step) {
+      const uint2 rv = next;
+      next = residual_at(row + row_step);
+      const float xs = sxs[row];
+      float4 v = sum4(row, xs, 0);
+      if constexpr (SWIGLU) {
+        const float4 u = sum4(row, xs, 1);
         v = make_float4(silu(v.x) * u.x, silu(v.y) * u.y, silu(v.z) * u.z, silu(v.w) * u.w);
       }
-      if (p.residual != nullptr) {
-        const float2 r0 = unpack_bf16x2(rv.x), r1 = unpack_bf16x2(rv.y);
-        v.x += r0.x;
-        v.y += r0.y;
-        v.z += r1.x;
-        v.w += r1.y;
-      }
-      *reinterpret_cast<uint2*>(p.C + m * p.ldc + col) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+      const float2 r0 = unpack_bf16x2(rv.x), r1 = unpack_bf16x2(rv.y);
+      *reinterpret_cast<uint2*>(p.C + (m0 + row) * p.ldc + col) =
+          make_uint2(pack_bf16x2(v.x + r0.x, v.y + r0.y), pack_bf16x2(v.z + r1.x, v.w + r1.y));
     }
   }
-  cluster_barrier();  // the partials live until every CTA has read them
+  if (cs > 1) cluster_barrier();  // the partials live until every CTA has read them
+  else __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);
 }
 
@@ -302,17 +313,21 @@ __global__ void __launch_bounds__(192, 2)
 // and of its 256 rows of W; the leader issues the MMAs (M = 256, N = 256, K = 32),
 // which accumulate rows [128 r, +128) in CTA r's tensor memory.  Loads of both
 // complete on the leader's `full` barrier, commits arrive in both CTAs.
-constexpr int BN = 256;
-constexpr int PAIR_STAGES = 5;
-constexpr int PAIR_TILE = 128 * BK;  // a CTA's half of X's, and of W's, k-block
 constexpr int PAIR_EPI_WARPS = 8;    // two to a quarter of TMEM's lanes, each with half of the tile's columns
-constexpr int PAIR_COLS = BN / 2;    // accumulator columns of an epilogue warp
 constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
 constexpr int PAIR_BOX = 32 * 64;    // epilogue staging: 32 rows x 32 bf16 columns
 constexpr int PAIR_BOXES = 3;        // of a warp: one is stored, one worked on, one being filled with residual
-constexpr int PAIR_EPI_BYTES = PAIR_EPI_WARPS * (PAIR_BOXES * PAIR_BOX + 2 * PAIR_COLS * 4);  // boxes; scales and bias
-constexpr int PAIR_SMEM = PAIR_STAGES * 2 * PAIR_TILE + PAIR_EPI_BYTES + 1024 + 512;
-constexpr int PAIR_TMEM = 2 * BN;
+template <int BN>
+struct PairCfg {
+  static constexpr int STAGES = BN == 256 ? 5 : 7;
+  static constexpr int X_BYTES = 128 * BK;      // a CTA's half of X's k-block
+  static constexpr int W_BYTES = BN / 2 * BK;   // and of W's
+  static constexpr int COLS = BN / 2;           // accumulator columns of an epilogue warp
+  static constexpr int EPI_BYTES = PAIR_EPI_WARPS * (PAIR_BOXES * PAIR_BOX + 2 * COLS * 4);  // boxes; scales and bias
+  static constexpr int SMEM = STAGES * (X_BYTES + W_BYTES) + EPI_BYTES + 1024 + 512;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
 
 // Groups of `group_m` row tiles, rows fastest inside a group: the tiles in flight
 // share few rows of X and of W, both from L2.
@@ -325,14 +340,16 @@ __device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, int group
   nb = r / gm;
 }
 
-template <bool SWIGLU>
+template <int BN, bool SWIGLU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     q8_pair_kernel(const __grid_constant__ Maps tm, const __grid_constant__ LLQ8Gemm p, int group_m, int* err) {
+  using Cfg = PairCfg<BN>;
+  constexpr int PAIR_STAGES = Cfg::STAGES, PAIR_COLS = Cfg::COLS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
-  uint8_t* sW = smem + PAIR_STAGES * PAIR_TILE;
-  uint8_t* sBox = sW + PAIR_STAGES * PAIR_TILE;                                              // [warps][boxes]
+  uint8_t* sW = smem + PAIR_STAGES * Cfg::X_BYTES;
+  uint8_t* sBox = sW + PAIR_STAGES * Cfg::W_BYTES;                                              // [warps][boxes]
   float* sCol = reinterpret_cast<float*>(sBox + PAIR_EPI_WARPS * PAIR_BOXES * PAIR_BOX);  // [warps][scales, bias]
   uint64_t* full = reinterpret_cast<uint64_t*>(sCol + PAIR_EPI_WARPS * 2 * PAIR_COLS);
   uint64_t* empty = full + PAIR_STAGES;
@@ -364,7 +381,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"((uint32_t)PAIR_TMEM)
+                 "r"((uint32_t)Cfg::TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -390,9 +407,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             break;
           }
           const uint32_t leader_full = mapa(smem_u32(&full[stage]), 0);
-          if (crank == 0) mbar_arrive_expect_tx(&full[stage], 4 * PAIR_TILE);
-          load_pair(sX + stage * PAIR_TILE, &tm.x, leader_full, kb * BK, mb * 256 + (int)crank * 128);
-          load_pair(sW + stage * PAIR_TILE, &tm.w, leader_full, kb * BK, nb * BN + (int)crank * 128);
+          if (crank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (Cfg::X_BYTES + Cfg::W_BYTES));
+          load_pair(sX + stage * Cfg::X_BYTES, &tm.x, leader_full, kb * BK, mb * 256 + (int)crank * 128);
+          load_pair(sW + stage * Cfg::W_BYTES, &tm.w, leader_full, kb * BK, nb * BN + (int)crank * (BN / 2));
           if (++stage == PAIR_STAGES) {
             stage = 0;
             phase ^= 1;
@@ -417,8 +434,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             break;
           }
           tc_fence_after();
-          const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sX + stage * PAIR_TILE));
-          const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sW + stage * PAIR_TILE));
+          const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sX + stage * Cfg::X_BYTES));
+          const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sW + stage * Cfg::W_BYTES));
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k) mma_pair(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
           commit_pair(&empty[stage]);
@@ -457,9 +474,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
       const int colw = nb * BN + half * PAIR_COLS;  // this warp's first accumulator column
       // what does not depend on the product, while it runs
       const float xs = row < p.M ? p.xs[row] : 1.f;
-      const int cl = colw + 4 * lane;  // N % 8 == 0: four columns are all there or none is
-      const float4 ws4 = cl < p.N ? *reinterpret_cast<const float4*>(p.ws + cl) : make_float4(0, 0, 0, 0);
-      const uint2 bias4 = p.bias != nullptr && cl < p.N ? *reinterpret_cast<const uint2*>(p.bias + cl) : make_uint2(0, 0);
+      // four columns a lane, of the first COLS / 4 lanes; N % 8 == 0: all four are there or none is
+      const int cl = colw + 4 * lane;
+      const bool mine = 4 * lane < PAIR_COLS;
+      const float4 ws4 = mine && cl < p.N ? *reinterpret_cast<const float4*>(p.ws + cl) : make_float4(0, 0, 0, 0);
+      const uint2 bias4 = p.bias != nullptr && mine && cl < p.N ? *reinterpret_cast<const uint2*>(p.bias + cl)
+                                                                 : make_uint2(0, 0);
       // fills box `at` with the residual of accumulator columns [c, c + STEP),
       // once the store that last read the box is done with it
       auto fetch_residual = [&](int at, int c) {
@@ -470,9 +490,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
       };
       fetch_residual(b, 0);
       __syncwarp();  // the tile before is read
-      *reinterpret_cast<float4*>(scol + 4 * lane) = ws4;
-      {
+      if (mine) {
         const float2 b0 = unpack_bf16x2(bias4.x), b1 = unpack_bf16x2(bias4.y);
+        *reinterpret_cast<float4*>(scol + 4 * lane) = ws4;
         *reinterpret_cast<float4*>(sbias + 4 * lane) = make_float4(b0.x, b0.y, b1.x, b1.y);
       }
       __syncwarp();
@@ -489,73 +509,75 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                            fmaf(__uint_as_float(r[i + 2]) * xs, s.z, b.z), fmaf(__uint_as_float(r[i + 3]) * xs, s.w, b.w));
       };
 #pragma unroll 1
-      for (int c = 0; c < PAIR_COLS; c += STEP) {
-        if (colw + c >= p.N || row0 >= p.M) break;  // the whole box is outside C
-        const int out0 = SWIGLU ? (colw + c) / 2 : colw + c;
-        float v[32];
-        if constexpr (SWIGLU) {
+      for (int c = 0; c < PAIR_COLS; c += 64) {
+        if (colw + c >= p.N || row0 >= p.M) break;  // outside C
+        uint32_t r[2][32];
+        tmem_ld_32x32b_x32(tbase + c, r[0]);
+        tmem_ld_32x32b_x32(tbase + c + 32, r[1]);
+        tmem_ld_wait();
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(tbase + c + 32 * h, r);
-            tmem_ld_wait();
+        for (int h = 0; h < 64 / STEP; ++h) {
+          const int cb = c + h * STEP;  // of this box
+          if (colw + cb >= p.N) break;
+          const int out0 = SWIGLU ? (colw + cb) / 2 : colw + cb;
+          float v[32];
+          if constexpr (SWIGLU) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const float4 g = scaled(r, c + 32 * h, i), u = scaled(r, c + 32 * h, i + 16);
-              v[16 * h + i] = silu_fast(g.x) * u.x;
-              v[16 * h + i + 1] = silu_fast(g.y) * u.y;
-              v[16 * h + i + 2] = silu_fast(g.z) * u.z;
-              v[16 * h + i + 3] = silu_fast(g.w) * u.w;
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) {
+                const float4 g = scaled(r[j], c + 32 * j, i), u = scaled(r[j], c + 32 * j, i + 16);
+                v[16 * j + i] = silu(g.x) * u.x;
+                v[16 * j + i + 1] = silu(g.y) * u.y;
+                v[16 * j + i + 2] = silu(g.z) * u.z;
+                v[16 * j + i + 3] = silu(g.w) * u.w;
+              }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 y = scaled(r[h], cb, i);
+              v[i] = y.x;
+              v[i + 1] = y.y;
+              v[i + 2] = y.z;
+              v[i + 3] = y.w;
             }
           }
-        } else {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(tbase + c, r);
-          tmem_ld_wait();
+          // 16-byte chunk k of row r is chunk k ^ ((r >> 1) & 3) of a box, the 64-byte
+          // swizzle of the maps; rows past M and columns past N are clipped there
+          uint4* d = reinterpret_cast<uint4*>(boxes + b * PAIR_BOX + lane * 64);
+          const int swz = (lane >> 1) & 3;
+          if (p.residual != nullptr) {
+            fetch_residual(b == PAIR_BOXES - 1 ? 0 : b + 1, cb + STEP);
+            if (!mbar_wait(&rbar[b], bphase, err, kErrTmaFullTimeout)) linger();
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 y = scaled(r, c, i);
-            v[i] = y.x;
-            v[i + 1] = y.y;
-            v[i + 2] = y.z;
-            v[i + 3] = y.w;
-          }
-        }
-        // 16-byte chunk k of row r is chunk k ^ ((r >> 1) & 3) of a box, the 64-byte
-        // swizzle of the maps; rows past M and columns past N are clipped there
-        uint4* d = reinterpret_cast<uint4*>(boxes + b * PAIR_BOX + lane * 64);
-        const int swz = (lane >> 1) & 3;
-        if (p.residual != nullptr) {
-          fetch_residual(b == PAIR_BOXES - 1 ? 0 : b + 1, c + STEP);
-          if (!mbar_wait(&rbar[b], bphase, err, kErrTmaFullTimeout)) linger();
+            for (int k = 0; k < 4; ++k) {
+              const uint4 rv = d[k ^ swz];
+              const uint32_t ru[4] = {rv.x, rv.y, rv.z, rv.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint4 rv = d[k ^ swz];
-            const uint32_t ru[4] = {rv.x, rv.y, rv.z, rv.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack_bf16x2(ru[j]);
-              v[8 * k + 2 * j] += f.x;
-              v[8 * k + 2 * j + 1] += f.y;
+              for (int j = 0; j < 4; ++j) {
+                const float2 f = unpack_bf16x2(ru[j]);
+                v[8 * k + 2 * j] += f.x;
+                v[8 * k + 2 * j + 1] += f.y;
+              }
             }
+          } else {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PAIR_BOXES - 1) : "memory");
+            __syncwarp();
           }
-        } else {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PAIR_BOXES - 1) : "memory");
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            d[k ^ swz] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                                    pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+          fence_proxy_async();
           __syncwarp();
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          d[k ^ swz] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                                  pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {
-          store_box(&tm.c, boxes + b * PAIR_BOX, out0, row0);
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
-        if (++b == PAIR_BOXES) {
-          b = 0;
-          bphase ^= 1;
+          if (lane == 0) {
+            store_box(&tm.c, boxes + b * PAIR_BOX, out0, row0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          if (++b == PAIR_BOXES) {
+            b = 0;
+            bphase ^= 1;
+          }
         }
       }
       tc_fence_before();
@@ -573,7 +595,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   cluster_barrier();
   tc_fence_after();
   if (warp == 1) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)PAIR_TMEM)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::TMEM_COLS)
                  : "memory");
   }
 }
@@ -664,18 +686,15 @@ static int split_launch(const LLQ8Gemm& p, int cs, int* err, cudaStream_t stream
   }
 }
 
-template <bool SWIGLU>
-static int pair_launch(const LLQ8Gemm& p, int* err, cudaStream_t stream) {
+template <int BN, bool SWIGLU>
+static int pair_launch(const LLQ8Gemm& p, int sms, int* err, cudaStream_t stream) {
+  using Cfg = PairCfg<BN>;
   Maps tm;
-  if (!operand_map(&tm.x, p.x, p.M, p.K, p.ldx, 128) || !operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) ||
+  if (!operand_map(&tm.x, p.x, p.M, p.K, p.ldx, 128) || !operand_map(&tm.w, p.w, p.N, p.K, p.ldw, BN / 2) ||
       !output_map(&tm.c, p.C, p.M, SWIGLU ? p.N / 2 : p.N, p.ldc))
     return -2;
   tm.r = tm.c;  // read with a residual only
   if (p.residual != nullptr && !output_map(&tm.r, p.residual, p.M, SWIGLU ? p.N / 2 : p.N, p.ldr)) return -2;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return -5;
   const int num_m = (p.M + 255) / 256;
   const int64_t tiles = (int64_t)num_m * ((p.N + BN - 1) / BN);
   if (tiles > (1ll << 30)) return -3;
@@ -685,24 +704,33 @@ static int pair_launch(const LLQ8Gemm& p, int* err, cudaStream_t stream) {
   group = group < 8 ? 8 : group;
   group = group > num_m ? num_m : group;
   static unsigned long long done = 0;
-  auto kern = q8_pair_kernel<SWIGLU>;
-  if (!smem_on_device(kern, PAIR_SMEM, done)) return -7;
-  const cudaError_t e = launch_pdl(kern, dim3(2 * pairs), dim3(PAIR_THREADS), PAIR_SMEM, stream, tm, p, (int)group, err);
+  auto kern = q8_pair_kernel<BN, SWIGLU>;
+  if (!smem_on_device(kern, Cfg::SMEM, done)) return -7;
+  const cudaError_t e = launch_pdl(kern, dim3(2 * pairs), dim3(PAIR_THREADS), Cfg::SMEM, stream, tm, p, (int)group, err);
   return e == cudaSuccess ? 0 : -5;
 }
 
 }  // namespace q8
 }  // namespace ll
 
-// `cluster`: 0 takes the kernel by the rule below, -1 the pair kernel, 1 to 8
-// the split kernel with that many CTAs to a feature tile.
-extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int cluster, int* err, cudaStream_t stream) {
+// `kernel`: 0 by the rule below; 1 to 8 the split kernel with that many CTAs to a
+// feature tile; 128 or 256 the pair kernel with tiles of so many features.
+extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, cudaStream_t stream) {
   using namespace ll::q8;
   if (p->M <= 0) return 0;
   if (p->N <= 0 || p->K <= 0 || (p->K % 16) || (p->N % 8) || (swiglu && (p->N % 32))) return -3;
-  if ((p->ldx % 16) || (p->ldw % 16) || (p->ldc % 8) || (p->ldr % 8) || cluster > SPLIT_MAX_CLUSTER) return -3;
-  const int64_t tiles = (int64_t)((p->N + 127) / 128) * ((p->M + 127) / 128);
-  const bool split = cluster > 0 || (cluster == 0 && (p->M <= 128 || tiles <= 200));
-  if (split) return swiglu ? split_launch<true>(*p, cluster, err, stream) : split_launch<false>(*p, cluster, err, stream);
-  return swiglu ? pair_launch<true>(*p, err, stream) : pair_launch<false>(*p, err, stream);
+  if ((p->ldx % 16) || (p->ldw % 16) || (p->ldc % 8) || (p->ldr % 8)) return -3;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return -5;
+  if (kernel == 0) {
+    const int64_t tiles = (int64_t)((p->N + 127) / 128) * ((p->M + 127) / 128);
+    if (p->M > 128 && tiles > 200) kernel = 256;
+  }
+  if (kernel >= 0 && kernel <= SPLIT_MAX_CLUSTER)
+    return swiglu ? split_launch<true>(*p, kernel, err, stream) : split_launch<false>(*p, kernel, err, stream);
+  if (kernel == 128) return swiglu ? pair_launch<128, true>(*p, sms, err, stream) : pair_launch<128, false>(*p, sms, err, stream);
+  if (kernel == 256) return swiglu ? pair_launch<256, true>(*p, sms, err, stream) : pair_launch<256, false>(*p, sms, err, stream);
+  return -3;
 }
