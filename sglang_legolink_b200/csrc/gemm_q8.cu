@@ -51,6 +51,56 @@ __device__ __forceinline__ void arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// One thread of a converged warp.  The main loops are one thread's, and what counts
+// beside a k-block's products (512 cycles for 256 x 256) are that thread's own
+// instructions.  The copies and MMAs take their operands from uniform registers:
+// behind `elect.sync`, in a warp whose number and accumulator address come from a
+// shuffle, the compiler keeps them there; behind `lane == 0` it moved each operand
+// over for every instruction, 80 cycles an MMA at least (39 now) and 510 to 545
+// cycles a k-block of any size.  For the same reason the loops are unrolled over
+// the stages, with shared addresses known up to a constant, and a wait's slow path
+// is out of line.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(p));
+  return p != 0;
+}
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* err, int code) {
+  return mbar_wait(reinterpret_cast<uint64_t*>(__cvta_shared_to_generic(bar)), parity, err, code);
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int* err, int code) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0 || wait_long(bar, parity, err, code);
+}
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void load(uint32_t dst, const void* tmap, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          dst),
+      "l"(tmap), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // Instruction descriptor of kind::f8f6f4: fp32 accumulator, both operands e4m3
 // (format 0) and K-major.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
@@ -76,10 +126,10 @@ __device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a, uint64_t b
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 // Arrives on the barrier at this offset in both CTAs of the pair.
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
+          bar),
       "h"((uint16_t)0x3)
       : "memory");
 }
@@ -87,10 +137,10 @@ __device__ __forceinline__ void commit_pair_local(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
-__device__ __forceinline__ void load_pair(void* dst, const void* tmap, uint32_t leader_bar, int x, int y) {
+__device__ __forceinline__ void load_pair(uint32_t dst, const void* tmap, uint32_t leader_bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
-      "%4}], [%2];" ::"r"(smem_u32(dst)),
+      "%4}], [%2];" ::"r"(dst),
       "l"(tmap), "r"(leader_bar), "r"(x), "r"(y)
       : "memory");
 }
@@ -153,7 +203,7 @@ __global__ void __launch_bounds__(192, 2)
   __shared__ uint32_t tmem_slot;
   __shared__ float sxs[BNX];
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int cs = gridDim.x, crank = blockIdx.x, nb = blockIdx.y;
   const int num_kb = (p.K + BK - 1) / BK, per = (num_kb + cs - 1) / cs;
   const int kb0 = min(num_kb, crank * per), kb1 = min(num_kb, kb0 + per);
@@ -172,47 +222,54 @@ __global__ void __launch_bounds__(192, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
+  const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), w0 = smem_u32(sW), x0 = smem_u32(sX);
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
+    if (elect_one()) {
       // every input may be an output of the kernel ahead
       for (int kb = kb0; kb < min(kb1, kb0 + STAGES); ++kb) prefetch_box(&tm.w, kb * BK, nb * 128);
       pdl_wait();
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
-          ok = false;
-          break;
-        }
-        mbar_arrive_expect_tx(&full[stage], Cfg::W_BYTES + Cfg::X_BYTES);
-        tma_load_2d(sW + stage * Cfg::W_BYTES, &tm.w, &full[stage], kb * BK, nb * 128);
-        tma_load_2d(sX + stage * Cfg::X_BYTES, &tm.x, &full[stage], kb * BK, m0);
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
+      bool ok = true;
+      uint32_t phase = 1;
+      for (int kb = kb0; kb < kb1 && ok; phase ^= 1) {
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) {
+          if (kb >= kb1) break;
+          if (!wait(empty0 + 8 * s, phase, err, kErrSmemEmptyTimeout)) {
+            ok = false;
+            break;
+          }
+          expect(full0 + 8 * s, Cfg::W_BYTES + Cfg::X_BYTES);
+          load(w0 + s * Cfg::W_BYTES, &tm.w, full0 + 8 * s, kb * BK, nb * 128);
+          load(x0 + s * Cfg::X_BYTES, &tm.x, full0 + 8 * s, kb * BK, m0);
+          ++kb;
         }
       }
       if (!ok) linger();
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = idesc_e4m3(128, BNX);
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) break;
-        tc_fence_after();
-        const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sW + stage * Cfg::W_BYTES));
-        const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sX + stage * Cfg::X_BYTES));
+      const uint64_t wd = umma_desc_sw128_kmajor(w0), xd = umma_desc_sw128_kmajor(x0);
+      bool ok = true;
+      uint32_t phase = 0, accumulate = 0;
+      for (int kb = kb0; kb < kb1 && ok; phase ^= 1) {
 #pragma unroll
-        for (int k = 0; k < BK / 32; ++k) mma(tmem, ad + 2 * k, bd + 2 * k, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
-        umma_commit(&empty[stage]);
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
+        for (int s = 0; s < STAGES; ++s) {
+          if (kb >= kb1) break;
+          if (!wait(full0 + 8 * s, phase, err, kErrTmaFullTimeout)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            mma(tmem, wd + (s * Cfg::W_BYTES >> 4) + 2 * k, xd + (s * Cfg::X_BYTES >> 4) + 2 * k, idesc,
+                k == 0 ? accumulate : 1u);
+          commit(empty0 + 8 * s);
+          accumulate = 1;
+          ++kb;
         }
       }
       umma_commit(&tfull);
@@ -359,7 +416,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   uint64_t* rfull = drain + 1;  // [warps][boxes]: residual has landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + PAIR_EPI_WARPS * PAIR_BOXES);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t crank = cluster_rank();
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int num_m = (p.M + 255) / 256, num_n = (p.N + BN - 1) / BN;
@@ -388,67 +445,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   tc_fence_before();
   cluster_barrier();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_wait();
 
+  const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), w0 = smem_u32(sW), x0 = smem_u32(sX);
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       prefetch_tmap(&tm.x);
       prefetch_tmap(&tm.w);
-      int stage = 0;
-      uint32_t phase = 0;
+      const uint32_t leader_full0 = mapa(full0, 0);
+      int t = pair, k = 0, mb = 0, nb = 0;
+      pair_tile(t, num_m, num_n, group_m, mb, nb);
+      int xrow = mb * 256 + (int)crank * 128, wrow = nb * BN + (int)crank * (BN / 2);
       bool ok = true;
-      for (int t = pair; t < ntiles && ok; t += npairs) {
-        int mb, nb;
-        pair_tile(t, num_m, num_n, group_m, mb, nb);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrSmemEmptyTimeout)) {
+      for (uint32_t phase = 1; t < ntiles && ok; phase ^= 1) {
+#pragma unroll
+        for (int s = 0; s < PAIR_STAGES; ++s) {
+          if (t >= ntiles) break;
+          if (!wait(empty0 + 8 * s, phase, err, kErrSmemEmptyTimeout)) {
             ok = false;
             break;
           }
-          const uint32_t leader_full = mapa(smem_u32(&full[stage]), 0);
-          if (crank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (Cfg::X_BYTES + Cfg::W_BYTES));
-          load_pair(sX + stage * Cfg::X_BYTES, &tm.x, leader_full, kb * BK, mb * 256 + (int)crank * 128);
-          load_pair(sW + stage * Cfg::W_BYTES, &tm.w, leader_full, kb * BK, nb * BN + (int)crank * (BN / 2));
-          if (++stage == PAIR_STAGES) {
-            stage = 0;
-            phase ^= 1;
+          if (crank == 0) expect(full0 + 8 * s, 2 * (Cfg::X_BYTES + Cfg::W_BYTES));
+          load_pair(x0 + s * Cfg::X_BYTES, &tm.x, leader_full0 + 8 * s, k, xrow);
+          load_pair(w0 + s * Cfg::W_BYTES, &tm.w, leader_full0 + 8 * s, k, wrow);
+          k += BK;
+          if (k >= p.K) {
+            k = 0;
+            t += npairs;
+            pair_tile(t, num_m, num_n, group_m, mb, nb);
+            xrow = mb * 256 + (int)crank * 128;
+            wrow = nb * BN + (int)crank * (BN / 2);
           }
         }
       }
       if (!ok) linger();
     }
   } else if (warp == 1) {
-    if (lane == 0 && crank == 0) {
+    if (crank == 0 && elect_one()) {
       constexpr uint32_t idesc = idesc_e4m3(256, BN);
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, aphase = 0;
+      const uint64_t xd = umma_desc_sw128_kmajor(x0), wd = umma_desc_sw128_kmajor(w0);
+      int t = pair, kb = 0, acc = 0;
+      uint32_t aphase = 1;
       bool ok = true;
-      for (int t = pair; t < ntiles && ok; t += npairs) {
-        if (!mbar_wait(&tempty[acc], aphase ^ 1, err, kErrTmemEmptyTimeout)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&full[stage], phase, err, kErrTmaFullTimeout)) {
+      for (uint32_t phase = 0; t < ntiles && ok; phase ^= 1) {
+#pragma unroll
+        for (int s = 0; s < PAIR_STAGES; ++s) {
+          if (t >= ntiles) break;
+          if (kb == 0) {
+            if (!wait(smem_u32(&tempty[acc]), aphase, err, kErrTmemEmptyTimeout)) {
+              ok = false;
+              break;
+            }
+          }
+          if (!wait(full0 + 8 * s, phase, err, kErrTmaFullTimeout)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t ad = umma_desc_sw128_kmajor(smem_u32(sX + stage * Cfg::X_BYTES));
-          const uint64_t bd = umma_desc_sw128_kmajor(smem_u32(sW + stage * Cfg::W_BYTES));
+          const uint32_t d_tmem = tmem_base + acc * BN;
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k) mma_pair(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
-          commit_pair(&empty[stage]);
-          if (++stage == PAIR_STAGES) {
-            stage = 0;
-            phase ^= 1;
+          for (int k = 0; k < BK / 32; ++k)
+            mma_pair(d_tmem, xd + (s * Cfg::X_BYTES >> 4) + 2 * k, wd + (s * Cfg::W_BYTES >> 4) + 2 * k, idesc,
+                     k == 0 ? (uint32_t)kb : 1u);
+          commit_pair(empty0 + 8 * s);
+          if (++kb == num_kb) {
+            commit_pair(smem_u32(&tfull[acc]));
+            kb = 0;
+            t += npairs;
+            if (++acc == 2) {
+              acc = 0;
+              aphase ^= 1;
+            }
           }
-        }
-        if (!ok) break;
-        commit_pair(&tfull[acc]);
-        if (++acc == 2) {
-          acc = 0;
-          aphase ^= 1;
         }
       }
       // every MMA issued is done before its accumulator is given back
