@@ -31,16 +31,14 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -176,17 +174,22 @@ struct alignas(64) Maps {
 // Few rows: D[128 features, BNX rows] = W_tile . X_tile^T over a CTA's share of
 // the k-blocks.  Bound by reading W: every CTA's first ring of weights is on its
 // way to L2 before the wait for the kernel ahead.  grid (cluster, feature tiles, row tiles).
-constexpr int SPLIT_RING = 108 * 1024;  // two CTAs a SM
+//
+// CTA o of a cluster sums and stores rows [o R, (o + 1) R): the others write their
+// partials of those rows into its shared memory as they read them from tensor
+// memory, behind one cluster barrier (XX).  That memory is beside the ring, since
+// the others may be done first; a lone CTA takes the ring.
 constexpr int SPLIT_MAX_CLUSTER = 8;
 template <int BNX>
 struct SplitCfg {
   static constexpr int W_BYTES = 128 * BK;
   static constexpr int X_BYTES = BNX * BK;
-  static constexpr int STAGES = SPLIT_RING / (W_BYTES + X_BYTES);
+  static constexpr int RECV_BYTES = BNX <= 64 ? (BNX + SPLIT_MAX_CLUSTER - 1) * 512 : 0;  // BNX 128: lone CTAs only
+  static constexpr int STAGES = (108 * 1024 - RECV_BYTES) / (W_BYTES + X_BYTES);          // two CTAs a SM
   static constexpr int TMEM_COLS = BNX < 32 ? 32 : BNX;
-  static constexpr int LD = 132;  // floats per row of the partials
-  static constexpr int SMEM = STAGES * (W_BYTES + X_BYTES) + 1024;
-  static_assert(BNX * LD * 4 <= STAGES * (W_BYTES + X_BYTES), "the partials overlay the ring");
+  static constexpr int LD = 132;  // floats per row of a lone CTA's sums
+  static constexpr int SMEM = STAGES * (W_BYTES + X_BYTES) + RECV_BYTES + 1024;
+  static_assert(BNX * LD * 4 <= STAGES * (W_BYTES + X_BYTES), "the sums overlay the ring");
 };
 
 template <int BNX, bool SWIGLU>
@@ -198,7 +201,8 @@ __global__ void __launch_bounds__(192, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sX = smem + STAGES * Cfg::W_BYTES;
-  float* part = reinterpret_cast<float*>(smem);  // [rows][LD], over the ring, once the product is done
+  float* part = reinterpret_cast<float*>(smem);  // a lone CTA: [rows][LD], over the ring, once the product is done
+  const float* recv = reinterpret_cast<const float*>(smem + STAGES * (Cfg::W_BYTES + Cfg::X_BYTES));  // [cs][R][128]
   __shared__ uint64_t full[STAGES], empty[STAGES], tfull;
   __shared__ uint32_t tmem_slot;
   __shared__ float sxs[BNX];
@@ -223,6 +227,7 @@ __global__ void __launch_bounds__(192, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  if (cs > 1) cluster_arrive();  // this CTA runs: the others may write into its shared memory
 
   const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), w0 = smem_u32(sW), x0 = smem_u32(sX);
   if (warp == 0) {
@@ -285,7 +290,8 @@ __global__ void __launch_bounds__(192, 2)
   const int g = tid % GROUPS, f = SWIGLU ? (g >> 2) * 32 + (g & 3) * 4 : 4 * g;
   const int col = SWIGLU ? nb * 64 + 4 * g : nb * 128 + f;
   const bool live = nb * 128 + f < p.N;
-  const int row0 = crank * PER + tid / GROUPS, row_step = cs * PER;
+  const int R = (rows + cs - 1) / cs, first = min(rows, crank * R), end = min(rows, first + R);  // this CTA's rows
+  const int row0 = first + tid / GROUPS;
   float4 ws[2] = {}, bias[2] = {};
 #pragma unroll
   for (int h = 0; h < (SWIGLU ? 2 : 1); ++h) {
@@ -298,7 +304,7 @@ __global__ void __launch_bounds__(192, 2)
     }
   }
   auto residual_at = [&](int row) {
-    return p.residual != nullptr && live && row < rows
+    return p.residual != nullptr && live && row < end
                ? *reinterpret_cast<const uint2*>(p.residual + (m0 + row) * p.ldr + col)
                : make_uint2(0, 0);
   };
@@ -306,16 +312,35 @@ __global__ void __launch_bounds__(192, 2)
   if (tid < rows) sxs[tid] = p.xs[m0 + tid];
   const bool ok = __syncthreads_and(mbar_wait(&tfull, 0, err, kErrTmemFullTimeout));
   tc_fence_after();
+  if (cs > 1) cluster_wait();
   if (warp >= 2) {  // TMEM lane quarter of this warp: features; columns: rows
     const int feat = (warp & 3) * 32 + lane;
+    const bool none = kb1 <= kb0;
+    int owner = 0, left = R;  // rows that are still the owner's
+    uint32_t to = mapa(smem_u32(recv), 0) + 4u * (crank * R * 128 + feat);
 #pragma unroll 1
     for (int c = 0; c < BNX && c < rows; c += 32) {
       uint32_t r[32];
       tmem_ld_32x32b_x32(tmem + (uint32_t((warp & 3) * 32) << 16) + c, r);  // BNX 16: columns 16.. unused
       tmem_ld_wait();
+      constexpr int COLS = BNX < 32 ? BNX : 32;
+      if (cs > 1) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c + i < rows && c + i < BNX) part[(c + i) * Cfg::LD + feat] = kb1 > kb0 ? __uint_as_float(r[i]) : 0.f;
+        for (int i = 0; i < COLS; ++i) {
+          if (c + i >= rows) break;
+          st_cluster(to, none ? 0.f : __uint_as_float(r[i]));
+          to += 512;
+          if (--left == 0) {
+            ++owner;
+            left = R;
+            to = mapa(smem_u32(recv), min(owner, cs - 1)) + 4u * (crank * R * 128 + feat);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < COLS; ++i)
+          if (c + i < rows) part[(c + i) * Cfg::LD + feat] = none ? 0.f : __uint_as_float(r[i]);
+      }
     }
   }
   tc_fence_before();
@@ -323,32 +348,31 @@ __global__ void __launch_bounds__(192, 2)
   else __syncthreads();
   tc_fence_after();
   if (ok && live) {
-    const uint32_t base = smem_u32(part);
-    // the partials of four features in split order, scales, bias
+    // four features of a row: the partials in split order, scales, bias
     auto sum4 = [&](int row, float xs, int h) {
-      const int at = row * Cfg::LD + f + 16 * h;
-      float4 v = *reinterpret_cast<const float4*>(part + at);
+      float4 v;
       if (cs > 1) {
-        float4 t[SPLIT_MAX_CLUSTER];
-#pragma unroll
-        for (int r = 0; r < SPLIT_MAX_CLUSTER; ++r)
-          t[r] = r < cs ? ld_cluster(mapa(base + 4 * at, r)) : make_float4(0, 0, 0, 0);
-        v = t[0];
+        const float* at = recv + (row - first) * 128 + f + 16 * h;
+        v = *reinterpret_cast<const float4*>(at);
 #pragma unroll
         for (int r = 1; r < SPLIT_MAX_CLUSTER; ++r) {
-          v.x += t[r].x;
-          v.y += t[r].y;
-          v.z += t[r].z;
-          v.w += t[r].w;
+          if (r >= cs) break;
+          const float4 t = *reinterpret_cast<const float4*>(at + r * R * 128);
+          v.x += t.x;
+          v.y += t.y;
+          v.z += t.z;
+          v.w += t.w;
         }
+      } else {
+        v = *reinterpret_cast<const float4*>(part + row * Cfg::LD + f + 16 * h);
       }
       return make_float4(fmaf(v.x * xs, ws[h].x, bias[h].x), fmaf(v.y * xs, ws[h].y, bias[h].y),
                          fmaf(v.z * xs, ws[h].z, bias[h].z), fmaf(v.w * xs, ws[h].w, bias[h].w));
     };
 #pragma unroll 2
-    for (int row = row0; row < rows; row += row_step) {
+    for (int row = row0; row < end; row += PER) {
       const uint2 rv = next;
-      next = residual_at(row + row_step);
+      next = residual_at(row + PER);
       const float xs = sxs[row];
       float4 v = sum4(row, xs, 0);
       if constexpr (SWIGLU) {
@@ -360,9 +384,7 @@ __global__ void __launch_bounds__(192, 2)
           make_uint2(pack_bf16x2(v.x + r0.x, v.y + r0.y), pack_bf16x2(v.z + r1.x, v.w + r1.y));
     }
   }
-  if (cs > 1) cluster_barrier();  // the partials live until every CTA has read them
-  else __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);
+  if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);  // every read of it is behind the barrier
 }
 
 // ---------------------------------------------------------------------------
@@ -370,17 +392,17 @@ __global__ void __launch_bounds__(192, 2)
 // and of its 256 rows of W; the leader issues the MMAs (M = 256, N = 256, K = 32),
 // which accumulate rows [128 r, +128) in CTA r's tensor memory.  Loads of both
 // complete on the leader's `full` barrier, commits arrive in both CTAs.
-constexpr int PAIR_EPI_WARPS = 8;    // two to a quarter of TMEM's lanes, each with half of the tile's columns
-constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
 constexpr int PAIR_BOX = 32 * 64;    // epilogue staging: 32 rows x 32 bf16 columns
 constexpr int PAIR_BOXES = 3;        // of a warp: one is stored, one worked on, one being filled with residual
 template <int BN>
 struct PairCfg {
-  static constexpr int STAGES = BN == 256 ? 5 : 7;
+  static constexpr int STAGES = BN == 256 ? 5 : (BN == 128 ? 7 : 8);
+  static constexpr int EPI_WARPS = BN == 64 ? 4 : 8;  // 8: two to a quarter of TMEM's lanes, each with half of the columns
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int X_BYTES = 128 * BK;      // a CTA's half of X's k-block
   static constexpr int W_BYTES = BN / 2 * BK;   // and of W's
-  static constexpr int COLS = BN / 2;           // accumulator columns of an epilogue warp
-  static constexpr int EPI_BYTES = PAIR_EPI_WARPS * (PAIR_BOXES * PAIR_BOX + 2 * COLS * 4);  // boxes; scales and bias
+  static constexpr int COLS = BN / (EPI_WARPS / 4);  // accumulator columns of an epilogue warp
+  static constexpr int EPI_BYTES = EPI_WARPS * (PAIR_BOXES * PAIR_BOX + 2 * COLS * 4);  // boxes; scales and bias
   static constexpr int SMEM = STAGES * (X_BYTES + W_BYTES) + EPI_BYTES + 1024 + 512;
   static constexpr int TMEM_COLS = 2 * BN;
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -398,10 +420,10 @@ __device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, int group
 }
 
 template <int BN, bool SWIGLU>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS, 1)
     q8_pair_kernel(const __grid_constant__ Maps tm, const __grid_constant__ LLQ8Gemm p, int group_m, int* err) {
   using Cfg = PairCfg<BN>;
-  constexpr int PAIR_STAGES = Cfg::STAGES, PAIR_COLS = Cfg::COLS;
+  constexpr int PAIR_STAGES = Cfg::STAGES, PAIR_COLS = Cfg::COLS, PAIR_EPI_WARPS = Cfg::EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
@@ -473,9 +495,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
           if (k >= p.K) {
             k = 0;
             t += npairs;
-            pair_tile(t, num_m, num_n, group_m, mb, nb);
-            xrow = mb * 256 + (int)crank * 128;
-            wrow = nb * BN + (int)crank * (BN / 2);
+            if (t < ntiles) {
+              pair_tile(t, num_m, num_n, group_m, mb, nb);
+              xrow = mb * 256 + (int)crank * 128;
+              wrow = nb * BN + (int)crank * (BN / 2);
+            }
           }
         }
       }
@@ -741,6 +765,7 @@ template <bool SWIGLU>
 static int split_launch(const LLQ8Gemm& p, int cs, int* err, cudaStream_t stream) {
   const int bnx = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
   if (cs <= 0) cs = split_rule(p.M, p.N, p.K, bnx);
+  if (bnx > 64) cs = 1;
   Maps tm;
   if (!operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) || !operand_map(&tm.x, p.x, p.M, p.K, p.ldx, bnx)) return -2;
   tm.c = tm.r = tm.x;  // not read
@@ -775,7 +800,7 @@ static int pair_launch(const LLQ8Gemm& p, int sms, int* err, cudaStream_t stream
   static unsigned long long done = 0;
   auto kern = q8_pair_kernel<BN, SWIGLU>;
   if (!smem_on_device(kern, Cfg::SMEM, done)) return -7;
-  const cudaError_t e = launch_pdl(kern, dim3(2 * pairs), dim3(PAIR_THREADS), Cfg::SMEM, stream, tm, p, (int)group, err);
+  const cudaError_t e = launch_pdl(kern, dim3(2 * pairs), dim3(Cfg::THREADS), Cfg::SMEM, stream, tm, p, (int)group, err);
   return e == cudaSuccess ? 0 : -5;
 }
 
@@ -783,7 +808,8 @@ static int pair_launch(const LLQ8Gemm& p, int sms, int* err, cudaStream_t stream
 }  // namespace ll
 
 // `kernel`: 0 by the rule below; 1 to 8 the split kernel with that many CTAs to a
-// feature tile; 128 or 256 the pair kernel with tiles of so many features.
+// feature tile (of one where there are more than 64 rows a tile); 64, 128 or 256
+// the pair kernel with tiles of so many features.
 extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, cudaStream_t stream) {
   using namespace ll::q8;
   if (p->M <= 0) return 0;
@@ -799,6 +825,7 @@ extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, c
   }
   if (kernel >= 0 && kernel <= SPLIT_MAX_CLUSTER)
     return swiglu ? split_launch<true>(*p, kernel, err, stream) : split_launch<false>(*p, kernel, err, stream);
+  if (kernel == 64) return swiglu ? pair_launch<64, true>(*p, sms, err, stream) : pair_launch<64, false>(*p, sms, err, stream);
   if (kernel == 128) return swiglu ? pair_launch<128, true>(*p, sms, err, stream) : pair_launch<128, false>(*p, sms, err, stream);
   if (kernel == 256) return swiglu ? pair_launch<256, true>(*p, sms, err, stream) : pair_launch<256, false>(*p, sms, err, stream);
   return -3;
