@@ -30,7 +30,7 @@ int ll_lora_gemv(const bf16* x, int64_t ldx, const bf16* w, bf16* C, int64_t ldc
 int ll_gemm_bf16_lora(const void* A, int lda, const void* W, int ldw, void* C, int ldc, const void* bias, int M,
                       int N, int K, int epilogue, const LLLora* lo, int* err, void* stream);
 int ll_sample(const LLSample* p, cudaStream_t stream);
-int ll_q8_rows(const LLQ8Rows* p, int variant, cudaStream_t stream);
+int ll_q8_rows(const LLQ8Rows* p, cudaStream_t stream);
 int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, cudaStream_t stream);
 int ll_rmsnorm(bf16* out, const bf16* x, bf16* residual, const bf16* w, int rows, int hidden, float eps,
                cudaStream_t stream);
@@ -517,11 +517,10 @@ bool same_place(const at::Tensor& a, const at::Tensor& b) {
 }
 
 // y = x (w null), rmsnorm(x) w, or rmsnorm(x + residual) w with the sum to `sum`.
-// `variant` names a kernel (ll_q8_rows), 0: by the sizes.
 std::tuple<at::Tensor, at::Tensor> q8_rows(const at::Tensor& x, const c10::optional<at::Tensor>& residual,
                                            const c10::optional<at::Tensor>& sum, const c10::optional<at::Tensor>& w,
                                            double eps, const c10::optional<at::Tensor>& q_,
-                                           const c10::optional<at::Tensor>& scale_, int64_t variant) {
+                                           const c10::optional<at::Tensor>& scale_) {
   CHECK_CUDA(x);
   TORCH_CHECK_VALUE(x.dim() == 2, "x must be [rows, K]");
   const int64_t rows = x.size(0), K = x.size(1);
@@ -569,7 +568,7 @@ std::tuple<at::Tensor, at::Tensor> q8_rows(const at::Tensor& x, const c10::optio
   p.rows = (int)rows;
   p.K = (int)K;
   p.eps = (float)eps;
-  check_rc(ll_q8_rows(&p, (int)variant, cur_stream()), "ll_q8_rows");
+  check_rc(ll_q8_rows(&p, cur_stream()), "ll_q8_rows");
   return {q, scale};
 }
 

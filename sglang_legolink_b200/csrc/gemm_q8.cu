@@ -214,14 +214,11 @@ __global__ void __launch_bounds__(192, 2)
   const int m0 = blockIdx.z * BNX, rows = min(BNX, p.M - m0);
   pdl_trigger();
 
-  if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(&tfull, 1);
+  if (tid <= 2 * STAGES) {
+    mbar_init(tid == 2 * STAGES ? &tfull : (tid < STAGES ? &full[tid] : &empty[tid - STAGES]), 1);
     fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 1) tmem_alloc(&tmem_slot, Cfg::TMEM_COLS);
   tc_fence_before();
   __syncthreads();
@@ -445,19 +442,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
   const int ntiles = num_m * num_n, num_kb = (p.K + BK - 1) / BK;
   pdl_trigger();
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < PAIR_STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 2 * PAIR_EPI_WARPS);  // of both CTAs (used on the leader)
-    }
-    mbar_init(drain, 1);
-    for (int i = 0; i < PAIR_EPI_WARPS * PAIR_BOXES; ++i) mbar_init(&rfull[i], 1);
+  // full, empty, tfull, tempty, drain and rfull lie in a row: a barrier a thread
+  static_assert(2 * PAIR_STAGES + 5 + PAIR_EPI_WARPS * PAIR_BOXES <= 64, "two warps initialise the barriers");
+  if (threadIdx.x < 2 * PAIR_STAGES + 5 + PAIR_EPI_WARPS * PAIR_BOXES) {
+    uint64_t* bar = full + threadIdx.x;
+    mbar_init(bar, bar == tempty || bar == tempty + 1 ? 2 * PAIR_EPI_WARPS : 1);  // tempty: warps of both CTAs, on the leader
     fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"((uint32_t)Cfg::TMEM_COLS)
@@ -468,6 +460,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
   cluster_barrier();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  if (warp == 0 && elect_one() && pair < ntiles) {  // the first ring of weights on its way to L2
+    int mb, nb;
+    pair_tile(pair, num_m, num_n, group_m, mb, nb);
+    for (int k = 0; k < min(p.K, PAIR_STAGES * BK); k += BK) prefetch_box(&tm.w, k, nb * BN + (int)crank * (BN / 2));
+  }
+  __syncwarp();
   pdl_wait();
 
   const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), w0 = smem_u32(sW), x0 = smem_u32(sX);
@@ -681,7 +679,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
         aphase ^= 1;
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the boxes are read
   }
 
   tc_fence_before();
@@ -749,23 +747,56 @@ static int launch(Kern kern, dim3 grid, int smem, int cluster, cudaStream_t stre
   return cudaLaunchKernelEx(&cfg, kern, tm, p, err) == cudaSuccess ? 0 : -5;
 }
 
-// CTAs that share a feature tile's K: as many as have places, two a SM; larger
-// clusters than pairs do not fill the SMs to the last place.
-constexpr int SPLIT_PLACES = 248;
-static int split_rule(int M, int N, int K, int bnx) {
-  const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + bnx - 1) / bnx);
+// CTAs that share a feature tile's K, for up to 64 rows: as many as have places,
+// two a SM (larger clusters than pairs do not fill the SMs to the last place), with
+// three k-blocks each or more; two for more tiles than places, whose last round
+// would be a long one.  Over 760 random sizes (1 to 64 rows) 1 % slower than the
+// best of 1 to 8 CTAs in the geometric mean (2 % with two k-blocks each and without
+// the second rule).
+constexpr int SPLIT_PLACES = 248, SPLIT_ROUND = 296;
+static int split_rule(int N, int K) {
+  const int tiles = (N + 127) / 128, num_kb = (K + BK - 1) / BK;
+  int cs = SPLIT_PLACES / tiles;
+  if ((tiles > SPLIT_PLACES / 2 && tiles <= SPLIT_ROUND / 2) || (tiles > SPLIT_ROUND && num_kb >= 64)) cs = 2;
+  cs = cs < num_kb / 3 ? cs : num_kb / 3;
+  return cs < 1 ? 1 : (cs > SPLIT_MAX_CLUSTER ? SPLIT_MAX_CLUSTER : cs);
+}
+
+// The kernel for more than 64 rows: the one with the least modelled time, a start
+// and then, for each round of tiles, the k-blocks and the part of the epilogue that
+// the next tile does not hide.  The figures (us) are fitted to 2033 random sizes (65
+// to 5000 rows) timed with every kernel: what it picks is 0.3 % slower than the
+// best of the four in the geometric mean; tiles of 64, 128 or 256 features
+// alone would be 32, 12 and 23 % slower, the split kernel 57 %.
+static int kernel_rule(int M, int N, int K, int sms) {
+  struct Cost {
+    int kernel, tile_rows, tile_features, places;
+    double start, block, tile;
+  };
+  const Cost costs[] = {{64, 256, 64, sms / 2, 3.6, 0.085, 0.9},
+                        {128, 256, 128, sms / 2, 3.3, 0.14, 1.15},
+                        {256, 256, 256, sms / 2, 3.85, 0.225, 1.15},
+                        {1, 128, 128, 2 * sms, 4.45, 0.34, 1.55}};
   const int num_kb = (K + BK - 1) / BK;
-  int cs = tiles <= 148 && tiles > SPLIT_PLACES / 2 ? 2 : (int)(SPLIT_PLACES / tiles);
-  if (cs > SPLIT_MAX_CLUSTER) cs = SPLIT_MAX_CLUSTER;
-  if (cs > (num_kb + 1) / 2) cs = (num_kb + 1) / 2;
-  return cs < 1 ? 1 : cs;
+  int best = 0;
+  double least = 0;
+  for (const Cost& c : costs) {
+    const int64_t tiles =
+        (int64_t)((M + c.tile_rows - 1) / c.tile_rows) * ((N + c.tile_features - 1) / c.tile_features);
+    const double t = c.start + (double)((tiles + c.places - 1) / c.places) * (num_kb * c.block + c.tile);
+    if (best == 0 || t < least) {
+      best = c.kernel;
+      least = t;
+    }
+  }
+  return best;
 }
 
 template <bool SWIGLU>
 static int split_launch(const LLQ8Gemm& p, int cs, int* err, cudaStream_t stream) {
   const int bnx = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
-  if (cs <= 0) cs = split_rule(p.M, p.N, p.K, bnx);
   if (bnx > 64) cs = 1;
+  else if (cs <= 0) cs = split_rule(p.N, p.K);
   Maps tm;
   if (!operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) || !operand_map(&tm.x, p.x, p.M, p.K, p.ldx, bnx)) return -2;
   tm.c = tm.r = tm.x;  // not read
@@ -819,10 +850,7 @@ extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, c
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return -5;
-  if (kernel == 0) {
-    const int64_t tiles = (int64_t)((p->N + 127) / 128) * ((p->M + 127) / 128);
-    if (p->M > 128 && tiles > 200) kernel = 256;
-  }
+  if (kernel == 0 && p->M > 64) kernel = kernel_rule(p->M, p->N, p->K, sms);
   if (kernel >= 0 && kernel <= SPLIT_MAX_CLUSTER)
     return swiglu ? split_launch<true>(*p, kernel, err, stream) : split_launch<false>(*p, kernel, err, stream);
   if (kernel == 64) return swiglu ? pair_launch<64, true>(*p, sms, err, stream) : pair_launch<64, false>(*p, sms, err, stream);

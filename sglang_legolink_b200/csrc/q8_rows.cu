@@ -37,32 +37,38 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// Sum and largest magnitude (as an integer) over the row's threads: a warp's
-// (WARP), else the CTA's.  The order is fixed, so a row's bits depend on K alone.
+// Sum, and largest magnitude (as an integer, where a NaN is the largest), over the
+// row's threads: a warp's (WARP), else the CTA's.  The order is fixed, so a row's
+// bits depend on K and the number of rows alone, never on other rows.
 template <bool WARP>
-__device__ __forceinline__ void row_reduce(float& sum, uint32_t& top, float* rsum, uint32_t* rtop) {
-  sum = warp_sum(sum);
-  top = __reduce_max_sync(0xffffffffu, top);
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = warp_sum(v);
   if constexpr (!WARP) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) {
-      rsum[warp] = sum;
-      rtop[warp] = top;
-    }
+    if (lane == 0) red[warp] = v;
     __syncthreads();
-    const bool in = lane < (blockDim.x >> 5);
-    sum = warp_sum(in ? rsum[lane] : 0.f);
-    top = __reduce_max_sync(0xffffffffu, in ? rtop[lane] : 0u);
+    v = warp_sum(lane < (blockDim.x >> 5) ? red[lane] : 0.f);
     __syncthreads();  // free again
   }
+  return v;
+}
+template <bool WARP>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, float* red) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if constexpr (!WARP) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) red[warp] = __uint_as_float(v);
+    __syncthreads();
+    v = __reduce_max_sync(0xffffffffu, lane < (blockDim.x >> 5) ? __float_as_uint(red[lane]) : 0u);
+  }
+  return v;
 }
 
 // WARP: a row a warp; else a row a CTA.  VPT vectors of 8 values a thread.
 template <int VPT, int MODE, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : 1024)
     q8_rows_kernel(const __grid_constant__ LLQ8Rows p) {
-  __shared__ float rsum[32];
-  __shared__ uint32_t rtop[32];
+  __shared__ float red[32];
   pdl_trigger();
   pdl_wait();
   const int tid = WARP ? (threadIdx.x & 31) : threadIdx.x, step = WARP ? 32 : blockDim.x;
@@ -113,41 +119,15 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024)
       }
     }
   }
-  float ss = 0.f, big = 0.f, rstd = 1.f;
-  uint32_t top;
-  if constexpr (MODE == kQ8Quantize) {
+  if constexpr (MODE != kQ8Quantize) {
+    float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) big = max_nan(big, fabsf(v[i][c]));
-    top = __float_as_uint(big);
-    row_reduce<WARP>(ss, top, rsum, rtop);
-  } else {
-    // max |y| = rstd max |v w|, so the sum of squares and the largest value come
-    // from one reduction (5087 rows x 3584: 14.2 us with two, XX with one); w is read again behind it, from L1
-    const uint4* wr = reinterpret_cast<const uint4*>(p.w);
-    auto times_w = [&](int i, auto f) {
-      const int j = tid + i * step;
-      const uint4 wv = j < nvec ? wr[j] : make_uint4(0, 0, 0, 0);
-      const uint32_t wu[4] = {wv.x, wv.y, wv.z, wv.w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float2 fw = unpack_bf16x2(wu[c]);
-        f(v[i][2 * c], fw.x);
-        f(v[i][2 * c + 1], fw.y);
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      times_w(i, [&](float& t, float w) {
-        ss = fmaf(t, t, ss);
-        big = max_nan(big, fabsf(t * w));
-      });
-    top = __float_as_uint(big);
-    row_reduce<WARP>(ss, top, rsum, rtop);
-    rstd = rsqrtf(ss / (float)p.K + p.eps);
-    const bool plain = ss < INFINITY && top < 0x7f800000u;
-    if (!plain) {  // squares past fp32's range, or a value that is not finite: 2^-80 as large
+      for (int c = 0; c < 8; ++c) ss = fmaf(v[i][c], v[i][c], ss);
+    ss = row_sum<WARP>(ss, red);
+    float rstd = rsqrtf(ss / (float)p.K + p.eps);
+    if (!(ss < INFINITY)) {  // squares past fp32's range, or a value that is not finite: the same, 2^-80 as large
       ss = 0.f;
 #pragma unroll
       for (int i = 0; i < VPT; ++i)
@@ -156,24 +136,29 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024)
           const float t = v[i][c] * 0x1p-80f;
           ss = fmaf(t, t, ss);
         }
-      top = 0;
-      row_reduce<WARP>(ss, top, rsum, rtop);
+      ss = row_sum<WARP>(ss, red);
       rstd = rsqrtf(ss / (float)p.K) * 0x1p-80f;
     }
-    big = 0.f;
+    const uint4* wr = reinterpret_cast<const uint4*>(p.w);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      times_w(i, [&](float& t, float w) {
-        t = t * rstd * w;
-        big = max_nan(big, fabsf(t));
-      });
-    if (!plain) {
-      top = __float_as_uint(big);
-      row_reduce<WARP>(ss, top, rsum, rtop);
-    } else {
-      top = __float_as_uint(__uint_as_float(top) * rstd);
+    for (int i = 0; i < VPT; ++i) {
+      const int j = tid + i * step;
+      const uint4 wv = j < nvec ? wr[j] : make_uint4(0, 0, 0, 0);
+      const uint32_t wu[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 fw = unpack_bf16x2(wu[c]);
+        v[i][2 * c] = v[i][2 * c] * rstd * fw.x;
+        v[i][2 * c + 1] = v[i][2 * c + 1] * rstd * fw.y;
+      }
     }
   }
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) big = max_nan(big, fabsf(v[i][c]));
+  const uint32_t top = row_max<WARP>(__float_as_uint(big), red);
   const float amax = __uint_as_float(top);
   const float scale = amax < INFINITY ? fmaxf(amax / kE4m3Max, kQ8MinScale) : __uint_as_float(0x7fffffffu);
   const float inv = 1.f / scale;
@@ -200,26 +185,26 @@ static cudaError_t q8_rows_launch(const LLQ8Rows& p, int grid, int threads, cuda
 
 using namespace ll;
 
-extern "C" int ll_q8_rows(const LLQ8Rows* p, int variant, cudaStream_t stream) {
+extern "C" int ll_q8_rows(const LLQ8Rows* p, cudaStream_t stream) {
   if (p->rows <= 0) return 0;
   if (p->K <= 0 || (p->K % 16) || p->K > LL_Q8_MAX_K) return -3;
   const int nvec = p->K / 8;
+  // A warp holds a row of up to 1024 values.  Longer ones are a CTA's: two vectors
+  // a thread while every row has a place at once, four for more rows, so that more
+  // bytes are on their way (us, 1 / 2 / 4 vectors: quantising 300 x 3584 1.8 / 2.2 /
+  // 2.3, 5087 x 3584 13.9 / 9.7 / 10.1; with the norm 2.6 / 2.9 / 4.0 and 19.8 /
+  // 15.0 / 14.2; a warp to a row there 15.1 and 22.0).
+  const int vpt = nvec <= 32 ? 1 : (nvec <= 64 ? 2 : (nvec <= 128 || nvec > 2048 || p->rows > 600 ? 4 : 2));
   cudaError_t e;
-  // SWEEP: variant = 100 * warp + vpt
-  if (variant == 0) variant = nvec <= 32 ? 101 : nvec <= 64 ? 102 : nvec <= 128 ? 104 : nvec <= 512 ? 1 : nvec <= 1024 ? 2 : 4;
-  const int vpt = variant % 100;
-  const int warps = p->rows < 8 ? p->rows : 8, grid = (p->rows + warps - 1) / warps;
-  const int threads = ((nvec + vpt - 1) / vpt + 31) / 32 * 32;
-  switch (variant) {
-    case 101: e = q8_rows_launch<1, true>(*p, grid, 32 * warps, stream); break;
-    case 102: e = q8_rows_launch<2, true>(*p, grid, 32 * warps, stream); break;
-    case 104: e = q8_rows_launch<4, true>(*p, grid, 32 * warps, stream); break;
-    case 108: e = q8_rows_launch<8, true>(*p, grid, 32 * warps, stream); break;
-    case 116: e = q8_rows_launch<16, true>(*p, grid, 32 * warps, stream); break;
-    case 1: e = q8_rows_launch<1, false>(*p, p->rows, threads, stream); break;
-    case 2: e = q8_rows_launch<2, false>(*p, p->rows, threads, stream); break;
-    case 4: e = q8_rows_launch<4, false>(*p, p->rows, threads, stream); break;
-    default: return -3;
+  if (nvec <= 128) {
+    const int warps = p->rows < 8 ? p->rows : 8, grid = (p->rows + warps - 1) / warps;
+    if (vpt == 1) e = q8_rows_launch<1, true>(*p, grid, 32 * warps, stream);
+    else if (vpt == 2) e = q8_rows_launch<2, true>(*p, grid, 32 * warps, stream);
+    else e = q8_rows_launch<4, true>(*p, grid, 32 * warps, stream);
+  } else {
+    const int threads = ((nvec + vpt - 1) / vpt + 31) / 32 * 32;
+    if (vpt == 2) e = q8_rows_launch<2, false>(*p, p->rows, threads, stream);
+    else e = q8_rows_launch<4, false>(*p, p->rows, threads, stream);
   }
   return e == cudaSuccess ? 0 : -5;
 }
