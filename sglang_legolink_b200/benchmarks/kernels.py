@@ -298,6 +298,44 @@ def bench_sample(pk, with_torch):
     return rows
 
 
+def bench_q8(pk, with_torch):
+    """Rows to 8 bits and products of two matrices in 8 bits.  The rows'
+    fraction is of their bytes at HBM rate; a product's of the longer of its
+    bytes at HBM rate and its operations at twice the bf16 GEMM rate."""
+    rows = []
+
+    def bf16(*shape):
+        return torch.randn(*shape, device="cuda", dtype=torch.bfloat16)
+
+    for M, K, kind in [(1, 3584, "norm"), (16, 5120, "add_norm"), (5087, 3584, "norm"), (5087, 3584, "add_norm"),
+                       (300, 512, "quantize"), (2048, 18944, "quantize")]:
+        x, r, to, w = bf16(M, K), bf16(M, K), bf16(M, K), bf16(K)
+        out = ops.empty_q8(M, K, "cuda")
+        fn = {"quantize": lambda: ops.quantize_q8(x, out=out), "norm": lambda: ops.rmsnorm_q8(x, w, 1e-6, out=out),
+              "add_norm": lambda: ops.fused_add_rmsnorm_q8(x, r, w, 1e-6, residual_out=to, out=out)}[kind]
+        ms = time_fn(fn)
+        gbs = M * K * (7 if kind == "add_norm" else 3) / ms / 1e6
+        rows.append({"op": f"{kind}_q8[{M}x{K}]", "ms": round(ms, 4), "gbs": round(gbs, 1),
+                     "frac_of_hbm": round(gbs / pk["hbm_gbs"], 3)})
+    for M, N, K, swiglu, residual in [(1, 4608, 3584, False, False), (16, 37888, 3584, True, False),
+                                      (61, 5120, 8192, False, True), (300, 1024, 512, False, False),
+                                      (5087, 4608, 3584, False, False), (2048, 37888, 3584, True, False),
+                                      (5087, 3584, 18944, False, True)]:
+        x, w = ops.quantize_q8(bf16(M, K)), ops.quantize_q8(bf16(N, K))
+        cols = N // 2 if swiglu else N
+        res, out = bf16(M, cols) if residual else None, bf16(M, cols)
+        ms = time_fn(lambda: ops.linear_q8(x, w, residual=res, out=out, swiglu_epilogue=swiglu))
+        byts = M * K + N * K + 2 * M * cols * (2 if residual else 1)
+        floor = max(byts / pk["hbm_gbs"] / 1e6, M * N * K / pk["bf16_tflops"] / 1e9)
+        row = {"op": f"linear_q8[M{M},N{N},K{K}{',swiglu' if swiglu else ''}{',residual' if residual else ''}]",
+               "ms": round(ms, 4), "tflops": round(2 * M * N * K / ms / 1e9, 1), "frac_of_floor": round(floor / ms, 3)}
+        if with_torch:  # the product with its scales; no SwiGLU, no residual
+            row["torch_scaled_mm_ms"] = round(time_fn(lambda: torch._scaled_mm(
+                x.values, w.values.t(), x.scale[:, None], w.scale[None], out_dtype=torch.bfloat16)), 4)
+        rows.append(row)
+    return rows
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--only", default="gemm,small_m,attn,kv_link")
@@ -306,7 +344,7 @@ def main():
     pk = peaks()
     fns = {"gemm": bench_gemm, "small_m": bench_small_m, "attn": bench_attention, "kv_link": bench_kv_link,
            "attn_variants": bench_attention_variants, "tp_reduce": bench_tp_reduce, "lora": bench_lora,
-           "sample": bench_sample}
+           "sample": bench_sample, "q8": bench_q8}
     for name in a.only.split(","):
         for r in fns[name](pk, a.torch):
             r["peaks"] = pk["src"]

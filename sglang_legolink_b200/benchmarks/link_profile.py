@@ -3,7 +3,7 @@ decode steps on the headline configuration (Qwen2.5-7B, 16K context, 12
 sub-contexts, 10 linked, repair window 32), from the CUDA activity trace of
 ``torch.profiler`` (kernel durations as the driver reports them; no replay).
 
-    python -m sglang_legolink_b200.benchmarks.link_profile [--decode 8]
+    python -m sglang_legolink_b200.benchmarks.link_profile [--decode 8] [--weights q8]
 
 Prints, per phase, each kernel's share of the phase's summed kernel time.
 """
@@ -68,9 +68,12 @@ def main():
     ap.add_argument("--model", default="qwen2.5-7b")
     ap.add_argument("--context", type=int, default=16384)
     ap.add_argument("--decode", type=int, default=8)
+    ap.add_argument("--weights", choices=("bf16", "q8"), default="bf16")
     a = ap.parse_args()
     cfg = PRESETS[a.model]
     model = QwenModel.random_init(cfg, seed=0, device="cuda", dtype=torch.bfloat16)
+    if a.weights == "q8":
+        model.quantize_weights()
     eng = Engine(model, page_size=16, max_context=a.context + 2048, mem_fraction=0.6)
     subs = synthetic_context(12, a.context, cfg.vocab_size, 0)
     for i in range(10):

@@ -35,10 +35,10 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_barrier() {
+__device__ __forceinline__ void cluster_barrier_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
   cluster_arrive();
-  cluster_wait();
+  cluster_barrier_wait();
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(192, 2)
   if (tid < rows) sxs[tid] = p.xs[m0 + tid];
   const bool ok = __syncthreads_and(mbar_wait(&tfull, 0, err, kErrTmemFullTimeout));
   tc_fence_after();
-  if (cs > 1) cluster_wait();
+  if (cs > 1) cluster_barrier_wait();
   if (warp >= 2) {  // TMEM lane quarter of this warp: features; columns: rows
     const int feat = (warp & 3) * 32 + lane;
     const bool none = kb1 <= kb0;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(192, 2)
     }
   }
   tc_fence_before();
-  if (cs > 1) cluster_barrier();
+  if (cs > 1) cluster_sync();
   else __syncthreads();
   tc_fence_after();
   if (ok && live) {
@@ -457,7 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  cluster_barrier();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   if (warp == 0 && elect_one() && pair < ntiles) {  // the first ring of weights on its way to L2
@@ -683,7 +683,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
   }
 
   tc_fence_before();
-  cluster_barrier();
+  cluster_sync();
   tc_fence_after();
   if (warp == 1) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::TMEM_COLS)

@@ -5,6 +5,9 @@ qwen2.py:63-311``): fused-add RMSNorm -> QKV GEMM (+bias on Qwen2) -> [Qwen3:
 per-head q/k RMSNorm] -> RoPE + paged KV write -> attention -> o_proj ->
 fused-add RMSNorm -> gate_up GEMM with SwiGLU epilogue -> down_proj.
 
+With its projections in 8 bits (:meth:`QwenModel.quantize_weights`) the norms
+write 8 bits and the residual is added in the projections' epilogues.
+
 One forward serves every batch kind through :class:`ForwardBatch`:
 
 * ``extend``  -- query rows at arbitrary positions of each request (a Compile
@@ -84,6 +87,8 @@ class QwenModel:
         self.lm_head: Optional[torch.Tensor] = None
         self.cos_sin: Optional[torch.Tensor] = None
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
+        self.quantized = False  # the layers' projections are in 8 bits (quantize_weights)
+        self.served = False  # an engine holds keys and values of these weights
         self.adapter_names: list[str] = []  # adapter i of a batch's plan
         self.adapter_digests: list[str] = []
         self._layer_adapters: list = []
@@ -225,6 +230,35 @@ class QwenModel:
     def save_pretrained(self, path: str, state: dict) -> None:
         save_safetensors_checkpoint(path, self.cfg, state)
 
+    # ----------------------------------------------------- weights in 8 bits
+    def quantize_weights(self) -> None:
+        """Puts the layers' projections into 8 bits (:func:`ops.quantize_q8`:
+        e4m3 with a scale per output feature) in place of the others; forwards
+        quantise their inputs row by row (:meth:`_forward_q8`).  The embedding,
+        the norms and the LM head stay.  Before an engine serves the model;
+        not with adapters, tensor parallelism or row-wise repair compute."""
+        if self.tp_size > 1:
+            raise ValueError("weights in 8 bits are not supported with tensor parallelism")
+        if self.adapter_names:
+            raise ValueError("weights in 8 bits are not supported with adapters")
+        if self.served:
+            raise ValueError("weights go into 8 bits before an engine holds keys and values of the others")
+        if self.quantized:
+            return
+        names = ("qkv_w", "o_w", "gu_w", "down_w")
+        for i, lw in enumerate(self.layers):  # all of them fit before any is replaced
+            for n in names:
+                w = getattr(lw, n)
+                if w.shape[1] % 16 or w.shape[1] > ops.Q8_MAX_K or w.shape[0] % (32 if n == "gu_w" else 8):
+                    raise ValueError(f"layer {i}: a projection of shape {tuple(w.shape)} does not go into 8 bits")
+                if not bool(torch.isfinite(w).all()):
+                    raise ValueError(f"layer {i}: the weights must be finite")
+        for lw in self.layers:
+            for n in names:
+                setattr(lw, n, ops.quantize_q8(getattr(lw, n)))
+        self.quantized = True
+        self.buf_generation += 1  # a captured graph may point at weights that are gone
+
     # ------------------------------------------------------------- adapters
     def add_adapter(self, name: str, adapter) -> int:
         """Adds a low-rank adapter (:class:`~.adapters.Adapter`); rows whose
@@ -236,6 +270,8 @@ class QwenModel:
 
         if self.tp_size > 1:
             raise ValueError("adapters are not supported with tensor parallelism")
+        if self.quantized:
+            raise ValueError("adapters are not supported with weights in 8 bits")
         if name in self.adapter_names:
             raise ValueError(f"adapter '{name}' is loaded already")
         bad = sorted({layer for layer, _ in adapter.mats if not 0 <= layer < self.cfg.num_layers})
@@ -281,6 +317,8 @@ class QwenModel:
         ``fb.logit_rows`` (all rows when None)."""
         c = self.cfg
         T = fb.num_rows
+        if self.quantized:
+            return self._forward_q8(fb, kv, return_hidden)
         if (fb.mode == "extend" and getattr(self.comm, "name", "") == "fused" and fb.input_ids.is_cuda
                 and self.comm.use_fused(T)):
             return self._forward_fused_tp(fb, kv, return_hidden)
@@ -334,21 +372,7 @@ class QwenModel:
                 cap.on_component(li, "qkv_projection", qkv=qkv)
                 cap.on_component(li, "rope", q=q)
             with mk.region("Attention", li, q=q):
-                if fb.mode == "decode":
-                    ops.attention_decode(q, kv.k[li], kv.v[li], fb.page_table, fb.kv_lens, self.scale,
-                                         nsplit=fb.decode_nsplit, out=attn)
-                else:
-                    ops.attention_prefill(q, kv.k, kv.v, li, fb.q_indptr, fb.positions, fb.page_table, fb.kv_lens,
-                                          self.scale, tiles=tiles, out=attn, nsplit=tiles_nsplit)
-                    if cmp_attn:  # diagnostic: native kernel vs the fp32 torch statement, sampled rows
-                        from ..runtime.repair_diagnostics import compare_attention
-                        from ..utils.trace import emit_trace
-
-                        row = compare_attention(li, q, attn, kv.k[li], kv.v[li], fb.q_indptr, fb.positions,
-                                                fb.page_table, fb.kv_lens, self.scale)
-                        if fb.repair_meta is not None:
-                            fb.repair_meta.setdefault("native_operator_comparisons", []).append(row)
-                        emit_trace("repair_attention_compare", **row)
+                self._attend(li, fb, kv, q, attn, tiles, tiles_nsplit, cmp_attn)
             # row-wise: each grouped row with the shapes it has alone
             if la is not None:
                 self._proj(attn, lw.o_w, None, la.o, fb, o)
@@ -379,6 +403,101 @@ class QwenModel:
         if return_hidden:
             return rows
         return self.logits(rows)
+
+    def _attend(self, li: int, fb: ForwardBatch, kv, q, attn, tiles, tiles_nsplit: int, cmp_attn: bool) -> None:
+        if fb.mode == "decode":
+            ops.attention_decode(q, kv.k[li], kv.v[li], fb.page_table, fb.kv_lens, self.scale,
+                                 nsplit=fb.decode_nsplit, out=attn)
+            return
+        ops.attention_prefill(q, kv.k, kv.v, li, fb.q_indptr, fb.positions, fb.page_table, fb.kv_lens,
+                              self.scale, tiles=tiles, out=attn, nsplit=tiles_nsplit)
+        if cmp_attn:  # diagnostic: native kernel vs the fp32 torch statement, sampled rows
+            from ..runtime.repair_diagnostics import compare_attention
+            from ..utils.trace import emit_trace
+
+            row = compare_attention(li, q, attn, kv.k[li], kv.v[li], fb.q_indptr, fb.positions,
+                                    fb.page_table, fb.kv_lens, self.scale)
+            if fb.repair_meta is not None:
+                fb.repair_meta.setdefault("native_operator_comparisons", []).append(row)
+            emit_trace("repair_attention_compare", **row)
+
+    def _forward_q8(self, fb: ForwardBatch, kv, return_hidden: bool = False) -> torch.Tensor:
+        """Forward of a model whose projections are in 8 bits.  A layer's four
+        products read rows in 8 bits: the norms write them, and the attention's
+        and the gated rows are quantised by a launch of their own, since a
+        row's scale needs all of it.  o_proj and down_proj add the residual in
+        their epilogue, in fp32; a diagnostic capture, which wants their
+        results by themselves, adds it in the norms instead."""
+        c, mk = self.cfg, self.markers
+        T = fb.num_rows
+        H, D, eps = c.hidden_size, c.head_dim, c.rms_norm_eps
+        cap = self.capture if fb.mode == "extend" else None
+        cmp_attn = False
+        if fb.mode == "extend":
+            from ..runtime.repair_diagnostics import compare_enabled, rowwise_slices
+
+            cmp_attn = compare_enabled("attention")
+            if fb.repair_meta is not None and (rowwise_slices(fb.repair_meta, T, "output_projection")
+                                               or rowwise_slices(fb.repair_meta, T, "ffn")):
+                raise ValueError("row-wise repair compute does not run with weights in 8 bits")
+        tiles, tiles_nsplit = fb.tiles, fb.tiles_nsplit
+        if fb.mode == "extend" and tiles is None and fb.input_ids.is_cuda:
+            tiles, tiles_nsplit = self._attn_tiles(fb)
+        residual = ops.embedding(fb.input_ids, self.embed, out=self._buf("res", (T, H)))
+        h = self._buf_q8("h8", T, H)
+        q = self._buf("q", (T, self.hq, D))
+        attn = self._buf("attn", (T, self.hq * D))
+        a8 = self._buf_q8("a8", T, self.hq * D)
+        qkv = self._buf("qkv", (T, (self.hq + 2 * self.hkv) * D))
+        mlp = self._buf("mlp", (T, self.inter))
+        m8 = self._buf_q8("m8", T, self.inter)
+        o = self._buf("o", (T, H)) if cap is not None else residual
+        add = None if cap is not None else residual
+        for li, lw in enumerate(self.layers):
+            if cap is None or li == 0:
+                ops.rmsnorm_q8(residual, lw.in_norm, eps, out=h)
+            else:
+                ops.fused_add_rmsnorm_q8(o, residual, lw.in_norm, eps, out=h)
+            wants = cap is not None and cap.wants(li)
+            if wants:
+                cap.on_component(li, "pre_attention_norm", hidden=h.float(), residual=residual)
+            ops.linear_q8(h, lw.qkv_w, lw.qkv_b, out=qkv)
+            ops.rope_qkv_write(qkv, fb.positions, fb.slots, self.cos_sin, q, kv.k[li], kv.v[li], self.hq, self.hkv,
+                               D, lw.q_norm, lw.k_norm, eps)
+            if wants:
+                cap.on_component(li, "qkv_projection", qkv=qkv)
+                cap.on_component(li, "rope", q=q)
+            with mk.region("Attention", li, q=q):
+                self._attend(li, fb, kv, q, attn, tiles, tiles_nsplit, cmp_attn)
+            ops.quantize_q8(attn, out=a8)
+            ops.linear_q8(a8, lw.o_w, residual=add, out=o)
+            if wants:
+                cap.on_component(li, "attention", attention_output=attn)
+                cap.on_component(li, "output_projection", projected_output=o)
+            if cap is None:
+                ops.rmsnorm_q8(residual, lw.post_norm, eps, out=h)
+            else:
+                ops.fused_add_rmsnorm_q8(o, residual, lw.post_norm, eps, out=h)
+            if wants:
+                cap.on_component(li, "post_attention_norm", hidden=h.float(), residual=residual)
+            with mk.region("FFN", li, hidden=residual):
+                ops.linear_q8(h, lw.gu_w, out=mlp, swiglu_epilogue=True)
+                ops.quantize_q8(mlp, out=m8)
+                ops.linear_q8(m8, lw.down_w, residual=add, out=o)
+            if cap is not None:
+                if wants:
+                    cap.on_component(li, "mlp", mlp_output=o)
+                cap.on_layer(li, hidden=o, residual=residual)
+        if cap is None:
+            out = ops.rmsnorm(residual, self.final_norm, eps, out=self._buf("h", (T, H)))
+        else:
+            ops.fused_add_rmsnorm(o, residual, self.final_norm, eps)
+            out = o
+        rows = out if fb.logit_rows is None else out.index_select(0, fb.logit_rows)
+        return rows if return_hidden else self.logits(rows)
+
+    def _buf_q8(self, name: str, rows: int, K: int) -> "ops.Q8":
+        return ops.Q8(self._buf(name, (rows, K), torch.float8_e4m3fn), self._buf(name + "s", (rows,), torch.float32))
 
     def _forward_decode_tp(self, fb: ForwardBatch, kv) -> torch.Tensor:
         """TP decode step whose row-parallel reductions are fused kernels:

@@ -23,14 +23,14 @@ import torch
 from . import reference as ref
 from ._ext import ExtensionMissing, cuda as _cuda  # noqa: F401
 from .lora import LORA_MAX_RANK, LoraPlan, LoraStack, lora_plan  # noqa: F401
-from .q8 import Q8, check_product, check_rows, empty_q8
+from .q8 import Q8, Q8_MAX_K, check_product, check_rows, empty_q8
 
 __all__ = [
     "ExtensionMissing", "linear", "rmsnorm", "fused_add_rmsnorm", "rope_qkv_write", "attention_prefill",
     "attention_decode", "swiglu", "embedding", "argmax", "kv_link_rope", "interleave_gate_up",
     "deinterleave_gate_up", "prefill_tiles", "workspace", "check_errors", "gemv_rownorm", "gemv_residual",
     "gemv_qkv_rope", "LoraStack", "LoraPlan", "lora_plan", "linear_lora", "sample",
-    "Q8", "empty_q8", "quantize_q8", "rmsnorm_q8", "fused_add_rmsnorm_q8", "linear_q8",
+    "Q8", "Q8_MAX_K", "empty_q8", "quantize_q8", "rmsnorm_q8", "fused_add_rmsnorm_q8", "linear_q8",
 ]
 
 SMALL_M_MAX = 128
@@ -393,8 +393,8 @@ def linear_q8(x: Q8, w: Q8, bias: Optional[torch.Tensor] = None, residual: Optio
     last bits may change with the number of rows, which chooses the kernel and
     its split of K, never with the other rows' values."""
     if x.values.is_cuda:
-        return _cuda().q8_linear(x.values, x.scale, w.values, w.scale, bias, residual, out, swiglu_epilogue, 0,
-                                 workspace(x.values.device).err)
+        ws = _WS.get(x.values.get_device()) or workspace(x.values.device)
+        return _cuda().q8_linear(x.values, x.scale, w.values, w.scale, bias, residual, out, swiglu_epilogue, 0, ws.err)
     cols = check_product(x, w, bias, residual, out, swiglu_epilogue)
     if out is None:
         out = torch.empty(x.values.shape[0], cols, dtype=torch.bfloat16)

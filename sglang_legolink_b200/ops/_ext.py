@@ -71,6 +71,7 @@ class _Counted:
             else:
                 fn = target
             self._cache[name] = fn
+            self.__dict__[name] = fn  # found without __getattr__ from now on
         return fn
 
 

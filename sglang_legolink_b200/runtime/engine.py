@@ -165,6 +165,7 @@ class Engine:
             raise ValueError("sampler must be 'torch' (per-row torch ops) or 'kernel' (one launch a batch)")
         self.sampler = sampler
         self.model = model
+        model.served = True
         self.cfg = model.cfg
         self.device = model.device
         self.page_size = page_size
@@ -238,7 +239,8 @@ class Engine:
     def _compat(self, over: dict) -> dict:
         c = self.cfg
         d = {
-            "model_fingerprint": f"{c.name}@{c.fingerprint()}",
+            # blocks of weights in 8 bits and of the others do not link
+            "model_fingerprint": f"{c.name}@{c.fingerprint()}" + ("+q8" if self.model.quantized else ""),
             "tokenizer_fingerprint": f"{c.name}:{c.vocab_size}",
             "kv_dtype": str(self.model.dtype),
             "rope_fingerprint": f'{{"max_position_embeddings":{c.max_position_embeddings},"rope_scaling":null,'

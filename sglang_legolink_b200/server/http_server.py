@@ -284,7 +284,7 @@ def serve(svc: RuntimeService, host: str = "127.0.0.1", port: int = 30000) -> Th
 def build_service(model: str = "tiny-qwen2", *, device: str = "cpu", tokenizer: Optional[str] = None,
                   legolink_only: Optional[bool] = True, page_size: int = 16, num_pages: Optional[int] = None,
                   max_context: int = 32768, seed: int = 0, layerwise_markers: bool = False,
-                  sampler: str = "torch", adapters=()) -> RuntimeService:
+                  sampler: str = "torch", adapters=(), weights: str = "bf16") -> RuntimeService:
     import torch
 
     from ..host.tokenizer import HashTokenizer, HFTokenizer
@@ -297,6 +297,8 @@ def build_service(model: str = "tiny-qwen2", *, device: str = "cpu", tokenizer: 
         m = QwenModel.from_pretrained(model, device=device, dtype=dtype)
     else:
         m = QwenModel.random_init(get_config(model), seed=seed, device=device, dtype=dtype)
+    if weights == "q8":
+        m.quantize_weights()
     if layerwise_markers:
         from ..utils.layer_markers import LayerMarkers
 
@@ -343,9 +345,13 @@ def main(argv=None) -> None:
                     help="sampled rows: per-row torch ops, or one launch for the batch (other seeded draws)")
     ap.add_argument("--adapter", action="append", default=[], type=adapter_arg, metavar="NAME=PATH",
                     help="load a PEFT low-rank adapter; requests choose it with adapter_id (repeatable)")
+    ap.add_argument("--weights", choices=("bf16", "q8"), default="bf16",
+                    help="the layers' projections: as loaded, or in 8 bits (e4m3, quantised at load)")
     a = ap.parse_args(argv)
     if a.adapter and a.tp_size > 1:
         ap.error("--adapter is not supported with --tp-size")
+    if a.weights != "bf16" and (a.adapter or a.tp_size > 1):
+        ap.error("--weights q8 is not supported with --adapter or --tp-size")
     if a.tp_size > 1 or a.dp_size > 1 or a.pp_size != 1:
         from .launch import launch
 
@@ -354,7 +360,7 @@ def main(argv=None) -> None:
     svc = build_service(a.model, device=a.device, tokenizer=a.tokenizer,
                         legolink_only=False if a.allow_plain_generation else None, page_size=a.page_size,
                         max_context=a.context_length, layerwise_markers=a.enable_layerwise_nvtx_marker,
-                        sampler=a.sampler, adapters=a.adapter)
+                        sampler=a.sampler, adapters=a.adapter, weights=a.weights)
     if not a.skip_warmup and os.getenv("SGLANG_PIC_WARMUP", "1") != "0":
         print("warmup", svc.warmup(int(os.getenv("SGLANG_PIC_WARMUP_BLOCK_TOKENS", "256")),
                                    int(os.getenv("SGLANG_PIC_WARMUP_LEGOLINK_K", "16"))), flush=True)

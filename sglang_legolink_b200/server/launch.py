@@ -246,6 +246,8 @@ def _build_rank(a, rank: int, world: int, local: int, ctrl=None):
     else:
         m = QwenModel.random_init(get_config(a.model), seed=a.seed, device=dev, dtype=dtype, tp_rank=tpr,
                                   tp_size=tps, comm=comm)
+    if getattr(a, "weights", "bf16") == "q8":
+        m.quantize_weights()
     if a.dp_size > 1:
         from ..parallel.dp import BlockDirectory
 
