@@ -851,6 +851,7 @@ extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, c
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return -5;
   if (kernel == 0 && p->M > 64) kernel = kernel_rule(p->M, p->N, p->K, sms);
+  if (kernel <= SPLIT_MAX_CLUSTER && p->N > 128 * 65535) kernel = 256;  // more feature tiles than a grid has places
   if (kernel >= 0 && kernel <= SPLIT_MAX_CLUSTER)
     return swiglu ? split_launch<true>(*p, kernel, err, stream) : split_launch<false>(*p, kernel, err, stream);
   if (kernel == 64) return swiglu ? pair_launch<64, true>(*p, sms, err, stream) : pair_launch<64, false>(*p, sms, err, stream);

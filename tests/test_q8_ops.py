@@ -396,3 +396,82 @@ def test_refusals_on_the_gpu():
     buf = torch.zeros(33, 32, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError):  # the output a row behind the residual
         ops.linear_q8(x, w, residual=buf[:32], out=buf[1:])
+
+
+@gpu
+def test_no_rows_on_the_gpu():
+    w = q8_like(32, 64, 1, "cuda")
+    x = ops.quantize_q8(torch.empty(0, 64, dtype=torch.bfloat16, device="cuda"))
+    assert x.values.shape == (0, 64) and x.scale.shape == (0,)
+    assert ops.linear_q8(x, w).shape == (0, 32)
+    r = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+    assert ops.fused_add_rmsnorm_q8(r, r.clone(), torch.ones(64, dtype=torch.bfloat16, device="cuda"), 1e-6).values.numel() == 0
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """More than 2^31 values of x and of the result: the last rows are right."""
+    M, K = 140000, 16384
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    last = rows_like(3, K, 5, device="cuda")
+    x[-3:] = last
+    got, want = ops.quantize_q8(x), ops.quantize_q8(last)
+    assert torch.equal(got.values[-3:].view(torch.uint8), want.values.view(torch.uint8))
+    assert torch.equal(got.scale[-3:], want.scale) and float(got.scale[0]) == 2.0 ** -126
+    del x, got
+    M, N, K = 70000, 32768, 64
+    a, b = integers_q8(M, K, 1, "cuda"), integers_q8(N, K, 2, "cuda")
+    r = torch.ones(M, N, dtype=torch.bfloat16, device="cuda")
+    y = ops.linear_q8(a, b, residual=r, out=r)
+    tail = slice(M - 300, M)
+    want = (a.values[tail].double() @ b.values.double().t()) * a.scale[tail, None].double() * b.scale.double() + 1
+    assert torch.equal(y[tail], want.to(torch.bfloat16))
+    assert ops.check_errors("cuda") == 0
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_a_row_of_nan_values_stays_its_own(M):
+    """NaN codes in one row of x and one of w: that row and that column, whatever lies behind the last row."""
+    x, w = q8_like(M, 272, 1, "cuda"), q8_like(136, 272, 2, "cuda")
+    want = ops.linear_q8(x, w)
+    nan = torch.tensor(math.nan, device="cuda")
+    x.values[M // 2] = nan.to(E4M3)
+    w.values[7] = nan.to(E4M3)
+    y = ops.linear_q8(x, w)
+    keep = torch.ones_like(want, dtype=torch.bool)
+    keep[M // 2], keep[:, 7] = False, False
+    assert torch.equal(y[keep], want[keep]) and bool(y[~keep].isnan().all())
+
+
+@gpu
+def test_two_graphs_replayed_on_two_streams():
+    """Nothing but the error word is shared between calls."""
+    x, w = q8_like(5, 2048, 1, "cuda"), q8_like(640, 2048, 2, "cuda")
+    want = ops.linear_q8(x, w)
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            for _ in range(8):
+                y = ops.linear_q8(x, w)
+        graphs.append(g)
+        outs.append(y)
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in outs) and ops.check_errors("cuda") == 0
+
+
+@gpu
+@pytest.mark.parametrize("K,N", [(64, 64), (2048, 5120), (18944, 384)])
+def test_a_row_alone_and_among_others(K, N):
+    """The kernels differ in the order of a row's sums alone."""
+    x, w = q8_like(700, K, 1, "cuda"), q8_like(N, K, 2, "cuda")
+    want, tol = product64(x, w, None, None, False)
+    for M in (1, 16, 17, 33, 64, 65, 128, 129, 256, 257, 700):
+        y = ops.linear_q8(Q8(x.values[:M], x.scale[:M]), w)
+        assert torch.all((y.cpu().double() - want[:M]).abs() <= tol[:M]), M
