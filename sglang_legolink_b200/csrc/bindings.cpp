@@ -582,7 +582,7 @@ at::Tensor q8_linear(const at::Tensor& x, const at::Tensor& xs, const at::Tensor
   TORCH_CHECK_VALUE(w.size(1) == K, "x has rows of ", num(K), " values, w of ", num(w.size(1)));
   TORCH_CHECK_VALUE(K > 0 && K % 16 == 0 && N > 0 && N % (swiglu ? 32 : 8) == 0, "K = ", num(K), ", N = ", num(N),
                     ": K must be a multiple of 16 and N of 8 (of 32: SwiGLU)");
-  TORCH_CHECK(M < (1 << 28) && N < (1 << 28) && K < (1ll << 31), "too large");
+  TORCH_CHECK(M < (1 << 28) && N < (1 << 28) && K < (1 << 30), "too large");
   const at::Device dev = x.device();
   check_matrix(x, at::kFloat8_e4m3fn, dev, M, K, "x");
   check_matrix(w, at::kFloat8_e4m3fn, dev, N, K, "w");

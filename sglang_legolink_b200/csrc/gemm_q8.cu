@@ -11,12 +11,17 @@
 //
 // * q8_split_kernel -- few rows.  The weight tile is the M = 128 side, the rows
 //   (up to 128) are the N side, and K is split over the CTAs of a cluster, whose
-//   fp32 partials meet in distributed shared memory.
-// * q8_pair_kernel -- many rows.  Pairs of CTAs (cta_group::2) on 256 x 256
-//   tiles, persistent, two accumulators in tensor memory, so that the epilogue of
-//   a tile runs beside the main loop of the next.
+//   fp32 partials meet in distributed shared memory.  Bound by reading W: 16 rows,
+//   3584 -> 37888 with SwiGLU, 22.0 us in a graph, 6.2 TB/s of its 137 MB.
+// * q8_pair_kernel -- many rows.  Pairs of CTAs (cta_group::2) on tiles of 256 rows
+//   x 64, 128 or 256 features, persistent, two accumulators in tensor memory, so
+//   that the epilogue of a tile runs beside the main loop of the next.  Bound by the
+//   tensor pipe and the power cap: 2048 rows, 3584 -> 37888 with SwiGLU, 178 us
+//   alone (3.1 PFLOP/s, tensor pipe 89 % active at 1.48 GHz), 222 back to back.
 #include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "q8.h"
@@ -34,8 +39,12 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_barrier_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_barrier_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
   cluster_arrive();
   cluster_barrier_wait();
@@ -177,8 +186,12 @@ struct alignas(64) Maps {
 //
 // CTA o of a cluster sums and stores rows [o R, (o + 1) R): the others write their
 // partials of those rows into its shared memory as they read them from tensor
-// memory, behind one cluster barrier (XX).  That memory is beside the ring, since
-// the others may be done first; a lone CTA takes the ring.
+// memory, and one cluster barrier later they are there.  (Partials that stay where
+// they are, read behind one barrier and kept alive by a second: 1 row, 3584 -> 4608,
+// 5.3 us for 5.1; 16 rows, 18944 -> 3584, 14.2 for 13.6.)  That memory is beside the
+// ring, since the others may be done first; a lone CTA takes the ring.  With more
+// than 64 rows the partials of a cluster would cost more than they save (128 rows,
+// 3584 -> 4608: 7 of 10 us behind the last product), so those have lone CTAs.
 constexpr int SPLIT_MAX_CLUSTER = 8;
 template <int BNX>
 struct SplitCfg {
@@ -386,15 +399,22 @@ __global__ void __launch_bounds__(192, 2)
 
 // ---------------------------------------------------------------------------
 // Many rows: CTA r of a pair loads rows [128 r, +128) of the tile's 256 rows of X
-// and of its 256 rows of W; the leader issues the MMAs (M = 256, N = 256, K = 32),
-// which accumulate rows [128 r, +128) in CTA r's tensor memory.  Loads of both
-// complete on the leader's `full` barrier, commits arrive in both CTAs.
+// and its half of the tile's BN rows of W; the leader issues the MMAs (M = 256, N =
+// BN, K = 32), which accumulate rows [128 r, +128) in CTA r's tensor memory.  Loads
+// of both complete on the leader's `full` barrier, commits arrive in both CTAs.
+//
+// The epilogue hides behind the next tile's k-blocks only if it is the shorter: four
+// warps that read scales and bias from global memory took 449 us for 2048 x 3584 ->
+// 37888 with SwiGLU, eight with both in shared memory and the approximate quotient
+// 203.  Results and residual go through boxes of 32 x 32 in shared memory, by bulk
+// tensor copies; residual loads by the threads cost 5087 x 3584 -> 3584 11 us, these 1.
 constexpr int PAIR_BOX = 32 * 64;    // epilogue staging: 32 rows x 32 bf16 columns
 constexpr int PAIR_BOXES = 3;        // of a warp: one is stored, one worked on, one being filled with residual
 template <int BN>
 struct PairCfg {
   static constexpr int STAGES = BN == 256 ? 5 : (BN == 128 ? 7 : 8);
-  static constexpr int EPI_WARPS = BN == 64 ? 4 : 8;  // 8: two to a quarter of TMEM's lanes, each with half of the columns
+  // eight: two to a quarter of TMEM's lanes, each with half of the tile's columns
+  static constexpr int EPI_WARPS = BN == 64 ? 4 : 8;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int X_BYTES = 128 * BK;      // a CTA's half of X's k-block
   static constexpr int W_BYTES = BN / 2 * BK;   // and of W's
@@ -446,7 +466,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
   static_assert(2 * PAIR_STAGES + 5 + PAIR_EPI_WARPS * PAIR_BOXES <= 64, "two warps initialise the barriers");
   if (threadIdx.x < 2 * PAIR_STAGES + 5 + PAIR_EPI_WARPS * PAIR_BOXES) {
     uint64_t* bar = full + threadIdx.x;
-    mbar_init(bar, bar == tempty || bar == tempty + 1 ? 2 * PAIR_EPI_WARPS : 1);  // tempty: warps of both CTAs, on the leader
+    // tempty: the epilogue warps of both CTAs, on the leader
+    mbar_init(bar, bar == tempty || bar == tempty + 1 ? 2 * PAIR_EPI_WARPS : 1);
     fence_mbar_init();
   }
   __syncwarp();
@@ -548,7 +569,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     }
     __syncwarp();
   } else {
-    // warp w reads TMEM lanes [32 (w % 4), +32) (lane = row) of the tile's columns [128 half, +128)
+    // warp w reads TMEM lanes [32 (w % 4), +32) (lane = row) of the tile's columns [COLS half, +COLS)
     const int q = warp & 3, e = warp - 2, half = e >> 2;
     const uint32_t leader_tempty0 = mapa(smem_u32(&tempty[0]), 0), leader_tempty1 = mapa(smem_u32(&tempty[1]), 0);
     uint8_t* boxes = sBox + e * PAIR_BOXES * PAIR_BOX;
@@ -595,9 +616,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
       const uint32_t tbase = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN + half * PAIR_COLS);
       // r[i] ws xs + bias of columns [c, c + 32); every lane reads the same of them
       auto scaled = [&](const uint32_t (&r)[32], int c, int i) {
-        const float4 s = *reinterpret_cast<const float4*>(scol + c + i), b = *reinterpret_cast<const float4*>(sbias + c + i);
-        return make_float4(fmaf(__uint_as_float(r[i]) * xs, s.x, b.x), fmaf(__uint_as_float(r[i + 1]) * xs, s.y, b.y),
-                           fmaf(__uint_as_float(r[i + 2]) * xs, s.z, b.z), fmaf(__uint_as_float(r[i + 3]) * xs, s.w, b.w));
+        const float4 s = *reinterpret_cast<const float4*>(scol + c + i);
+        const float4 t = *reinterpret_cast<const float4*>(sbias + c + i);
+        return make_float4(fmaf(__uint_as_float(r[i]) * xs, s.x, t.x), fmaf(__uint_as_float(r[i + 1]) * xs, s.y, t.y),
+                           fmaf(__uint_as_float(r[i + 2]) * xs, s.z, t.z),
+                           fmaf(__uint_as_float(r[i + 3]) * xs, s.w, t.w));
       };
 #pragma unroll 1
       for (int c = 0; c < PAIR_COLS; c += 64) {
@@ -679,14 +702,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
         aphase ^= 1;
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the boxes are read
+    // the boxes are read; the grid's end completes the writes
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
 
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
   if (warp == 1) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::TMEM_COLS)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"((uint32_t)Cfg::TMEM_COLS)
                  : "memory");
   }
 }
@@ -831,7 +856,8 @@ static int pair_launch(const LLQ8Gemm& p, int sms, int* err, cudaStream_t stream
   static unsigned long long done = 0;
   auto kern = q8_pair_kernel<BN, SWIGLU>;
   if (!smem_on_device(kern, Cfg::SMEM, done)) return -7;
-  const cudaError_t e = launch_pdl(kern, dim3(2 * pairs), dim3(Cfg::THREADS), Cfg::SMEM, stream, tm, p, (int)group, err);
+  const cudaError_t e =
+      launch_pdl(kern, dim3(2 * pairs), dim3(Cfg::THREADS), Cfg::SMEM, stream, tm, p, (int)group, err);
   return e == cudaSuccess ? 0 : -5;
 }
 
@@ -852,10 +878,13 @@ extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, c
     return -5;
   if (kernel == 0 && p->M > 64) kernel = kernel_rule(p->M, p->N, p->K, sms);
   if (kernel <= SPLIT_MAX_CLUSTER && p->N > 128 * 65535) kernel = 256;  // more feature tiles than a grid has places
-  if (kernel >= 0 && kernel <= SPLIT_MAX_CLUSTER)
-    return swiglu ? split_launch<true>(*p, kernel, err, stream) : split_launch<false>(*p, kernel, err, stream);
-  if (kernel == 64) return swiglu ? pair_launch<64, true>(*p, sms, err, stream) : pair_launch<64, false>(*p, sms, err, stream);
-  if (kernel == 128) return swiglu ? pair_launch<128, true>(*p, sms, err, stream) : pair_launch<128, false>(*p, sms, err, stream);
-  if (kernel == 256) return swiglu ? pair_launch<256, true>(*p, sms, err, stream) : pair_launch<256, false>(*p, sms, err, stream);
-  return -3;
+  const auto run = [&](auto gated) {
+    constexpr bool G = decltype(gated)::value;
+    if (kernel >= 0 && kernel <= SPLIT_MAX_CLUSTER) return split_launch<G>(*p, kernel, err, stream);
+    if (kernel == 64) return pair_launch<64, G>(*p, sms, err, stream);
+    if (kernel == 128) return pair_launch<128, G>(*p, sms, err, stream);
+    if (kernel == 256) return pair_launch<256, G>(*p, sms, err, stream);
+    return -3;
+  };
+  return swiglu ? run(std::true_type{}) : run(std::false_type{});
 }

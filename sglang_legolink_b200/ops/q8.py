@@ -37,7 +37,7 @@ def check_q8(t: Q8, name: str) -> None:
     if v.dtype != torch.float8_e4m3fn or s.dtype != torch.float32:
         raise ValueError(f"{name}: values must be float8_e4m3fn and scales float32, got {v.dtype} and {s.dtype}")
     if v.dim() != 2 or tuple(s.shape) != (v.shape[0],):
-        raise ValueError(f"{name}: values must be [rows, K] with a scale a row, got {tuple(v.shape)} and {tuple(s.shape)}")
+        raise ValueError(f"{name}: values must be [rows, K] with a scale a row, got {tuple(v.shape)}, {tuple(s.shape)}")
     if v.device != s.device:
         raise ValueError(f"{name}: values are on {v.device}, scales on {s.device}")
 
