@@ -121,6 +121,7 @@ class QwenModel:
         """``get(name)`` returns the full (unsharded) HF tensor for ``name``."""
         c, D, r = self.cfg, self.cfg.head_dim, self.tp_rank
         self.layers = []
+        self.quantized = False
         for i in range(c.num_layers):
             p = f"model.layers.{i}."
             lw = LayerWeights()
@@ -236,15 +237,14 @@ class QwenModel:
         e4m3 with a scale per output feature) in place of the others; forwards
         quantise their inputs row by row (:meth:`_forward_q8`).  The embedding,
         the norms and the LM head stay.  Before an engine serves the model;
-        not with adapters, tensor parallelism or row-wise repair compute."""
-        if self.tp_size > 1:
-            raise ValueError("weights in 8 bits are not supported with tensor parallelism")
+        not with adapters or row-wise repair compute.  A rank of a sharded
+        model quantises its shards, with scales of their own."""
+        if self.quantized:
+            return
         if self.adapter_names:
             raise ValueError("weights in 8 bits are not supported with adapters")
         if self.served:
             raise ValueError("weights go into 8 bits before an engine holds keys and values of the others")
-        if self.quantized:
-            return
         names = ("qkv_w", "o_w", "gu_w", "down_w")
         for i, lw in enumerate(self.layers):  # all of them fit before any is replaced
             for n in names:
@@ -426,8 +426,9 @@ class QwenModel:
         products read rows in 8 bits: the norms write them, and the attention's
         and the gated rows are quantised by a launch of their own, since a
         row's scale needs all of it.  o_proj and down_proj add the residual in
-        their epilogue, in fp32; a diagnostic capture, which wants their
-        results by themselves, adds it in the norms instead."""
+        their epilogue, in fp32, and the next norm reads the sum.  Where their
+        results are wanted by themselves, as terms of a sum over tensor-parallel
+        ranks or by a diagnostic capture, the norms add it instead."""
         c, mk = self.cfg, self.markers
         T = fb.num_rows
         H, D, eps = c.hidden_size, c.head_dim, c.rms_norm_eps
@@ -451,10 +452,12 @@ class QwenModel:
         qkv = self._buf("qkv", (T, (self.hq + 2 * self.hkv) * D))
         mlp = self._buf("mlp", (T, self.inter))
         m8 = self._buf_q8("m8", T, self.inter)
-        o = self._buf("o", (T, H)) if cap is not None else residual
-        add = None if cap is not None else residual
+        comm = self.comm if self.tp_size > 1 else None
+        apart = cap is not None or comm is not None
+        o = self._buf("o", (T, H)) if apart else residual
+        add = None if apart else residual
         for li, lw in enumerate(self.layers):
-            if cap is None or li == 0:
+            if not apart or li == 0:
                 ops.rmsnorm_q8(residual, lw.in_norm, eps, out=h)
             else:
                 ops.fused_add_rmsnorm_q8(o, residual, lw.in_norm, eps, out=h)
@@ -471,10 +474,12 @@ class QwenModel:
                 self._attend(li, fb, kv, q, attn, tiles, tiles_nsplit, cmp_attn)
             ops.quantize_q8(attn, out=a8)
             ops.linear_q8(a8, lw.o_w, residual=add, out=o)
+            if comm is not None:
+                comm.allreduce(o)
             if wants:
                 cap.on_component(li, "attention", attention_output=attn)
                 cap.on_component(li, "output_projection", projected_output=o)
-            if cap is None:
+            if not apart:
                 ops.rmsnorm_q8(residual, lw.post_norm, eps, out=h)
             else:
                 ops.fused_add_rmsnorm_q8(o, residual, lw.post_norm, eps, out=h)
@@ -484,11 +489,13 @@ class QwenModel:
                 ops.linear_q8(h, lw.gu_w, out=mlp, swiglu_epilogue=True)
                 ops.quantize_q8(mlp, out=m8)
                 ops.linear_q8(m8, lw.down_w, residual=add, out=o)
+            if comm is not None:
+                comm.allreduce(o)
             if cap is not None:
                 if wants:
                     cap.on_component(li, "mlp", mlp_output=o)
                 cap.on_layer(li, hidden=o, residual=residual)
-        if cap is None:
+        if not apart:
             out = ops.rmsnorm(residual, self.final_norm, eps, out=self._buf("h", (T, H)))
         else:
             ops.fused_add_rmsnorm(o, residual, self.final_norm, eps)

@@ -386,8 +386,8 @@ def linear_q8(x: Q8, w: Q8, bias: Optional[torch.Tensor] = None, residual: Optio
     interleaved gate/up product (half width); with ``residual`` [M, N] (half
     width, likewise) that is added last.  Sums in fp32, one rounding to bf16.
 
-    K a multiple of 16, N of 8 (of 32 with SwiGLU), rows on 16-byte
-    boundaries; ``out`` may be ``residual`` itself, and shares memory with no
+    K a multiple of 16, N of 8 (of 32 with SwiGLU); on CUDA rows, ``bias`` and
+    ``w.scale`` on 16-byte boundaries; ``out`` may be ``residual`` itself, and shares memory with no
     other input.  One launch without scratch, so calls on several streams may
     share everything but ``out``.  The same call gives the same bits; a row's
     last bits may change with the number of rows, which chooses the kernel and

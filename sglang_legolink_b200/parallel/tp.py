@@ -63,6 +63,9 @@ class NcclTPComm:
 
     def gemm_allreduce(self, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> None:
         ops.linear(x, w, out=out)
+        self.allreduce(out)
+
+    def allreduce(self, out: torch.Tensor) -> None:
         dist.all_reduce(out, group=self.group)
 
     def all_gather_vocab(self, local: torch.Tensor, vocab: int) -> torch.Tensor:

@@ -350,8 +350,8 @@ def main(argv=None) -> None:
     a = ap.parse_args(argv)
     if a.adapter and a.tp_size > 1:
         ap.error("--adapter is not supported with --tp-size")
-    if a.weights != "bf16" and (a.adapter or a.tp_size > 1):
-        ap.error("--weights q8 is not supported with --adapter or --tp-size")
+    if a.weights != "bf16" and a.adapter:
+        ap.error("--weights q8 is not supported with --adapter")
     if a.tp_size > 1 or a.dp_size > 1 or a.pp_size != 1:
         from .launch import launch
 

@@ -23,8 +23,10 @@ def tokens(n, vocab, seed):
     return torch.randint(0, vocab, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
 
 
-def statement(m, toks):
-    """Logits of the last token: every product on quantised rows, in 64 bits."""
+def statement(m, toks, ranks=()):
+    """Logits of the last token: every product on quantised rows, in 64 bits.
+    ``ranks``: the shards of a tensor-parallel model (``m`` is its first),
+    whose row-parallel products are sums of the ranks' own."""
     c, D = m.cfg, m.cfg.head_dim
     dbl = lambda t: t.detach().cpu().double()  # noqa: E731
 
@@ -36,12 +38,13 @@ def statement(m, toks):
     def norm(x, w):
         return x / torch.sqrt((x * x).mean(-1, keepdim=True) + c.rms_norm_eps) * dbl(w)
 
+    ranks = ranks or (m,)
     n = len(toks)
     r = dbl(m.embed)[torch.tensor(toks)]
     cos, sin = dbl(m.cos_sin)[:n].chunk(2, -1)
     mask = torch.full((n, n), float("-inf"), dtype=torch.float64).triu(1)
-    for lw in m.layers:
-        qkv = product(norm(r, lw.in_norm), lw.qkv_w, lw.qkv_b).view(n, -1, D)
+    def attention(m, lw, h):
+        qkv = product(h, lw.qkv_w, lw.qkv_b).view(n, -1, D)
         q, k, v = qkv[:, : m.hq], qkv[:, m.hq : m.hq + m.hkv], qkv[:, m.hq + m.hkv :]
         if lw.q_norm is not None:
             q, k = norm(q, lw.q_norm), norm(k, lw.k_norm)
@@ -53,11 +56,19 @@ def statement(m, toks):
         q, k = rope(q), rope(k).repeat_interleave(m.hq // m.hkv, 1)
         v = v.repeat_interleave(m.hq // m.hkv, 1)
         p = torch.softmax(torch.einsum("qhd,khd->hqk", q, k) * m.scale + mask, -1)
-        r = r + product(torch.einsum("hqk,khd->qhd", p, v).reshape(n, -1), lw.o_w)
-        gu = product(norm(r, lw.post_norm), lw.gu_w).view(n, -1, 2, 16)
+        return product(torch.einsum("hqk,khd->qhd", p, v).reshape(n, -1), lw.o_w)
+
+    def mlp(lw, h):
+        gu = product(h, lw.gu_w).view(n, -1, 2, 16)
         g, u = gu[:, :, 0], gu[:, :, 1]
-        r = r + product((g * torch.sigmoid(g) * u).reshape(n, -1), lw.down_w)
-    return norm(r, m.final_norm)[-1] @ dbl(m.lm_head).t()
+        return product((g * torch.sigmoid(g) * u).reshape(n, -1), lw.down_w)
+
+    for i, lw in enumerate(m.layers):
+        h = norm(r, lw.in_norm)
+        r = r + sum(attention(s, s.layers[i], h) for s in ranks)
+        h = norm(r, lw.post_norm)
+        r = r + sum(mlp(s.layers[i], h) for s in ranks)
+    return norm(r, m.final_norm)[-1] @ torch.cat([dbl(s.lm_head) for s in ranks])[: c.vocab_size].t()
 
 
 def logits_of(eng, toks):
@@ -79,6 +90,52 @@ def test_the_forward_follows_its_statement():
     assert close(logits_of(Engine(m, num_pages=64, max_context=256), toks), statement(m, toks), 0.02)
 
 
+def _rank(rank, port, q):
+    import os
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE="2")
+    import torch.distributed as dist
+
+    from sglang_legolink_b200.parallel.tp import NcclTPComm
+
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    try:
+        cfg = PRESETS["tiny-qwen2"]
+        m = QwenModel.random_init(cfg, seed=3, tp_rank=rank, tp_size=2, comm=NcclTPComm())
+        m.quantize_weights()
+        eng = Engine(m, num_pages=64, max_context=256)
+        toks = tokens(40, cfg.vocab_size, 1)
+        pages = eng.alloc.alloc(3)
+        fb = eng._extend_batch([(toks, list(range(40)), pages, 40)])
+        logits = m.full_logits(m.forward(fb, eng.kv))[-1]
+        seq = eng.prefill(toks)
+        eng.decode([seq], 4)
+        q.put((rank, logits.tolist(), seq.output_ids))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_two_tensor_parallel_ranks_follow_their_statement():
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_rank, args=(r, port, q)) for r in range(2)]
+    [p.start() for p in procs]
+    got = {r: (logits, ids) for r, logits, ids in (q.get(timeout=300) for _ in procs)}
+    [p.join(timeout=60) for p in procs]
+    assert all(p.exitcode == 0 for p in procs) and got[0][1] == got[1][1]
+    cfg = PRESETS["tiny-qwen2"]
+    shards = [QwenModel.random_init(cfg, seed=3, tp_rank=r, tp_size=2) for r in range(2)]
+    [m.quantize_weights() for m in shards]
+    assert close(torch.tensor(got[0][0]), statement(shards[0], tokens(40, cfg.vocab_size, 1), shards), 0.02)
+
+
 def test_a_capture_sees_the_parts_and_changes_little(tmp_path):
     from sglang_legolink_b200.runtime.repair_diagnostics import COMPONENTS, RepairStateCapture
 
@@ -97,8 +154,6 @@ def test_a_capture_sees_the_parts_and_changes_little(tmp_path):
 
 def test_refusals(tmp_path):
     cfg = PRESETS["tiny-qwen2"]
-    with pytest.raises(ValueError, match="tensor parallelism"):
-        QwenModel.random_init(cfg, tp_rank=0, tp_size=2).quantize_weights()
     m = QwenModel.random_init(cfg)
     m.layers[1].o_w[3, 4] = float("nan")
     with pytest.raises(ValueError, match="layer 1"):
@@ -152,7 +207,7 @@ def test_the_service_with_weights_in_8_bits():
 def test_the_command_line_refuses_what_does_not_go_together(capsys):
     from sglang_legolink_b200.server.http_server import main
 
-    for more in (["--adapter", "a=b"], ["--tp-size", "2"], ["--weights", "q4"]):
+    for more in (["--adapter", "a=b"], ["--weights", "q4"]):
         with pytest.raises(SystemExit):
             main(["--weights", "q8", *more])
         assert "--weights" in capsys.readouterr().err
