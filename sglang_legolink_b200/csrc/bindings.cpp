@@ -2,6 +2,7 @@
 // plain C entry points; this file checks tensors and forwards pointers and
 // the current CUDA stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_bf16.h>
 #include <torch/extension.h>
@@ -483,6 +484,11 @@ void sample(const at::Tensor& logits, const at::Tensor& u, const c10::optional<a
   check_rc(rc, "ll_sample");
 }
 
+// A new tensor on the current device, without the dispatcher's round (0.4 us of a call).
+at::Tensor empty_here(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, dev, c10::nullopt));
+}
+
 // Matrices in 8 bits (q8.h): e4m3 values [rows, K] with one fp32 scale a row.
 // Elements from a row to the next; of a single row it is never used.
 int64_t row_step(const at::Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
@@ -530,8 +536,8 @@ std::tuple<at::Tensor, at::Tensor> q8_rows(const at::Tensor& x, const c10::optio
   const at::Device dev = x.device();
   check_matrix(x, at::kBFloat16, dev, rows, K, "x");
   c10::cuda::CUDAGuard g(dev);
-  at::Tensor q = q_.has_value() ? *q_ : at::empty({rows, K}, x.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor scale = scale_.has_value() ? *scale_ : at::empty({rows}, x.options().dtype(at::kFloat));
+  at::Tensor q = q_.has_value() ? *q_ : empty_here({rows, K}, at::kFloat8_e4m3fn, dev);
+  at::Tensor scale = scale_.has_value() ? *scale_ : empty_here({rows}, at::kFloat, dev);
   LLQ8Rows p{};
   if (q_.has_value() || scale_.has_value()) {
     check_matrix(q, at::kFloat8_e4m3fn, dev, rows, K, "the values");
@@ -591,7 +597,7 @@ at::Tensor q8_linear(const at::Tensor& x, const at::Tensor& xs, const at::Tensor
   TORCH_CHECK(err.device() == dev, "the error word must be on ", dev.str());
   TORCH_CHECK(row_step(x) >= K && row_step(w) >= K, "rows of x or w share memory");
   c10::cuda::CUDAGuard g(dev);
-  at::Tensor out = out_.has_value() ? *out_ : at::empty({M, cols}, x.options().dtype(at::kBFloat16));
+  at::Tensor out = out_.has_value() ? *out_ : empty_here({M, cols}, at::kBFloat16, dev);
   LLQ8Gemm p{};
   if (out_.has_value()) {
     check_matrix(out, at::kBFloat16, dev, M, cols, "out");

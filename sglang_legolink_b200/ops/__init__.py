@@ -341,7 +341,7 @@ def _rows_q8(x: torch.Tensor, out: Optional[Q8], w: Optional[torch.Tensor] = Non
              residual: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None) -> Q8:
     if x.is_cuda:
         q, s = (None, None) if out is None else out
-        return Q8(*_cuda().q8_rows(x, residual, residual_out, w, eps, q, s))
+        return Q8._make(_cuda().q8_rows(x, residual, residual_out, w, eps, q, s))
     out = check_rows(x, out, w, residual, residual_out)
     if x.shape[0] == 0:
         return out
