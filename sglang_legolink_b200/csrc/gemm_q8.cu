@@ -188,7 +188,9 @@ struct alignas(64) Maps {
 // partials of those rows into its shared memory as they read them from tensor
 // memory, and one cluster barrier later they are there.  (Partials that stay where
 // they are, read behind one barrier and kept alive by a second: 1 row, 3584 -> 4608,
-// 5.3 us for 5.1; 16 rows, 18944 -> 3584, 14.2 for 13.6.)  That memory is beside the
+// 5.3 us for 5.1; 16 rows, 18944 -> 3584, 14.2 for 13.6.  Bulk copies from one CTA's
+// shared memory to another's in place of the stores: 5.2 and 13.9; 61 rows, 3584 ->
+// 3584, 7.6 for 7.0.)  That memory is beside the
 // ring, since the others may be done first; a lone CTA takes the ring.  With more
 // than 64 rows the partials of a cluster would cost more than they save (128 rows,
 // 3584 -> 4608: 7 of 10 us behind the last product), so those have lone CTAs.
@@ -353,6 +355,7 @@ __global__ void __launch_bounds__(192, 2)
       }
     }
   }
+  __syncwarp();
   tc_fence_before();
   if (cs > 1) cluster_sync();
   else __syncthreads();
@@ -394,6 +397,7 @@ __global__ void __launch_bounds__(192, 2)
           make_uint2(pack_bf16x2(v.x + r0.x, v.y + r0.y), pack_bf16x2(v.z + r1.x, v.w + r1.y));
     }
   }
+  __syncwarp();
   if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);  // every read of it is behind the barrier
 }
 
@@ -706,6 +710,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
 
+  __syncwarp();
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
