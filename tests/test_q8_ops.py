@@ -475,3 +475,47 @@ def test_a_row_alone_and_among_others(K, N):
     for M in (1, 16, 17, 33, 64, 65, 128, 129, 256, 257, 700):
         y = ops.linear_q8(Q8(x.values[:M], x.scale[:M]), w)
         assert torch.all((y.cpu().double() - want[:M]).abs() <= tol[:M]), M
+
+
+@gpu
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_sums_that_cancel_over_a_wide_range(kernel):
+    """Values over the whole of e4m3, the second half of K against the first but
+    for a few: the sums of magnitudes are 1e3 to 1e5 times the results."""
+    g = torch.Generator().manual_seed(6)
+
+    def wide(R, K):
+        v = torch.exp2(torch.randint(-9, 9, (R, K), generator=g).float()) * (1 + torch.randint(0, 8, (R, K), generator=g) / 8)
+        return (torch.where(torch.rand(R, K, generator=g) < 0.5, -v, v)).clamp(-448, 448)
+
+    M, K, N = 70, 4096, 264
+    x, w = wide(M, K), wide(N, K)
+    x[:, K // 2:] = x[:, : K // 2]
+    w[:, K // 2:] = -w[:, : K // 2] * torch.where(torch.rand(N, K // 2, generator=g) < 0.01, 0.5, 1.0)
+    x, w = (Q8(t.to(E4M3).cuda(), torch.ones(t.shape[0], device="cuda")) for t in (x, w))
+    want, tol = product64(x, w, None, None, False)
+    assert torch.all((raw(x, w, kernel=kernel).cpu().double() - want).abs() <= tol)
+
+
+@gpu
+@pytest.mark.parametrize("M,K,N", [(1, 256, 256), (40, 512, 384), (300, 128, 512), (1000, 256, 1024)])
+def test_results_are_there_for_the_kernel_behind(M, K, N):
+    """Every launch may start before the one ahead of it ends: what it reads has to be complete."""
+    xs = [q8_like(M, K, s, "cuda") for s in range(4)]
+    w, w2 = q8_like(N, K, 9, "cuda"), q8_like(256, N, 10, "cuda")
+    norm = torch.ones(256, dtype=torch.bfloat16, device="cuda")
+    y, q = torch.empty(M, N, dtype=torch.bfloat16, device="cuda"), ops.empty_q8(M, N, "cuda")
+    z, n = torch.empty(M, 256, dtype=torch.bfloat16, device="cuda"), ops.empty_q8(M, 256, "cuda")
+
+    def step(x, wait):
+        for f in (lambda: ops.linear_q8(x, w, out=y), lambda: ops.quantize_q8(y, out=q), lambda: ops.linear_q8(q, w2, out=z),
+                  lambda: ops.rmsnorm_q8(z, norm, 1e-6, out=n)):
+            f()
+            if wait:
+                torch.cuda.synchronize()
+        return n.values.view(torch.uint8).clone(), n.scale.clone()
+
+    want = [step(x, True) for x in xs]
+    for _ in range(50):
+        got = [step(x, False) for x in xs]
+        assert all(torch.equal(a, b) for g, t in zip(got, want) for a, b in zip(g, t))
