@@ -191,26 +191,31 @@ struct alignas(64) Maps {
 // 5.3 us for 5.1; 16 rows, 18944 -> 3584, 14.2 for 13.6.  Bulk copies from one CTA's
 // shared memory to another's in place of the stores: 5.2 and 13.9; 61 rows, 3584 ->
 // 3584, 7.6 for 7.0.)  That memory is beside the
-// ring, since the others may be done first; a lone CTA takes the ring.  With more
-// than 64 rows the partials of a cluster would cost more than they save (128 rows,
-// 3584 -> 4608: 7 of 10 us behind the last product), so those have lone CTAs.
+// ring, since the others may be done first; a lone CTA takes the ring.
+//
+// DEEP: one CTA a SM with a ring of 220 KB for two with 108 KB each.  Half as many
+// CTAs hold as many bytes on their way and read X half as often, and that is a third
+// of the reads of 64 rows.  61 rows, 18944 -> 3584: 15.4 us for 16.5 with two a SM;
+// 3584 -> 3584: 6.4 for 7.6.  128 rows: 18944 -> 3584 in clusters of four 21.2 us, for
+// 28.1 in pairs of CTAs on tiles of 64 features.
 constexpr int SPLIT_MAX_CLUSTER = 8;
-template <int BNX>
+constexpr int SPLIT_DEEP = 10;  // added to a cluster's size: the deep ring
+template <int BNX, bool DEEP>
 struct SplitCfg {
   static constexpr int W_BYTES = 128 * BK;
   static constexpr int X_BYTES = BNX * BK;
-  static constexpr int RECV_BYTES = BNX <= 64 ? (BNX + SPLIT_MAX_CLUSTER - 1) * 512 : 0;  // BNX 128: lone CTAs only
-  static constexpr int STAGES = (108 * 1024 - RECV_BYTES) / (W_BYTES + X_BYTES);          // two CTAs a SM
+  static constexpr int RECV_BYTES = BNX <= 64 || DEEP ? (BNX + SPLIT_MAX_CLUSTER - 1) * 512 : 0;  // else lone
+  static constexpr int STAGES = ((DEEP ? 220 : 108) * 1024 - RECV_BYTES) / (W_BYTES + X_BYTES);
   static constexpr int TMEM_COLS = BNX < 32 ? 32 : BNX;
   static constexpr int LD = 132;  // floats per row of a lone CTA's sums
   static constexpr int SMEM = STAGES * (W_BYTES + X_BYTES) + RECV_BYTES + 1024;
   static_assert(BNX * LD * 4 <= STAGES * (W_BYTES + X_BYTES), "the sums overlay the ring");
 };
 
-template <int BNX, bool SWIGLU>
-__global__ void __launch_bounds__(192, 2)
+template <int BNX, bool SWIGLU, bool DEEP>
+__global__ void __launch_bounds__(192, DEEP ? 1 : 2)
     q8_split_kernel(const __grid_constant__ Maps tm, const __grid_constant__ LLQ8Gemm p, int* err) {
-  using Cfg = SplitCfg<BNX>;
+  using Cfg = SplitCfg<BNX, DEEP>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(192, 2)
   pdl_wait();  // the scales and the residual are the previous kernel's; C may still be read by it
   // A thread keeps its four features (with SwiGLU four gate features and the
   // matching up features, 16 further on) over the rows of its share; what the
-  // epilogue reads of them, and its first row's residual, is on its way while the
+  // epilogue reads of them, and its first rows' residual, is on its way while the
   // product runs.
   constexpr int GROUPS = SWIGLU ? 16 : 32, PER = 192 / GROUPS;  // groups of four outputs a row, rows at once
   const int g = tid % GROUPS, f = SWIGLU ? (g >> 2) * 32 + (g & 3) * 4 : 4 * g;
@@ -320,7 +325,10 @@ __global__ void __launch_bounds__(192, 2)
                ? *reinterpret_cast<const uint2*>(p.residual + (m0 + row) * p.ldr + col)
                : make_uint2(0, 0);
   };
-  uint2 next = residual_at(row0);
+  constexpr int AHEAD = BNX / 16;  // residual rows on their way (one for 61 rows, 8192 -> 5120: 13.6 us; four 12.4)
+  uint2 next[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) next[i] = residual_at(row0 + i * PER);
   if (tid < rows) sxs[tid] = p.xs[m0 + tid];
   const bool ok = __syncthreads_and(mbar_wait(&tfull, 0, err, kErrTmemFullTimeout));
   tc_fence_after();
@@ -382,19 +390,23 @@ __global__ void __launch_bounds__(192, 2)
       return make_float4(fmaf(v.x * xs, ws[h].x, bias[h].x), fmaf(v.y * xs, ws[h].y, bias[h].y),
                          fmaf(v.z * xs, ws[h].z, bias[h].z), fmaf(v.w * xs, ws[h].w, bias[h].w));
     };
-#pragma unroll 2
-    for (int row = row0; row < end; row += PER) {
-      const uint2 rv = next;
-      next = residual_at(row + PER);
-      const float xs = sxs[row];
-      float4 v = sum4(row, xs, 0);
-      if constexpr (SWIGLU) {
-        const float4 u = sum4(row, xs, 1);
-        v = make_float4(silu(v.x) * u.x, silu(v.y) * u.y, silu(v.z) * u.z, silu(v.w) * u.w);
+    for (int base = row0; base < end; base += AHEAD * PER) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int row = base + i * PER;
+        if (row >= end) break;
+        const uint2 rv = next[i];
+        next[i] = residual_at(row + AHEAD * PER);
+        const float xs = sxs[row];
+        float4 v = sum4(row, xs, 0);
+        if constexpr (SWIGLU) {
+          const float4 u = sum4(row, xs, 1);
+          v = make_float4(silu(v.x) * u.x, silu(v.y) * u.y, silu(v.z) * u.z, silu(v.w) * u.w);
+        }
+        const float2 r0 = unpack_bf16x2(rv.x), r1 = unpack_bf16x2(rv.y);
+        *reinterpret_cast<uint2*>(p.C + (m0 + row) * p.ldc + col) =
+            make_uint2(pack_bf16x2(v.x + r0.x, v.y + r0.y), pack_bf16x2(v.z + r1.x, v.w + r1.y));
       }
-      const float2 r0 = unpack_bf16x2(rv.x), r1 = unpack_bf16x2(rv.y);
-      *reinterpret_cast<uint2*>(p.C + (m0 + row) * p.ldc + col) =
-          make_uint2(pack_bf16x2(v.x + r0.x, v.y + r0.y), pack_bf16x2(v.z + r1.x, v.w + r1.y));
     }
   }
   __syncwarp();
@@ -777,27 +789,49 @@ static int launch(Kern kern, dim3 grid, int smem, int cluster, cudaStream_t stre
   return cudaLaunchKernelEx(&cfg, kern, tm, p, err) == cudaSuccess ? 0 : -5;
 }
 
-// CTAs that share a feature tile's K, for up to 64 rows: as many as have places,
-// two a SM (larger clusters than pairs do not fill the SMs to the last place), with
-// three k-blocks each or more; two for more tiles than places, whose last round
-// would be a long one.  Over 760 random sizes (1 to 64 rows) 1 % slower than the
-// best of 1 to 8 CTAs in the geometric mean (2 % with two k-blocks each and without
-// the second rule).
+// CTAs that share a feature tile's K, two a SM: as many as have places (larger
+// clusters than pairs do not fill the SMs to the last place), with three k-blocks
+// each or more; two for more tiles than places, whose last round would be a long
+// one.  Over 760 random sizes (1 to 64 rows) 1 % slower than the best of 1 to 8 CTAs
+// in the geometric mean (2 % with two k-blocks each and without the second rule).
 constexpr int SPLIT_PLACES = 248, SPLIT_ROUND = 296;
-static int split_rule(int N, int K) {
-  const int tiles = (N + 127) / 128, num_kb = (K + BK - 1) / BK;
+static int split_rule(int tiles, int num_kb) {
   int cs = SPLIT_PLACES / tiles;
   if ((tiles > SPLIT_PLACES / 2 && tiles <= SPLIT_ROUND / 2) || (tiles > SPLIT_ROUND && num_kb >= 64)) cs = 2;
   cs = cs < num_kb / 3 ? cs : num_kb / 3;
   return cs < 1 ? 1 : (cs > SPLIT_MAX_CLUSTER ? SPLIT_MAX_CLUSTER : cs);
 }
 
+// The same with one CTA a SM: the largest cluster with which all tiles run at once
+// and every CTA has three k-blocks; 0 for more tiles than SMs.  The places are what
+// the occupancy calculator gives clusters of each size: they lie within a GPC, whose
+// SMs clusters of seven and eight do not fill.
+static int deep_rule(int64_t tiles, int num_kb) {
+  constexpr int places[SPLIT_MAX_CLUSTER + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+  for (int cs = SPLIT_MAX_CLUSTER; cs >= 1; --cs)
+    if (tiles * cs <= places[cs] && (cs == 1 || num_kb >= 3 * cs)) return cs;
+  return 0;
+}
+
+// The kernel for 33 to 64 rows.  Up to 74 feature tiles, half the SMs, the deep ring
+// (with more it loses as often as it wins); of those the few and short pairs of CTAs,
+// whose epilogue has twice the warps (61 rows, 512 -> 1024: 3.5 us for 4.4).  Over
+// 1134 random sizes 1.1 % slower than the best of all; without the pairs 2.0 %, without
+// the deep ring too 8 %.
+static int middle_rule(int N, int K) {
+  const int tiles = (N + 127) / 128, num_kb = (K + BK - 1) / BK;
+  if (tiles > 74) return split_rule(tiles, num_kb);
+  return tiles <= 24 && num_kb <= 4 ? 64 : SPLIT_DEEP + deep_rule(tiles, num_kb);
+}
+
 // The kernel for more than 64 rows: the one with the least modelled time, a start
 // and then, for each round of tiles, the k-blocks and the part of the epilogue that
-// the next tile does not hide.  The figures (us) are fitted to 2033 random sizes (65
-// to 5000 rows) timed with every kernel: what it picks is 0.3 % slower than the
-// best of the four in the geometric mean; tiles of 64, 128 or 256 features
-// alone would be 32, 12 and 23 % slower, the split kernel 57 %.
+// the next tile does not hide; for the deep split kernel a CTA's k-blocks, and the
+// partials by rows and by CTAs.  The figures (us) are fitted to 2033 random sizes (65
+// to 5000 rows) timed with every kernel but that one, 0.3 % slower than the best in
+// the geometric mean (tiles of 64, 128 or 256 features alone 32, 12 and 23 %), and to
+// 525 sizes (65 to 160 rows) with it; over 861 others 0.3 % slower than the best (over the
+// 525 0.7 %, and 14 % without it).
 static int kernel_rule(int M, int N, int K, int sms) {
   struct Cost {
     int kernel, tile_rows, tile_features, places;
@@ -819,26 +853,35 @@ static int kernel_rule(int M, int N, int K, int sms) {
       least = t;
     }
   }
+  const int cs = deep_rule((int64_t)((M + 127) / 128) * ((N + 127) / 128), num_kb);
+  if (cs > 0) {
+    const double t = 2.3 + (num_kb + cs - 1) / cs * 0.15 + 4.7 * (M < 128 ? M : 128) / 128 + 0.07 * cs;
+    if (t < least) best = SPLIT_DEEP + cs;
+  }
   return best;
 }
 
-template <bool SWIGLU>
-static int split_launch(const LLQ8Gemm& p, int cs, int* err, cudaStream_t stream) {
-  const int bnx = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
-  if (bnx > 64) cs = 1;
-  else if (cs <= 0) cs = split_rule(p.N, p.K);
+template <int BNX, bool SWIGLU, bool DEEP = false>
+static int split_run(const LLQ8Gemm& p, int cs, int* err, cudaStream_t stream) {
   Maps tm;
-  if (!operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) || !operand_map(&tm.x, p.x, p.M, p.K, p.ldx, bnx)) return -2;
+  if (!operand_map(&tm.w, p.w, p.N, p.K, p.ldw, 128) || !operand_map(&tm.x, p.x, p.M, p.K, p.ldx, BNX)) return -2;
   tm.c = tm.r = tm.x;  // not read
-  const dim3 grid(cs, (p.N + 127) / 128, (p.M + bnx - 1) / bnx);
+  const dim3 grid(cs, (p.N + 127) / 128, (p.M + BNX - 1) / BNX);
   if (grid.y > 65535 || grid.z > 65535) return -3;
-  static unsigned long long done[4] = {0, 0, 0, 0};
-  switch (bnx) {
-    case 16: return launch(q8_split_kernel<16, SWIGLU>, grid, SplitCfg<16>::SMEM, cs, stream, done[0], tm, p, err);
-    case 32: return launch(q8_split_kernel<32, SWIGLU>, grid, SplitCfg<32>::SMEM, cs, stream, done[1], tm, p, err);
-    case 64: return launch(q8_split_kernel<64, SWIGLU>, grid, SplitCfg<64>::SMEM, cs, stream, done[2], tm, p, err);
-    default: return launch(q8_split_kernel<128, SWIGLU>, grid, SplitCfg<128>::SMEM, cs, stream, done[3], tm, p, err);
-  }
+  static unsigned long long done = 0;
+  return launch(q8_split_kernel<BNX, SWIGLU, DEEP>, grid, SplitCfg<BNX, DEEP>::SMEM, cs, stream, done, tm, p, err);
+}
+template <bool SWIGLU>
+static int split_launch(const LLQ8Gemm& p, int kernel, int* err, cudaStream_t stream) {
+  const int tiles = (p.N + 127) / 128, num_kb = (p.K + BK - 1) / BK;
+  const bool deep = kernel > SPLIT_DEEP;
+  const int cs = deep ? kernel - SPLIT_DEEP : (p.M > 64 ? 1 : (kernel > 0 ? kernel : split_rule(tiles, num_kb)));
+  if (deep && p.M > 64) return split_run<128, SWIGLU, true>(p, cs, err, stream);
+  if (deep) return split_run<64, SWIGLU, true>(p, cs, err, stream);
+  if (p.M > 64) return split_run<128, SWIGLU>(p, cs, err, stream);
+  if (p.M <= 16) return split_run<16, SWIGLU>(p, cs, err, stream);
+  if (p.M <= 32) return split_run<32, SWIGLU>(p, cs, err, stream);
+  return split_run<64, SWIGLU>(p, cs, err, stream);
 }
 
 template <int BN, bool SWIGLU>
@@ -870,8 +913,8 @@ static int pair_launch(const LLQ8Gemm& p, int sms, int* err, cudaStream_t stream
 }  // namespace ll
 
 // `kernel`: 0 by the rule below; 1 to 8 the split kernel with that many CTAs to a
-// feature tile (of one where there are more than 64 rows a tile); 64, 128 or 256
-// the pair kernel with tiles of so many features.
+// feature tile (of one where there are more than 64 rows), 11 to 18 the same with the
+// deep ring and 1 to 8; 64, 128 or 256 the pair kernel with tiles of so many features.
 extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, cudaStream_t stream) {
   using namespace ll::q8;
   if (p->M <= 0) return 0;
@@ -882,10 +925,13 @@ extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, c
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return -5;
   if (kernel == 0 && p->M > 64) kernel = kernel_rule(p->M, p->N, p->K, sms);
+  else if (kernel == 0 && p->M > 32) kernel = middle_rule(p->N, p->K);
   if (kernel <= SPLIT_MAX_CLUSTER && p->N > 128 * 65535) kernel = 256;  // more feature tiles than a grid has places
   const auto run = [&](auto gated) {
     constexpr bool G = decltype(gated)::value;
-    if (kernel >= 0 && kernel <= SPLIT_MAX_CLUSTER) return split_launch<G>(*p, kernel, err, stream);
+    if ((kernel >= 0 && kernel <= SPLIT_MAX_CLUSTER) ||
+        (kernel > SPLIT_DEEP && kernel <= SPLIT_DEEP + SPLIT_MAX_CLUSTER))
+      return split_launch<G>(*p, kernel, err, stream);
     if (kernel == 64) return pair_launch<64, G>(*p, sms, err, stream);
     if (kernel == 128) return pair_launch<128, G>(*p, sms, err, stream);
     if (kernel == 256) return pair_launch<256, G>(*p, sms, err, stream);

@@ -246,7 +246,7 @@ def test_norm_of_extreme_rows(K):
 
 def raw(x, w, bias=None, residual=None, swiglu=False, kernel=0):
     """The product by a named kernel (64, 128, 256: pairs of CTAs on tiles of so many
-    features; up to 8: as many CTAs to a feature tile)."""
+    features; up to 8: as many CTAs to a feature tile; 11 to 18: the same, one to a SM)."""
     M, N = x.values.shape[0], w.values.shape[0]
     out = torch.full((M + 2, N // 2 if swiglu else N), 3.0, dtype=torch.bfloat16, device="cuda")
     ops._cuda().q8_linear(x.values, x.scale, w.values, w.scale, bias, residual, out[:M], swiglu, kernel,
@@ -255,7 +255,7 @@ def raw(x, w, bias=None, residual=None, swiglu=False, kernel=0):
     return out[:M]
 
 
-KERNELS = [256, 128, 64, 1, 2, 3, 8]
+KERNELS = [256, 128, 64, 1, 2, 3, 8, 11, 13, 18]
 
 
 @gpu
