@@ -821,7 +821,7 @@ static int deep_rule(int64_t tiles, int num_kb) {
 static int middle_rule(int N, int K) {
   const int tiles = (N + 127) / 128, num_kb = (K + BK - 1) / BK;
   if (tiles > 74) return split_rule(tiles, num_kb);
-  return tiles <= 24 && num_kb <= 4 ? 64 : SPLIT_DEEP + deep_rule(tiles, num_kb);
+  return tiles <= 16 && num_kb <= 4 ? 64 : SPLIT_DEEP + deep_rule(tiles, num_kb);
 }
 
 // The kernel for more than 64 rows: the one with the least modelled time, a start
