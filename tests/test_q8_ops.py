@@ -244,6 +244,31 @@ def test_norm_of_extreme_rows(K):
     assert bool(s.scale[4:].isnan().all())
 
 
+@gpu
+@pytest.mark.parametrize("M,K", [(5000, 1040), (2600, 2048), (1400, 3584), (640, 8192)])
+def test_many_rows(M, K):
+    """More rows than have places at once, some of them extreme: the same bits
+    as the statement, and norms as far from 64 bits as those of few rows."""
+    x, r = rows_like(M, K, 4), rows_like(M, K, 5)
+    x[7], r[7] = 0, 0
+    x[8], r[8] = x[8] * 1e30, r[8] * 1e30
+    x[9], r[9] = x[9] * 1e-38, r[9] * 1e-38
+    x[M - 3, 0], x[M - 2, K // 2], x[M - 1, K - 1] = math.inf, math.nan, -math.inf
+    w = (1 + 0.1 * torch.randn(K, generator=torch.Generator().manual_seed(6))).to(torch.bfloat16)
+    ok = slice(0, M - 3)
+    got, want = ops.quantize_q8(x.cuda()), ops.quantize_q8(x)
+    assert torch.equal(got.scale[ok].cpu(), want.scale[ok]) and bool(got.scale[M - 3:].isnan().all())
+    assert torch.equal(got.values[ok].cpu().view(torch.uint8), want.values[ok].view(torch.uint8))
+    got = ops.rmsnorm_q8(x.cuda(), w.cuda(), 1e-6)
+    check_rows_q8(Q8(got.values[ok], got.scale[ok]), norm64(x[ok], w, 1e-6)[0], 2e-5)
+    assert bool(got.scale[M - 3:].isnan().all())
+    y, s = norm64(x[ok], w, 1e-6, r[ok])
+    total = r.cuda()
+    got = ops.fused_add_rmsnorm_q8(x.cuda(), total, w.cuda(), 1e-6)
+    check_rows_q8(Q8(got.values[ok], got.scale[ok]), y, 2e-5)
+    assert torch.equal(total[ok].cpu(), s.to(torch.bfloat16)) and bool(got.scale[M - 3:].isnan().all())
+
+
 def raw(x, w, bias=None, residual=None, swiglu=False, kernel=0):
     """The product by a named kernel (64, 128, 256: pairs of CTAs on tiles of so many
     features; up to 8: as many CTAs to a feature tile; 11 to 18: the same, one to a SM)."""
