@@ -36,8 +36,16 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+// A store of 16 bytes that the barrier `bar`, of the same CTA as `addr`, counts as they arrive.
+__device__ __forceinline__ void st_async(uint32_t addr, float4 v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr),
+               "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)),
+               "r"(__float_as_uint(v.w)), "r"(bar)
+               : "memory");
+}
+// Says that this CTA's stores are issued; orders nothing.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -184,32 +192,48 @@ struct alignas(64) Maps {
 // the k-blocks.  Bound by reading W: every CTA's first ring of weights is on its
 // way to L2 before the wait for the kernel ahead.  grid (cluster, feature tiles, row tiles).
 //
-// CTA o of a cluster sums and stores rows [o R, (o + 1) R): the others write their
-// partials of those rows into its shared memory as they read them from tensor
-// memory, and one cluster barrier later they are there.  (Partials that stay where
-// they are, read behind one barrier and kept alive by a second: 1 row, 3584 -> 4608,
-// 5.3 us for 5.1; 16 rows, 18944 -> 3584, 14.2 for 13.6.  Bulk copies from one CTA's
-// shared memory to another's in place of the stores: 5.2 and 13.9; 61 rows, 3584 ->
-// 3584, 7.6 for 7.0.)  That memory is beside the
-// ring, since the others may be done first; a lone CTA takes the ring.
+// Each CTA of a cluster sums and stores a share of the groups of four rows.  The others
+// send it their partials of them as they read them from tensor memory, 16 bytes (four
+// rows of a feature) a thread, by stores that its barrier counts: no barrier of the
+// cluster is waited for until everything is stored.  (Four bytes a store and one
+// cluster barrier behind them, us: 1 row, 3584 -> 3584, 4.4 for 4.0; 32 rows 5.6 for 4.6; 61
+// rows, 8192 -> 5120, 11.8 for 11.0; counted stores of four bytes 3.9, 5.5 and 13.0.
+// Before that, partials that stay where they are, read behind one barrier: 16 rows, 18944 ->
+// 3584, 14.2 for 13.6; bulk copies between shared memories 13.9.)  They have memory of
+// their own beside the ring, since the others may be done first; a lone CTA's take the ring.
+//
+// The epilogue's code is met cold by every CTA, so its loop is not unrolled (twice: 61 rows,
+// 8192 -> 5120, 11.2 us for 11.0), and scales and bias are fetched by the warps that wait for
+// the product: fetched by all six, the two that feed it come late (1 row, 512 -> 1024, 3.1 us
+// for 2.9).
 //
 // DEEP: one CTA a SM with a ring of 220 KB for two with 108 KB each.  Half as many
 // CTAs hold as many bytes on their way and read X half as often, and that is a third
 // of the reads of 64 rows.  61 rows, 18944 -> 3584: 15.4 us for 16.5 with two a SM;
-// 3584 -> 3584: 6.4 for 7.6.  128 rows: 18944 -> 3584 in clusters of four 21.2 us, for
-// 28.1 in pairs of CTAs on tiles of 64 features.
+// 3584 -> 3584: 6.4 for 7.6 (now 14.6 and 5.3).  128 rows: 18944 -> 3584 in clusters of
+// four 19.7 us, for 28.1 in pairs of CTAs on tiles of 64 features.
 constexpr int SPLIT_MAX_CLUSTER = 8;
 constexpr int SPLIT_DEEP = 10;  // added to a cluster's size: the deep ring
 template <int BNX, bool DEEP>
 struct SplitCfg {
   static constexpr int W_BYTES = 128 * BK;
   static constexpr int X_BYTES = BNX * BK;
-  static constexpr int RECV_BYTES = BNX <= 64 || DEEP ? (BNX + SPLIT_MAX_CLUSTER - 1) * 512 : 0;  // else lone
+  static constexpr int MAX_CLUSTER = DEEP || BNX < 64 ? SPLIT_MAX_CLUSTER : (BNX == 64 ? 3 : 1);
+  // partials: for each CTA of the cluster its share of the groups of four rows, 128 features each
+  static constexpr int recv_groups() {
+    int most = 0;
+    for (int cs = 2; cs <= MAX_CLUSTER; ++cs) {
+      const int n = cs * ((BNX + 4 * cs - 1) / (4 * cs));
+      most = n > most ? n : most;
+    }
+    return most;
+  }
+  static constexpr int GROUP_BYTES = 4 * 128 * 4;
+  static constexpr int RECV_BYTES = recv_groups() * GROUP_BYTES;
   static constexpr int STAGES = ((DEEP ? 220 : 108) * 1024 - RECV_BYTES) / (W_BYTES + X_BYTES);
   static constexpr int TMEM_COLS = BNX < 32 ? 32 : BNX;
-  static constexpr int LD = 132;  // floats per row of a lone CTA's sums
   static constexpr int SMEM = STAGES * (W_BYTES + X_BYTES) + RECV_BYTES + 1024;
-  static_assert(BNX * LD * 4 <= STAGES * (W_BYTES + X_BYTES), "the sums overlay the ring");
+  static_assert(BNX / 4 * GROUP_BYTES <= STAGES * (W_BYTES + X_BYTES), "a lone CTA's sums overlay the ring");
 };
 
 template <int BNX, bool SWIGLU, bool DEEP>
@@ -221,22 +245,30 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sX = smem + STAGES * Cfg::W_BYTES;
-  float* part = reinterpret_cast<float*>(smem);  // a lone CTA: [rows][LD], over the ring, once the product is done
-  const float* recv = reinterpret_cast<const float*>(smem + STAGES * (Cfg::W_BYTES + Cfg::X_BYTES));  // [cs][R][128]
-  __shared__ uint64_t full[STAGES], empty[STAGES], tfull;
+  __shared__ uint64_t full[STAGES], empty[STAGES], tfull, rfull;  // rfull: the other CTAs' partials
   __shared__ uint32_t tmem_slot;
-  __shared__ float sxs[BNX];
+  __shared__ __align__(16) float sxs[BNX];
+  __shared__ float2 scol[128];  // scale and bias of a feature
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int cs = gridDim.x, crank = blockIdx.x, nb = blockIdx.y;
   const int num_kb = (p.K + BK - 1) / BK, per = (num_kb + cs - 1) / cs;
   const int kb0 = min(num_kb, crank * per), kb1 = min(num_kb, kb0 + per);
   const int m0 = blockIdx.z * BNX, rows = min(BNX, p.M - m0);
+  // groups of four rows: all of them, a CTA's share, this CTA's first one and number
+  const int groups = (rows + 3) / 4, share = (groups + cs - 1) / cs;
+  const int first = min(groups, crank * share), mine = min(groups - first, share);
+  // partials [cs][share][128 features][4 rows]; a lone CTA's lie over the ring, once the product is done
+  float4* part = reinterpret_cast<float4*>(cs > 1 ? smem + STAGES * (Cfg::W_BYTES + Cfg::X_BYTES) : smem);
   pdl_trigger();
 
   if (tid <= 2 * STAGES) {
     mbar_init(tid == 2 * STAGES ? &tfull : (tid < STAGES ? &full[tid] : &empty[tid - STAGES]), 1);
     fence_mbar_init();
+  } else if (tid == 2 * STAGES + 1) {
+    mbar_init(&rfull, 1);
+    fence_mbar_init();
+    mbar_arrive_expect_tx(&rfull, Cfg::GROUP_BYTES * mine * (cs - 1));
   }
   __syncwarp();
   if (warp == 1) tmem_alloc(&tmem_slot, Cfg::TMEM_COLS);
@@ -299,118 +331,127 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
   }
   __syncwarp();
   pdl_wait();  // the scales and the residual are the previous kernel's; C may still be read by it
-  // A thread keeps its four features (with SwiGLU four gate features and the
-  // matching up features, 16 further on) over the rows of its share; what the
-  // epilogue reads of them, and its first rows' residual, is on its way while the
-  // product runs.
-  constexpr int GROUPS = SWIGLU ? 16 : 32, PER = 192 / GROUPS;  // groups of four outputs a row, rows at once
-  const int g = tid % GROUPS, f = SWIGLU ? (g >> 2) * 32 + (g & 3) * 4 : 4 * g;
-  const int col = SWIGLU ? nb * 64 + 4 * g : nb * 128 + f;
-  const bool live = nb * 128 + f < p.N;
-  const int R = (rows + cs - 1) / cs, first = min(rows, crank * R), end = min(rows, first + R);  // this CTA's rows
-  const int row0 = first + tid / GROUPS;
-  float4 ws[2] = {}, bias[2] = {};
-#pragma unroll
-  for (int h = 0; h < (SWIGLU ? 2 : 1); ++h) {
-    if (!live) break;
-    ws[h] = *reinterpret_cast<const float4*>(p.ws + nb * 128 + f + 16 * h);
-    if (p.bias != nullptr) {
-      const uint2 b = *reinterpret_cast<const uint2*>(p.bias + nb * 128 + f + 16 * h);
-      const float2 b0 = unpack_bf16x2(b.x), b1 = unpack_bf16x2(b.y);
-      bias[h] = make_float4(b0.x, b0.y, b1.x, b1.y);
-    }
-  }
-  auto residual_at = [&](int row) {
-    return p.residual != nullptr && live && row < end
-               ? *reinterpret_cast<const uint2*>(p.residual + (m0 + row) * p.ldr + col)
-               : make_uint2(0, 0);
+  // A warp's turn is four rows of 32 features, a feature a lane; two lanes then trade,
+  // so that each has two rows of two features (with SwiGLU of a gate and its up, 16 further
+  // on).  What the epilogue reads is fetched while the product runs, by the warps that
+  // have nothing else to do, which also have the first turns.
+  const int turns = mine * 4, turn0 = (warp + 4) % 6;  // of the CTA; this warp's first one
+  const bool high = SWIGLU ? lane >= 16 : lane & 1;     // has the last two rows
+  // of a turn: this lane's first row and column of C
+  auto row_of = [&](int turn) { return (first + (turn >> 2)) * 4 + (high ? 2 : 0); };
+  auto col_of = [&](int turn) {
+    return SWIGLU ? nb * 64 + (turn & 3) * 16 + (lane & 15) : nb * 128 + (turn & 3) * 32 + (lane & ~1);
   };
-  constexpr int AHEAD = BNX / 16;  // residual rows on their way (one for 61 rows, 8192 -> 5120: 13.6 us; four 12.4)
-  uint2 next[AHEAD];
+  const int cols = SWIGLU ? p.N / 2 : p.N;
+  auto residual_at = [&](int turn, int i) -> uint32_t {
+    const int row = row_of(turn) + i, col = col_of(turn);
+    if (p.residual == nullptr || turn >= turns || row >= rows || col >= cols) return 0;
+    const __nv_bfloat16* at = p.residual + (m0 + row) * p.ldr + col;
+    return SWIGLU ? *reinterpret_cast<const uint16_t*>(at) : *reinterpret_cast<const uint32_t*>(at);
+  };
+  constexpr int AHEAD = BNX / 16;  // turns (one for 61 rows, 8192 -> 5120: 13.6 us; four 12.4)
+  uint32_t next[AHEAD][2];
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) next[i] = residual_at(row0 + i * PER);
-  if (tid < rows) sxs[tid] = p.xs[m0 + tid];
-  const bool ok = __syncthreads_and(mbar_wait(&tfull, 0, err, kErrTmemFullTimeout));
+  for (int i = 0; i < AHEAD; ++i) {
+    next[i][0] = residual_at(turn0 + 6 * i, 0);
+    next[i][1] = residual_at(turn0 + 6 * i, 1);
+  }
+  if (warp >= 2) {
+    const int i = tid - 64, n = nb * 128 + i;
+    if (i < BNX) sxs[i] = i < rows ? p.xs[m0 + i] : 0.f;
+    const float bias = p.bias != nullptr && n < p.N ? __bfloat162float(p.bias[n]) : 0.f;
+    scol[i] = make_float2(n < p.N ? p.ws[n] : 0.f, bias);
+  }
+  const bool done = mbar_wait(&tfull, 0, err, kErrTmemFullTimeout);
   tc_fence_after();
   if (cs > 1) cluster_barrier_wait();
   if (warp >= 2) {  // TMEM lane quarter of this warp: features; columns: rows
     const int feat = (warp & 3) * 32 + lane;
     const bool none = kb1 <= kb0;
-    int owner = 0, left = R;  // rows that are still the owner's
-    uint32_t to = mapa(smem_u32(recv), 0) + 4u * (crank * R * 128 + feat);
+    float4* slot = part + crank * share * 128 + feat;  // of this CTA, in every CTA
+    const uint32_t slot_addr = smem_u32(slot), bar_addr = smem_u32(&rfull);
+    int owner = 0, left = share;  // groups that are still the owner's
+    uint32_t to = mapa(slot_addr, 0), bar = mapa(bar_addr, 0);
 #pragma unroll 1
     for (int c = 0; c < BNX && c < rows; c += 32) {
       uint32_t r[32];
       tmem_ld_32x32b_x32(tmem + (uint32_t((warp & 3) * 32) << 16) + c, r);  // BNX 16: columns 16.. unused
       tmem_ld_wait();
       constexpr int COLS = BNX < 32 ? BNX : 32;
-      if (cs > 1) {
 #pragma unroll
-        for (int i = 0; i < COLS; ++i) {
-          if (c + i >= rows) break;
-          st_cluster(to, none ? 0.f : __uint_as_float(r[i]));
-          to += 512;
-          if (--left == 0) {
-            ++owner;
-            left = R;
-            to = mapa(smem_u32(recv), min(owner, cs - 1)) + 4u * (crank * R * 128 + feat);
-          }
+      for (int i = 0; i < COLS; i += 4) {
+        if (c + i >= rows) break;
+        float4 v = make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]),
+                               __uint_as_float(r[i + 3]));
+        if (none) v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (owner == crank) slot[(share - left) * 128] = v;
+        else st_async(to + (share - left) * Cfg::GROUP_BYTES, v, bar);
+        if (--left == 0) {
+          ++owner;
+          left = share;
+          to = mapa(slot_addr, min(owner, cs - 1));
+          bar = mapa(bar_addr, min(owner, cs - 1));
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < COLS; ++i)
-          if (c + i < rows) part[(c + i) * Cfg::LD + feat] = none ? 0.f : __uint_as_float(r[i]);
       }
     }
   }
   __syncwarp();
+  if (cs > 1) cluster_arrive_relaxed();
+  const bool received = cs == 1 || mbar_wait(&rfull, 0, err, kErrSmemEmptyTimeout);
   tc_fence_before();
-  if (cs > 1) cluster_sync();
-  else __syncthreads();
+  const bool ok = __syncthreads_and(done && received);
   tc_fence_after();
-  if (ok && live) {
-    // four features of a row: the partials in split order, scales, bias
-    auto sum4 = [&](int row, float xs, int h) {
-      float4 v;
-      if (cs > 1) {
-        const float* at = recv + (row - first) * 128 + f + 16 * h;
-        v = *reinterpret_cast<const float4*>(at);
+  if (ok) {
+#pragma unroll 1
+    for (int turn = turn0; turn < turns; turn += 6) {
+      const uint32_t r0 = next[0][0], r1 = next[0][1];
+      if (p.residual != nullptr) {
 #pragma unroll
-        for (int r = 1; r < SPLIT_MAX_CLUSTER; ++r) {
-          if (r >= cs) break;
-          const float4 t = *reinterpret_cast<const float4*>(at + r * R * 128);
-          v.x += t.x;
-          v.y += t.y;
-          v.z += t.z;
-          v.w += t.w;
+        for (int i = 0; i + 1 < AHEAD; ++i) {
+          next[i][0] = next[i + 1][0];
+          next[i][1] = next[i + 1][1];
         }
-      } else {
-        v = *reinterpret_cast<const float4*>(part + row * Cfg::LD + f + 16 * h);
+        next[AHEAD - 1][0] = residual_at(turn + 6 * AHEAD, 0);
+        next[AHEAD - 1][1] = residual_at(turn + 6 * AHEAD, 1);
       }
-      return make_float4(fmaf(v.x * xs, ws[h].x, bias[h].x), fmaf(v.y * xs, ws[h].y, bias[h].y),
-                         fmaf(v.z * xs, ws[h].z, bias[h].z), fmaf(v.w * xs, ws[h].w, bias[h].w));
-    };
-    for (int base = row0; base < end; base += AHEAD * PER) {
+      // the partials in split order, scales, bias
+      const float4* at = part + turn * 32 + lane;
+      float4 v = *at;
+      if (cs > 1) {
+        float4 t[Cfg::MAX_CLUSTER];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int row = base + i * PER;
-        if (row >= end) break;
-        const uint2 rv = next[i];
-        next[i] = residual_at(row + AHEAD * PER);
-        const float xs = sxs[row];
-        float4 v = sum4(row, xs, 0);
-        if constexpr (SWIGLU) {
-          const float4 u = sum4(row, xs, 1);
-          v = make_float4(silu(v.x) * u.x, silu(v.y) * u.y, silu(v.z) * u.z, silu(v.w) * u.w);
-        }
-        const float2 r0 = unpack_bf16x2(rv.x), r1 = unpack_bf16x2(rv.y);
-        *reinterpret_cast<uint2*>(p.C + (m0 + row) * p.ldc + col) =
-            make_uint2(pack_bf16x2(v.x + r0.x, v.y + r0.y), pack_bf16x2(v.z + r1.x, v.w + r1.y));
+        for (int r = 1; r < Cfg::MAX_CLUSTER; ++r)
+          t[r] = r < cs ? at[r * share * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 1; r < Cfg::MAX_CLUSTER; ++r)
+          v = make_float4(v.x + t[r].x, v.y + t[r].y, v.z + t[r].z, v.w + t[r].w);
+      }
+      const float2 s = scol[(turn & 3) * 32 + lane];
+      const float4 xs = *reinterpret_cast<const float4*>(sxs + (first + (turn >> 2)) * 4);
+      v = make_float4(fmaf(v.x * xs.x, s.x, s.y), fmaf(v.y * xs.y, s.x, s.y), fmaf(v.z * xs.z, s.x, s.y),
+                      fmaf(v.w * xs.w, s.x, s.y));
+      const float a0 = __shfl_xor_sync(0xffffffffu, high ? v.x : v.z, SWIGLU ? 16 : 1);
+      const float a1 = __shfl_xor_sync(0xffffffffu, high ? v.y : v.w, SWIGLU ? 16 : 1);
+      const int row = row_of(turn), col = col_of(turn);
+      const bool one = col < cols && row < rows, two = col < cols && row + 1 < rows;
+      __nv_bfloat16* c = p.C + (m0 + row) * p.ldc + col;
+      if constexpr (SWIGLU) {
+        const float y0 = high ? silu(a0) * v.z : silu(v.x) * a0, y1 = high ? silu(a1) * v.w : silu(v.y) * a1;
+        if (one) c[0] = __float2bfloat16_rn(y0 + __uint_as_float(r0 << 16));
+        if (two) c[p.ldc] = __float2bfloat16_rn(y1 + __uint_as_float(r1 << 16));
+      } else {
+        const float2 f0 = unpack_bf16x2(r0), f1 = unpack_bf16x2(r1);
+        const float2 y0 = high ? make_float2(a0, v.z) : make_float2(v.x, a0);
+        const float2 y1 = high ? make_float2(a1, v.w) : make_float2(v.y, a1);
+        if (one) *reinterpret_cast<uint32_t*>(c) = pack_bf16x2(y0.x + f0.x, y0.y + f0.y);
+        if (two) *reinterpret_cast<uint32_t*>(c + p.ldc) = pack_bf16x2(y1.x + f1.x, y1.y + f1.y);
       }
     }
   }
+  if (!received) linger();
   __syncwarp();
   if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);  // every read of it is behind the barrier
+  if (cs > 1) cluster_barrier_wait();  // no CTA leaves before the others' stores to it are issued
 }
 
 // ---------------------------------------------------------------------------
@@ -875,7 +916,11 @@ template <bool SWIGLU>
 static int split_launch(const LLQ8Gemm& p, int kernel, int* err, cudaStream_t stream) {
   const int tiles = (p.N + 127) / 128, num_kb = (p.K + BK - 1) / BK;
   const bool deep = kernel > SPLIT_DEEP;
-  const int cs = deep ? kernel - SPLIT_DEEP : (p.M > 64 ? 1 : (kernel > 0 ? kernel : split_rule(tiles, num_kb)));
+  int cs = deep ? kernel - SPLIT_DEEP : (kernel > 0 ? kernel : split_rule(tiles, num_kb));
+  if (!deep && p.M > 32) {
+    const int most = p.M > 64 ? SplitCfg<128, false>::MAX_CLUSTER : SplitCfg<64, false>::MAX_CLUSTER;
+    cs = cs < most ? cs : most;
+  }
   if (deep && p.M > 64) return split_run<128, SWIGLU, true>(p, cs, err, stream);
   if (deep) return split_run<64, SWIGLU, true>(p, cs, err, stream);
   if (p.M > 64) return split_run<128, SWIGLU>(p, cs, err, stream);
@@ -913,8 +958,9 @@ static int pair_launch(const LLQ8Gemm& p, int sms, int* err, cudaStream_t stream
 }  // namespace ll
 
 // `kernel`: 0 by the rule below; 1 to 8 the split kernel with that many CTAs to a
-// feature tile (of one where there are more than 64 rows), 11 to 18 the same with the
-// deep ring and 1 to 8; 64, 128 or 256 the pair kernel with tiles of so many features.
+// feature tile (at most three for more than 32 rows, one for more than 64), 11 to 18
+// the same with the deep ring and 1 to 8; 64, 128 or 256 the pair kernel with tiles of so
+// many features.
 extern "C" int ll_q8_gemm(const LLQ8Gemm* p, int swiglu, int kernel, int* err, cudaStream_t stream) {
   using namespace ll::q8;
   if (p->M <= 0) return 0;
