@@ -830,49 +830,43 @@ static int launch(Kern kern, dim3 grid, int smem, int cluster, cudaStream_t stre
   return cudaLaunchKernelEx(&cfg, kern, tm, p, err) == cudaSuccess ? 0 : -5;
 }
 
-// CTAs that share a feature tile's K, two a SM: as many as have places (larger
-// clusters than pairs do not fill the SMs to the last place), with three k-blocks
-// each or more; two for more tiles than places, whose last round would be a long
-// one.  Over 760 random sizes (1 to 64 rows) 1 % slower than the best of 1 to 8 CTAs
-// in the geometric mean (2 % with two k-blocks each and without the second rule).
+// CTAs that share a feature tile's K, two a SM: as many as have places (larger clusters
+// than pairs do not fill the SMs to the last place), also where K is shorter than
+// that, since they share the epilogue too; two for more tiles than places, whose last
+// round would be a long one.  Over 1133 random sizes (1 to 32 rows, behind their
+// quantisation) 1.0 % slower than the best of 1 to 8 CTAs in the geometric mean.
 constexpr int SPLIT_PLACES = 248, SPLIT_ROUND = 296;
 static int split_rule(int tiles, int num_kb) {
   int cs = SPLIT_PLACES / tiles;
   if ((tiles > SPLIT_PLACES / 2 && tiles <= SPLIT_ROUND / 2) || (tiles > SPLIT_ROUND && num_kb >= 64)) cs = 2;
-  cs = cs < num_kb / 3 ? cs : num_kb / 3;
   return cs < 1 ? 1 : (cs > SPLIT_MAX_CLUSTER ? SPLIT_MAX_CLUSTER : cs);
 }
 
-// The same with one CTA a SM: the largest cluster with which all tiles run at once
-// and every CTA has three k-blocks; 0 for more tiles than SMs.  The places are what
-// the occupancy calculator gives clusters of each size: they lie within a GPC, whose
-// SMs clusters of seven and eight do not fill.
-static int deep_rule(int64_t tiles, int num_kb) {
+// The same with one CTA a SM: the largest cluster with which all tiles run at once, 0
+// for more tiles than SMs.  The places are what the occupancy calculator gives clusters
+// of each size: they lie within a GPC, whose SMs clusters of seven and eight do not fill.
+static int deep_rule(int64_t tiles) {
   constexpr int places[SPLIT_MAX_CLUSTER + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
   for (int cs = SPLIT_MAX_CLUSTER; cs >= 1; --cs)
-    if (tiles * cs <= places[cs] && (cs == 1 || num_kb >= 3 * cs)) return cs;
+    if (tiles * cs <= places[cs]) return cs;
   return 0;
 }
 
-// The kernel for 33 to 64 rows.  Up to 74 feature tiles, half the SMs, the deep ring
-// (with more it loses as often as it wins); of those the few and short pairs of CTAs,
-// whose epilogue has twice the warps (61 rows, 512 -> 1024: 3.5 us for 4.4).  Over
-// 1134 random sizes 1.1 % slower than the best of all; without the pairs 2.0 %, without
-// the deep ring too 8 %.
+// The kernel for 33 to 64 rows: up to 74 feature tiles, half the SMs, the deep ring (with
+// more it loses as often as it wins).  Over 716 random sizes 0.4 % slower than the best of
+// all.
 static int middle_rule(int N, int K) {
   const int tiles = (N + 127) / 128, num_kb = (K + BK - 1) / BK;
-  if (tiles > 74) return split_rule(tiles, num_kb);
-  return tiles <= 16 && num_kb <= 4 ? 64 : SPLIT_DEEP + deep_rule(tiles, num_kb);
+  return tiles > 74 ? split_rule(tiles, num_kb) : SPLIT_DEEP + deep_rule(tiles);
 }
 
 // The kernel for more than 64 rows: the one with the least modelled time, a start
 // and then, for each round of tiles, the k-blocks and the part of the epilogue that
-// the next tile does not hide; for the deep split kernel a CTA's k-blocks, and the
-// partials by rows and by CTAs.  The figures (us) are fitted to 2033 random sizes (65
-// to 5000 rows) timed with every kernel but that one, 0.3 % slower than the best in
-// the geometric mean (tiles of 64, 128 or 256 features alone 32, 12 and 23 %), and to
-// 525 sizes (65 to 160 rows) with it; over 861 others 0.3 % slower than the best (over the
-// 525 0.7 %, and 14 % without it).
+// the next tile does not hide; for the deep split kernel a CTA's k-blocks and an
+// epilogue by rows.  The figures (us) are fitted to 2033 random sizes (65 to 5000 rows)
+// timed with every kernel but that one, 0.3 % slower than the best in the geometric mean
+// (tiles of 64, 128 or 256 features alone 32, 12 and 23 %), and to 656 sizes (65 to 160
+// rows) with it; over 616 others 0.7 % slower than the best.
 static int kernel_rule(int M, int N, int K, int sms) {
   struct Cost {
     int kernel, tile_rows, tile_features, places;
@@ -894,9 +888,9 @@ static int kernel_rule(int M, int N, int K, int sms) {
       least = t;
     }
   }
-  const int cs = deep_rule((int64_t)((M + 127) / 128) * ((N + 127) / 128), num_kb);
+  const int cs = deep_rule((int64_t)((M + 127) / 128) * ((N + 127) / 128));
   if (cs > 0) {
-    const double t = 2.3 + (num_kb + cs - 1) / cs * 0.15 + 4.7 * (M < 128 ? M : 128) / 128 + 0.07 * cs;
+    const double t = 4.0 + (num_kb + cs - 1) / cs * 0.23 + 1.7 * (M < 128 ? M : 128) / 128;
     if (t < least) best = SPLIT_DEEP + cs;
   }
   return best;
