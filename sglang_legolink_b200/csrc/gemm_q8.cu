@@ -203,15 +203,17 @@ struct alignas(64) Maps {
 // their own beside the ring, since the others may be done first; a lone CTA's take the ring.
 //
 // The epilogue's code is met cold by every CTA, so its loop is not unrolled (twice: 61 rows,
-// 8192 -> 5120, 11.2 us for 11.0), and scales and bias are fetched by the warps that wait for
-// the product: fetched by all six, the two that feed it come late (1 row, 512 -> 1024, 3.1 us
-// for 2.9).
+// 8192 -> 5120, 11.2 us for 11.0); the warps that wait for the product fetch scales and bias,
+// and the two that feed it, which come late, do nothing before the sums (1 row, 512 ->
+// 1024, 2.3 us for 2.9).  It costs a lone CTA of many rows up to 4 % more than one
+// row a thread did (61 rows, 3584 -> 37888, 25.9 for 25.2) and is up to a fifth faster in
+// clusters.
 //
 // DEEP: one CTA a SM with a ring of 220 KB for two with 108 KB each.  Half as many
 // CTAs hold as many bytes on their way and read X half as often, and that is a third
 // of the reads of 64 rows.  61 rows, 18944 -> 3584: 15.4 us for 16.5 with two a SM;
-// 3584 -> 3584: 6.4 for 7.6 (now 14.6 and 5.3).  128 rows: 18944 -> 3584 in clusters of
-// four 19.7 us, for 28.1 in pairs of CTAs on tiles of 64 features.
+// 3584 -> 3584: 6.4 for 7.6 (now 14.4 and 5.2).  128 rows: 18944 -> 3584 in clusters of
+// four 19.8 us, for 28.1 in pairs of CTAs on tiles of 64 features.
 constexpr int SPLIT_MAX_CLUSTER = 8;
 constexpr int SPLIT_DEEP = 10;  // added to a cluster's size: the deep ring
 template <int BNX, bool DEEP>
@@ -345,25 +347,28 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
   const int cols = SWIGLU ? p.N / 2 : p.N;
   auto residual_at = [&](int turn, int i) -> uint32_t {
     const int row = row_of(turn) + i, col = col_of(turn);
-    if (p.residual == nullptr || turn >= turns || row >= rows || col >= cols) return 0;
+    if (turn >= turns || row >= rows || col >= cols) return 0;
     const __nv_bfloat16* at = p.residual + (m0 + row) * p.ldr + col;
     return SWIGLU ? *reinterpret_cast<const uint16_t*>(at) : *reinterpret_cast<const uint32_t*>(at);
   };
   constexpr int AHEAD = BNX / 16;  // turns (one for 61 rows, 8192 -> 5120: 13.6 us; four 12.4)
-  uint32_t next[AHEAD][2];
+  uint32_t next[AHEAD][2] = {};
+  if (p.residual != nullptr) {
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    next[i][0] = residual_at(turn0 + 6 * i, 0);
-    next[i][1] = residual_at(turn0 + 6 * i, 1);
+    for (int i = 0; i < AHEAD; ++i) {
+      next[i][0] = residual_at(turn0 + 6 * i, 0);
+      next[i][1] = residual_at(turn0 + 6 * i, 1);
+    }
   }
+  bool done = true;
   if (warp >= 2) {
     const int i = tid - 64, n = nb * 128 + i;
     if (i < BNX) sxs[i] = i < rows ? p.xs[m0 + i] : 0.f;
     const float bias = p.bias != nullptr && n < p.N ? __bfloat162float(p.bias[n]) : 0.f;
     scol[i] = make_float2(n < p.N ? p.ws[n] : 0.f, bias);
+    done = mbar_wait(&tfull, 0, err, kErrTmemFullTimeout);
+    tc_fence_after();
   }
-  const bool done = mbar_wait(&tfull, 0, err, kErrTmemFullTimeout);
-  tc_fence_after();
   if (cs > 1) cluster_barrier_wait();
   if (warp >= 2) {  // TMEM lane quarter of this warp: features; columns: rows
     const int feat = (warp & 3) * 32 + lane;
