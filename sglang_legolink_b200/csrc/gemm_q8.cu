@@ -4,7 +4,10 @@
 //   C[m, n] = act(xs[m] ws[n] sum_k X[m, k] W[n, k] + bias[n]) + residual[m, n],
 //
 // with X and W in e4m3 and the sum in fp32 in tensor memory.  A scale belongs to
-// a whole row, so it leaves the sum and is one product per output; a 128-byte
+// a whole row, so it leaves the sum and is one product per output: the weight's
+// first, which is the one of moderate size (a row of x may hold numbers up to bf16's
+// largest, and its scale times a sum may pass fp32's range where the result does
+// not; for weights from 1e-29 to 1e29 the sum times their scale does not).  A 128-byte
 // swizzled row of an operand tile holds 128 values, and one tcgen05.mma of
 // kind::f8f6f4 takes 32 of them: the same bytes per instruction as in bf16, twice
 // the products.
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
         next[AHEAD - 1][0] = residual_at(turn + 6 * AHEAD, 0);
         next[AHEAD - 1][1] = residual_at(turn + 6 * AHEAD, 1);
       }
-      // the partials in split order, scales, bias
+      // the partials in split order, the scales (the weight's first), bias
       const float4* at = part + turn * 32 + lane;
       float4 v = *at;
       if (cs > 1) {
@@ -433,8 +436,8 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
       }
       const float2 s = scol[(turn & 3) * 32 + lane];
       const float4 xs = *reinterpret_cast<const float4*>(sxs + (first + (turn >> 2)) * 4);
-      v = make_float4(fmaf(v.x * xs.x, s.x, s.y), fmaf(v.y * xs.y, s.x, s.y), fmaf(v.z * xs.z, s.x, s.y),
-                      fmaf(v.w * xs.w, s.x, s.y));
+      v = make_float4(fmaf(v.x * s.x, xs.x, s.y), fmaf(v.y * s.x, xs.y, s.y), fmaf(v.z * s.x, xs.z, s.y),
+                      fmaf(v.w * s.x, xs.w, s.y));
       const float a0 = __shfl_xor_sync(0xffffffffu, high ? v.x : v.z, SWIGLU ? 16 : 1);
       const float a1 = __shfl_xor_sync(0xffffffffu, high ? v.y : v.w, SWIGLU ? 16 : 1);
       const int row = row_of(turn), col = col_of(turn);
@@ -676,13 +679,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
       }
       tc_fence_after();
       const uint32_t tbase = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN + half * PAIR_COLS);
-      // r[i] ws xs + bias of columns [c, c + 32); every lane reads the same of them
+      // (r[i] ws) xs + bias of columns [c, c + 32); every lane reads the same of them
       auto scaled = [&](const uint32_t (&r)[32], int c, int i) {
         const float4 s = *reinterpret_cast<const float4*>(scol + c + i);
         const float4 t = *reinterpret_cast<const float4*>(sbias + c + i);
-        return make_float4(fmaf(__uint_as_float(r[i]) * xs, s.x, t.x), fmaf(__uint_as_float(r[i + 1]) * xs, s.y, t.y),
-                           fmaf(__uint_as_float(r[i + 2]) * xs, s.z, t.z),
-                           fmaf(__uint_as_float(r[i + 3]) * xs, s.w, t.w));
+        return make_float4(fmaf(__uint_as_float(r[i]) * s.x, xs, t.x), fmaf(__uint_as_float(r[i + 1]) * s.y, xs, t.y),
+                           fmaf(__uint_as_float(r[i + 2]) * s.z, xs, t.z),
+                           fmaf(__uint_as_float(r[i + 3]) * s.w, xs, t.w));
       };
 #pragma unroll 1
       for (int c = 0; c < PAIR_COLS; c += 64) {

@@ -385,6 +385,8 @@ def linear_q8(x: Q8, w: Q8, bias: Optional[torch.Tensor] = None, residual: Optio
     + bias[n]``; with ``swiglu_epilogue`` then ``silu(gate) * up`` of the
     interleaved gate/up product (half width); with ``residual`` [M, N] (half
     width, likewise) that is added last.  Sums in fp32, one rounding to bf16.
+    The weight's scale is multiplied first: rows of ``x`` may be of any size, those
+    of ``w`` between 1e-29 and 1e29 (beyond, the sum times its scale may leave fp32's range).
 
     K a multiple of 16, N of 8 (of 32 with SwiGLU); on CUDA rows, ``bias`` and
     ``w.scale`` on 16-byte boundaries; ``out`` may be ``residual`` itself, and shares memory with no

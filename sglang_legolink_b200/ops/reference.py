@@ -193,8 +193,9 @@ def rmsnorm_q8(x: torch.Tensor, w: torch.Tensor, eps: float):
 
 def linear_q8(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """fp32 ``xs[m] ws[n] sum_k xq[m, k] wq[n, k] + bias[n]``."""
-    y = (xq.float() @ wq.float().t()) * xs[:, None] * ws
+    """fp32 ``xs[m] ws[n] sum_k xq[m, k] wq[n, k] + bias[n]``; the weight's scale
+    goes first, the sum times that of a row of large numbers may pass fp32's range."""
+    y = (xq.float() @ wq.float().t()) * ws * xs[:, None]
     return y if bias is None else y + bias.float()
 
 

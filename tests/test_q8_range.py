@@ -1,0 +1,81 @@
+"""The product of two matrices in 8 bits (``ops.linear_q8``) over the whole range
+of its operands and sizes.
+
+Tolerances.  The kernels add 32 products at a time to a sum in fp32, and then the
+partial sums of at most eight CTAs: K / 32 + 8 steps.  A step is off by at most
+2^-22 of the larger of the sum so far and its products, however it rounds; with
+terms of random signs that is at most 6 sqrt(sum of the terms' squares), so a
+product is off by (K / 32 + 8) 2^-22 of that, and by six steps of 2^-24 of
+itself for the scales, the bias and the residual.  silu(g) u is off by what g and u
+are off by (|silu'| <= 1.1) and, relatively, by the fast exponential's 2^-21 and 2^-23
+of its argument, as long as exp(-g) is within fp32, |g| < 90.  The result is
+rounded once, 2^-8 of itself; below bf16's normal numbers, a step is 2^-133.
+"""
+
+import pytest
+import torch
+
+from sglang_legolink_b200 import ops
+from sglang_legolink_b200.ops import Q8
+from test_q8_ops import KERNELS, q8_like, raw, rows_like
+
+gpu = pytest.mark.gpu
+
+
+def result64(x, w, bias, residual, swiglu):
+    """The result in 64 bits and how far one may be off."""
+    a, b = (t.values.cpu().double() * t.scale.cpu().double()[:, None] for t in (x, w))
+    y = a @ b.t()
+    tol = (a.shape[1] / 32 + 8) * 2.0 ** -22 * 6 * torch.sqrt((a * a) @ (b * b).t()) + 2.0 ** -22 * y.abs()
+    if bias is not None:
+        y = y + bias.cpu().double()
+        tol = tol + 2.0 ** -23 * y.abs()
+    if swiglu:
+        c = torch.arange(y.shape[1])
+        g, u, tg, tu = y[:, c % 32 < 16], y[:, c % 32 >= 16], tol[:, c % 32 < 16], tol[:, c % 32 >= 16]
+        s = g * torch.sigmoid(g)
+        y = s * u
+        tol = 1.1 * tg * (u.abs() + tu) + s.abs() * tu + (2.0 ** -20 + 2.0 ** -22 * g.abs().clamp(max=90)) * y.abs()
+    if residual is not None:
+        y = y + residual.cpu().double()
+        tol = tol + 2.0 ** -23 * y.abs()
+    return y, tol * (1 + 2.0 ** -8) + 2.0 ** -8 * y.abs() + 2.0 ** -133
+
+
+def far_rows(M, K, N, swiglu, device="cpu"):
+    """Rows of x of very different sizes, up to 1e37, against weights of ordinary
+    size: results within bf16's range whose factors may leave fp32's.  With SwiGLU
+    the up rows are 1e-34 as large, so that gate times up stays finite."""
+    g = torch.Generator().manual_seed(11)
+    size = torch.tensor([1e36, 1.0, 1e35, 1e-30, 3e37 if not swiglu else 1e34, 1e20])[torch.arange(M) % 6]
+    x, w = q8_like(M, K, 12), q8_like(N, K, 13)
+    x = Q8(x.values, (size / 448 * (0.5 + torch.rand(M, generator=g))).float())
+    ws = 0.05 / 448 * (0.5 + torch.rand(N, generator=g))
+    if swiglu:
+        ws = torch.where(torch.arange(N) % 32 < 16, ws, ws * 1e-34)
+    w = Q8(w.values, ws.float())
+    bias = rows_like(1, N, 14)[0].contiguous() * 1e-30
+    residual = rows_like(M, N // 2 if swiglu else N, 15) * 1e30
+    return tuple(Q8(*(t.to(device) for t in q)) for q in (x, w)) + (bias.to(device), residual.to(device))
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_rows_of_large_numbers(swiglu):
+    """The bf16 product of such rows is finite, and so is this one."""
+    x, w, b, r = far_rows(13, 512, 96, swiglu)
+    want, tol = result64(x, w, b, r, swiglu)
+    assert 1e36 < float(want.abs().max()) < 2e38
+    y = ops.linear_q8(x, w, b, residual=r, swiglu_epilogue=swiglu)
+    assert torch.all((y.double() - want).abs() <= tol)
+
+
+@gpu
+@pytest.mark.parametrize("kernel", [0] + KERNELS)
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("M", [1, 16, 61, 300])
+def test_rows_of_large_numbers_on_the_gpu(M, swiglu, kernel):
+    x, w, b, r = far_rows(M, 512, 160, swiglu, "cuda")
+    for bias, res in ((None, None), (b, r)):
+        want, tol = result64(x, w, bias, res, swiglu)
+        y = raw(x, w, bias, res, swiglu, kernel)
+        assert torch.all((y.cpu().double() - want).abs() <= tol)
