@@ -888,6 +888,8 @@ static int kernel_rule(int M, int N, int K, int sms) {
   int best = 0;
   double least = 0;
   for (const Cost& c : costs) {
+    // more row tiles than a grid has places along z: short rows, few features
+    if (c.kernel <= SPLIT_MAX_CLUSTER && M > 128 * 65535) continue;
     const int64_t tiles =
         (int64_t)((M + c.tile_rows - 1) / c.tile_rows) * ((N + c.tile_features - 1) / c.tile_features);
     const double t = c.start + (double)((tiles + c.places - 1) / c.places) * (num_kb * c.block + c.tile);

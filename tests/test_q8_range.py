@@ -17,7 +17,7 @@ import torch
 
 from sglang_legolink_b200 import ops
 from sglang_legolink_b200.ops import Q8
-from test_q8_ops import KERNELS, q8_like, raw, rows_like
+from test_q8_ops import KERNELS, integers_q8, q8_like, raw, rows_like
 
 gpu = pytest.mark.gpu
 
@@ -79,3 +79,18 @@ def test_rows_of_large_numbers_on_the_gpu(M, swiglu, kernel):
         want, tol = result64(x, w, bias, res, swiglu)
         y = raw(x, w, bias, res, swiglu, kernel)
         assert torch.all((y.cpu().double() - want).abs() <= tol)
+
+
+@gpu
+@pytest.mark.parametrize("K,N", [(64, 64), (16, 128), (128, 8)])
+def test_more_row_tiles_than_a_grid_has_places(K, N):
+    """65535 tiles of 128 rows and one row more, of few and short features."""
+    M = 65535 * 128 + 1
+    x = Q8(torch.randint(-3, 4, (M, K), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda",
+                         dtype=torch.int8).to(torch.float8_e4m3fn), torch.full((M,), 0.5, device="cuda"))
+    w = integers_q8(N, K, 2, "cuda")
+    y = ops.linear_q8(x, w)
+    for rows in (slice(0, 300), slice(M // 2, M // 2 + 300), slice(M - 300, M)):
+        want = x.values[rows].double() @ w.values.double().t() * 0.5 * w.scale.double()
+        assert torch.equal(y[rows], want.to(torch.bfloat16))
+    assert bool(torch.isfinite(y).all()) and ops.check_errors("cuda") == 0
