@@ -184,7 +184,9 @@ __device__ __forceinline__ void prefetch_box(const void* tmap, int x, int y) {
 // The approximate quotient is off by 2 ulp, and 0 for a divisor past 2^126, where x
 // is below -87 and silu(x) below 1e-36.
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
-// Lets the copies in flight land before a CTA that gave up exits.
+// Lets what is in flight land (copies, products, other CTAs' stores) before a CTA of
+// which a wait ran out exits.  Such a CTA stores no result that is not whole: what it
+// would have written stays as it was, and the error word says so.
 __device__ __forceinline__ void linger() {
   const unsigned long long t0 = globaltimer_ns();
   while (globaltimer_ns() - t0 < 2000000ull) {
@@ -289,6 +291,7 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
   if (cs > 1) cluster_arrive();  // this CTA runs: the others may write into its shared memory
 
   const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), w0 = smem_u32(sW), x0 = smem_u32(sX);
+  bool done = true;  // no wait of this thread ran out
   if (warp == 0) {
     if (elect_one()) {
       // every input may be an output of the kernel ahead
@@ -310,10 +313,11 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
           ++kb;
         }
       }
-      if (!ok) linger();
+      done = ok;
     }
   } else if (warp == 1) {
     if (elect_one()) {
+      pdl_wait();  // a wait's limit is for the copies, not for the kernel ahead
       constexpr uint32_t idesc = idesc_e4m3(128, BNX);
       const uint64_t wd = umma_desc_sw128_kmajor(w0), xd = umma_desc_sw128_kmajor(x0);
       bool ok = true;
@@ -336,7 +340,8 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
           ++kb;
         }
       }
-      umma_commit(&tfull);
+      if (ok) umma_commit(&tfull);  // else the sums are not whole: those who wait for them give up too
+      done = ok;
     }
   }
   __syncwarp();
@@ -368,7 +373,6 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
       next[i][1] = residual_at(turn0 + 6 * i, 1);
     }
   }
-  bool done = true;
   if (warp >= 2) {
     const int i = tid - 64, n = nb * 128 + i;
     if (i < BNX) sxs[i] = i < rows ? p.xs[m0 + i] : 0.f;
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
     tc_fence_after();
   }
   if (cs > 1) cluster_barrier_wait_lanes();
-  if (warp >= 2) {  // TMEM lane quarter of this warp: features; columns: rows
+  if (warp >= 2 && done) {  // TMEM lane quarter of this warp: features; columns: rows
     const int feat = (warp & 3) * 32 + lane;
     const bool none = kb1 <= kb0;
     float4* slot = part + crank * share * 128 + feat;  // of this CTA, in every CTA
@@ -462,10 +466,13 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
       }
     }
   }
-  if (!received) linger();
+  if (!ok) linger();  // products and copies in flight
   __syncwarp();
   if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);  // every read of it is behind the barrier
-  if (cs > 1) cluster_barrier_wait();  // no CTA leaves before the others' stores to it are issued
+  if (cs > 1) {
+    cluster_barrier_wait();  // no CTA leaves before the others' stores to it are issued
+    if (!ok) linger();       // nor, where it did not count them, before they land
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -561,6 +568,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
   pdl_wait();
 
   const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), w0 = smem_u32(sW), x0 = smem_u32(sX);
+  bool done = true;  // no wait of this thread ran out
   if (warp == 0) {
     if (elect_one()) {
       prefetch_tmap(&tm.x);
@@ -593,7 +601,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
           }
         }
       }
-      if (!ok) linger();
+      done = ok;
     }
   } else if (warp == 1) {
     if (crank == 0 && elect_one()) {
@@ -637,6 +645,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
       // every MMA issued is done before its accumulator is given back
       commit_pair_local(drain);
       mbar_wait(drain, 0, nullptr, 0);
+      done = ok;
     }
     __syncwarp();
   } else {
@@ -679,11 +688,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
         *reinterpret_cast<float4*>(sbias + 4 * lane) = make_float4(b0.x, b0.y, b1.x, b1.y);
       }
       __syncwarp();
-      if (!mbar_wait(&tfull[acc], aphase, err, kErrTmemFullTimeout)) {
-        if (p.residual != nullptr) linger();
+      // lanes leave a wait one by one; the loads below take a whole warp
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], aphase, err, kErrTmemFullTimeout))) {
+        done = false;
         break;
       }
-      __syncwarp();  // lanes leave a wait one by one; the loads below take a whole warp
       tc_fence_after();
       const uint32_t tbase = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN + half * PAIR_COLS);
       // (r[i] ws) xs + bias of columns [c, c + 32); every lane reads the same of them
@@ -695,7 +704,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
                            fmaf(__uint_as_float(r[i + 3]) * s.w, xs, t.w));
       };
 #pragma unroll 1
-      for (int c = 0; c < PAIR_COLS; c += 64) {
+      for (int c = 0; c < PAIR_COLS && done; c += 64) {
         if (colw + c >= p.N || row0 >= p.M) break;  // outside C
         uint32_t r[2][32];
         tmem_ld_32x32b_x32(tbase + c, r[0]);
@@ -734,7 +743,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
           const int swz = (lane >> 1) & 3;
           if (p.residual != nullptr) {
             fetch_residual(b == PAIR_BOXES - 1 ? 0 : b + 1, cb + STEP);
-            if (!mbar_wait(&rbar[b], bphase, err, kErrTmaFullTimeout)) linger();
+            if (!__all_sync(0xffffffffu, mbar_wait(&rbar[b], bphase, err, kErrTmaFullTimeout))) {
+              done = false;
+              break;
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const uint4 rv = d[k ^ swz];
@@ -767,6 +779,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
           }
         }
       }
+      if (!done) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(acc == 0 ? leader_tempty0 : leader_tempty1);
@@ -779,6 +792,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
 
+  if (!done) linger();  // neither CTA leaves before
   __syncwarp();
   tc_fence_before();
   cluster_sync();

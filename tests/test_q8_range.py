@@ -94,3 +94,25 @@ def test_more_row_tiles_than_a_grid_has_places(K, N):
         want = x.values[rows].double() @ w.values.double().t() * 0.5 * w.scale.double()
         assert torch.equal(y[rows], want.to(torch.bfloat16))
     assert bool(torch.isfinite(y).all()) and ops.check_errors("cuda") == 0
+
+
+@gpu
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1, 128, 128), (16, 3584, 512), (61, 8192, 640), (128, 18944, 256), (300, 2048, 1056)])
+def test_a_call_that_gives_up_stores_whole_results_only(M, K, N, swiglu, kernel):
+    """With an error on record waits return at once: what a call stores all the
+    same is right, and the rest of its output is left as it was."""
+    x, w = integers_q8(M, K, 1, "cuda"), integers_q8(N, K, 2, "cuda")
+    r = torch.randint(-64, 65, (M, N // 2 if swiglu else N)).to(torch.bfloat16).cuda()
+    err = ops.workspace("cuda").err
+    for res in (None, r):
+        want = raw(x, w, None, res, swiglu, kernel)
+        for _ in range(5):
+            out = torch.full_like(want, 1234.0)
+            err.fill_(6)
+            ops._cuda().q8_linear(x.values, x.scale, w.values, w.scale, None, res, out, swiglu, kernel, err)
+            assert ops.check_errors("cuda") == 6
+            assert bool(((out == want) | (out == 1234)).all())
+        assert torch.equal(raw(x, w, None, res, swiglu, kernel), want)
+    assert ops.check_errors("cuda") == 0
