@@ -245,6 +245,7 @@ class QwenModel:
             raise ValueError("weights in 8 bits are not supported with adapters")
         if self.served:
             raise ValueError("weights go into 8 bits before an engine holds keys and values of the others")
+        self.check_rowwise_q8()
         names = ("qkv_w", "o_w", "gu_w", "down_w")
         for i, lw in enumerate(self.layers):  # all of them fit before any is replaced
             for n in names:
@@ -258,6 +259,15 @@ class QwenModel:
                 setattr(lw, n, ops.quantize_q8(getattr(lw, n)))
         self.quantized = True
         self.buf_generation += 1  # a captured graph may point at weights that are gone
+
+    @staticmethod
+    def check_rowwise_q8() -> None:
+        """Row-wise compute is used by grouped Compiles alone: a setting that weights
+        in 8 bits cannot follow is refused ahead of all of them."""
+        from ..runtime.repair_diagnostics import rowwise_setting
+
+        if rowwise_setting():
+            raise ValueError(f"weights in 8 bits are not supported with row-wise repair compute ({rowwise_setting()})")
 
     # ------------------------------------------------------------- adapters
     def add_adapter(self, name: str, adapter) -> int:

@@ -163,6 +163,8 @@ class Engine:
                  sampler: str = "torch"):
         if sampler not in ("torch", "kernel"):
             raise ValueError("sampler must be 'torch' (per-row torch ops) or 'kernel' (one launch a batch)")
+        if model.quantized:
+            model.check_rowwise_q8()
         self.sampler = sampler
         self.model = model
         model.served = True

@@ -50,6 +50,11 @@ def _flag(name: str) -> bool:
     return os.getenv(name, "0").strip().lower() in {"1", "true", "yes", "on"}
 
 
+def rowwise_setting() -> str:
+    """The first environment setting that asks for row-wise compute; "" when none does."""
+    return next((env for _, env, _ in _ROWWISE.values() if _flag(env)), "")
+
+
 def rowwise_slices(meta: Optional[dict], token_count: int, which: str) -> tuple[slice, ...]:
     """Flattened token slices, one per grouped execution row, for a
     row-by-row ``which`` ("ffn" or "output_projection"); () when disabled or

@@ -352,6 +352,11 @@ def main(argv=None) -> None:
         ap.error("--adapter is not supported with --tp-size")
     if a.weights != "bf16" and a.adapter:
         ap.error("--weights q8 is not supported with --adapter")
+    if a.weights != "bf16":
+        from ..runtime.repair_diagnostics import rowwise_setting
+
+        if rowwise_setting():
+            ap.error(f"--weights q8 is not supported with {rowwise_setting()}")
     if a.tp_size > 1 or a.dp_size > 1 or a.pp_size != 1:
         from .launch import launch
 

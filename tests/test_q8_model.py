@@ -278,3 +278,28 @@ def test_decode_step_equals_the_prefill_of_the_same_tokens():
                       kv_lens=torch.tensor([50], dtype=torch.int32, device=dev))
     got = eng.model.forward(fb, eng.kv)[0].float().cpu()
     assert close(got, want, 0.05)
+
+
+@pytest.mark.parametrize("which", ["FFN", "OUTPUT_PROJECTION"])
+def test_a_setting_of_row_wise_repair_is_refused_ahead_of_the_first_request(monkeypatch, capsys, which):
+    """It acts on grouped Compiles alone: a server that starts with it would fail under load."""
+    from sglang_legolink_b200.server.http_server import build_service, main
+
+    name = "SGLANG_PIC_SPARSE_REPAIR_ROWWISE_" + which
+    ready = QwenModel.random_init(PRESETS["tiny-qwen2"])
+    ready.quantize_weights()
+    monkeypatch.setenv(name, "1")
+    m = QwenModel.random_init(PRESETS["tiny-qwen2"])
+    with pytest.raises(ValueError, match=name):
+        m.quantize_weights()
+    assert not m.quantized and isinstance(m.layers[0].qkv_w, torch.Tensor)
+    with pytest.raises(ValueError, match=name):
+        Engine(ready, num_pages=64, max_context=256)
+    with pytest.raises(ValueError, match=name):
+        build_service("tiny-qwen2", max_context=1024, legolink_only=False, weights="q8")
+    with pytest.raises(SystemExit):
+        main(["--weights", "q8"])
+    assert name in capsys.readouterr().err
+    Engine(m, num_pages=64, max_context=256)  # as before for the other weights
+    monkeypatch.setenv(name, "0")
+    Engine(ready, num_pages=64, max_context=256)
