@@ -58,7 +58,7 @@ __device__ __forceinline__ void cluster_barrier_wait() {
 }
 // For lanes that may have parted: behind loads that some of them skip, a
 // __syncwarp() for the wait above costs 61 rows, 8192 -> 5120 11.63 us for 11.50.
-__device__ __forceinline__ void cluster_barrier_wait_lanes() {
+__device__ __forceinline__ void cluster_lanes_barrier_wait() {
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(192, DEEP ? 1 : 2)
     done = __all_sync(0xffffffffu, mbar_wait(&tfull, 0, err, kErrTmemFullTimeout));
     tc_fence_after();
   }
-  if (cs > 1) cluster_barrier_wait_lanes();
+  if (cs > 1) cluster_lanes_barrier_wait();
   if (warp >= 2 && done) {  // TMEM lane quarter of this warp: features; columns: rows
     const int feat = (warp & 3) * 32 + lane;
     const bool none = kb1 <= kb0;
