@@ -167,7 +167,6 @@ class Engine:
             model.check_rowwise_q8()
         self.sampler = sampler
         self.model = model
-        model.served = True
         self.cfg = model.cfg
         self.device = model.device
         self.page_size = page_size
@@ -219,6 +218,7 @@ class Engine:
             # split-K partials for M <= 128 rows over the widest weight
             widest = max(2 * model.inter, (model.hq + 2 * model.hkv) * self.cfg.head_dim, self.cfg.hidden_size)
             ws.reserve_gemm(8 * 128 * max(widest, model.lm_head.shape[0]) // 2, 4096)
+        model.served = True
 
     def release_graphs(self) -> None:
         """Drops the captured decode graphs.  A TP model's graphs hold NCCL

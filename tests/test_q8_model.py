@@ -303,3 +303,13 @@ def test_a_setting_of_row_wise_repair_is_refused_ahead_of_the_first_request(monk
     Engine(m, num_pages=64, max_context=256)  # as before for the other weights
     monkeypatch.setenv(name, "0")
     Engine(ready, num_pages=64, max_context=256)
+
+
+def test_an_engine_that_was_not_made_holds_nothing():
+    """An engine whose arguments do not fit leaves the model as it was."""
+    m = QwenModel.random_init(PRESETS["tiny-qwen2"])
+    for bad in (dict(page_size="16"), dict(max_blocks="many"), dict(num_pages="64")):
+        with pytest.raises((TypeError, ValueError)):
+            Engine(m, **{"num_pages": 64, "max_context": 256, **bad})
+    m.quantize_weights()
+    assert m.quantized
