@@ -292,6 +292,8 @@ def build_service(model: str = "tiny-qwen2", *, device: str = "cpu", tokenizer: 
     from ..models.qwen import QwenModel
     from ..runtime.engine import Engine
 
+    if weights not in ("bf16", "q8"):
+        raise ValueError("weights must be 'bf16' (as loaded) or 'q8' (the layers' projections in 8 bits)")
     dtype = torch.bfloat16 if device.startswith("cuda") else torch.float32
     if os.path.isdir(model) and any(f.endswith(".safetensors") for f in os.listdir(model)):
         m = QwenModel.from_pretrained(model, device=device, dtype=dtype)

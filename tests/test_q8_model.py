@@ -313,3 +313,10 @@ def test_an_engine_that_was_not_made_holds_nothing():
             Engine(m, **{"num_pages": 64, "max_context": 256, **bad})
     m.quantize_weights()
     assert m.quantized
+
+
+def test_the_service_refuses_weights_that_it_does_not_know():
+    from sglang_legolink_b200.server.http_server import build_service
+
+    with pytest.raises(ValueError, match="weights"):
+        build_service("tiny-qwen2", max_context=1024, legolink_only=False, weights="fp8")
