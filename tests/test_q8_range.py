@@ -8,8 +8,9 @@ terms of random signs that is at most 6 sqrt(sum of the terms' squares), so a
 product is off by (K / 32 + 8) 2^-22 of that, and by six steps of 2^-24 of
 itself for the scales, the bias and the residual.  silu(g) u is off by what g and u
 are off by (|silu'| <= 1.1) and, relatively, by the fast exponential's 2^-21 and 2^-23
-of its argument, as long as exp(-g) is within fp32, |g| < 90.  The result is
-rounded once, 2^-8 of itself; below bf16's normal numbers, a step is 2^-133.
+of its argument, as long as exp(-g) is within fp32, |g| < 90; where 1 + exp(-g) is past
+2^126 silu(g) is 0, which is off by less than 2^-119.  The result is rounded once,
+2^-8 of itself; below bf16's normal numbers, a step is 2^-133.
 """
 
 import pytest
@@ -36,6 +37,7 @@ def result64(x, w, bias, residual, swiglu):
         s = g * torch.sigmoid(g)
         y = s * u
         tol = 1.1 * tg * (u.abs() + tu) + s.abs() * tu + (2.0 ** -20 + 2.0 ** -22 * g.abs().clamp(max=90)) * y.abs()
+        tol = tol + 2.0 ** -119 * u.abs()
     if residual is not None:
         y = y + residual.cpu().double()
         tol = tol + 2.0 ** -23 * y.abs()
@@ -103,7 +105,22 @@ def test_more_row_tiles_than_a_grid_has_places(K, N):
 def test_a_call_that_gives_up_stores_whole_results_only(M, K, N, swiglu, kernel):
     """With an error on record waits return at once: what a call stores all the
     same is right, and the rest of its output is left as it was."""
-    x, w = integers_q8(M, K, 1, "cuda"), integers_q8(N, K, 2, "cuda")
+    gives_up(integers_q8(M, K, 1, "cuda"), integers_q8(N, K, 2, "cuda"), swiglu, kernel)
+
+
+@gpu
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_a_long_call_that_gives_up_leaves_its_output(swiglu, kernel):
+    """A product that takes longer than the waits for it look away from the error word."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, w = (Q8(torch.randint(-3, 4, (R, 1 << 22), generator=g, device="cuda", dtype=torch.int8).to(torch.float8_e4m3fn),
+               torch.ones(R, device="cuda")) for R in (16, 64))
+    gives_up(x, w, swiglu, kernel)
+
+
+def gives_up(x, w, swiglu, kernel):
+    M, N = x.values.shape[0], w.values.shape[0]
     r = torch.randint(-64, 65, (M, N // 2 if swiglu else N)).to(torch.bfloat16).cuda()
     err = ops.workspace("cuda").err
     for res in (None, r):
@@ -116,3 +133,111 @@ def test_a_call_that_gives_up_stores_whole_results_only(M, K, N, swiglu, kernel)
             assert bool(((out == want) | (out == 1234)).all())
         assert torch.equal(raw(x, w, None, res, swiglu, kernel), want)
     assert ops.check_errors("cuda") == 0
+
+
+# ------------------------------------------------- every cluster, long sums
+CLUSTERS = [4, 5, 6, 7, 12, 14, 15, 16, 17]  # CTAs to a feature tile that the rules choose beside those of KERNELS
+
+
+@gpu
+@pytest.mark.parametrize("kernel", CLUSTERS)
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1, 640, 128), (9, 1808, 160), (29, 512, 96), (33, 1040, 288), (61, 3584, 352), (64, 128, 128),
+                                   (125, 1808, 288), (128, 8192, 128), (150, 912, 64)])
+def test_clusters_of_every_size(M, K, N, swiglu, kernel):
+    """Groups of rows and k-blocks that do not divide among the CTAs; some CTAs have none."""
+    x, w = integers_q8(M, K, 1, "cuda"), integers_q8(N, K, 2, "cuda")
+    b = torch.randint(-64, 65, (N,), generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    cols = N // 2 if swiglu else N
+    r = torch.randint(-64, 65, (M, cols), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    for bias, res in ((None, None), (b, r)):
+        y = raw(x, w, bias, res, swiglu, kernel).cpu().double()
+        want, tol = result64(x, w, bias, res, swiglu)
+        # without SwiGLU every step is exact, and the result is rounded once
+        ok = (y - want).abs() <= tol if swiglu else y == want.to(torch.bfloat16).double()
+        assert torch.all(ok)
+    assert ops.check_errors("cuda") == 0
+
+
+def wide_whole(M, N, K, device="cpu"):
+    """Whole numbers whose running sum rises to 2^21 or 2^22 over the first half of K and
+    falls back over the second, with small ones beside them: each sum of any part
+    is a whole number below 2^24, exact in fp32, and the end is what the small ones give."""
+    g = torch.Generator().manual_seed(K)
+    big = 2.0 ** (6 if K <= 8192 else 5)
+    x, w = (torch.randint(-3, 4, (R, K), generator=g).float() for R in (M, N))
+    k = torch.arange(K)
+    x[:, k % 4 == 0] = big
+    w[:, (k % 4 == 0) & (k < K // 2)] = big
+    w[:, (k % 4 == 0) & (k >= K // 2)] = -big
+    scale = [torch.exp2(torch.randint(-3, 4, (R,), generator=g).float()) for R in (M, N)]
+    return tuple(Q8(t.to(torch.float8_e4m3fn).to(device), s.to(device)) for t, s in zip((x, w), scale))
+
+
+def product_of(x, w, ks=slice(None)):
+    a, b = (t.values.cpu().double()[:, ks] for t in (x, w))
+    return a @ b.t() * x.scale.cpu().double()[:, None] * w.scale.cpu().double()
+
+
+@pytest.mark.parametrize("K", [8192, 18944])
+def test_the_long_sums_tell_mistakes_apart(K):
+    """Of products without an MMA's 32 values, or whose sum keeps 14 bits, few pass."""
+    x, w = wide_whole(61, 128, K)
+    want = product_of(x, w).to(torch.bfloat16)
+    assert float((want.double() / x.scale[:, None] / w.scale).abs().max()) < 2 ** 12
+    for at in (0, 32 * (K // 64), K - 32):
+        keep = torch.ones(K, dtype=torch.bool)
+        keep[at:at + 32] = False
+        assert float((product_of(x, w, keep).to(torch.bfloat16) == want).float().mean()) < 0.2
+    total = torch.zeros(61, 128, dtype=torch.float64)
+    for k in range(0, K, 32):
+        total += x.values.double()[:, k:k + 32] @ w.values.double()[:, k:k + 32].t()
+        step = torch.exp2(torch.floor(torch.log2(total.abs().clamp(min=1))) - 13)
+        total = torch.trunc(total / step) * step
+    cut = (total * x.scale.double()[:, None] * w.scale.double()).to(torch.bfloat16)
+    assert float((cut == want).float().mean()) < 0.2
+
+
+@gpu
+@pytest.mark.parametrize("kernel", KERNELS + CLUSTERS)
+@pytest.mark.parametrize("M", [1, 61, 128, 300])
+@pytest.mark.parametrize("K", [8192, 18944])
+def test_long_sums_are_exact(K, M, kernel):
+    N = 264
+    x, w = wide_whole(M, N, K, "cuda")
+    want = product_of(x, w)
+    assert torch.equal(raw(x, w, kernel=kernel).cpu(), want.to(torch.bfloat16))
+    b = torch.randint(-64, 65, (N,), generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    r = torch.randint(-64, 65, (M, N), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    y = raw(x, w, b, r, kernel=kernel)
+    assert torch.equal(y.cpu(), (want + b.cpu().double() + r.cpu().double()).to(torch.bfloat16))
+    assert ops.check_errors("cuda") == 0
+
+
+LONG = [(5, 18944, 96), (61, 8192, 640), (128, 18944, 160), (300, 8192, 288)]
+
+
+@pytest.mark.parametrize("M,K,N", LONG[:2])
+def test_the_bound_of_a_long_product_is_sharp(M, K, N):
+    """A product without an MMA's 32 values is refused nearly everywhere."""
+    x, w = q8_like(M, K, 1), q8_like(N, K, 2)
+    want, tol = result64(x, w, None, None, False)
+    for at in (0, 32 * (K // 64), K - 32):
+        keep = torch.ones(K, dtype=torch.bool)
+        keep[at:at + 32] = False
+        off = (product_of(x, w, keep).to(torch.bfloat16).double() - want).abs() > tol
+        assert float(off.float().mean()) > 0.7
+
+
+@gpu
+@pytest.mark.parametrize("kernel", KERNELS + CLUSTERS)
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("M,K,N", LONG)
+def test_long_products(M, K, N, swiglu, kernel):
+    x, w = q8_like(M, K, 1, "cuda"), q8_like(N, K, 2, "cuda")
+    w = Q8(w.values, w.scale * 0.02)
+    b = rows_like(1, N, 3, device="cuda")[0].contiguous()
+    r = rows_like(M, N // 2 if swiglu else N, 4, 8, "cuda")
+    for bias, res in ((None, None), (b, r)):
+        want, tol = result64(x, w, bias, res, swiglu)
+        assert torch.all((raw(x, w, bias, res, swiglu, kernel).cpu().double() - want).abs() <= tol)
