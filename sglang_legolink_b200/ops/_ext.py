@@ -51,27 +51,23 @@ class _Counted:
 
     def __init__(self, mod):
         self._mod = mod
-        self._cache = {}
 
     def __getattr__(self, name):
-        fn = self._cache.get(name)
-        if fn is None:
-            target = getattr(self._mod, name)
-            from ..utils import launch_count
+        target = getattr(self._mod, name)
+        from ..utils import launch_count
 
-            k = self._KERNELS.get(name, 1)
-            if name == "attn_decode":
-                def fn(*a, **kw):
-                    launch_count.add(2 if a[8] > 1 else 1)
-                    return target(*a, **kw)
-            elif k:
-                def fn(*a, **kw):
-                    launch_count.add(k)
-                    return target(*a, **kw)
-            else:
-                fn = target
-            self._cache[name] = fn
-            self.__dict__[name] = fn  # found without __getattr__ from now on
+        k = self._KERNELS.get(name, 1)
+        if name == "attn_decode":
+            def fn(*a, **kw):
+                launch_count.add(2 if a[8] > 1 else 1)
+                return target(*a, **kw)
+        elif k:
+            def fn(*a, **kw):
+                launch_count.add(k)
+                return target(*a, **kw)
+        else:
+            fn = target
+        self.__dict__[name] = fn  # found without __getattr__ from now on
         return fn
 
 
