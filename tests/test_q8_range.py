@@ -241,3 +241,36 @@ def test_long_products(M, K, N, swiglu, kernel):
     for bias, res in ((None, None), (b, r)):
         want, tol = result64(x, w, bias, res, swiglu)
         assert torch.all((raw(x, w, bias, res, swiglu, kernel).cpu().double() - want).abs() <= tol)
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 40, 100, 300])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_what_lies_beside_the_output_stays(M, swiglu):
+    """Rows and columns of a larger buffer, with a width that ends inside the kernels' boxes."""
+    K, N = 272, 544 if swiglu else 520
+    cols = N // 2 if swiglu else N
+    x, w = integers_q8(M, K, 1, "cuda"), integers_q8(N, K, 2, "cuda")
+    want = ops.linear_q8(x, w, swiglu_epilogue=swiglu)
+    for kernel in [0] + KERNELS:
+        buf = torch.full((M + 3, cols + 40), 7.0, dtype=torch.bfloat16, device="cuda")
+        out = buf[1:M + 1, 16:cols + 16]
+        ops._cuda().q8_linear(x.values, x.scale, w.values, w.scale, None, None, out, swiglu, kernel, ops.workspace("cuda").err)
+        if not swiglu:
+            assert torch.equal(out, want)
+        buf[1:M + 1, 16:cols + 16] = 7
+        assert bool((buf == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 40, 70])
+def test_more_feature_tiles_than_a_grid_has_places(M):
+    K, N = 16, 65535 * 128 + 8
+    x = integers_q8(M, K, 1, "cuda")
+    w = Q8(torch.randint(-3, 4, (N, K), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda",
+                         dtype=torch.int8).to(torch.float8_e4m3fn), torch.full((N,), 0.5, device="cuda"))
+    y = ops.linear_q8(x, w)
+    for cols in (slice(0, 300), slice(N // 2, N // 2 + 300), slice(N - 300, N)):
+        want = x.values.double() @ w.values[cols].double().t() * 0.5 * x.scale[:, None].double()
+        assert torch.equal(y[:, cols], want.to(torch.bfloat16))
+    assert bool(torch.isfinite(y).all()) and ops.check_errors("cuda") == 0
