@@ -93,7 +93,10 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, float* red) {
 // (quantising, long rows): they stay as they were loaded, so that more of the large CTAs
 // fit a SM: 3000 x 25600 36.0 us for 47; short rows have places enough, and unpacking
 // them behind the maximum costs 8192 x 2048 10.1 for 9.0.
-template <int VPT, int MODE, bool WARP, bool PACKED>
+// LOW: an eps below 2^-80, beside which squares below fp32's range count.  A kernel of its
+// own, since its registers cost the norm 2 to 16 % (5087 x 3584 14.2 us for 13.9, 5087 x
+// 1024 6.3 for 5.4).
+template <int VPT, int MODE, bool WARP, bool PACKED, bool LOW>
 __global__ void __launch_bounds__(WARP ? 256 : 1024)
     q8_rows_kernel(const __grid_constant__ LLQ8Rows p) {
   __shared__ float red[3][32];
@@ -112,6 +115,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024)
     in[i] = j < nvec ? xr[j] : make_uint4(0, 0, 0, 0);
   }
   uint32_t top = 0;  // the largest magnitude's bits
+  float up = 1.f;    // what is held of y is 1 / up of it
   float2 v[PACKED ? 1 : VPT][4];  // the row in fp32
   if constexpr (MODE == kQ8Quantize) {
     if constexpr (PACKED) {
@@ -191,17 +195,22 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024)
       }
     float ss = row_sum<WARP>((sq.x + sq.y) + (sq2.x + sq2.y), red[0]);
     float rstd = rsqrtf(ss / (float)p.K + p.eps);
-    if (!(ss < INFINITY)) {  // squares past fp32's range, or a value that is not finite: the same, 2^-80 as large
+    // squares past fp32's range, or a value that is not finite: the same, 2^-80 as large;
+    // squares below it: 2^80 as large
+    if (!(ss < INFINITY) || (LOW && ss < 0x1p-80f)) {
+      const float f = LOW && ss < 1.f ? 0x1p80f : 0x1p-80f;
       ss = 0.f;
 #pragma unroll
       for (int i = 0; i < VPT; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float a = v[i][c].x * 0x1p-80f, b = v[i][c].y * 0x1p-80f;
+          const float a = v[i][c].x * f, b = v[i][c].y * f;
           ss = fmaf(a, a, fmaf(b, b, ss));
         }
       ss = row_sum<WARP>(ss, red[2]);
-      rstd = rsqrtf(ss / (float)p.K) * 0x1p-80f;
+      rstd = rsqrtf(ss / (float)p.K + (LOW ? p.eps * f * f : 0.f));
+      if (LOW && rstd * f == INFINITY) up = f;  // itself past the range: until the row is quantised
+      else rstd *= f;
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -222,9 +231,10 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024)
       }
     top = __float_as_uint(max_nan(big, big2, 0.f));
   }
-  const float amax = __uint_as_float(row_max<WARP>(top, red[1]));
+  const float amax = __uint_as_float(row_max<WARP>(top, red[1])) * (LOW ? up : 1.f);
   const float scale = amax < INFINITY ? fmaxf(amax / kE4m3Max, kQ8MinScale) : __uint_as_float(0x7fffffffu);
-  const float inv = 1.f / scale;
+  float inv = 1.f / scale;
+  if (LOW && up > 1.f) inv = inv * up == INFINITY ? 0x1p127f : inv * up;  // zeros stay zeros
   const float2 inv2 = make_float2(inv, inv);
   uint2* qr = reinterpret_cast<uint2*>(p.q + row * p.ldq);
 #pragma unroll
@@ -241,16 +251,19 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024)
 
 template <int VPT, bool WARP>
 static cudaError_t q8_rows_launch(const LLQ8Rows& p, int grid, int threads, cudaStream_t stream) {
+  const auto run = [&](auto kernel) { return launch_pdl(kernel, dim3(grid), dim3(threads), 0, stream, p); };
   if (p.w == nullptr) {
     if constexpr (!WARP && VPT == 4) {
-      if (threads > 256)
-        return launch_pdl(q8_rows_kernel<VPT, kQ8Quantize, WARP, true>, dim3(grid), dim3(threads), 0, stream, p);
+      if (threads > 256) return run(q8_rows_kernel<VPT, kQ8Quantize, WARP, true, false>);
     }
-    return launch_pdl(q8_rows_kernel<VPT, kQ8Quantize, WARP, false>, dim3(grid), dim3(threads), 0, stream, p);
+    return run(q8_rows_kernel<VPT, kQ8Quantize, WARP, false, false>);
   }
+  const bool low = p.eps < 0x1p-80f;
   if (p.residual == nullptr)
-    return launch_pdl(q8_rows_kernel<VPT, kQ8Norm, WARP, false>, dim3(grid), dim3(threads), 0, stream, p);
-  return launch_pdl(q8_rows_kernel<VPT, kQ8AddNorm, WARP, false>, dim3(grid), dim3(threads), 0, stream, p);
+    return low ? run(q8_rows_kernel<VPT, kQ8Norm, WARP, false, true>)
+               : run(q8_rows_kernel<VPT, kQ8Norm, WARP, false, false>);
+  return low ? run(q8_rows_kernel<VPT, kQ8AddNorm, WARP, false, true>)
+             : run(q8_rows_kernel<VPT, kQ8AddNorm, WARP, false, false>);
 }
 
 }  // namespace ll

@@ -186,9 +186,9 @@ def quantize_q8(y: torch.Tensor):
 
 def rmsnorm_q8(x: torch.Tensor, w: torch.Tensor, eps: float):
     xf = x.float()
-    # squares in 64 bits: fp32 ones of values past 2^64 are infinite
-    rstd = torch.rsqrt(xf.double().pow(2).mean(-1, keepdim=True) + eps).float()
-    return quantize_q8(xf * rstd * w.float())
+    # in 64 bits: fp32 squares of values past 2^64 are infinite, of those below 2^-75 zero
+    rstd = torch.rsqrt(xf.double().pow(2).mean(-1, keepdim=True) + eps)
+    return quantize_q8((xf * rstd).float() * w.float())
 
 
 def linear_q8(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,

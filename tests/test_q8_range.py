@@ -18,7 +18,7 @@ import torch
 
 from sglang_legolink_b200 import ops
 from sglang_legolink_b200.ops import Q8
-from test_q8_ops import KERNELS, integers_q8, q8_like, raw, rows_like
+from test_q8_ops import KERNELS, check_rows_q8, integers_q8, norm64, q8_like, raw, rows_like
 
 gpu = pytest.mark.gpu
 
@@ -274,3 +274,24 @@ def test_more_feature_tiles_than_a_grid_has_places(M):
         want = x.values.double() @ w.values[cols].double().t() * 0.5 * x.scale[:, None].double()
         assert torch.equal(y[:, cols], want.to(torch.bfloat16))
     assert bool(torch.isfinite(y).all()) and ops.check_errors("cuda") == 0
+
+
+def small_rows(K):
+    """Rows whose squares leave fp32 at its lower end, down to bf16's least number."""
+    x = torch.randn(7, K, generator=torch.Generator().manual_seed(3))
+    return (x * torch.tensor([1.0, 1e-12, 1e-18, 1e-20, 1e-25, 1e-36, 0.0])[:, None]).to(torch.bfloat16).index_fill_(
+        0, torch.tensor([6]), 2.0 ** -133)
+
+
+@pytest.mark.parametrize("K", [64, 4096])
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-30])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_norm_of_small_rows_with_a_small_eps(K, eps, device):
+    x, r = small_rows(K).to(device), (small_rows(K).flip(1) / 2).to(device)
+    w = (1 + 0.1 * torch.randn(K, generator=torch.Generator().manual_seed(1))).to(torch.bfloat16).to(device)
+    check_rows_q8(ops.rmsnorm_q8(x, w, eps), norm64(x, w, eps)[0], 2e-5)
+    want, s = norm64(x, w, eps, r)
+    check_rows_q8(ops.fused_add_rmsnorm_q8(x, r, w, eps), want, 2e-5)
+    assert torch.equal(r.cpu(), s.to(torch.bfloat16))
+    none = ops.rmsnorm_q8(torch.zeros(2, K, dtype=torch.bfloat16, device=device), w, eps)
+    assert bool(none.scale.isnan().all()) if eps == 0 else bool((none.values.float() == 0).all())
