@@ -15,12 +15,12 @@
 // * q8_split_kernel -- few rows.  The weight tile is the M = 128 side, the rows
 //   (up to 128) are the N side, and K is split over the CTAs of a cluster, whose
 //   fp32 partials meet in distributed shared memory.  Bound by reading W: 16 rows,
-//   3584 -> 37888 with SwiGLU, 22.0 us in a graph, 6.2 TB/s of its 137 MB.
+//   3584 -> 37888 with SwiGLU, 22.4 us in a graph, 6.1 TB/s of its 137 MB.
 // * q8_pair_kernel -- many rows.  Pairs of CTAs (cta_group::2) on tiles of 256 rows
 //   x 64, 128 or 256 features, persistent, two accumulators in tensor memory, so
 //   that the epilogue of a tile runs beside the main loop of the next.  Bound by the
-//   tensor pipe and the power cap: 2048 rows, 3584 -> 37888 with SwiGLU, 178 us
-//   alone (3.1 PFLOP/s, tensor pipe 89 % active at 1.48 GHz), 222 back to back.
+//   tensor pipe and the power cap: 2048 rows, 3584 -> 37888 with SwiGLU, 176 us
+//   alone (3.1 PFLOP/s, tensor pipe 89 % active at 1.49 GHz), 222 back to back.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

@@ -10,11 +10,12 @@
 // as integers, where a NaN is the largest), so every product of that row is NaN.
 //
 // Bound by memory: each value is read once, kept in registers through the
-// reductions, and written as one byte.  In a graph, of bytes that cannot be saved at
-// 6551 GB/s: quantising 2048 x 18944 18.4 us of 17.8, the norm with the residual's
-// addition of 5087 x 3584 20.5 of 19.5; a few rows 1.0 to 2 us.  The norm alone, 12.6 us
-// of 8.4, issues an instruction in 70 % of the cycles (quantising 60 %), so products go
-// two and maxima three values an instruction (13.7 us before; 5087 x 18944 58.5 for 98).
+// reductions, and written as one byte.  In a graph over rows that L2 does not hold, of
+// bytes that cannot be saved at 6551 GB/s: quantising 2048 x 18944 18.4 us of 17.8, the
+// norm with the residual's addition of 5087 x 3584 21.4 of 19.5; a few rows 1.2 to 2 us.
+// The norm alone, 13.9 us of 8.4, issues an instruction in 65 % of the cycles (with the
+// addition 63 %, quantising 53 %), with products two and maxima three values an
+// instruction (one each issued in 70 %, and 5087 x 18944 took 98 us for 60).
 // Persistent CTAs that fetch rows ahead into shared memory by bulk copies were slower
 // (quantising 5087 x 3584 10.4 us for 9.5, the norm 14.9 for 13.8), and so was one
 // reduction for both the squares and the largest |x w| (15.5 for 13.7: the weight is
